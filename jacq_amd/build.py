@@ -15,7 +15,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libjacq_kivi.so")
 TORCH_LIB = os.path.join(HERE, "libjacq_kivi_torch.so")
-SOURCES = ["kivi_api.hip", "kivi_writer.hip", "kivi_decode.hip", "kivi_decode_mfma.hip"]
+SOURCES = ["kivi_api.hip", "kivi_writer.hip", "kivi_decode.hip", "kivi_decode_mfma.hip",
+           "q8_api.hip", "q8_writer.hip", "q8_decode.hip", "q8_prefill.hip", "q8_evict.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -45,7 +46,9 @@ def hipcc() -> str:
 
 # Kernels that must not spill: a spill makes the kernel need scratch memory,
 # which cost the decode about 17 us (13%) when a 12-byte spill crept in.
-NO_SCRATCH = ("kivi_decode_stream_kernel", "kivi_decode_chunk_kernel", "kivi_append_kernel")
+NO_SCRATCH = ("kivi_decode_stream_kernel", "kivi_decode_chunk_kernel", "kivi_append_kernel",
+              "q8_append_kernel", "q8_read_kernel", "q8_decode_kernel", "q8_join_kernel",
+              "q8_weights_kernel", "q8_prefill_kernel", "q8_evict_kernel")
 
 
 def kernel_resources(remarks: str) -> dict:

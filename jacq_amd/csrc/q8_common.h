@@ -1,0 +1,178 @@
+// q8_common.h -- shared definitions of the 8-bit paged cache's kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "jacq_q8.h"
+
+namespace jacq {
+namespace q8 {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr float kFloor = 0x1p-24f;   // a block's largest magnitude counts as at least this
+constexpr float kHalfMax = 65504.0f;
+constexpr int kTile = 64;            // tokens per step of the attention kernels
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Geo {
+  int nh, nkv, hd, page, page_log2, max_pages, num_pages, gqa, codes;
+};
+
+struct Pool {
+  const uint8_t* k_code;
+  const float* k_scale;
+  const uint8_t* v_code;
+  const float* v_scale;
+  const uint16_t* k_tail;
+  const uint16_t* v_tail;
+};
+
+struct AppendArgs {
+  jacq_q8_pool pool;
+  const uint16_t* new_k;
+  const uint16_t* new_v;
+  int64_t k_stride, v_stride;
+  const int32_t* cu;      // null: one token per sequence
+  const int32_t* start;
+  const int32_t* tables;
+  int total, max_new, bf16;
+};
+
+struct AttendArgs {
+  Pool pool;
+  const uint16_t* q;
+  const int32_t* cu;      // null: one query per sequence
+  const int32_t* lens;
+  const int32_t* tables;
+  void* o;
+  float* lse;             // null: not wanted
+  float* weights;
+  int64_t q_stride;
+  int q_bf16, o_type;     // o_type: JACQ_Q8_*
+  int batch, total_q, max_q;
+  int window, sinks;      // window 0: none
+  float scale;            // log2(e) included
+  float decay;
+  // split pieces and the sums of 16-token groups (decode kernel)
+  float* part_ml;         // [2 runs][rows][2]
+  float* part_acc;        // [2 runs][rows][HD]
+  float* group_lse;       // [batch][nkv][row blocks][groups][rows]
+  float* row_lse;         // [total_q][nh], base 2
+  int runs;               // workgroups of the stream; 0: one workgroup per segment
+  int rows;               // rows of a segment at most (<= 16 NB)
+  int row_blocks;         // row blocks of a sequence at most
+  int min_units;          // units of a run at least
+  int groups;             // 16-token groups a table addresses
+};
+
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float log2_(float x) { return __builtin_amdgcn_logf(x); }
+__device__ inline float bf2f(uint32_t h) { return __uint_as_float(h << 16); }
+__device__ inline uint16_t f2bf(float f) {  // round to nearest even; NaN stays NaN
+  return __builtin_bit_cast(uint16_t, (__bf16)f);
+}
+// by value: a bit_cast of a vector's element in place takes the vector's first
+__device__ inline uint16_t h_bits(_Float16 x) { return __builtin_bit_cast(uint16_t, x); }
+__device__ inline uint16_t f2h_(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+__device__ inline float h2f_(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+
+// Four codes (one dword) as fp16, exactly: what the matrix cores take.
+//  int8: the byte u = code + 128 under the exponent of 1024 is 1024 + u; minus 1152 is the code.
+//  e4m3: the conversion instruction with scale 1.
+template <bool E4M3>
+__device__ inline void codes4(uint32_t w, h2& lo, h2& hi) {
+  if constexpr (E4M3) {
+    lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true);
+  } else {
+    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    lo = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off;
+    hi = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off;
+  }
+}
+
+template <bool E4M3>
+__device__ inline h8 codes8(uint32_t w0, uint32_t w1) {
+  h2 a, b, c, d;
+  codes4<E4M3>(w0, a, b);
+  codes4<E4M3>(w1, c, d);
+  h8 r;
+  r.s01 = a;
+  r.s23 = b;
+  r.s45 = c;
+  r.s67 = d;
+  return r;
+}
+
+__device__ inline int clamp_len(const Geo& g, int n) {
+  const int cap = g.max_pages << g.page_log2;  // the host checked that this fits
+  return n < 0 ? 0 : n > cap ? cap : n;
+}
+
+// Queries of sequence b: rows [q0, q0 + m) of Q, whatever the table of offsets holds.
+__device__ inline void queries_of(const AttendArgs& a, int b, int* q0, int* m) {
+  if (!a.cu) {
+    *q0 = b;
+    *m = 1;
+    return;
+  }
+  int lo = a.cu[b], hi = a.cu[b + 1];
+  lo = lo < 0 ? 0 : lo > a.total_q ? a.total_q : lo;
+  hi = hi < lo ? lo : hi > a.total_q ? a.total_q : hi;
+  *q0 = lo;
+  *m = hi - lo > a.max_q ? a.max_q : hi - lo;
+}
+
+// The tiles of kTile tokens that the queries of a sequence of n tokens may see, in order: the
+// sinks' tiles, the window's, then the tail (fp16) as a unit of its own.
+struct Span {
+  int n;        // tokens
+  int nq;       // of them quantised
+  int w0;       // first tile of the window
+  int ns;       // tiles of the sinks before it
+  int tiles;    // quantised tiles in all
+  int units;    // units of a segment, at least 1 (a segment without tokens still writes its zeros)
+  __device__ Span() {}
+  // first: the lowest position of a query (may be negative)
+  __device__ Span(const Geo& g, int n_, int first, int window, int sinks) {
+    n = n_;
+    nq = n >> g.page_log2 << g.page_log2;
+    tiles = (nq + kTile - 1) / kTile;
+    w0 = ns = 0;
+    if (window > 0 && first >= window) {
+      w0 = (first - window + 1) / kTile;
+      w0 = w0 > tiles ? tiles : w0;
+      const int s = sinks < n ? sinks : n;
+      ns = (int)(((int64_t)s + kTile - 1) / kTile);
+      ns = ns > w0 ? w0 : ns;
+    }
+    units = ns + tiles - w0 + (n > nq ? 1 : 0);
+    units = units < 1 ? 1 : units;
+  }
+  __device__ int tile_of(int u) const { return u < ns ? u : w0 + u - ns; }  // == tiles: the tail
+};
+
+__device__ inline bool sees(int j, int pos, int window, int sinks) {
+  return j <= pos && (window <= 0 || j < sinks || j > pos - window);
+}
+
+hipError_t launch_append(const Geo& g, const AppendArgs& a, int batch, hipStream_t s);
+hipError_t launch_read(const Geo& g, const Pool& p, const int32_t* starts, const int32_t* ends,
+                       const int32_t* tables, int batch, int total, void* k, void* v, int type,
+                       hipStream_t s);
+hipError_t launch_decode(const Geo& g, const AttendArgs& a, int nb, hipStream_t s);
+hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s);
+hipError_t launch_evict(const Geo& g, const float* w, const int32_t* lens, const int32_t* tables,
+                        int batch, int keep, int sink, int recent, int32_t* tables_out,
+                        int32_t* lens_out, float* w_out, int32_t* evicted, hipStream_t s);
+
+}  // namespace q8
+}  // namespace jacq
