@@ -135,7 +135,7 @@ constexpr int kMinUnits = 4;   // units of a run at least
 
 struct Plan {
   bool prefill;
-  int nb, rows, row_blocks, runs, min_units, groups;
+  int rb, nb, rows, row_blocks, runs, min_units, groups;
   size_t ml, acc, group_lse, row_lse, bytes;  // offsets into the workspace, and its size
 };
 
@@ -143,7 +143,10 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
   Plan p = {};
   const int64_t rows = (int64_t)max_q * g.gqa;
   p.prefill = !weighted && rows > kFewRows;
-  if (p.prefill) return p;
+  if (p.prefill) {
+    p.rb = getenv("JRB") ? atoi(getenv("JRB")) : 2;
+    return p;
+  }
   p.nb = rows <= 16 ? 1 : 2;
   p.rows = (int)std::min<int64_t>(rows, 16 * p.nb);
   p.row_blocks = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
@@ -287,7 +290,7 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 ||
         (int64_t)a.batch * g.nkv * std::max(1, p.row_blocks) > INT32_MAX)
       return fail(JACQ_KIVI_EINVAL, "too many query rows in one call");
-    if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, stream), "prefill");
+    if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, p.rb, stream), "prefill");
     if (p.bytes && (!workspace || workspace_bytes < p.bytes))
       return fail(JACQ_KIVI_ENOMEM, "the workspace needs " + std::to_string(p.bytes) +
                                         " bytes, got " +

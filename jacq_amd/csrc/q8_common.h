@@ -169,7 +169,7 @@ hipError_t launch_read(const Geo& g, const Pool& p, const int32_t* starts, const
                        const int32_t* tables, int batch, int total, void* k, void* v, int type,
                        hipStream_t s);
 hipError_t launch_decode(const Geo& g, const AttendArgs& a, int nb, hipStream_t s);
-hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s);
+hipError_t launch_prefill(const Geo& g, const AttendArgs& a, int rb, hipStream_t s);
 hipError_t launch_evict(const Geo& g, const float* w, const int32_t* lens, const int32_t* tables,
                         int batch, int keep, int sink, int recent, int32_t* tables_out,
                         int32_t* lens_out, float* w_out, int32_t* evicted, hipStream_t s);

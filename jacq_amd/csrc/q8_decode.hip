@@ -51,6 +51,7 @@ struct Wave {
     u4 k[4][KL];
     u4 v[DT];
     float ks, vs;
+    bool there;  // a page outside the pool reads as NaN
   };
 
   __device__ Wave(const Geo& g_, const AttendArgs& a_, int lane_)
@@ -103,12 +104,16 @@ struct Wave {
     }
   }
 
-  // The physical page of the 16 tokens from t on, -1 where the table names none.
+  // The table's entry for the 16 tokens from t on; it is looked at when its page is loaded, so
+  // that nothing waits for it before.
   __device__ int page_of(const Segment& s, int t) const {
     const int last = s.span.nq - 16;  // never past the sequence's own entries
     t = t < last ? t : last;
-    const int p = a.tables[(int64_t)s.b * g.max_pages + (t >> g.page_log2)];
-    return p >= 0 && p < g.num_pages ? p : -1;
+    return a.tables[(int64_t)s.b * g.max_pages + (t >> g.page_log2)];
+  }
+  __device__ bool exists(int page) const { return page >= 0 && page < g.num_pages; }
+  __device__ int64_t slot_of(const Segment& s, int page) const {
+    return (int64_t)(exists(page) ? page : 0) * g.nkv + s.h;
   }
 
   __device__ void pages(const Segment& s, int tile, int& pk, int& pv) const {
@@ -119,19 +124,19 @@ struct Wave {
   // A quantised tile's K codes with the scales, and its V codes.
   __device__ void load_k(const Segment& s, int tile, int pk, int pv, Codes& c) const {
     const int tk = (tile * kTile + n16 / 4 * 16) & (g.page - 1);
-    const int64_t sk = (int64_t)(pk < 0 ? 0 : pk) * g.nkv + s.h;
-    const int64_t sv = (int64_t)(pv < 0 ? 0 : pv) * g.nkv + s.h;
+    const int64_t sk = slot_of(s, pk), sv = slot_of(s, pv);
     const uint8_t* k = a.pool.k_code + (sk * g.page + tk + (n16 & 3)) * HD + kq * 16;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int j = 0; j < KL; ++j) c.k[t][j] = *(const u4*)(k + t * 4 * HD + j * 64);
-    c.ks = pv < 0 ? __builtin_nanf("") : a.pool.k_scale[sv];
+    c.ks = a.pool.k_scale[sv];
+    c.there = exists(pv);
     c.vs = a.pool.v_scale[sv];
   }
   __device__ void load_v(const Segment& s, int tile, int pv, Codes& c) const {
     const int tv = (tile * kTile + kq * 16) & (g.page - 1);
-    const int64_t sv = (int64_t)(pv < 0 ? 0 : pv) * g.nkv + s.h;
+    const int64_t sv = slot_of(s, pv);
     const uint8_t* v = a.pool.v_code + (sv * HD + n16) * g.page + tv;
 #pragma unroll
     for (int d = 0; d < DT; ++d) c.v[d] = *(const u4*)(v + d * 16 * g.page);
@@ -281,7 +286,7 @@ struct Wave {
         const bool masked = needs_mask(s, t0, sp.nq);
         f4 sc[NB][4];
         scores(c, sc);
-        const float ks = c.ks, vs = c.vs;
+        const float ks = c.there ? c.ks : __builtin_nanf(""), vs = c.vs;
         if (next >= 0) load_k(s, next, nk, nv, c);
         h8 p[NB][2];
 #pragma unroll

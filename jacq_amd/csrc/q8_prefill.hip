@@ -1,15 +1,16 @@
 // q8_prefill.hip -- attention of prompts over the 8-bit cache.
 //
-// A workgroup has 32 kWaves query rows of one kv head (row = query token x
-// head of the group), 32 a wavefront, and goes through the tiles of 64 tokens
-// that any of its rows sees.  A tile's codes are converted to fp16 once and
-// shared through the LDS, two tiles deep: the next one's codes are in flight
-// while this one is computed.  S^T = K Q^T and O^T += V^T P^T on
+// A workgroup has 128 RB query rows of one kv head (row = query token x head of
+// the group), 32 RB for each of 4 wavefronts, and goes through the tiles of 64
+// tokens that any of its rows sees.  A tile's codes are converted to fp16 once
+// and shared through the LDS.  S^T = K Q^T and O^T += V^T P^T on
 // v_mfma_f32_32x32x16_f16; a lane's column is a query row, so its maximum, sum
 // and rescaling are the lane's own (and its partner's, 32 lanes on), and the
 // order in which K's rows enter makes P the next operand as it stands.
 // The scales of 16 tokens are the wavefront's: t = s (ks q) + log2(vs), as in
 // q8_decode.hip, where the reason is.
+#include <type_traits>
+
 #include "q8_common.h"
 
 namespace jacq {
@@ -17,7 +18,6 @@ namespace q8 {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;
 constexpr float kSlack = 8.0f;  // the running maximum moves only by more than this (base 2)
 constexpr float kNegInf = -__builtin_inff();
 
@@ -25,8 +25,15 @@ template <int HD>
 struct Lds {
   uint16_t k[2][kTile][HD];    // 16-byte chunks of a row are XOR-ed with the row
   uint16_t v[2][HD][kTile];
-  float ks[2][4], lvs[2][4], ivs[2][4];  // per 16 tokens: K scale, log2 and inverse of V's
+  float ks[4][4], lvs[4][4], ivs[4][4];  // per 16 tokens: K scale, log2 and inverse of V's
 };
+
+// LDS writes are done, loads from memory may be in flight.
+__device__ inline void turn() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // Where chunk c (8 values) of a row lies, so that 16 rows' same chunk covers all banks.
 template <int HD>
@@ -35,11 +42,25 @@ __device__ inline int k_chunk(int row, int c) {
 }
 __device__ inline int v_chunk(int d, int c) { return c ^ (d >> 1 & 7); }
 
-template <int HD, bool E4M3>
-__global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendArgs a, int tiles) {
+// The value of the lane 32 on (or back).
+__device__ inline float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
+}
+
+// Bits 0 to n - 1; n in any range.
+__device__ inline uint64_t low_bits(int n) {
+  return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
+}
+
+template <int HD, bool E4M3, int RB>
+__global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_prefill_kernel(
+    Geo g, AttendArgs a, int tiles) {
+  constexpr int kRows = 32 * RB * kWaves;
   constexpr int KS = HD / 16;                        // k-steps of S^T
   constexpr int DT = HD / 32;                        // channel tiles
-  constexpr int KC = kTile * HD / 16 / kThreads;     // 16-code chunks of K a thread stages
+  constexpr int KC = kTile * HD / 16 / kThreads;     // 16-code chunks of K (and of V) a thread stages
   extern __shared__ __align__(16) uint8_t shared_bytes[];
   Lds<HD>& lds = *(Lds<HD>*)shared_bytes;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -53,20 +74,30 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   const int rows = m * g.gqa;
   if (rt * kRows >= rows) return;
   const int n = uniform(clamp_len(g, a.lens[b]));
-  const int row = rt * kRows + wave * 32 + n32;
-  const bool ok = row < rows;
-  const int tok = ok ? row / g.gqa : 0, head = h * g.gqa + row % g.gqa;
-  const int pos = ok ? n - m + tok : -1;
   // positions of the workgroup's and the wavefront's rows
   const int end_row = rows < (rt + 1) * kRows ? rows : (rt + 1) * kRows;
-  const int pfirst = n - m + rt * kRows / g.gqa, plast = n - m + (end_row - 1) / g.gqa;
-  const int wr0 = rt * kRows + wave * 32;
-  const int wr1 = wr0 + 32 < rows ? wr0 + 32 : rows;
-  const int wfirst = n - m + wr0 / g.gqa, wlast = wr0 < rows ? n - m + (wr1 - 1) / g.gqa : -1;
+  const int pfirst = uniform(n - m + rt * kRows / g.gqa);
+  const int plast = uniform(n - m + (end_row - 1) / g.gqa);
+  const int wr0 = rt * kRows + wave * 32 * RB;
+  const int wr1 = wr0 + 32 * RB < rows ? wr0 + 32 * RB : rows;
+  const int wfirst = uniform(n - m + wr0 / g.gqa);
+  const int wlast = uniform(wr0 < rows ? n - m + (wr1 - 1) / g.gqa : -1);
 
-  h8 q[KS];
-  float qs = a.scale;
-  {
+  h8 q[RB][KS];
+  float qs[RB], mx[RB], l[RB];
+  int pos[RB];
+  f16v acc[RB][DT];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = wr0 + rb * 32 + n32;
+    const bool ok = row < rows;
+    const int tok = ok ? row / g.gqa : 0, head = h * g.gqa + row % g.gqa;
+    pos[rb] = ok ? n - m + tok : -1;
+    mx[rb] = kNegInf;
+    l[rb] = 0.0f;
+    qs[rb] = a.scale;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[rb][d] = f16v{};
     const uint16_t* src = a.q + (int64_t)(q0 + tok) * a.q_stride + head * HD + hh * 8;
     u4 raw[KS];
 #pragma unroll
@@ -79,97 +110,119 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
         for (int c = 0; c < 8; ++c)
           big = fmaxf(big, __builtin_fabsf(__uint_as_float(c & 1 ? raw[i][c / 2] & 0xffff0000u
                                                                  : raw[i][c / 2] << 16)));
-      big = fmaxf(big, __shfl_xor(big, 32));
+      big = fmaxf(big, other_half(big));
       const bool plain = !(big > 0.0f && big < __builtin_inff());
       const int e = plain ? 0 : 14 - __builtin_amdgcn_frexp_expf(big);
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int c = 0; c < 8; ++c)
-          q[i][c] = (_Float16)__builtin_amdgcn_ldexpf(
+          q[rb][i][c] = (_Float16)__builtin_amdgcn_ldexpf(
               __uint_as_float(c & 1 ? raw[i][c / 2] & 0xffff0000u : raw[i][c / 2] << 16), e);
-      qs = __builtin_amdgcn_ldexpf(a.scale, -e);
+      qs[rb] = __builtin_amdgcn_ldexpf(a.scale, -e);
     } else {
 #pragma unroll
-      for (int i = 0; i < KS; ++i) q[i] = __builtin_bit_cast(h8, raw[i]);
+      for (int i = 0; i < KS; ++i) q[rb][i] = __builtin_bit_cast(h8, raw[i]);
     }
   }
 
-  // Units: the sinks' tiles, the window's up to the last row's position, the tail.
+  // Tiles: the sinks', the window's up to the last row's position; then the tail.
   const Span sp(g, n, pfirst, a.window, a.sinks);
-  int top = plast < 0 ? 0 : plast / kTile + 1;
+  int top = plast < 0 ? 0 : (plast >> 6) + 1;
   top = top > sp.tiles ? sp.tiles : top;
   const int quant = plast < 0 ? 0 : sp.ns + (top > sp.w0 ? top - sp.w0 : 0);
-  const int units = quant + (plast >= sp.nq && n > sp.nq ? 1 : 0);
 
-  // ---- staging: this thread's chunks of a tile ----
+  // ---- staging: a thread has KC chunks of K and of V ----
+  // K chunk i: 16 codes (kcc) of row kr + i 64 / KC.  V chunk i: 16 tokens (group vg) of channel
+  // vd; those of a page side by side in memory.  A wavefront's chunks are 8 or 16 rows of K, and
+  // at most a page of V: one page each, so the table is read once per wavefront.
+  const int per = g.page >> 4, per_log2 = g.page_log2 - 4;
+  const int kr = tid / (HD / 16), kcc = tid % (HD / 16);
+  constexpr int KR = kTile / KC;
+  uint32_t k_off[KC], v_off[KC];
+  int kt[KC], vt[KC], ks0[KC], ks1[KC], vs0[KC], vs1[KC];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    const int r = kr + i * KR;
+    k_off[i] = (h * g.page + (r & (g.page - 1))) * HD + kcc * 16;
+    kt[i] = uniform(r & -16);
+    ks0[i] = r * HD + k_chunk<HD>(r, 2 * kcc) * 8;
+    ks1[i] = r * HD + k_chunk<HD>(r, 2 * kcc + 1) * 8;
+    const int chunk = tid + i * kThreads, in = chunk & (HD * per - 1), vd = in >> per_log2;
+    const int vg = (chunk / HD >> per_log2 << per_log2) + (in & (per - 1));
+    v_off[i] = (h * HD + vd) * g.page + ((vg * 16) & (g.page - 1));
+    vt[i] = uniform(vg * 16 & -g.page);
+    vs0[i] = vd * kTile + v_chunk(vd, 2 * vg) * 8;
+    vs1[i] = vd * kTile + v_chunk(vd, 2 * vg + 1) * 8;
+  }
+  const int64_t stride = (int64_t)g.nkv * g.page * HD;
+  const int32_t* table = a.tables + (int64_t)b * g.max_pages;
+  // Units past the last one are fetched as the last one again, and never used: the loop's loads
+  // have no branches around them, so each is waited for by itself, a unit after its issue.
+  auto tile_at = [&](int u) { return sp.tile_of(u < quant ? u : quant - 1) * kTile; };
+  auto page_at = [&](int t) {
+    const int last = sp.nq - 16;
+    return table[(t < last ? t : last) >> g.page_log2];
+  };
+  auto exists = [&](int page) { return page >= 0 && page < g.num_pages; };
   u4 kc[KC], vc[KC];
   float scale_k = 0, scale_v = 0;
-  const int per = g.page >> 4;                  // 16-token chunks of a V row in its page
-  const int per_log2 = g.page_log2 - 4;
-  auto page_at = [&](int t) {  // of the 16 tokens at t; -1: none
-    const int last = sp.nq - 16;
-    t = t < last ? t : last;
-    const int p = a.tables[(int64_t)b * g.max_pages + (t >> g.page_log2)];
-    return p >= 0 && p < g.num_pages ? p : -1;
+  bool no_page = false;
+  int pk[KC], pv[KC], ps = 0;
+  auto pages_k = [&](int u) {
+    const int t0 = tile_at(u);
+#pragma unroll
+    for (int i = 0; i < KC; ++i) pk[i] = page_at(t0 + kt[i]);
+    if (wave == 0) ps = page_at(t0 + (lane & 3) * 16);
   };
-  // V chunk i of this thread: 16 tokens group vg of channel vd, side by side in memory
-  auto v_place = [&](int i, int& vd, int& vg) {
-    const int c = tid + kThreads * i;
-    const int in = c & (HD * per - 1);
-    vd = in >> per_log2;
-    vg = (c / HD >> per_log2 << per_log2) + (in & (per - 1));
+  auto pages_v = [&](int u) {
+    const int t0 = tile_at(u);
+#pragma unroll
+    for (int i = 0; i < KC; ++i) pv[i] = page_at(t0 + vt[i]);
   };
-  int pk[KC], pv[KC], ps;
-  auto fetch_pages = [&](int u) {
-    const int t0 = sp.tile_of(u) * kTile;
+  auto fetch_k = [&] {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      pk[i] = page_at(t0 + (tid + kThreads * i) / (HD / 16) / 16 * 16);
-      int vd, vg;
-      v_place(i, vd, vg);
-      pv[i] = page_at(t0 + vg * 16);
+      const int page = uniform(pk[i]);
+      kc[i] = *(const u4*)(a.pool.k_code + (exists(page) ? page : 0) * stride + k_off[i]);
     }
-    ps = page_at(t0 + (tid & 3) * 16);
+    if (wave == 0) {
+      const int64_t s = (int64_t)(exists(ps) ? ps : 0) * g.nkv + h;
+      scale_k = a.pool.k_scale[s];
+      scale_v = a.pool.v_scale[s];
+      no_page = !exists(ps);
+    }
   };
-  auto fetch = [&](int u) {
-    const int t0 = sp.tile_of(u) * kTile;
+  auto fetch_v = [&] {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      const int c = tid + kThreads * i;
-      const int r = c / (HD / 16), cc = c % (HD / 16);
-      const int64_t s = (int64_t)(pk[i] < 0 ? 0 : pk[i]) * g.nkv + h;
-      kc[i] = *(const u4*)(a.pool.k_code + (s * g.page + ((t0 + r) & (g.page - 1))) * HD + cc * 16);
-      int vd, vg;
-      v_place(i, vd, vg);
-      const int64_t sv = (int64_t)(pv[i] < 0 ? 0 : pv[i]) * g.nkv + h;
-      vc[i] = *(const u4*)(a.pool.v_code + (sv * HD + vd) * g.page +
-                           ((t0 + vg * 16) & (g.page - 1)));
+      const int page = uniform(pv[i]);
+      vc[i] = *(const u4*)(a.pool.v_code + (exists(page) ? page : 0) * stride + v_off[i]);
     }
-    const int64_t s = (int64_t)(ps < 0 ? 0 : ps) * g.nkv + h;
-    scale_k = ps < 0 ? __builtin_nanf("") : a.pool.k_scale[s];
-    scale_v = a.pool.v_scale[s];
   };
-  auto stage = [&](int buf) {
+  auto stage_k = [&](int u) {
+    uint16_t* dst = &lds.k[u & 1][0][0];
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      const int c = tid + kThreads * i;
-      const int r = c / (HD / 16), cc = c % (HD / 16);
-      *(h8*)&lds.k[buf][r][k_chunk<HD>(r, 2 * cc) * 8] = codes8<E4M3>(kc[i].x, kc[i].y);
-      *(h8*)&lds.k[buf][r][k_chunk<HD>(r, 2 * cc + 1) * 8] = codes8<E4M3>(kc[i].z, kc[i].w);
-      int vd, vg;
-      v_place(i, vd, vg);
-      *(h8*)&lds.v[buf][vd][v_chunk(vd, 2 * vg) * 8] = codes8<E4M3>(vc[i].x, vc[i].y);
-      *(h8*)&lds.v[buf][vd][v_chunk(vd, 2 * vg + 1) * 8] = codes8<E4M3>(vc[i].z, vc[i].w);
+      *(h8*)(dst + ks0[i]) = codes8<E4M3>(kc[i].x, kc[i].y);
+      *(h8*)(dst + ks1[i]) = codes8<E4M3>(kc[i].z, kc[i].w);
     }
-    if (tid < 4) {
-      lds.ks[buf][tid] = scale_k;
-      lds.lvs[buf][tid] = log2_(scale_v);
-      lds.ivs[buf][tid] = 1.0f / scale_v;
+    if (wave == 0 && lane < 4) {
+      lds.ks[u & 3][lane] = no_page ? __builtin_nanf("") : scale_k;
+      lds.lvs[u & 3][lane] = log2_(scale_v);
+      lds.ivs[u & 3][lane] = scale_v == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(scale_v);  // unwritten
+    }
+  };
+  auto stage_v = [&](int u) {
+    uint16_t* dst = &lds.v[u & 1][0][0];
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      *(h8*)(dst + vs0[i]) = codes8<E4M3>(vc[i].x, vc[i].y);
+      *(h8*)(dst + vs1[i]) = codes8<E4M3>(vc[i].z, vc[i].w);
     }
   };
   // The tail, straight to the LDS: rows behind the last token are 0, never what lies there.
-  auto stage_tail = [&](int buf) {
+  auto stage_tail = [&] {
     const int64_t base = ((int64_t)b * g.nkv + h) * g.page * HD;
     const int have = n - sp.nq;
     for (int c = tid; c < kTile * (HD / 8); c += kThreads) {
@@ -179,151 +232,234 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
         k = *(const h8*)(a.pool.k_tail + base + r * HD + cc * 8);
         v = *(const h8*)(a.pool.v_tail + base + r * HD + cc * 8);
       }
-      *(h8*)&lds.k[buf][r][k_chunk<HD>(r, cc) * 8] = k;
+      *(h8*)&lds.k[0][r][k_chunk<HD>(r, cc) * 8] = k;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int d = cc * 8 + i;
-        lds.v[buf][d][v_chunk(d, r / 8) * 8 + (r & 7)] = h_bits(v[i]);
+        lds.v[0][d][v_chunk(d, r / 8) * 8 + (r & 7)] = h_bits(v[i]);
       }
     }
     if (tid < 4) {
-      lds.ks[buf][tid] = 1.0f;
-      lds.lvs[buf][tid] = 0.0f;
-      lds.ivs[buf][tid] = 1.0f;
+      lds.ks[0][tid] = 1.0f;
+      lds.lvs[0][tid] = 0.0f;
+      lds.ivs[0][tid] = 1.0f;
     }
   };
 
-  f16v acc[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) acc[d] = f16v{};
-  float mx = kNegInf, l = 0.0f;
   // K row of this lane in a tile of 32: the scores of a lane are then tokens 8 hh ... + 7 of
   // either half
   const int krow = (n32 & 16) | (n32 & 4) << 1 | (n32 & 8) >> 1 | (n32 & 3);
+  // LDS offsets (values) of this lane's chunks: a K row's k-steps, a V row's
+  int ko[KS], vo[4];
+#pragma unroll
+  for (int i = 0; i < KS; ++i) ko[i] = krow * HD + k_chunk<HD>(krow, 2 * i + hh) * 8;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) vo[k] = n32 * kTile + v_chunk(n32, 2 * k + hh) * 8;
 
-  auto compute = [&](int buf, int t0, int end) {
-    if (t0 > wlast) return;  // the wavefront's rows are all before the tile
-    if (a.window > 0 && t0 + kTile - 1 <= wfirst - a.window && t0 >= a.sinks) return;
-    const bool masked = t0 + kTile > end || t0 + kTile - 1 > wfirst ||
-                        (a.window > 0 && t0 <= wlast - a.window && t0 + kTile > a.sinks);
-    f16v s[2];
+  f16v s[RB][2];
+  h8 p[RB][4];
+  auto scores = [&](int u) {
+    const uint16_t* kb = &lds.k[u & 1][0][0];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = f16v{};
-      const int r = t * 32 + krow;
+    for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const h8 k = *(const h8*)&lds.k[buf][r][k_chunk<HD>(r, 2 * i + hh) * 8];
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], s[t], 0, 0, 0);
+      for (int t = 0; t < 2; ++t) {
+        const h8 k = *(const h8*)(kb + t * 32 * HD + ko[i]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          s[rb][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[rb][i], i ? s[rb][t] : f16v{}, 0,
+                                                            0, 0);
       }
-    }
-    float top = kNegInf;
+  };
+  // What a tile is to the wavefront's rows: nothing (behind them all, or before their windows),
+  // seen by all of them, or in part.
+  auto nothing = [&](int t0) {
+    return t0 > wlast ||
+           (a.window > 0 && t0 + kTile - 1 <= wfirst - a.window && t0 >= a.sinks);
+  };
+  auto whole = [&](int t0, int end) {
+    return t0 + kTile <= end && t0 + kTile - 1 <= wfirst &&
+           (a.window <= 0 || t0 > wlast - a.window || t0 + kTile <= a.sinks);
+  };
+  auto soften = [&](int u, int t0, int end) {
+    const bool masked = !whole(t0, end);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int rb = 0; rb < RB; ++rb) {
+      // A group of 16 tokens has one scale: its largest t is that of its largest score.
+      float ga[4], gb[4], gi[4], top = kNegInf;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int grp = t * 2 + i / 8;
-        s[t][i] = __builtin_fmaf(s[t][i], lds.ks[buf][grp] * qs, lds.lvs[buf][grp]);
-        if (masked) {
-          const int j = t0 + grp * 16 + hh * 8 + (i & 7);
-          s[t][i] = j < end && sees(j, pos, a.window, a.sinks) ? s[t][i] : kNegInf;
+      for (int k = 0; k < 4; ++k) {
+        ga[k] = lds.ks[u & 3][k] * qs[rb];
+        gb[k] = lds.lvs[u & 3][k];
+        gi[k] = lds.ivs[u & 3][k];
+      }
+      if (masked) {
+        // bit j: token t0 + j is there and seen
+        uint64_t see = low_bits((end < pos[rb] + 1 ? end : pos[rb] + 1) - t0);
+        if (a.window > 0)
+          see &= ~low_bits(pos[rb] + 1 - a.window - t0) | low_bits(a.sinks - t0);
+        see >>= hh * 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t bits = (uint32_t)(see >> (16 * k)) & 255u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            s[rb][k / 2][(k & 1) * 8 + i] = bits >> i & 1 ? s[rb][k / 2][(k & 1) * 8 + i] : kNegInf;
+          // scales that nothing sees may be anything; and -inf times one stays -inf
+          ga[k] = bits == 0 ? 1.0f : ga[k] < 0x1p-100f ? 0x1p-100f : ga[k];
+          gb[k] = bits == 0 ? 0.0f : gb[k];
+          gi[k] = bits == 0 ? 0.0f : gi[k];
         }
-        top = fmaxf(top, s[t][i]);
       }
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__ballot(top > mx + kSlack)) {
-      const float to = top > mx + kSlack ? top : mx;
-      const float f = to > mx ? exp2_(mx - to) : 1.0f;
-      mx = to;
-      l *= f;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) acc[d] *= f;
-    }
-    const float base = mx == kNegInf ? 0.0f : mx;
-    h8 p[4];
+      for (int k = 0; k < 4; ++k) {
+        float x = kNegInf;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = exp2_(s[k / 2][(k & 1) * 8 + i] - base);
-        sum += w;
-        p[k][i] = (_Float16)w;
+        for (int i = 0; i < 8; i += 2)
+          x = fmaxf(fmaxf(x, s[rb][k / 2][(k & 1) * 8 + i]), s[rb][k / 2][(k & 1) * 8 + i + 1]);
+        top = fmaxf(top, __builtin_fmaf(x, ga[k], gb[k]));
       }
-      l += sum == 0.0f ? 0.0f : sum * lds.ivs[buf][k];  // a scale that nothing sees may be any
+      top = fmaxf(top, other_half(top));
+      if (__ballot(top > mx[rb] + kSlack)) {
+        const float to = top > mx[rb] + kSlack ? top : mx[rb];
+        const float f = to > mx[rb] ? exp2_(mx[rb] - to) : 1.0f;
+        mx[rb] = to;
+        l[rb] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[rb][d] *= f;
+      }
+      const float base = mx[rb] == kNegInf ? 0.0f : mx[rb];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float sum = 0.0f;
+        const float off = gb[k] - base;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float w = exp2_(__builtin_fmaf(s[rb][k / 2][(k & 1) * 8 + i], ga[k], off));
+          sum += w;
+          p[rb][k][i] = (_Float16)w;
+        }
+        l[rb] = __builtin_fmaf(sum, gi[k], l[rb]);
+      }
     }
+  };
+  auto values = [&](int u) {
+    const uint16_t* vb = &lds.v[u & 1][0][0];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const int r = d * 32 + n32;
-        const h8 v = *(const h8*)&lds.v[buf][r][v_chunk(r, 2 * k + hh) * 8];
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[k], acc[d], 0, 0, 0);
+        const h8 v = *(const h8*)(vb + d * 32 * kTile + vo[k]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          acc[rb][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[rb][k], acc[rb][d], 0, 0, 0);
       }
   };
 
   if (quant > 0) {
-    fetch_pages(0);
-    fetch(0);
-    if (quant > 1) fetch_pages(1);
-    stage(0);
-  } else if (units > 0) {
-    stage_tail(0);
-  }
-  __syncthreads();
-  for (int u = 0; u < units; ++u) {
-    const int buf = u & 1;
-    if (u + 1 < quant) {
-      fetch(u + 1);
-      if (u + 2 < quant) fetch_pages(u + 2);
+    // K of tiles 0 and 1 and V of tile 0 to the LDS, K of 2 and V of 1 on their way
+    pages_k(0);
+    pages_v(0);
+    fetch_k();
+    fetch_v();
+    pages_k(1);
+    pages_v(1);
+    stage_k(0);
+    stage_v(0);
+    fetch_k();
+    fetch_v();
+    pages_k(2);
+    pages_v(2);
+    stage_k(1);
+    fetch_k();
+    pages_k(3);
+    turn();
+    if (!nothing(tile_at(0))) scores(0);
+    turn();
+    for (int u = 0; u < quant; ++u) {
+      // K of u + 2 takes the place of u's, whose scores are done; V of u + 1 that of u - 1
+      stage_k(u + 2);
+      stage_v(u + 1);
+      fetch_k();
+      fetch_v();
+      pages_k(u + 4);
+      pages_v(u + 3);
+      const int t0 = tile_at(u);
+      if (!nothing(t0)) {
+        soften(u, t0, sp.nq);
+        values(u);
+      }
+      if (u + 1 < quant && !nothing(tile_at(u + 1))) scores(u + 1);
+      turn();
     }
-    if (u < quant) compute(buf, sp.tile_of(u) * kTile, sp.nq);
-    else compute(buf, sp.nq, n);
-    if (u + 1 < quant) stage(buf ^ 1);
-    else if (u + 1 < units) stage_tail(buf ^ 1);
-    __syncthreads();
+  }
+  if (plast >= sp.nq && n > sp.nq) {
+    stage_tail();
+    turn();
+    if (wlast >= sp.nq) {
+      scores(0);
+      soften(0, sp.nq, n);
+      values(0);
+    }
   }
 
-  l += __shfl_xor(l, 32);
-  if (!ok) return;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int64_t at = ((int64_t)(q0 + tok) * g.nh + head) * HD;
-  if (a.lse && hh == 0)
-    a.lse[(int64_t)(q0 + tok) * g.nh + head] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = wr0 + rb * 32 + n32;
+    l[rb] += other_half(l[rb]);
+    if (row >= rows) continue;
+    const int tok = row / g.gqa, head = h * g.gqa + row % g.gqa;
+    const float inv = l[rb] == 0.0f ? 0.0f : 1.0f / l[rb];
+    const int64_t at = ((int64_t)(q0 + tok) * g.nh + head) * HD;
+    if (a.lse && hh == 0)
+      a.lse[(int64_t)(q0 + tok) * g.nh + head] =
+          l[rb] == 0.0f ? kNegInf : (mx[rb] + log2_(l[rb])) / kLog2e;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int ch = d * 32 + i * 8 + hh * 4;
-      const f4 x = {acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv, acc[d][4 * i + 2] * inv,
-                    acc[d][4 * i + 3] * inv};
-      if (a.o_type == JACQ_Q8_FP32) {
-        *(f4*)((float*)a.o + at + ch) = x;
-      } else {
-        const bool bf = a.o_type == JACQ_Q8_BF16;
-        const uint32_t x0 = bf ? f2bf(x.x) : f2h_(x.x), x1 = bf ? f2bf(x.y) : f2h_(x.y);
-        const uint32_t x2 = bf ? f2bf(x.z) : f2h_(x.z), x3 = bf ? f2bf(x.w) : f2h_(x.w);
-        *(u2*)((uint16_t*)a.o + at + ch) = u2{x0 | x1 << 16, x2 | x3 << 16};
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ch = d * 32 + i * 8 + hh * 4;
+        const f4 x = {acc[rb][d][4 * i] * inv, acc[rb][d][4 * i + 1] * inv,
+                      acc[rb][d][4 * i + 2] * inv, acc[rb][d][4 * i + 3] * inv};
+        if (a.o_type == JACQ_Q8_FP32) {
+          *(f4*)((float*)a.o + at + ch) = x;
+        } else {
+          const bool bf = a.o_type == JACQ_Q8_BF16;
+          const uint32_t x0 = bf ? f2bf(x.x) : f2h_(x.x), x1 = bf ? f2bf(x.y) : f2h_(x.y);
+          const uint32_t x2 = bf ? f2bf(x.z) : f2h_(x.z), x3 = bf ? f2bf(x.w) : f2h_(x.w);
+          *(u2*)((uint16_t*)a.o + at + ch) = u2{x0 | x1 << 16, x2 | x3 << 16};
+        }
       }
-    }
+  }
 }
 
-hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s) {
+template <int HD, bool E4M3, int RB>
+static hipError_t prefill_rows(const Geo& g, const AttendArgs& a, hipStream_t s) {
   const int64_t rows = (int64_t)a.max_q * g.gqa;
+  constexpr int kRows = 32 * RB * kWaves;
   const int tiles = (int)((rows + kRows - 1) / kRows);
   const dim3 grid((unsigned)tiles * g.nkv, a.batch);
-#define JACQ_PREFILL(HD, E)                                                                  \
-  hipLaunchKernelGGL((q8_prefill_kernel<HD, E>), grid, dim3(kThreads), sizeof(Lds<HD>), s, g, a, \
-                     tiles)
-  if (g.hd == 128) {
-    if (g.codes == JACQ_Q8_E4M3) JACQ_PREFILL(128, true);
-    else JACQ_PREFILL(128, false);
-  } else {
-    if (g.codes == JACQ_Q8_E4M3) JACQ_PREFILL(64, true);
-    else JACQ_PREFILL(64, false);
+  if (sizeof(Lds<HD>) > 65536) {  // past 64 KiB a kernel asks for its LDS
+    const hipError_t e = hipFuncSetAttribute((const void*)q8_prefill_kernel<HD, E4M3, RB>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)sizeof(Lds<HD>));
+    if (e != hipSuccess) return e;
   }
-#undef JACQ_PREFILL
+  hipLaunchKernelGGL((q8_prefill_kernel<HD, E4M3, RB>), grid, dim3(kThreads), sizeof(Lds<HD>), s,
+                     g, a, tiles);
   return hipGetLastError();
+}
+
+template <int HD, bool E4M3>
+static hipError_t prefill_codes(const Geo& g, const AttendArgs& a, int rb, hipStream_t s) {
+  return rb == 2 ? prefill_rows<HD, E4M3, 2>(g, a, s) : prefill_rows<HD, E4M3, 1>(g, a, s);
+}
+
+hipError_t launch_prefill(const Geo& g, const AttendArgs& a, int rb, hipStream_t s) {
+  const bool e = g.codes == JACQ_Q8_E4M3;
+  if (g.hd == 128)
+    return e ? prefill_codes<128, true>(g, a, rb, s) : prefill_codes<128, false>(g, a, rb, s);
+  return e ? prefill_codes<64, true>(g, a, rb, s) : prefill_codes<64, false>(g, a, rb, s);
 }
 
 }  // namespace q8
