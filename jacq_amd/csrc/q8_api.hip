@@ -129,22 +129,65 @@ int device_cus() {
 }
 
 // ---- how an attention call runs ----
-constexpr int kFewRows = 64;   // query rows of a kv head up to which the decode kernel runs
+// The decode kernel reads the cache once per 32 rows of a kv head and splits it freely; the
+// prefill kernel shares it among 128 rows.  The first is used up to 32 rows, and for so few rows
+// in all that the second leaves most of the chip idle: 40/8 heads of 128, 16384 tokens, one
+// sequence: 8 queries 29 us against 36, 16 queries 41 against 38; four sequences: 8 queries 62
+// against 55; 14/2 heads of 64: 64 queries 35 against 33.
+constexpr int kFewRows = 32;
+constexpr int kFewHeads = 1024;  // queries x query heads of the call
 constexpr int kWholeUnits = 8; // units up to which a workgroup takes a segment whole
 constexpr int kMinUnits = 4;   // units of a run at least
+constexpr int kSliceUnits = 8; // units of a prefill's slice at least, by the table's width
 
 struct Plan {
   bool prefill;
-  int rb, nb, rows, row_blocks, runs, min_units, groups;
+  int slices, nb, rows, row_blocks, runs, min_units, groups;
   size_t ml, acc, group_lse, row_lse, bytes;  // offsets into the workspace, and its size
 };
+
+// Workgroups that share the tokens of a prefill's row tile.  A workgroup alone on a CU takes about
+// 1.7 us a tile of 64 tokens, two 2.5 us (HD 128): `groups` row tiles in S slices take about
+// c(groups S / CUs) / S, c(x) = 1 up to one per CU and 3/4 for each begun one from there, with an
+// end that is not full; the slices' partial sums and their join cost about S 400 / tokens of the
+// whole.  The table's width stands for the tokens.  Measured (us, 40/8 heads of 128): 32 queries
+// over 16384 tokens 430 in one slice, 47 in 16; 511 queries of each of 4 sequences of up to 16001
+// 493 in one, 443 in 2, 446 in 4; a prompt of 8191 825 in one, 907 in 2.
+int plan_slices(double groups, int64_t tokens) {
+  const double load = groups / device_cus();
+  const int most = (int)std::min<int64_t>(32, tokens / (kSliceUnits * jacq::q8::kTile));
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= std::max(1, most); ++s) {
+    const double c = load * s <= 1 ? 1.0 : 0.75 * std::ceil(load * s);
+    const double t = (c + 0.3) / s + (s > 1 ? 0.75 * load * s * 400.0 / (double)tokens : 0.0);
+    if (s == 1 || t < least) {
+      best = s;
+      least = t;
+    }
+  }
+  return best;
+}
 
 Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted) {
   Plan p = {};
   const int64_t rows = (int64_t)max_q * g.gqa;
-  p.prefill = !weighted && rows > kFewRows;
+  p.prefill = !weighted && rows > kFewRows && (int64_t)batch * max_q * g.nh > kFewHeads;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
   if (p.prefill) {
-    p.rb = getenv("JRB") ? atoi(getenv("JRB")) : 2;
+    p.slices = plan_slices((double)jacq::q8::prefill_tiles(g, max_q) * g.nkv * batch,
+                           (int64_t)g.max_pages * g.page);
+    if (p.slices > 1) {
+      const size_t rows_all = (size_t)p.slices * total_q * g.nh;
+      p.ml = take(rows_all * 2 * sizeof(float));
+      p.acc = take(rows_all * g.hd * sizeof(float));
+    }
+    p.bytes = at;
     return p;
   }
   p.nb = rows <= 16 ? 1 : 2;
@@ -159,12 +202,6 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
     p.runs = (int)std::max<int64_t>(
         1, std::min(resident, (segments * most + p.min_units - 1) / p.min_units));
   }
-  size_t at = 0;
-  auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += (bytes + 255) / 256 * 256;
-    return here;
-  };
   p.ml = take((size_t)2 * p.runs * p.rows * 2 * sizeof(float));
   p.acc = take((size_t)2 * p.runs * p.rows * g.hd * sizeof(float));
   p.group_lse = take(weighted ? (size_t)segments * p.groups * p.rows * sizeof(float) : 0);
@@ -290,7 +327,6 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 ||
         (int64_t)a.batch * g.nkv * std::max(1, p.row_blocks) > INT32_MAX)
       return fail(JACQ_KIVI_EINVAL, "too many query rows in one call");
-    if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, p.rb, stream), "prefill");
     if (p.bytes && (!workspace || workspace_bytes < p.bytes))
       return fail(JACQ_KIVI_ENOMEM, "the workspace needs " + std::to_string(p.bytes) +
                                         " bytes, got " +
@@ -300,6 +336,8 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.part_acc = (float*)(ws + p.acc);
     a.group_lse = a.weights ? (float*)(ws + p.group_lse) : nullptr;
     a.row_lse = a.weights ? (float*)(ws + p.row_lse) : nullptr;
+    a.slices = p.slices;
+    if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, stream), "prefill");
     a.runs = p.runs;
     a.rows = p.rows;
     a.row_blocks = p.row_blocks;

@@ -60,9 +60,9 @@ struct AttendArgs {
   int window, sinks;      // window 0: none
   float scale;            // log2(e) included
   float decay;
-  // split pieces and the sums of 16-token groups (decode kernel)
-  float* part_ml;         // [2 runs][rows][2]
-  float* part_acc;        // [2 runs][rows][HD]
+  // split pieces and the sums of 16-token groups
+  float* part_ml;         // decode: [2 runs][rows][2]; prefill: [slices][total_q][nh][2]
+  float* part_acc;        // the same [HD]
   float* group_lse;       // [batch][nkv][row blocks][groups][rows]
   float* row_lse;         // [total_q][nh], base 2
   int runs;               // workgroups of the stream; 0: one workgroup per segment
@@ -70,6 +70,7 @@ struct AttendArgs {
   int row_blocks;         // row blocks of a sequence at most
   int min_units;          // units of a run at least
   int groups;             // 16-token groups a table addresses
+  int slices;             // prefill: workgroups that share a row tile's tokens
 };
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -169,7 +170,8 @@ hipError_t launch_read(const Geo& g, const Pool& p, const int32_t* starts, const
                        const int32_t* tables, int batch, int total, void* k, void* v, int type,
                        hipStream_t s);
 hipError_t launch_decode(const Geo& g, const AttendArgs& a, int nb, hipStream_t s);
-hipError_t launch_prefill(const Geo& g, const AttendArgs& a, int rb, hipStream_t s);
+hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s);
+int prefill_tiles(const Geo& g, int max_q);  // workgroups of a kv head and slice
 hipError_t launch_evict(const Geo& g, const float* w, const int32_t* lens, const int32_t* tables,
                         int batch, int keep, int sink, int recent, int32_t* tables_out,
                         int32_t* lens_out, float* w_out, int32_t* evicted, hipStream_t s);

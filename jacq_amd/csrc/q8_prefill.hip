@@ -1,8 +1,8 @@
 // q8_prefill.hip -- attention of prompts over the 8-bit cache.
 //
-// A workgroup has 128 RB query rows of one kv head (row = query token x head of
-// the group), 32 RB for each of 4 wavefronts, and goes through the tiles of 64
-// tokens that any of its rows sees.  A tile's codes are converted to fp16 once
+// A workgroup has 128 query rows of one kv head (row = query token x head of
+// the group), 32 for each of 4 wavefronts, and goes through the tiles of 64
+// tokens that any of its rows sees, or through one of several slices of them.  A tile's codes are converted to fp16 once
 // and shared through the LDS.  S^T = K Q^T and O^T += V^T P^T on
 // v_mfma_f32_32x32x16_f16; a lane's column is a query row, so its maximum, sum
 // and rescaling are the lane's own (and its partner's, 32 lanes on), and the
@@ -18,6 +18,7 @@ namespace q8 {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
+constexpr int kRows = 32 * kWaves;
 constexpr float kSlack = 8.0f;  // the running maximum moves only by more than this (base 2)
 constexpr float kNegInf = -__builtin_inff();
 
@@ -49,15 +50,25 @@ __device__ inline float other_half(float x) {
   return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
 }
 
+// 4 values of O, in its type.
+__device__ inline void store4(const AttendArgs& a, int64_t at, f4 x) {
+  if (a.o_type == JACQ_Q8_FP32) {
+    *(f4*)((float*)a.o + at) = x;
+    return;
+  }
+  const bool bf = a.o_type == JACQ_Q8_BF16;
+  const uint32_t x0 = bf ? f2bf(x.x) : f2h_(x.x), x1 = bf ? f2bf(x.y) : f2h_(x.y);
+  const uint32_t x2 = bf ? f2bf(x.z) : f2h_(x.z), x3 = bf ? f2bf(x.w) : f2h_(x.w);
+  *(u2*)((uint16_t*)a.o + at) = u2{x0 | x1 << 16, x2 | x3 << 16};
+}
+
 // Bits 0 to n - 1; n in any range.
 __device__ inline uint64_t low_bits(int n) {
   return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
 }
 
-template <int HD, bool E4M3, int RB>
-__global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_prefill_kernel(
-    Geo g, AttendArgs a, int tiles) {
-  constexpr int kRows = 32 * RB * kWaves;
+template <int HD, bool E4M3>
+__global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendArgs a, int tiles) {
   constexpr int KS = HD / 16;                        // k-steps of S^T
   constexpr int DT = HD / 32;                        // channel tiles
   constexpr int KC = kTile * HD / 16 / kThreads;     // 16-code chunks of K (and of V) a thread stages
@@ -67,6 +78,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
   const int n32 = lane & 31, hh = lane >> 5;
   const int b = blockIdx.y, h = blockIdx.x % g.nkv;
   const int rt = tiles - 1 - (int)blockIdx.x / g.nkv;  // the longest first
+  const int slice = blockIdx.z;
   int q0, m;
   queries_of(a, b, &q0, &m);
   q0 = uniform(q0);
@@ -78,26 +90,21 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
   const int end_row = rows < (rt + 1) * kRows ? rows : (rt + 1) * kRows;
   const int pfirst = uniform(n - m + rt * kRows / g.gqa);
   const int plast = uniform(n - m + (end_row - 1) / g.gqa);
-  const int wr0 = rt * kRows + wave * 32 * RB;
-  const int wr1 = wr0 + 32 * RB < rows ? wr0 + 32 * RB : rows;
+  const int wr0 = rt * kRows + wave * 32;
+  const int wr1 = wr0 + 32 < rows ? wr0 + 32 : rows;
   const int wfirst = uniform(n - m + wr0 / g.gqa);
   const int wlast = uniform(wr0 < rows ? n - m + (wr1 - 1) / g.gqa : -1);
 
-  h8 q[RB][KS];
-  float qs[RB], mx[RB], l[RB];
-  int pos[RB];
-  f16v acc[RB][DT];
+  const int row = wr0 + n32;
+  const bool ok = row < rows;
+  const int tok = ok ? row / g.gqa : 0, head = h * g.gqa + row % g.gqa;
+  const int pos = ok ? n - m + tok : -1;
+  h8 q[KS];
+  float qs = a.scale, mx = kNegInf, l = 0.0f;
+  f16v acc[DT];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int row = wr0 + rb * 32 + n32;
-    const bool ok = row < rows;
-    const int tok = ok ? row / g.gqa : 0, head = h * g.gqa + row % g.gqa;
-    pos[rb] = ok ? n - m + tok : -1;
-    mx[rb] = kNegInf;
-    l[rb] = 0.0f;
-    qs[rb] = a.scale;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) acc[rb][d] = f16v{};
+  for (int d = 0; d < DT; ++d) acc[d] = f16v{};
+  {
     const uint16_t* src = a.q + (int64_t)(q0 + tok) * a.q_stride + head * HD + hh * 8;
     u4 raw[KS];
 #pragma unroll
@@ -117,20 +124,23 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
       for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int c = 0; c < 8; ++c)
-          q[rb][i][c] = (_Float16)__builtin_amdgcn_ldexpf(
+          q[i][c] = (_Float16)__builtin_amdgcn_ldexpf(
               __uint_as_float(c & 1 ? raw[i][c / 2] & 0xffff0000u : raw[i][c / 2] << 16), e);
-      qs[rb] = __builtin_amdgcn_ldexpf(a.scale, -e);
+      qs = __builtin_amdgcn_ldexpf(a.scale, -e);
     } else {
 #pragma unroll
-      for (int i = 0; i < KS; ++i) q[rb][i] = __builtin_bit_cast(h8, raw[i]);
+      for (int i = 0; i < KS; ++i) q[i] = __builtin_bit_cast(h8, raw[i]);
     }
   }
 
-  // Tiles: the sinks', the window's up to the last row's position; then the tail.
+  // Tiles: the sinks', the window's up to the last row's position; of them this slice's, from
+  // `from` on.  Then the tail, the last slice's.
   const Span sp(g, n, pfirst, a.window, a.sinks);
   int top = plast < 0 ? 0 : (plast >> 6) + 1;
   top = top > sp.tiles ? sp.tiles : top;
-  const int quant = plast < 0 ? 0 : sp.ns + (top > sp.w0 ? top - sp.w0 : 0);
+  const int every = plast < 0 ? 0 : sp.ns + (top > sp.w0 ? top - sp.w0 : 0);
+  const int from = uniform((int)((int64_t)every * slice / a.slices));
+  const int quant = uniform((int)((int64_t)every * (slice + 1) / a.slices)) - from;
 
   // ---- staging: a thread has KC chunks of K and of V ----
   // K chunk i: 16 codes (kcc) of row kr + i 64 / KC.  V chunk i: 16 tokens (group vg) of channel
@@ -159,7 +169,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
   const int32_t* table = a.tables + (int64_t)b * g.max_pages;
   // Units past the last one are fetched as the last one again, and never used: the loop's loads
   // have no branches around them, so each is waited for by itself, a unit after its issue.
-  auto tile_at = [&](int u) { return sp.tile_of(u < quant ? u : quant - 1) * kTile; };
+  auto tile_at = [&](int u) { return sp.tile_of(from + (u < quant ? u : quant - 1)) * kTile; };
   auto page_at = [&](int t) {
     const int last = sp.nq - 16;
     return table[(t < last ? t : last) >> g.page_log2];
@@ -256,8 +266,8 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
 #pragma unroll
   for (int k = 0; k < 4; ++k) vo[k] = n32 * kTile + v_chunk(n32, 2 * k + hh) * 8;
 
-  f16v s[RB][2];
-  h8 p[RB][4];
+  f16v s[2];
+  h8 p[4];
   auto scores = [&](int u) {
     const uint16_t* kb = &lds.k[u & 1][0][0];
 #pragma unroll
@@ -265,10 +275,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const h8 k = *(const h8*)(kb + t * 32 * HD + ko[i]);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          s[rb][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[rb][i], i ? s[rb][t] : f16v{}, 0,
-                                                            0, 0);
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], i ? s[t] : f16v{}, 0, 0, 0);
       }
   };
   // What a tile is to the wavefront's rows: nothing (behind them all, or before their windows),
@@ -283,64 +290,61 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
   };
   auto soften = [&](int u, int t0, int end) {
     const bool masked = !whole(t0, end);
+    // A group of 16 tokens has one scale: its largest t is that of its largest score.
+    float ga[4], gb[4], gi[4], top = kNegInf;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      // A group of 16 tokens has one scale: its largest t is that of its largest score.
-      float ga[4], gb[4], gi[4], top = kNegInf;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        ga[k] = lds.ks[u & 3][k] * qs[rb];
-        gb[k] = lds.lvs[u & 3][k];
-        gi[k] = lds.ivs[u & 3][k];
-      }
-      if (masked) {
-        // bit j: token t0 + j is there and seen
-        uint64_t see = low_bits((end < pos[rb] + 1 ? end : pos[rb] + 1) - t0);
-        if (a.window > 0)
-          see &= ~low_bits(pos[rb] + 1 - a.window - t0) | low_bits(a.sinks - t0);
-        see >>= hh * 8;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t bits = (uint32_t)(see >> (16 * k)) & 255u;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            s[rb][k / 2][(k & 1) * 8 + i] = bits >> i & 1 ? s[rb][k / 2][(k & 1) * 8 + i] : kNegInf;
-          // scales that nothing sees may be anything; and -inf times one stays -inf
-          ga[k] = bits == 0 ? 1.0f : ga[k] < 0x1p-100f ? 0x1p-100f : ga[k];
-          gb[k] = bits == 0 ? 0.0f : gb[k];
-          gi[k] = bits == 0 ? 0.0f : gi[k];
-        }
-      }
+    for (int k = 0; k < 4; ++k) {
+      ga[k] = lds.ks[u & 3][k] * qs;
+      gb[k] = lds.lvs[u & 3][k];
+      gi[k] = lds.ivs[u & 3][k];
+    }
+    if (masked) {
+      // bit j: token t0 + j is there and seen
+      uint64_t see = low_bits((end < pos + 1 ? end : pos + 1) - t0);
+      if (a.window > 0)
+        see &= ~low_bits(pos + 1 - a.window - t0) | low_bits(a.sinks - t0);
+      see >>= hh * 8;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float x = kNegInf;
+        const uint32_t bits = (uint32_t)(see >> (16 * k)) & 255u;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2)
-          x = fmaxf(fmaxf(x, s[rb][k / 2][(k & 1) * 8 + i]), s[rb][k / 2][(k & 1) * 8 + i + 1]);
-        top = fmaxf(top, __builtin_fmaf(x, ga[k], gb[k]));
+        for (int i = 0; i < 8; ++i)
+          s[k / 2][(k & 1) * 8 + i] = bits >> i & 1 ? s[k / 2][(k & 1) * 8 + i] : kNegInf;
+        // scales that nothing sees may be anything; and -inf times one stays -inf
+        ga[k] = bits == 0 ? 1.0f : ga[k] < 0x1p-100f ? 0x1p-100f : ga[k];
+        gb[k] = bits == 0 ? 0.0f : gb[k];
+        gi[k] = bits == 0 ? 0.0f : gi[k];
       }
-      top = fmaxf(top, other_half(top));
-      if (__ballot(top > mx[rb] + kSlack)) {
-        const float to = top > mx[rb] + kSlack ? top : mx[rb];
-        const float f = to > mx[rb] ? exp2_(mx[rb] - to) : 1.0f;
-        mx[rb] = to;
-        l[rb] *= f;
+    }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[rb][d] *= f;
+    for (int k = 0; k < 4; ++k) {
+      float x = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2)
+        x = fmaxf(fmaxf(x, s[k / 2][(k & 1) * 8 + i]), s[k / 2][(k & 1) * 8 + i + 1]);
+      top = fmaxf(top, __builtin_fmaf(x, ga[k], gb[k]));
+    }
+    top = fmaxf(top, other_half(top));
+    if (__ballot(top > mx + kSlack)) {
+      const float to = top > mx + kSlack ? top : mx;
+      const float f = to > mx ? exp2_(mx - to) : 1.0f;
+      mx = to;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] *= f;
+    }
+    const float base = mx == kNegInf ? 0.0f : mx;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float sum = 0.0f;
+      const float off = gb[k] - base;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = exp2_(__builtin_fmaf(s[k / 2][(k & 1) * 8 + i], ga[k], off));
+        sum += w;
+        p[k][i] = (_Float16)w;
       }
-      const float base = mx[rb] == kNegInf ? 0.0f : mx[rb];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float sum = 0.0f;
-        const float off = gb[k] - base;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float w = exp2_(__builtin_fmaf(s[rb][k / 2][(k & 1) * 8 + i], ga[k], off));
-          sum += w;
-          p[rb][k][i] = (_Float16)w;
-        }
-        l[rb] = __builtin_fmaf(sum, gi[k], l[rb]);
-      }
+      l = __builtin_fmaf(sum, gi[k], l);
     }
   };
   auto values = [&](int u) {
@@ -350,9 +354,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const h8 v = *(const h8*)(vb + d * 32 * kTile + vo[k]);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          acc[rb][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[rb][k], acc[rb][d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[k], acc[d], 0, 0, 0);
       }
   };
 
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
       turn();
     }
   }
-  if (plast >= sp.nq && n > sp.nq) {
+  if (plast >= sp.nq && n > sp.nq && slice == a.slices - 1) {
     stage_tail();
     turn();
     if (wlast >= sp.nq) {
@@ -403,63 +405,88 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RB == 2 ? 1 : 2) void q8_pre
     }
   }
 
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int row = wr0 + rb * 32 + n32;
-    l[rb] += other_half(l[rb]);
-    if (row >= rows) continue;
-    const int tok = row / g.gqa, head = h * g.gqa + row % g.gqa;
-    const float inv = l[rb] == 0.0f ? 0.0f : 1.0f / l[rb];
-    const int64_t at = ((int64_t)(q0 + tok) * g.nh + head) * HD;
-    if (a.lse && hh == 0)
-      a.lse[(int64_t)(q0 + tok) * g.nh + head] =
-          l[rb] == 0.0f ? kNegInf : (mx[rb] + log2_(l[rb])) / kLog2e;
+  l += other_half(l);
+  if (!ok) return;
+  const int64_t at = (int64_t)(q0 + tok) * g.nh + head;
+  if (a.slices > 1) {  // q8_merge_kernel joins the slices
+    const int64_t part = (int64_t)slice * a.total_q * g.nh + at;
+    if (hh == 0) {
+      a.part_ml[2 * part] = mx;
+      a.part_ml[2 * part + 1] = l;
+    }
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ch = d * 32 + i * 8 + hh * 4;
-        const f4 x = {acc[rb][d][4 * i] * inv, acc[rb][d][4 * i + 1] * inv,
-                      acc[rb][d][4 * i + 2] * inv, acc[rb][d][4 * i + 3] * inv};
-        if (a.o_type == JACQ_Q8_FP32) {
-          *(f4*)((float*)a.o + at + ch) = x;
-        } else {
-          const bool bf = a.o_type == JACQ_Q8_BF16;
-          const uint32_t x0 = bf ? f2bf(x.x) : f2h_(x.x), x1 = bf ? f2bf(x.y) : f2h_(x.y);
-          const uint32_t x2 = bf ? f2bf(x.z) : f2h_(x.z), x3 = bf ? f2bf(x.w) : f2h_(x.w);
-          *(u2*)((uint16_t*)a.o + at + ch) = u2{x0 | x1 << 16, x2 | x3 << 16};
-        }
-      }
+      for (int i = 0; i < 4; ++i)
+        *(f4*)(a.part_acc + part * HD + d * 32 + i * 8 + hh * 4) =
+            f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+    return;
   }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (a.lse && hh == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store4(a, at * HD + d * 32 + i * 8 + hh * 4,
+             f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]} * inv);
 }
 
-template <int HD, bool E4M3, int RB>
-static hipError_t prefill_rows(const Geo& g, const AttendArgs& a, hipStream_t s) {
-  const int64_t rows = (int64_t)a.max_q * g.gqa;
-  constexpr int kRows = 32 * RB * kWaves;
-  const int tiles = (int)((rows + kRows - 1) / kRows);
-  const dim3 grid((unsigned)tiles * g.nkv, a.batch);
+// Joins the slices of every row, in their order: a thread per 4 channels.  blockIdx.y: sequence.
+template <int HD>
+__global__ __launch_bounds__(256) void q8_merge_kernel(Geo g, AttendArgs a) {
+  int q0, m;
+  queries_of(a, blockIdx.y, &q0, &m);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int ch = (int)(i % (HD / 4)) * 4;
+  if (i / (HD / 4) >= (int64_t)m * g.nh) return;
+  const int64_t at = (int64_t)q0 * g.nh + i / (HD / 4), rows = (int64_t)a.total_q * g.nh;
+  float mx = kNegInf, l = 0.0f;
+  f4 acc = {0, 0, 0, 0};
+  for (int s = 0; s < a.slices; ++s) {
+    const float pm = a.part_ml[2 * (s * rows + at)], pl = a.part_ml[2 * (s * rows + at) + 1];
+    const f4 pa = *(const f4*)(a.part_acc + (s * rows + at) * HD + ch);
+    const float to = fmaxf(mx, pm);
+    // a part without a maximum saw nothing, or only NaN: l tells
+    const float f0 = mx == kNegInf ? 1.0f : exp2_(mx - to);
+    const float f1 = pm == kNegInf ? 1.0f : exp2_(pm - to);
+    acc = acc * f0 + pa * f1;
+    l = l * f0 + pl * f1;
+    mx = to;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  store4(a, at * HD + ch, acc * inv);
+  if (a.lse && ch == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
+}
+
+template <int HD, bool E4M3>
+static hipError_t prefill_codes(const Geo& g, const AttendArgs& a, hipStream_t s) {
+  const int tiles = prefill_tiles(g, a.max_q);
+  const dim3 grid((unsigned)tiles * g.nkv, a.batch, a.slices);
   if (sizeof(Lds<HD>) > 65536) {  // past 64 KiB a kernel asks for its LDS
-    const hipError_t e = hipFuncSetAttribute((const void*)q8_prefill_kernel<HD, E4M3, RB>,
+    const hipError_t e = hipFuncSetAttribute((const void*)q8_prefill_kernel<HD, E4M3>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)sizeof(Lds<HD>));
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((q8_prefill_kernel<HD, E4M3, RB>), grid, dim3(kThreads), sizeof(Lds<HD>), s,
-                     g, a, tiles);
+  hipLaunchKernelGGL((q8_prefill_kernel<HD, E4M3>), grid, dim3(kThreads), sizeof(Lds<HD>), s, g, a,
+                     tiles);
+  if (a.slices > 1) {
+    const int64_t threads = (int64_t)a.max_q * g.nh * (HD / 4);
+    hipLaunchKernelGGL((q8_merge_kernel<HD>), dim3((unsigned)((threads + 255) / 256), a.batch),
+                       dim3(256), 0, s, g, a);
+  }
   return hipGetLastError();
 }
 
-template <int HD, bool E4M3>
-static hipError_t prefill_codes(const Geo& g, const AttendArgs& a, int rb, hipStream_t s) {
-  return rb == 2 ? prefill_rows<HD, E4M3, 2>(g, a, s) : prefill_rows<HD, E4M3, 1>(g, a, s);
+int prefill_tiles(const Geo& g, int max_q) {
+  return (int)(((int64_t)max_q * g.gqa + kRows - 1) / kRows);
 }
 
-hipError_t launch_prefill(const Geo& g, const AttendArgs& a, int rb, hipStream_t s) {
+hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s) {
   const bool e = g.codes == JACQ_Q8_E4M3;
-  if (g.hd == 128)
-    return e ? prefill_codes<128, true>(g, a, rb, s) : prefill_codes<128, false>(g, a, rb, s);
-  return e ? prefill_codes<64, true>(g, a, rb, s) : prefill_codes<64, false>(g, a, rb, s);
+  if (g.hd == 128) return e ? prefill_codes<128, true>(g, a, s) : prefill_codes<128, false>(g, a, s);
+  return e ? prefill_codes<64, true>(g, a, s) : prefill_codes<64, false>(g, a, s);
 }
 
 }  // namespace q8

@@ -426,6 +426,28 @@ def test_prefill_window_and_sinks(q8, window, sinks, few):
     check_attention(cache, tables, lens, q, cu, got, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads,m,n", [((40, 8, 128), 60, 9000), ((14, 2, 64), 300, 5003),
+                                       ((8, 8, 128), 700, 2049), ((16, 1, 64), 70, 20001)])
+def test_prefill_in_slices(q8, codes, heads, m, n):
+    """Few row tiles over long contexts: several workgroups share a tile's tokens."""
+    nh, nkv, hd = heads
+    lens, ms = [n, 40, n // 3], [m, 40, 0]
+    cache, tables, seq = make(q8, nh, nkv, hd, 32, codes, lens, seed=45)
+    spoil(cache, tables, lens)
+    size = q8.lib().jacq_q8_attend_workspace_size(cache.geo.ref, 3, m + 40, m, 0)
+    assert size >= 2 * (m + 40) * nh * (hd + 2) * 4  # in slices indeed
+    gen = torch.Generator("cuda").manual_seed(46)
+    cu = [0, m, m + 40, m + 40]
+    q = randn(gen, cu[-1] + 2, nh, hd, dtype=torch.bfloat16)
+    for window, sinks in ((None, 0), (500, 3)):
+        out = torch.full((cu[-1] + 2, nh, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((cu[-1] + 2, nh), 7.0, device="cuda")
+        cache.prefill(q, ints(*cu), m, seq, tables, window=window, sinks=sinks, out=out, lse=lse)
+        check_attention(cache, tables, lens, q, cu, out, lse, window=window, sinks=sinks)
+        assert bool((out[cu[-1]:] == 7).all()) and bool((lse[cu[-1]:] == 7).all())
+
+
 @pytest.mark.parametrize("heads", [(4, 4, 64), (10, 2, 128), (16, 1, 64)])
 @pytest.mark.parametrize("m", [2, 3, 4, 8, 13])
 def test_few_queries(q8, heads, m):
