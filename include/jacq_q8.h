@@ -98,7 +98,8 @@ int jacq_q8_append(const jacq_q8_geometry* geo, const jacq_q8_pool* pool, const 
  * CU_Q[b] to CU_Q[b + 1] of Q (one each when CU_Q is NULL), its last tokens:
  * query i of m stands at position SEQ_LENS[b] - m + i and sees the tokens
  * j <= position with j < sinks or j > position - window (all j <= position
- * when window is 0).  A query that sees nothing gives 0 (lse -inf).
+ * when window is 0).  A query that sees nothing gives 0 (lse -inf).  Scores
+ * are scale (> 0) times the products.
  *   Q        [total_q, NH, HD] of q_dtype, token rows q_stride elements apart
  *   O        [total_q, NH, HD] of o_dtype (q_dtype or fp32), contiguous
  *   LSE      NULL or [total_q, NH] fp32: log of the sum of exp(scaled scores)

@@ -136,13 +136,14 @@ int device_cus() {
 // against 55; 14/2 heads of 64: 64 queries 35 against 33.
 constexpr int kFewRows = 32;
 constexpr int kFewHeads = 1024;  // queries x query heads of the call
-constexpr int kWholeUnits = 8; // units up to which a workgroup takes a segment whole
-constexpr int kMinUnits = 4;   // units of a run at least
+// Units up to which the decode kernel does not cut a segment (slice_units would not either): no
+// plan, no join.  The table's width bounds them, so a narrow table saves about 4 us.
+constexpr int kWholeUnits = 16;
 constexpr int kSliceUnits = 8; // units of a prefill's slice at least, by the table's width
 
 struct Plan {
   bool prefill;
-  int slices, nb, rows, row_blocks, runs, min_units, groups;
+  int slices, nb, rows, row_blocks, target, groups;
   size_t ml, acc, group_lse, row_lse, bytes;  // offsets into the workspace, and its size
 };
 
@@ -194,16 +195,12 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
   p.rows = (int)std::min<int64_t>(rows, 16 * p.nb);
   p.row_blocks = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
   p.groups = g.max_pages * (g.page / 16);
-  p.min_units = kMinUnits;
   const int64_t most = ((int64_t)p.groups + 3) / 4 + 1;  // units of a segment at most
   const int64_t segments = (int64_t)batch * g.nkv * p.row_blocks;
-  if (most > kWholeUnits) {
-    const int64_t resident = (int64_t)device_cus() * (p.nb == 1 ? 2 : 1);
-    p.runs = (int)std::max<int64_t>(
-        1, std::min(resident, (segments * most + p.min_units - 1) / p.min_units));
-  }
-  p.ml = take((size_t)2 * p.runs * p.rows * 2 * sizeof(float));
-  p.acc = take((size_t)2 * p.runs * p.rows * g.hd * sizeof(float));
+  if (most > kWholeUnits) p.target = 4 * device_cus();
+  const size_t parts = p.target ? (size_t)p.target + segments : 0;
+  p.ml = take(parts * p.rows * 2 * sizeof(float));
+  p.acc = take(parts * p.rows * g.hd * sizeof(float));
   p.group_lse = take(weighted ? (size_t)segments * p.groups * p.rows * sizeof(float) : 0);
   p.row_lse = take(weighted ? (size_t)total_q * g.nh * sizeof(float) : 0);
   p.bytes = at;
@@ -289,8 +286,8 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
       return fail(JACQ_KIVI_EINVAL, "without CU_Q every sequence has one query");
     if (x->window < 0 || x->sinks < 0)
       return fail(JACQ_KIVI_EINVAL, "window and sinks must not be negative");
-    if (!std::isfinite(x->scale) || !std::isfinite(x->decay) || x->decay < 0)
-      return fail(JACQ_KIVI_EINVAL, "scale and decay must be finite, decay not negative");
+    if (!std::isfinite(x->scale) || x->scale <= 0 || !std::isfinite(x->decay) || x->decay < 0)
+      return fail(JACQ_KIVI_EINVAL, "scale must be positive and finite, decay not negative");
     if (x->WEIGHTS && x->max_q > JACQ_Q8_MAX_WEIGHTED_QUERIES)
       return fail(JACQ_KIVI_EINVAL, "block weights take at most 64 queries per sequence, got " +
                                         std::to_string(x->max_q));
@@ -338,10 +335,9 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.row_lse = a.weights ? (float*)(ws + p.row_lse) : nullptr;
     a.slices = p.slices;
     if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, stream), "prefill");
-    a.runs = p.runs;
+    a.target = p.target;
     a.rows = p.rows;
     a.row_blocks = p.row_blocks;
-    a.min_units = p.min_units;
     a.groups = p.groups;
     return launched(jacq::q8::launch_decode(g, a, p.nb, stream), "decode");
   });

@@ -61,14 +61,13 @@ struct AttendArgs {
   float scale;            // log2(e) included
   float decay;
   // split pieces and the sums of 16-token groups
-  float* part_ml;         // decode: [2 runs][rows][2]; prefill: [slices][total_q][nh][2]
+  float* part_ml;         // decode: [target + segments][rows][2]; prefill: [slices][total_q][nh][2]
   float* part_acc;        // the same [HD]
   float* group_lse;       // [batch][nkv][row blocks][groups][rows]
   float* row_lse;         // [total_q][nh], base 2
-  int runs;               // workgroups of the stream; 0: one workgroup per segment
+  int target;             // decode: slices to aim at, 4 a CU; 0: segments stay whole
   int rows;               // rows of a segment at most (<= 16 NB)
   int row_blocks;         // row blocks of a sequence at most
-  int min_units;          // units of a run at least
   int groups;             // 16-token groups a table addresses
   int slices;             // prefill: workgroups that share a row tile's tokens
 };

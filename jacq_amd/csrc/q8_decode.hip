@@ -20,7 +20,7 @@
 namespace jacq {
 namespace q8 {
 
-constexpr int kWaves = 4;         // wavefronts of a workgroup: they share a run, unit by unit
+constexpr int kWaves = 4;         // wavefronts of a workgroup: they share a slice, unit by unit
 constexpr float kSlack = 8.0f;    // the running maximum moves only by more than this (base 2)
 constexpr float kNegInf = -__builtin_inff();
 
@@ -331,63 +331,113 @@ __device__ inline void finish_row(const Geo& g, const AttendArgs& a, const Segme
   }
 }
 
-// The stream: all segments' units one after another, sequence by sequence, cut into `runs` equal
-// runs of at least min_units.  Segment x of the stream starts at `first`.
-struct Stream {
-  int64_t total;
-  int runs;
-  __device__ int64_t begin(int r) const { return total * r / runs; }
-  __device__ int run_of(int64_t unit) const {  // the run that holds it
-    int r = (int)(((unit + 1) * runs - 1) / total);
-    while (r + 1 < runs && begin(r + 1) <= unit) ++r;
-    while (r > 0 && begin(r) > unit) --r;
-    return r;
+// Inclusive prefix over the 64 lanes, by DPP: shifts within rows of 16 lanes, then the last lanes of
+// rows (0 is the identity of both operations on what is summed here).
+template <class Op>
+__device__ inline int wave_prefix(int x, Op op) {
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr:1
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return x;
+}
+struct Sum {
+  __device__ int operator()(int a, int b) const { return a + b; }
+};
+struct SumF {  // of fp32 bits
+  __device__ int operator()(int a, int b) const {
+    return __float_as_int(__int_as_float(a) + __int_as_float(b));
   }
 };
+struct Max {  // of numbers that are not negative
+  __device__ int operator()(int a, int b) const { return a > b ? a : b; }
+};
+__device__ inline int lane63(int x) { return __builtin_amdgcn_readlane(x, 63); }
 
 template <int ROWS>
 __device__ inline void sequence_span(const Geo& g, const AttendArgs& a, int b, int* q0, int* m,
-                                     Span* span, int64_t* units) {
+                                     Span* span, int* blocks) {
   queries_of(a, b, q0, m);
   const int n = clamp_len(g, a.lens[b]);
   *span = Span(g, n, n - *m, a.window, a.sinks);
-  const int blocks = (*m * g.gqa + ROWS - 1) / ROWS;
-  *units = (int64_t)span->units * blocks * g.nkv;
+  *blocks = (*m * g.gqa + ROWS - 1) / ROWS;
 }
 
-// Total units of the batch (over the lanes of one wavefront), and the sequence that holds `unit`
-// with the units before it; unit < 0 only totals.
+// How the call's segments are cut: into slices of about `size` units each, at most a.target of
+// them more than there are segments.  A sequence's slices are numbered from `before` on, kv head
+// by kv head fastest, then row block, then slice.
+struct Slices {
+  int size;
+  int b;
+  int before;
+};
+
+__device__ inline int slices_of(const Span& s, int size) { return (s.units + size - 1) / size; }
+
+// Units of a slice, from the call's units, its segments and the longest one's units.
+//  - Uncut, if that takes no longer: a workgroup alone on a CU needs about 0.4 us a unit (HD 128),
+//    the memory 0.8 us a unit and CU, a cut call about 6 us more; and where segments outnumber CUs
+//    only if they are about equally long.  40/8 heads of 128, uncut against cut (us): 64 sequences
+//    of 2048 tokens 47 against 52, of 4096 99 against 107; 16 of 4096 37 against 32; 64 of 1024 to
+//    16384 254 against 228; one of 4096 32 against 14.
+//  - Else about 4 slices a CU, of 4 to 16 units where there is less work.
+__device__ inline int slice_units(const AttendArgs& a, float all, float segments, int longest) {
+  const float cus = 0.25f * (float)a.target;
+  if ((float)longest <= 1.4f * all / cus + 16.0f &&
+      (segments <= cus || all >= 0.75f * segments * (float)longest))
+    return longest;
+  const int fair = (int)(all / cus) + 1;  // one slice a CU
+  const int few = fair < 4 ? 4 : fair > 16 ? 16 : fair;
+  const int many = (int)(all / (float)a.target) + 1;
+  return many > few ? many : few;
+}
+
+// The cut, and the sequence that has slice `want` (b >= batch: none), or, with want < 0, the place
+// of sequence `b`.  Over the lanes of each wavefront alike.
 template <int ROWS>
-__device__ inline int64_t scan(const Geo& g, const AttendArgs& a, int lane, int64_t unit, int* seq,
-                               int64_t* before) {
-  int64_t sum = 0;
+__device__ inline Slices cut(const Geo& g, const AttendArgs& a, int lane, int want, int b) {
+  // the sums are fp32: they choose the size, alike in every wavefront, and no more
+  float total = 0.0f, segments = 0.0f;
+  int q0, m, blocks = 0, longest = 1;
+  Span sp;
   for (int base = 0; base < a.batch; base += 64) {
-    int64_t u = 0;
+    float u = 0.0f, n = 0.0f;
+    int most = 0;
     if (base + lane < a.batch) {
-      int q0, m;
-      Span sp;
-      sequence_span<ROWS>(g, a, base + lane, &q0, &m, &sp, &u);
+      sequence_span<ROWS>(g, a, base + lane, &q0, &m, &sp, &blocks);
+      n = (float)(blocks * g.nkv);
+      u = (float)sp.units * n;
+      most = blocks ? sp.units : 0;
     }
-    int64_t inc = u;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t x = __shfl_up(inc, d);
-      if (lane >= d) inc += x;
-    }
-    const uint64_t past = __ballot(sum + inc > unit && u > 0);
-    if (unit >= 0 && past) {
-      const int l = __builtin_ctzll(past);
-      *seq = base + l;
-      *before = sum + __shfl(inc - u, l);
-      return sum;  // not the total: the caller has it
-    }
-    sum += __shfl(inc, 63);
+    total += __int_as_float(lane63(wave_prefix(__float_as_int(u), SumF())));
+    segments += __int_as_float(lane63(wave_prefix(__float_as_int(n), SumF())));
+    most = lane63(wave_prefix(most, Max()));
+    longest = most > longest ? most : longest;
   }
-  return sum;
+  const int size = uniform(slice_units(a, total, segments, longest));
+  int sum = 0;
+  for (int base = 0; base < a.batch; base += 64) {
+    int n = 0;
+    if (base + lane < a.batch) {
+      if (a.batch > 64) sequence_span<ROWS>(g, a, base + lane, &q0, &m, &sp, &blocks);
+      n = slices_of(sp, size) * blocks * g.nkv;
+    }
+    const int inc = wave_prefix(n, Sum());
+    if (want < 0) {
+      if (b < base + 64) return {size, b, sum + __builtin_amdgcn_readlane(inc - n, uniform(b - base))};
+    } else if (const uint64_t past = __ballot(sum + inc > want && n > 0)) {
+      const int l = __builtin_ctzll(past);
+      return {size, base + l, sum + __builtin_amdgcn_readlane(inc - n, l)};
+    }
+    sum += lane63(inc);
+  }
+  return {size, a.batch, 0};
 }
 
-// Workgroups of kWaves wavefronts.  runs > 0: run blockIdx.x of the stream; else the segment
-// blockIdx.x = (sequence, kv head, row block) whole.
+// A workgroup of kWaves wavefronts has a slice of a segment.  target > 0: slice blockIdx.x of the
+// cut; else the segment blockIdx.x = (sequence, row block, kv head) whole.
 template <int HD, bool E4M3, int NB>
 __global__ __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) void q8_decode_kernel(Geo g,
                                                                                  AttendArgs a) {
@@ -397,192 +447,161 @@ __global__ __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) void q8_decode_kernel
   __shared__ float ml[kWaves][ROWS][2];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   Wave<HD, E4M3, NB> w(g, a, lane);
-
-  Stream st;
-  int64_t at, end;  // units left of this workgroup's run
   Segment s;
-  int64_t seg0;     // the sequence's first unit
-  int run = blockIdx.x;
-  if (a.runs) {
-    st.total = scan<ROWS>(g, a, lane, -1, nullptr, nullptr);
-    int64_t most = (st.total + a.min_units - 1) / a.min_units;
-    st.runs = (int)(most < a.runs ? most : a.runs);
-    if (run >= st.runs) return;
-    at = st.begin(run);
-    end = st.begin(run + 1);
-    scan<ROWS>(g, a, lane, at, &s.b, &seg0);
-    s.b = uniform(s.b);
+  int u0 = 0, u1, blocks;
+  bool whole = true;
+  if (a.target) {
+    const Slices c = cut<ROWS>(g, a, lane, blockIdx.x, 0);
+    if (c.b >= a.batch) return;
+    s.b = c.b;
+    sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
+    int x = blockIdx.x - c.before;
+    s.h = uniform(x % g.nkv);
+    x /= g.nkv;
+    s.rb = uniform(x % blocks);
+    const int z = uniform(x / blocks), n = uniform(slices_of(s.span, c.size));
+    u0 = uniform((int)((int64_t)s.span.units * z / n));
+    u1 = uniform((int)((int64_t)s.span.units * (z + 1) / n));
+    whole = n == 1;
   } else {
     s.b = blockIdx.x / (g.nkv * a.row_blocks);
-    seg0 = at = 0;
-    end = 1;
+    s.h = blockIdx.x % g.nkv;
+    s.rb = blockIdx.x / g.nkv % a.row_blocks;
+    sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
+    if (s.rb >= blocks) return;
+    u1 = s.span.units;
   }
+  const int left = s.m * g.gqa - s.rb * ROWS;
+  s.nrows = left < ROWS ? left : ROWS;
+  w.start(s);
+  w.units(s, u0 + wave, u1);
 
-  while (at < end) {
-    int64_t units;
-    sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &units);
-    const int blocks = (s.m * g.gqa + ROWS - 1) / ROWS;
-    int u0, u1;
-    bool whole;
-    if (a.runs) {
-      if (blocks == 0 || at >= seg0 + units) {  // on to the next sequence
-        seg0 += units;
-        ++s.b;
-        continue;
-      }
-      const int x = (int)((at - seg0) / s.span.units);
-      s.h = uniform(x / blocks);
-      s.rb = uniform(x % blocks);
-      const int64_t first = seg0 + (int64_t)x * s.span.units;
-      u0 = uniform((int)(at - first));
-      const int64_t e = end - first;
-      u1 = uniform(e < s.span.units ? (int)e : s.span.units);
-      whole = u0 == 0 && u1 == s.span.units;
-      at = first + u1;
+  // Fold the wavefronts' parts: each leaves (m, l, acc) as they are, the reader scales.
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float l = w.l[nb];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (lane < 16) {
+      ml[wave][nb * 16 + lane][0] = w.m[nb];
+      ml[wave][nb * 16 + lane][1] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d)
+      *(f4*)&red[wave][nb * 16 + w.n16][d * 16 + w.kq * 4] = w.acc[nb][d];
+  }
+  __syncthreads();
+  constexpr int PER = HD / 16;  // channels of a thread
+  for (int i = threadIdx.x; i < s.nrows * 16; i += 64 * kWaves) {
+    const int row = i / 16, ch = i % 16 * PER;
+    float mm = kNegInf, l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, ml[v][row][0]);
+    float x[PER];
+#pragma unroll
+    for (int c = 0; c < PER; ++c) x[c] = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      // a part without a maximum saw nothing, or only NaN: l tells
+      const float mv = ml[v][row][0];
+      const float f = mv == kNegInf ? 1.0f : exp2_(mv - mm);
+      l += ml[v][row][1] * f;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) x[c] += red[v][row][ch + c] * f;
+    }
+    if (whole) {
+      finish_row(g, a, s, row, HD, ch, x, PER, l, mm);
     } else {
-      const int x = blockIdx.x % (g.nkv * a.row_blocks);
-      s.h = x / a.row_blocks;
-      s.rb = x % a.row_blocks;
-      if (s.rb >= blocks) return;
-      u0 = 0;
-      u1 = s.span.units;
-      whole = true;
-      at = end;
-    }
-    const int left = s.m * g.gqa - s.rb * ROWS;
-    s.nrows = left < ROWS ? left : ROWS;
-    w.start(s);
-    w.units(s, u0 + wave, u1);
-
-    // Fold the wavefronts' pieces: each leaves (m, l, acc) as they are, the reader scales.
+      const int64_t at = (int64_t)blockIdx.x * a.rows + row;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float l = w.l[nb];
-      l += __shfl_xor(l, 16);
-      l += __shfl_xor(l, 32);
-      if (lane < 16) {
-        ml[wave][nb * 16 + lane][0] = w.m[nb];
-        ml[wave][nb * 16 + lane][1] = l;
-      }
-#pragma unroll
-      for (int d = 0; d < HD / 16; ++d)
-        *(f4*)&red[wave][nb * 16 + w.n16][d * 16 + w.kq * 4] = w.acc[nb][d];
-    }
-    __syncthreads();
-    constexpr int PER = HD / 16;  // channels of a thread
-    for (int i = threadIdx.x; i < s.nrows * 16; i += 64 * kWaves) {
-      const int row = i / 16, ch = i % 16 * PER;
-      float mm = kNegInf, l = 0.0f;
-#pragma unroll
-      for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, ml[v][row][0]);
-      float x[PER];
-#pragma unroll
-      for (int c = 0; c < PER; ++c) x[c] = 0.0f;
-#pragma unroll
-      for (int v = 0; v < kWaves; ++v) {
-        // a piece without a maximum saw nothing, or only NaN: l tells
-        const float mv = ml[v][row][0];
-        const float f = mv == kNegInf ? 1.0f : exp2_(mv - mm);
-        l += ml[v][row][1] * f;
-#pragma unroll
-        for (int c = 0; c < PER; ++c) x[c] += red[v][row][ch + c] * f;
-      }
-      if (whole) {
-        finish_row(g, a, s, row, HD, ch, x, PER, l, mm);
-      } else {
-        const int64_t slot = (int64_t)2 * run + (u0 > 0 ? 0 : 1);
-        float* dst = a.part_acc + (slot * a.rows + row) * HD + ch;
-#pragma unroll
-        for (int c = 0; c < PER; c += 4) *(f4*)(dst + c) = *(f4*)(x + c);
-        if (ch == 0) {
-          a.part_ml[(slot * a.rows + row) * 2] = mm;
-          a.part_ml[(slot * a.rows + row) * 2 + 1] = l;
-        }
+      for (int c = 0; c < PER; c += 4) *(f4*)(a.part_acc + at * HD + ch + c) = *(f4*)(x + c);
+      if (ch == 0) {
+        a.part_ml[at * 2] = mm;
+        a.part_ml[at * 2 + 1] = l;
       }
     }
-    __syncthreads();  // the fold's LDS, before the next piece's
   }
 }
 
-// Joins the pieces of the segments that runs cut, in the order of the runs.  blockIdx.x: segment,
-// blockIdx.y: row.
-template <int HD, int NB>
+// Joins a segment's slices, in their order.  blockIdx.x: segment.  MANY: of the row blockIdx.y, the
+// threads side by side share the slices; else they share the rows.
+template <int HD, int NB, bool MANY>
 __global__ __launch_bounds__(256) void q8_join_kernel(Geo g, AttendArgs a) {
   constexpr int ROWS = 16 * NB;
-  constexpr int TC = HD / 4;      // threads of a piece's row
-  constexpr int PG = 256 / TC;    // pieces at a time
-  __shared__ __align__(16) float red[PG][HD];
-  __shared__ float ml[PG][2];
-  const int lane = threadIdx.x & 63, row = blockIdx.y;
+  constexpr int TC = HD / 4;      // threads of a row
+  constexpr int PG = 256 / TC;    // rows, or slices, at a time
+  const int lane = threadIdx.x & 63;
   Segment s;
+  int blocks;
   s.b = blockIdx.x / (g.nkv * a.row_blocks);
-  const int x = blockIdx.x % (g.nkv * a.row_blocks);
-  int64_t units, before = 0, total = 0;
-  // the units of the sequences before b, and of all
-  for (int base = 0; base < a.batch; base += 64) {
-    int64_t u = 0;
-    if (base + lane < a.batch) {
-      int q0, m;
-      Span sp;
-      sequence_span<ROWS>(g, a, base + lane, &q0, &m, &sp, &u);
-    }
-    int64_t v = base + lane < s.b ? u : 0;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-      u += __shfl_xor(u, d);
-      v += __shfl_xor(v, d);
-    }
-    total += u;
-    before += v;
-  }
-  sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &units);
-  const int blocks = (s.m * g.gqa + ROWS - 1) / ROWS;
-  // row blocks of the grid that this sequence lacks have nothing to do
-  s.h = x / a.row_blocks;
-  s.rb = x % a.row_blocks;
+  s.h = blockIdx.x % g.nkv;
+  s.rb = blockIdx.x / g.nkv % a.row_blocks;
+  sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
   if (s.rb >= blocks) return;
   const int left = s.m * g.gqa - s.rb * ROWS;
   s.nrows = left < ROWS ? left : ROWS;
-  if (row >= s.nrows) return;
-  Stream st;
-  st.total = total;
-  const int64_t most = (total + a.min_units - 1) / a.min_units;
-  st.runs = (int)(most < a.runs ? most : a.runs);
-  const int64_t first = before + (int64_t)(s.h * blocks + s.rb) * s.span.units;
-  const int r0 = st.run_of(first), r1 = st.run_of(first + s.span.units - 1);
-  if (r0 == r1) return;  // one run had all of it
-  const int grp = threadIdx.x / TC, c = threadIdx.x % TC * 4;
-  float mm = kNegInf, l = 0.0f;
-  f4 acc = {0, 0, 0, 0};
-  for (int r = r0 + grp; r <= r1; r += PG) {
-    const int64_t slot = (int64_t)2 * r + (st.begin(r) > first ? 0 : 1);
-    const float pm = a.part_ml[(slot * a.rows + row) * 2];
-    const float pl = a.part_ml[(slot * a.rows + row) * 2 + 1];
-    const f4 pa = *(const f4*)(a.part_acc + (slot * a.rows + row) * HD + c);
+  if (MANY && (int)blockIdx.y >= s.nrows) return;
+  const Slices c = cut<ROWS>(g, a, lane, -1, s.b);
+  const int n = uniform(slices_of(s.span, c.size));
+  if (n == 1) return;
+  const int64_t first = c.before + s.rb * g.nkv + s.h;
+  const int step = blocks * g.nkv;
+  const int grp = threadIdx.x / TC, ch = threadIdx.x % TC * 4;
+  auto add = [&](float pm, float pl, f4 pa, float& mm, float& l, f4& acc) {
     const float to = fmaxf(mm, pm);
     const float f0 = mm == kNegInf ? 1.0f : exp2_(mm - to);
     const float f1 = pm == kNegInf ? 1.0f : exp2_(pm - to);
     acc = acc * f0 + pa * f1;
     l = l * f0 + pl * f1;
     mm = to;
+  };
+  // slices z0, z0 + by, ... of a row, 4 in flight
+  auto sum = [&](int row, int z0, int by, float& mm, float& l, f4& acc) {
+    for (int z = z0; z < n; z += 4 * by) {
+      float pm[4], pl[4];
+      f4 pa[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int zz = z + i * by < n ? z + i * by : z;
+        const int64_t at = (first + (int64_t)zz * step) * a.rows + row;
+        pm[i] = a.part_ml[at * 2];
+        pl[i] = a.part_ml[at * 2 + 1];
+        pa[i] = *(const f4*)(a.part_acc + at * HD + ch);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (z + i * by < n) add(pm[i], pl[i], pa[i], mm, l, acc);
+    }
+  };
+  if constexpr (!MANY) {
+    for (int row = grp; row < s.nrows; row += PG) {
+      float mm = kNegInf, l = 0.0f;
+      f4 acc = {0, 0, 0, 0};
+      sum(row, 0, 1, mm, l, acc);
+      float o[4] = {acc.x, acc.y, acc.z, acc.w};
+      finish_row(g, a, s, row, HD, ch, o, 4, l, mm);
+    }
+  } else {
+    __shared__ __align__(16) float red[PG][HD];
+    __shared__ float ml[PG][2];
+    const int row = blockIdx.y;
+    float mm = kNegInf, l = 0.0f;
+    f4 acc = {0, 0, 0, 0};
+    sum(row, grp, PG, mm, l, acc);
+    *(f4*)&red[grp][ch] = acc;
+    if (ch == 0) {
+      ml[grp][0] = mm;
+      ml[grp][1] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= TC) return;
+    mm = kNegInf;
+    l = 0.0f;
+    acc = f4{0, 0, 0, 0};
+    for (int i = 0; i < PG; ++i) add(ml[i][0], ml[i][1], *(const f4*)&red[i][ch], mm, l, acc);
+    float o[4] = {acc.x, acc.y, acc.z, acc.w};
+    finish_row(g, a, s, row, HD, ch, o, 4, l, mm);
   }
-  *(f4*)&red[grp][c] = acc;
-  if (c == 0) {
-    ml[grp][0] = mm;
-    ml[grp][1] = l;
-  }
-  __syncthreads();
-  if (threadIdx.x >= TC) return;
-  mm = kNegInf;
-  for (int i = 0; i < PG; ++i) mm = fmaxf(mm, ml[i][0]);
-  l = 0.0f;
-  float o[4] = {0, 0, 0, 0};
-  for (int i = 0; i < PG; ++i) {
-    const float f = ml[i][0] == kNegInf ? 1.0f : exp2_(ml[i][0] - mm);
-    l += ml[i][1] * f;
-    for (int k = 0; k < 4; ++k) o[k] += red[i][c + k] * f;
-  }
-  finish_row(g, a, s, row, HD, c, o, 4, l, mm);
 }
 
 // Adds up the weight of every block: a thread per 16 tokens, over kv heads, row blocks and rows in
@@ -591,11 +610,9 @@ template <int NB>
 __global__ __launch_bounds__(256) void q8_weights_kernel(Geo g, AttendArgs a) {
   constexpr int ROWS = 16 * NB;
   const int b = blockIdx.y, grp = blockIdx.x * 256 + threadIdx.x;
-  int q0, m;
+  int q0, m, blocks;
   Span sp;
-  int64_t units;
-  sequence_span<ROWS>(g, a, b, &q0, &m, &sp, &units);
-  const int blocks = (m * g.gqa + ROWS - 1) / ROWS;
+  sequence_span<ROWS>(g, a, b, &q0, &m, &sp, &blocks);
   const int t0 = grp * 16, tile = t0 / kTile;
   // groups that no unit covers were not written by this call
   const bool there = t0 < sp.n && m > 0 && (t0 >= sp.nq || tile < sp.ns || tile >= sp.w0);
@@ -625,10 +642,16 @@ __global__ __launch_bounds__(256) void q8_weights_kernel(Geo g, AttendArgs a) {
 template <int HD, bool E4M3, int NB>
 static void decode_kernels(const Geo& g, const AttendArgs& a, hipStream_t s) {
   const int segments = a.batch * g.nkv * a.row_blocks;
-  const unsigned blocks = a.runs ? a.runs : segments;
+  const unsigned blocks = a.target ? a.target + segments : segments;
   hipLaunchKernelGGL((q8_decode_kernel<HD, E4M3, NB>), dim3(blocks), dim3(64 * kWaves), 0, s, g, a);
-  if (a.runs)
-    hipLaunchKernelGGL((q8_join_kernel<HD, NB>), dim3(segments, a.rows), dim3(256), 0, s, g, a);
+  if (a.target) {
+    // from about 8 slices a segment on, a workgroup per row: its threads share the slices
+    if (a.target >= 8 * segments)
+      hipLaunchKernelGGL((q8_join_kernel<HD, NB, true>), dim3(segments, a.rows), dim3(256), 0, s, g,
+                         a);
+    else
+      hipLaunchKernelGGL((q8_join_kernel<HD, NB, false>), dim3(segments), dim3(256), 0, s, g, a);
+  }
   if (a.weights)
     hipLaunchKernelGGL((q8_weights_kernel<NB>), dim3((a.groups + 255) / 256, a.batch), dim3(256), 0,
                        s, g, a);

@@ -20,12 +20,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
 
 from jacq_amd import kivi as _kivi
-from jacq_amd.kivi import KiviLaunchError, _check, _raw_stream, check_shape
+from jacq_amd.kivi import KiviLaunchError, _check, check_shape
 
 CODES = {"int8": 0, "e4m3": 1}
 DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
@@ -41,6 +42,10 @@ class _Geometry(ctypes.Structure):
 
 class _Pool(ctypes.Structure):
     _fields_ = [(n, _vp) for n in ("k_code", "k_scale", "v_code", "v_scale", "k_tail", "v_tail")]
+
+
+# _AttendArgs packed at once: setting its fields one by one takes as long as a launch
+_ATTEND = struct.Struct("@7Pq7i2f4x")
 
 
 class _AttendArgs(ctypes.Structure):
@@ -72,7 +77,7 @@ def lib() -> ctypes.CDLL:
     L.jacq_q8_append.restype = ctypes.c_int
     L.jacq_q8_attend_workspace_size.argtypes = [geo, _i32, _i32, _i32, _i32]
     L.jacq_q8_attend_workspace_size.restype = ctypes.c_size_t
-    L.jacq_q8_attend.argtypes = [geo, pool, ctypes.POINTER(_AttendArgs), _vp, ctypes.c_size_t, _vp]
+    L.jacq_q8_attend.argtypes = [geo, pool, _vp, _vp, ctypes.c_size_t, _vp]  # args: packed bytes
     L.jacq_q8_attend.restype = ctypes.c_int
     L.jacq_q8_read.argtypes = [geo, pool, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp]
     L.jacq_q8_read.restype = ctypes.c_int
@@ -84,11 +89,6 @@ def lib() -> ctypes.CDLL:
 
 def last_error() -> str:
     return lib().jacq_q8_last_error().decode()
-
-
-def _done(rc: int) -> None:
-    if rc != 0:
-        raise KiviLaunchError(last_error())
 
 
 def _ptr(t: torch.Tensor | None) -> int:
@@ -195,6 +195,10 @@ class PagedQ8Cache:
         self._index = self.device.index if self.device.type == "cuda" else -1
         self._record = _Pool(*(t[n].data_ptr() for n in POOL))
         self._pool = ctypes.byref(self._record)
+        # what a call's tensors are compared with, and the workspace sizes asked for so far
+        self._q_row, self._kv_row = (g.num_heads, g.head_dim), (g.num_kv_heads, g.head_dim)
+        self._lens_shape, self._table_shape = (batch,), (batch, g.max_pages_per_seq)
+        self._sizes = {}
 
     def sequence_view(self, b: int) -> "PagedQ8Cache":
         """A one-sequence cache sharing this cache's pool and sequence b's tail."""
@@ -241,13 +245,29 @@ class PagedQ8Cache:
         check_shape(w, (self.batch, self.geo.max_pages_per_seq), name)
         _check(w.dtype == torch.float32 and w.is_contiguous(), name, " must be contiguous fp32")
 
+    # The checks of a call in one expression each: the named ones take the host longer than a
+    # small call takes the GPU.  A call that fails one goes to the named checks, which say why.
+
+    def _fits(self, lens: torch.Tensor, tables: torch.Tensor) -> bool:
+        return (lens.shape == self._lens_shape and lens.dtype is torch.int32
+                and lens.is_contiguous() and tables.shape == self._table_shape
+                and tables.dtype is torch.int32 and tables.is_contiguous()
+                and lens.get_device() == self._index == tables.get_device())
+
+    def _fits_rows(self, t: torch.Tensor, row: tuple) -> bool:
+        return (t.dim() == 3 and t.shape[1:] == row and t.is_contiguous()
+                and (t.dtype is torch.float16 or t.dtype is torch.bfloat16)
+                and t.get_device() == self._index)
+
     def _call(self, fn, *args) -> None:
         """The call with the cache's device current, on its current stream."""
-        if torch.cuda.current_device() == self._index:
-            _done(fn(*args, _raw_stream(self.k_code)))
+        if torch._C._cuda_getDevice() == self._index:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._index))
         else:
             with torch.cuda.device(self._index):
-                _done(fn(*args, _raw_stream(self.k_code)))
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._index))
+        if rc != 0:
+            raise KiviLaunchError(last_error())
 
     # ---- calls ----
 
@@ -261,24 +281,30 @@ class PagedQ8Cache:
         the table's capacity are dropped.  The first block of a sequence's new tokens takes
         its tail in, so appending the same tokens twice is not the same as once."""
         nkv = self.geo.num_kv_heads
-        self._rows(new_k, nkv, "NEW_K")
-        self._rows(new_v, nkv, "NEW_V")
-        total = new_k.shape[0]
-        _check(new_v.shape[0] == total and new_v.dtype == new_k.dtype,
-               "NEW_V must have NEW_K's tokens and type")
-        self._tables(start_lens, block_tables, "START_LENS")
+        total = new_k.shape[0] if new_k.dim() else 0
+        fits = (self._index >= 0 and self._fits_rows(new_k, self._kv_row)
+                and self._fits_rows(new_v, self._kv_row) and new_v.shape[0] == total
+                and new_v.dtype is new_k.dtype and self._fits(start_lens, block_tables))
+        if not fits:
+            self._rows(new_k, nkv, "NEW_K")
+            self._rows(new_v, nkv, "NEW_V")
+            _check(new_v.shape[0] == total and new_v.dtype == new_k.dtype,
+                   "NEW_V must have NEW_K's tokens and type")
+            self._tables(start_lens, block_tables, "START_LENS")
         if cu_new is None:
             _check(total == self.batch, "without CU_NEW there is one new token per sequence: ",
                    self.batch, ", got ", total)
-            _check(max_new in (None, 1), "MAX_NEW is for CU_NEW")
+            _check(max_new is None or max_new == 1, "MAX_NEW is for CU_NEW")
             max_new = 1
         else:
             self._ints(cu_new, self.batch + 1, "CU_NEW")
             max_new = total if max_new is None else max_new
             _check(max_new >= 0, "MAX_NEW must not be negative")
-        self._here(("NEW_K", new_k), ("NEW_V", new_v), ("START_LENS", start_lens),
-                   ("BLOCK_TABLES", block_tables), ("CU_NEW", cu_new))
-        self._call(lib().jacq_q8_append, self.geo.ref, self._pool, new_k.data_ptr(),
+            fits = fits and cu_new.get_device() == self._index
+        if not fits:
+            self._here(("NEW_K", new_k), ("NEW_V", new_v), ("START_LENS", start_lens),
+                       ("BLOCK_TABLES", block_tables), ("CU_NEW", cu_new))
+        self._call(_lib.jacq_q8_append, self.geo.ref, self._pool, new_k.data_ptr(),
                    new_v.data_ptr(), DTYPES[new_k.dtype], self._stride(new_k, nkv),
                    self._stride(new_v, nkv), _ptr(cu_new), start_lens.data_ptr(),
                    block_tables.data_ptr(), total, max_new, self.batch)
@@ -286,43 +312,59 @@ class PagedQ8Cache:
     def _attend(self, q, cu_q, max_q, seq_lens, block_tables, window, sinks, scale, weights, decay,
                 out, lse, workspace) -> torch.Tensor:
         g = self.geo
-        nh = g.num_heads
-        self._rows(q, nh, "Q")
+        nh, hd = self._q_row
+        fits = (self._index >= 0 and self._fits_rows(q, self._q_row)
+                and self._fits(seq_lens, block_tables))
+        if not fits:
+            self._rows(q, nh, "Q")
+            self._tables(seq_lens, block_tables)
         total = q.shape[0]
-        self._tables(seq_lens, block_tables)
-        _check(window is None or window >= 1, "WINDOW must be positive, or None")
-        _check(0 <= sinks, "SINKS must not be negative")
-        if out is None:
-            out = torch.empty((total, nh, g.head_dim), dtype=q.dtype, device=q.device)
+        if window is None:
+            window = 0
         else:
-            check_shape(out, (total, nh, g.head_dim), "O")
-            _check(out.dtype in (q.dtype, torch.float32) and out.is_contiguous(),
-                   "O must be contiguous, of Q's type or fp32")
-        if lse is not None:
-            check_shape(lse, (total, nh), "LSE")
-            _check(lse.dtype == torch.float32 and lse.is_contiguous(), "LSE must be contiguous fp32")
+            _check(window >= 1, "WINDOW must be positive, or None")
+        _check(sinks >= 0, "SINKS must not be negative")
+        scale = hd ** -0.5 if scale is None else float(scale)
+        _check(0.0 < scale < math.inf, "SCALE must be positive and finite")
+        if cu_q is not None:
+            self._ints(cu_q, self.batch + 1, "CU_Q")
         if weights is not None:
             self._weights(weights)
             _check(max_q <= MAX_WEIGHTED_QUERIES, "WEIGHTS take at most ", MAX_WEIGHTED_QUERIES,
                    " queries per sequence, got ", max_q)
-            _check(decay >= 0 and math.isfinite(decay), "DECAY must be finite and not negative")
-        scale = g.head_dim ** -0.5 if scale is None else float(scale)
-        _check(math.isfinite(scale), "SCALE must be finite")
-        self._here(("Q", q), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables), ("CU_Q", cu_q),
-                   ("O", out), ("LSE", lse), ("WEIGHTS", weights), ("workspace", workspace))
+            _check(0.0 <= decay < math.inf, "DECAY must be finite and not negative")
+        if out is None:
+            out = torch.empty((total, nh, hd), dtype=q.dtype, device=q.device)
+        else:
+            check_shape(out, (total, nh, hd), "O")
+            _check(out.dtype in (q.dtype, torch.float32) and out.is_contiguous(),
+                   "O must be contiguous, of Q's type or fp32")
+            fits = fits and out.get_device() == self._index
+        if lse is not None:
+            check_shape(lse, (total, nh), "LSE")
+            _check(lse.dtype == torch.float32 and lse.is_contiguous(), "LSE must be contiguous fp32")
+        if not (fits and cu_q is None and lse is None and weights is None and workspace is None):
+            self._here(("Q", q), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
+                       ("CU_Q", cu_q), ("O", out), ("LSE", lse), ("WEIGHTS", weights),
+                       ("workspace", workspace))
         if workspace is None:
-            size = lib().jacq_q8_attend_workspace_size(g.ref, self.batch, total, max_q,
-                                                       weights is not None)
+            key = (total, max_q, weights is not None)
+            size = self._sizes.get(key)
+            if size is None:
+                if len(self._sizes) > 4096:
+                    self._sizes.clear()
+                size = self._sizes[key] = _lib.jacq_q8_attend_workspace_size(
+                    g.ref, self.batch, total, max_q, weights is not None)
             if size:
                 workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         else:
             _check(workspace.is_contiguous(), "workspace must be contiguous")
-        args = _AttendArgs(q.data_ptr(), _ptr(cu_q), seq_lens.data_ptr(), block_tables.data_ptr(),
-                           out.data_ptr(), _ptr(lse), _ptr(weights), self._stride(q, nh),
-                           DTYPES[q.dtype], DTYPES[out.dtype], self.batch, total, max_q,
-                           min(window or 0, 1 << 30), min(sinks, 1 << 30), scale, decay)
-        self._call(lib().jacq_q8_attend, g.ref, self._pool, ctypes.byref(args), _ptr(workspace),
-                   0 if workspace is None else workspace.numel() * workspace.element_size())
+            size = workspace.numel() * workspace.element_size()
+        args = _ATTEND.pack(q.data_ptr(), _ptr(cu_q), seq_lens.data_ptr(), block_tables.data_ptr(),
+                            out.data_ptr(), _ptr(lse), _ptr(weights), self._stride(q, nh),
+                            DTYPES[q.dtype], DTYPES[out.dtype], self.batch, total, max_q,
+                            min(window, 1 << 30), min(sinks, 1 << 30), scale, decay)
+        self._call(_lib.jacq_q8_attend, g.ref, self._pool, args, _ptr(workspace), size)
         return out
 
     def decode(self, q: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.Tensor,
@@ -355,7 +397,7 @@ class PagedQ8Cache:
         max_q.  Rows outside every sequence are left as they are (undefined in a fresh
         output).  weights, as in ``decode``, take at most 64 queries per sequence: the last
         ones of a prompt, in a call of their own."""
-        self._ints(cu_q, self.batch + 1, "CU_Q")
+        _check(cu_q is not None, "CU_Q must be given")
         _check(max_q >= 0, "MAX_Q must not be negative")
         return self._attend(q, cu_q, int(max_q), seq_lens, block_tables, window, sinks, scale,
                             weights, decay, out, lse, workspace)
@@ -366,13 +408,17 @@ class PagedQ8Cache:
         sequence after another: K, V [total, NKV, HD].  total is their number: tokens past it
         are dropped, rows that none fills undefined."""
         g = self.geo
-        self._tables(ends, block_tables, "ENDS")
-        self._ints(starts, self.batch, "STARTS")
+        fits = (self._index >= 0 and self._fits(ends, block_tables)
+                and self._fits(starts, block_tables))
+        if not fits:
+            self._tables(ends, block_tables, "ENDS")
+            self._ints(starts, self.batch, "STARTS")
         _check(dtype in DTYPES, "values are read as fp16, bf16 or fp32, not ", dtype)
         _check(total >= 0, "TOTAL must not be negative")
-        self._here(("STARTS", starts), ("ENDS", ends), ("BLOCK_TABLES", block_tables))
+        if not fits:
+            self._here(("STARTS", starts), ("ENDS", ends), ("BLOCK_TABLES", block_tables))
         k, v = torch.empty((2, total, g.num_kv_heads, g.head_dim), dtype=dtype, device=self.device)
-        self._call(lib().jacq_q8_read, g.ref, self._pool, starts.data_ptr(), ends.data_ptr(),
+        self._call(_lib.jacq_q8_read, g.ref, self._pool, starts.data_ptr(), ends.data_ptr(),
                    block_tables.data_ptr(), self.batch, total, k.data_ptr(), v.data_ptr(),
                    DTYPES[dtype])
         return k, v
@@ -387,20 +433,28 @@ class PagedQ8Cache:
         A table row's kept entries move to its front; the evicted ones follow, so the
         sequence's next blocks reuse their pages unless the program takes them; no page is
         moved or copied.  Lengths count the tokens that are left."""
-        self._tables(seq_lens, block_tables)
-        self._weights(weights)
+        fits = (self._index >= 0 and self._fits(seq_lens, block_tables)
+                and weights.shape == self._table_shape and weights.dtype is torch.float32
+                and weights.is_contiguous() and weights.get_device() == self._index)
+        if not fits:
+            self._tables(seq_lens, block_tables)
+            self._weights(weights)
         _check(sink_pages >= 0 and recent_pages >= 0 and sink_pages + recent_pages <= keep,
                "KEEP must be at least SINK_PAGES + RECENT_PAGES, neither negative")
         if out is None:
             out = (torch.empty_like(block_tables), torch.empty_like(seq_lens),
                    torch.empty_like(weights), torch.empty_like(seq_lens))
-        tables_out, lens_out, weights_out, evicted = out
-        self._tables(lens_out, tables_out)
-        self._weights(weights_out)
-        self._ints(evicted, self.batch, "EVICTED")
-        self._here(("WEIGHTS", weights), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
-                   *(("an output", t) for t in out))
-        self._call(lib().jacq_q8_evict, self.geo.ref, weights.data_ptr(), seq_lens.data_ptr(),
+            tables_out, lens_out, weights_out, evicted = out
+        else:
+            tables_out, lens_out, weights_out, evicted = out
+            self._tables(lens_out, tables_out, "the lengths given for output")
+            self._weights(weights_out, "the weights given for output")
+            self._ints(evicted, self.batch, "EVICTED")
+            fits = False
+        if not fits:
+            self._here(("WEIGHTS", weights), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
+                       *(("an output", t) for t in out))
+        self._call(_lib.jacq_q8_evict, self.geo.ref, weights.data_ptr(), seq_lens.data_ptr(),
                    block_tables.data_ptr(), self.batch, min(int(keep), (1 << 31) - 1),
                    int(sink_pages), int(recent_pages), tables_out.data_ptr(), lens_out.data_ptr(),
                    weights_out.data_ptr(), evicted.data_ptr())

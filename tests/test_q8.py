@@ -60,14 +60,14 @@ class Record:
         for k, v in kw.items():
             setattr(self.args, k, v)
         return q8.lib().jacq_q8_attend(self.geo.ref, ctypes.byref(pool or self.pool),
-                                       ctypes.byref(self.args), ws, ws_bytes, None)
+                                       bytes(self.args), ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("kw,text", [
     (dict(batch=-1), "batch"), (dict(batch=65536), "batch"), (dict(q_dtype=2), "fp16 or bf16"),
     (dict(o_dtype=1), "queries' type"), (dict(total_q=-1), "negative"),
     (dict(CU_Q=0), "one query"), (dict(window=-1), "negative"), (dict(sinks=-1), "negative"),
-    (dict(scale=float("nan")), "finite"), (dict(decay=-0.5), "finite"),
+    (dict(scale=float("nan")), "finite"), (dict(scale=-0.5), "positive"), (dict(decay=-0.5), "finite"),
     (dict(WEIGHTS=0x60000, max_q=65, total_q=200), "64 queries"), (dict(q_stride=500), "stride"),
     (dict(q_stride=516), "stride"), (dict(Q=0), "null"), (dict(O=0), "null"),
     (dict(SEQ_LENS=0), "null"), (dict(Q=0x10008), "16-byte"), (dict(LSE=0x60002), "4-byte")])
@@ -92,6 +92,11 @@ def test_pool_refusals():
         error(r.attend(pool=q8._Pool(*p)), EINVAL, "null")
         p[i] = 4096 * (i + 1) + (2 if i in (1, 3) else 8)
         error(r.attend(pool=q8._Pool(*p)), EINVAL, "aligned")
+
+
+def test_packed_arguments_are_the_record():
+    values = (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 0.5, 0.25)
+    assert q8._ATTEND.pack(*values) == bytes(q8._AttendArgs(*values))
 
 
 def test_nothing_to_do_is_no_error():
@@ -179,6 +184,7 @@ def test_python_refusals(cache):
     no("WINDOW", cache.decode, q, lens, tables, window=0)
     no("SINKS", cache.decode, q, lens, tables, sinks=-1)
     no("SCALE", cache.decode, q, lens, tables, scale=float("inf"))
+    no("SCALE", cache.decode, q, lens, tables, scale=0.0)
     no("DECAY", cache.decode, q, lens, tables, weights=w, decay=-1.0)
     no("WEIGHTS", cache.decode, q, lens, tables, weights=w.double())
     no("O must", cache.decode, q, lens, tables, out=q.to(torch.bfloat16))
