@@ -358,6 +358,8 @@ int jacq_q8_read(const jacq_q8_geometry* geo, const jacq_q8_pool* pool, const in
       return fail(JACQ_KIVI_EINVAL, "a tensor pointer is null");
     if (!aligned({K, V}, 16) || !aligned({STARTS, ENDS, BLOCK_TABLES}, 4))
       return fail(JACQ_KIVI_EINVAL, "K and V must be 16-byte aligned, tables 4-byte");
+    if ((int64_t)geo->num_kv_heads * (total / 16 + 2 * batch) > INT32_MAX)
+      return fail(JACQ_KIVI_EINVAL, "too many tokens in one read");
     return launched(jacq::q8::launch_read(make_geo(*geo), read_pool(*pool), STARTS, ENDS,
                                           BLOCK_TABLES, batch, total, K, V, dtype, stream),
                     "read");

@@ -112,6 +112,31 @@ __device__ inline h8 codes8(uint32_t w0, uint32_t w1) {
   return r;
 }
 
+// Inclusive prefix over the 64 lanes, by DPP: shifts within rows of 16 lanes, then the last lanes of
+// rows (0 is the identity of both operations on what is summed here).
+template <class Op>
+__device__ inline int wave_prefix(int x, Op op) {
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr:1
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return x;
+}
+struct Sum {
+  __device__ int operator()(int a, int b) const { return a + b; }
+};
+struct SumF {  // of fp32 bits
+  __device__ int operator()(int a, int b) const {
+    return __float_as_int(__int_as_float(a) + __int_as_float(b));
+  }
+};
+struct Max {  // of numbers that are not negative
+  __device__ int operator()(int a, int b) const { return a > b ? a : b; }
+};
+__device__ inline int lane63(int x) { return __builtin_amdgcn_readlane(x, 63); }
+
 __device__ inline int clamp_len(const Geo& g, int n) {
   const int cap = g.max_pages << g.page_log2;  // the host checked that this fits
   return n < 0 ? 0 : n > cap ? cap : n;

@@ -1,51 +1,60 @@
 // q8_writer.hip -- append to the 8-bit paged cache, and reading it back.
 //
-// A wavefront per (sequence, kv head, block that the new tokens touch); none
-// waits for another.  The wavefront of the first block also owns the tail: it
-// reads the rows that the block takes in before it writes the rows that
-// remain.  All rows of a block are in registers (lane = NI consecutive tokens
-// x 8 channels), so the block's largest magnitude is one pass and a shuffle,
-// a row of K codes leaves as it came, and the lane already holds NI
+// Append: a workgroup per (sequence, kv head, block that the new tokens touch);
+// none waits for another.  The workgroup of the first block also owns the tail:
+// it has read the rows that the block takes in before it writes the rows that
+// remain.  One half of its wavefronts has K, the other V, all rows in registers
+// (lane = NI consecutive tokens x 8 channels), so the largest magnitude is one
+// pass, a row of K codes leaves as it came, and the lane already holds NI
 // consecutive tokens of each channel for the transposed V.
 #include "q8_common.h"
 
 namespace jacq {
 namespace q8 {
 
-// 8 new or held values as fp16: bf16 is converted, magnitudes saturate at fp16's largest, NaN
-// stays.
-__device__ inline h8 as_half(u4 raw, bool bf16) {
-  h8 r;
+// 8 new or held values as fp16; what is past fp16 is infinite here, and saturated by `finite`.
+__device__ inline u4 as_half(u4 raw, bool bf16) {
+  if (!bf16) return raw;
+  u4 r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t w = raw[i / 2];
-    const uint32_t b = i & 1 ? w >> 16 : w & 0xffffu;
-    float f = bf16 ? bf2f(b) : h2f_((uint16_t)b);
-    f = f > kHalfMax ? kHalfMax : f;
-    f = f < -kHalfMax ? -kHalfMax : f;
-    r[i] = (_Float16)f;
+  for (int i = 0; i < 4; ++i) {
+    const h2 x = {(_Float16)__uint_as_float(raw[i] << 16),
+                  (_Float16)__uint_as_float(raw[i] & 0xffff0000u)};
+    r[i] = __builtin_bit_cast(uint32_t, x);
   }
   return r;
 }
 
-__device__ inline bool has_nan(h8 x) {
-  bool n = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) n |= x[i] != x[i];
-  return n;
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+
+// The largest magnitude of fp16 pairs, as bits: past 0x7c00 there is a NaN, at 0x7c00 an infinity.
+__device__ inline uint32_t magnitude2(uint32_t m, uint32_t x) {
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_elementwise_max(__builtin_bit_cast(us2, m),
+                                                      __builtin_bit_cast(us2, x & 0x7fff7fffu)));
+}
+__device__ inline uint32_t magnitude8(u4 x) {
+  const uint32_t m = magnitude2(magnitude2(magnitude2(magnitude2(0, x.x), x.y), x.z), x.w);
+  const uint32_t lo = m & 0xffffu, hi = m >> 16;
+  return lo > hi ? lo : hi;
 }
 
-// The token row of this lane holds a NaN in some channel of K or V: rows are CH lanes side by side.
-template <int CH>
-__device__ inline void couple_nan(h8& k, h8& v, int lane) {
-  const uint64_t bad = __ballot(has_nan(k) || has_nan(v));
-  if (__builtin_expect(bad == 0, 1)) return;
-  const uint64_t row = (((uint64_t)1 << CH) - 1) << (lane / CH * CH);
-  if (bad & row) {
-    const _Float16 nan = __builtin_bit_cast(_Float16, (uint16_t)0x7e00);
-    k = h8{nan, nan, nan, nan, nan, nan, nan, nan};
-    v = h8{};
+// Infinities become fp16's largest.
+__device__ inline u4 finite(u4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w = x[i];
+    if ((w & 0x7fffu) == 0x7c00u) w -= 1;
+    if ((w & 0x7fff0000u) == 0x7c000000u) w -= 0x10000u;
+    x[i] = w;
   }
+  return x;
+}
+
+// Every lane of a row of CH lanes side by side: has one of them its bit in `lanes`?
+template <int CH>
+__device__ inline bool row_in(uint64_t lanes, int lane) {
+  return (lanes >> (lane / CH * CH) & (((uint64_t)1 << CH) - 1)) != 0;
 }
 
 // The quotient top x / a, rounded so that every tie between codes is seen as one: n = top x is
@@ -72,80 +81,66 @@ __device__ inline uint32_t code4(float y0, float y1, float y2, float y3) {
   }
 }
 
-template <int NI>
-__device__ inline float largest(const h8 (&x)[NI]) {
-  float a = kFloor;
-#pragma unroll
-  for (int i = 0; i < NI; ++i)
-#pragma unroll
-    for (int c = 0; c < 8; ++c) a = fmaxf(a, __builtin_fabsf((float)x[i][c]));  // a NaN is dropped
-#pragma unroll
-  for (int s = 32; s; s >>= 1) a = fmaxf(a, __shfl_xor(a, s));
-  return a;
+__device__ inline float half_at(u4 x, int i) {
+  const uint32_t w = x[i / 2];  // by value, as in h_bits
+  const h2 p = __builtin_bit_cast(h2, w);
+  return (float)(i & 1 ? p.y : p.x);
 }
 
 // Codes of K: a lane's 8 channels of a token are 8 bytes of its row.
-template <int HD, int P, bool E4M3>
-__device__ inline void store_k(const jacq_q8_pool& pool, const h8 (&x)[P * HD / 512], int64_t slot,
-                               int t0, int ch, int lane) {
-  constexpr int NI = P * HD / 512;
+template <int HD, int NI, bool E4M3>
+__device__ inline void store_k(uint8_t* dst, const u4 (&x)[NI], float a, bool poisoned) {
   constexpr float top = E4M3 ? 448.0f : 127.0f;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < NI; ++i) nan |= x[i][0] != x[i][0];  // couple_nan fills whole rows
-  const bool poisoned = __ballot(nan) != 0;
-  const float a = largest(x), inv = 1.0f / a;
-  uint8_t* dst = pool.k_code + slot * (P * HD) + t0 * HD + ch;
+  const float inv = 1.0f / a;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     float y[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      y[c] = quotient((float)x[i][c] * top, a, inv);
-      if (poisoned) y[c] = 0.0f;  // no NaN codes: the scale says it
-    }
+    for (int c = 0; c < 8; ++c) y[c] = quotient(half_at(x[i], c) * top, a, inv);
     u2 w = {code4<E4M3>(y[0], y[1], y[2], y[3]), code4<E4M3>(y[4], y[5], y[6], y[7])};
+    if (poisoned) w = E4M3 ? u2{0, 0} : u2{0x80808080u, 0x80808080u};  // zeros: the scale is NaN
     *(u2*)(dst + i * HD) = w;
   }
-  if (lane == 0) pool.k_scale[slot] = poisoned ? __builtin_nanf("") : a / top;
 }
 
 // Codes of V: a lane's NI tokens of a channel are NI bytes of that channel's row.
-template <int HD, int P, bool E4M3>
-__device__ inline void store_v(const jacq_q8_pool& pool, const h8 (&x)[P * HD / 512], int64_t slot,
-                               int t0, int ch, int lane) {
-  constexpr int NI = P * HD / 512;
+template <int P, int NI, bool E4M3>
+__device__ inline void store_v(uint8_t* dst, const u4 (&x)[NI], float a) {
   constexpr float top = E4M3 ? 448.0f : 127.0f;
-  const float a = largest(x), inv = 1.0f / a;
-  uint8_t* dst = pool.v_code + slot * (P * HD) + ch * P + t0;
+  const float inv = 1.0f / a;
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
-    float y[NI < 4 ? 4 : NI];
+    float y[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < NI; ++i) y[i] = quotient((float)x[i][c] * top, a, inv);
-    if constexpr (NI == 2) {
-      *(uint16_t*)(dst + c * P) = (uint16_t)code4<E4M3>(y[0], y[1], 0.0f, 0.0f);
-    } else if constexpr (NI == 4) {
-      *(uint32_t*)(dst + c * P) = code4<E4M3>(y[0], y[1], y[2], y[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NI; i += 8) {
-        u2 w = {code4<E4M3>(y[i], y[i + 1], y[i + 2], y[i + 3]),
-                code4<E4M3>(y[i + 4], y[i + 5], y[i + 6], y[i + 7])};
-        *(u2*)(dst + c * P + i) = w;
-      }
-    }
+    for (int i = 0; i < NI; ++i) y[i] = quotient(half_at(x[i], c) * top, a, inv);
+    const uint32_t w = code4<E4M3>(y[0], y[1], y[2], y[3]);
+    if constexpr (NI == 2) *(uint16_t*)(dst + c * P) = (uint16_t)w;
+    else *(uint32_t*)(dst + c * P) = w;
   }
-  if (lane == 0) pool.v_scale[slot] = a / top;
 }
+
+// How a block is dealt: NI tokens a lane, PARTS wavefronts for K and as many for V.
+template <int HD, int P>
+struct Deal {
+  static constexpr int CH = HD / 8;  // lanes of a token row
+  static constexpr int NI = P * HD / 512 < 4 ? P * HD / 512 : 4;
+  static constexpr int PARTS = P * HD / 512 / NI;
+  static constexpr int THREADS = 128 * PARTS;
+};
 
 // blockIdx.x: kv head + NKV * block from the sequence's first touched one; blockIdx.y: sequence.
 template <int HD, int P, bool E4M3>
-__global__ __launch_bounds__(64) void q8_append_kernel(Geo g, AppendArgs a) {
-  constexpr int CH = HD / 8;    // lanes of a token row
-  constexpr int NI = P * HD / 512;  // tokens of a lane
+__global__ __launch_bounds__((Deal<HD, P>::THREADS)) void q8_append_kernel(Geo g, AppendArgs a) {
+  typedef Deal<HD, P> D;
+  constexpr int CH = D::CH, NI = D::NI, PARTS = D::PARTS;
+  constexpr float top = E4M3 ? 448.0f : 127.0f;
+  __shared__ uint32_t most[2 * PARTS];             // largest magnitudes, as bits
+  __shared__ uint64_t bad[2][PARTS][NI];           // lanes with a NaN
+  __shared__ uint32_t mended[2 * PARTS];
   const int b = blockIdx.y, h = blockIdx.x % g.nkv, j = blockIdx.x / g.nkv;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const bool is_v = wave >= PARTS;
+  const int part = is_v ? wave - PARTS : wave;
   int row0 = b, n = 1;
   if (a.cu) {
     int lo = a.cu[b], hi = a.cu[b + 1];
@@ -162,42 +157,96 @@ __global__ __launch_bounds__(64) void q8_append_kernel(Geo g, AppendArgs a) {
   const int off = start % P, first = start / P;
   const int done = (off + n) / P;  // blocks that become full
   if (j > 0 && j >= done) return;
-  const int t0 = lane / CH * NI, ch = lane % CH * 8;
+  const int ch = lane % CH * 8;
   const uint16_t* nk = a.new_k + (int64_t)row0 * a.k_stride + (int64_t)h * HD + ch;
   const uint16_t* nv = a.new_v + (int64_t)row0 * a.v_stride + (int64_t)h * HD + ch;
   const int64_t tail = ((int64_t)b * g.nkv + h) * (P * HD) + ch;
   const bool bf16 = a.bf16 != 0;
 
   if (done > j) {  // block first + j: the tail's rows (of the first block), then new ones
-    h8 k[NI], v[NI];
+    const int t0 = part * (P / PARTS) + lane / CH * NI;
+    const uint16_t* src = is_v ? nv : nk;
+    const uint16_t* held_rows = is_v ? a.pool.v_tail : a.pool.k_tail;
+    const int64_t stride = is_v ? a.v_stride : a.k_stride;
+    const int page = uniform(a.tables[(int64_t)b * g.max_pages + first + j]);
+    u4 x[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int t = j * P + t0 + i - off;  // new token, or a row of the tail where negative
-      const bool held = t < 0;
-      const u4 rk = *(const u4*)(held ? a.pool.k_tail + tail + (t + off) * HD
-                                      : nk + (int64_t)t * a.k_stride);
-      const u4 rv = *(const u4*)(held ? a.pool.v_tail + tail + (t + off) * HD
-                                      : nv + (int64_t)t * a.v_stride);
-      k[i] = as_half(rk, bf16 && !held);
-      v[i] = as_half(rv, bf16 && !held);
-      couple_nan<CH>(k[i], v[i], lane);
+      x[i] = *(const u4*)(t < 0 ? held_rows + tail + (t + off) * HD : src + (int64_t)t * stride);
     }
-    const int page = uniform(a.tables[(int64_t)b * g.max_pages + first + j]);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      x[i] = as_half(x[i], bf16 && j * P + t0 + i >= off);
+      const uint32_t mi = magnitude8(x[i]);
+      m = mi > m ? mi : m;
+      const uint64_t nans = __ballot(mi > 0x7c00u);
+      if (lane == 0) bad[is_v][part][i] = nans;
+    }
+    m = (uint32_t)lane63(wave_prefix((int)m, Max()));
+    if (lane == 0) most[wave] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 2 * PARTS; ++i) m = most[i] > m ? most[i] : m;
+    const bool rare = uniform(m) >= 0x7c00;
+    bool poisoned = false;
+    if (__builtin_expect(rare, 0)) {
+      // Infinities saturate.  A NaN in a token's K or V: its V is 0, and K's scale NaN.
+      m = 0;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if (row_in<CH>(bad[0][part][i] | bad[1][part][i], lane)) x[i] = u4{0, 0, 0, 0};
+        x[i] = finite(x[i]);
+        const uint32_t mi = magnitude8(x[i]);
+        m = mi > m ? mi : m;
+      }
+      for (int q = 0; q < PARTS; ++q)
+        for (int i = 0; i < NI; ++i) poisoned |= (bad[0][q][i] | bad[1][q][i]) != 0;
+      m = (uint32_t)lane63(wave_prefix((int)m, Max()));
+      if (lane == 0) mended[wave] = m;
+      __syncthreads();
+    }
+    uint32_t own = 0;  // this tensor's largest
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const uint32_t v = rare ? mended[is_v * PARTS + i] : most[is_v * PARTS + i];
+      own = v > own ? v : own;
+    }
+    const float most_own = h2f_((uint16_t)own);
+    const float big = most_own > kFloor ? most_own : kFloor;
     if (page >= 0 && page < g.num_pages) {
       const int64_t slot = (int64_t)page * g.nkv + h;
-      store_k<HD, P, E4M3>(a.pool, k, slot, t0, ch, lane);
-      store_v<HD, P, E4M3>(a.pool, v, slot, t0, ch, lane);
+      if (is_v) {
+        store_v<P, NI, E4M3>(a.pool.v_code + slot * (P * HD) + ch * P + t0, x, big);
+        if (part == 0 && lane == 0) a.pool.v_scale[slot] = big / top;
+      } else {
+        store_k<HD, NI, E4M3>(a.pool.k_code + slot * (P * HD) + t0 * HD + ch, x, big, poisoned);
+        if (part == 0 && lane == 0)
+          a.pool.k_scale[slot] = poisoned ? __builtin_nanf("") : big / top;
+      }
     }
   }
   if (j > 0) return;
-  // The block in progress: all of the new tokens, or those behind the last full block.
+  // The block in progress: all of the new tokens, or those behind the last full block.  The tail's
+  // rows that a block took in have been read by all of the workgroup.
   const int left = done ? (off + n) % P : n, from = n - left, to = done ? 0 : off;
-  for (int r = lane / CH; r < left; r += 64 / CH) {
-    h8 k = as_half(*(const u4*)(nk + (int64_t)(from + r) * a.k_stride), bf16);
-    h8 v = as_half(*(const u4*)(nv + (int64_t)(from + r) * a.v_stride), bf16);
-    couple_nan<CH>(k, v, lane);
-    *(h8*)(a.pool.k_tail + tail + (to + r) * HD) = k;
-    *(h8*)(a.pool.v_tail + tail + (to + r) * HD) = v;
+  for (int r = threadIdx.x / CH; r < left; r += D::THREADS / CH) {
+    u4 k = as_half(*(const u4*)(nk + (int64_t)(from + r) * a.k_stride), bf16);
+    u4 v = as_half(*(const u4*)(nv + (int64_t)(from + r) * a.v_stride), bf16);
+    const uint32_t mk = magnitude8(k), mv = magnitude8(v);
+    if (__ballot(mk >= 0x7c00u || mv >= 0x7c00u)) {
+      const uint64_t nans = __ballot(mk > 0x7c00u || mv > 0x7c00u);
+      k = finite(k);
+      v = finite(v);
+      if (row_in<CH>(nans, lane)) {
+        k = u4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+        v = u4{0, 0, 0, 0};
+      }
+    }
+    *(u4*)(a.pool.k_tail + tail + (to + r) * HD) = k;
+    *(u4*)(a.pool.v_tail + tail + (to + r) * HD) = v;
   }
 }
 
@@ -207,9 +256,10 @@ static void append_codes(const Geo& g, const AppendArgs& a, int batch, hipStream
   const int blocks = a.max_new / P + 1;
   const dim3 grid((unsigned)g.nkv * blocks, batch);
   if (g.codes == JACQ_Q8_E4M3)
-    hipLaunchKernelGGL((q8_append_kernel<HD, P, true>), grid, dim3(64), 0, s, g, a);
+    hipLaunchKernelGGL((q8_append_kernel<HD, P, true>), grid, dim3(Deal<HD, P>::THREADS), 0, s, g, a);
   else
-    hipLaunchKernelGGL((q8_append_kernel<HD, P, false>), grid, dim3(64), 0, s, g, a);
+    hipLaunchKernelGGL((q8_append_kernel<HD, P, false>), grid, dim3(Deal<HD, P>::THREADS), 0, s, g,
+                       a);
 }
 
 hipError_t launch_append(const Geo& g, const AppendArgs& a, int batch, hipStream_t s) {
@@ -255,37 +305,43 @@ __device__ inline void store8(void* p, int64_t at, const float (&x)[8], int type
   *(u4*)((uint16_t*)p + at) = w;
 }
 
-// One wavefront per (kv head, 16 tokens from the sequence's first group of 16); blockIdx.y:
-// sequence.  Its rows of the output start where those of the sequences before end.
+// One wavefront per (16 tokens of a sequence, kv head): blockIdx.x counts them, kv heads fastest.
 template <int HD, bool E4M3>
 __global__ __launch_bounds__(64) void q8_read_kernel(Geo g, ReadArgs a) {
   constexpr int CH = HD / 8;
   __shared__ __align__(16) uint16_t lds[16 * (HD + 8)];
-  const int b = blockIdx.y, h = blockIdx.x % g.nkv, lane = threadIdx.x;
-  int64_t before = 0;  // a call's tokens may outnumber 32 bits: what is past `total` is dropped
-  int start = 0, end = 0;
-  for (int base = 0; base <= b; base += 64) {
+  const int h = blockIdx.x % g.nkv, lane = threadIdx.x;
+  const int want = blockIdx.x / g.nkv;
+  // The sequence of the wanted 16, which of its 16s it is, and the rows of the sequences before.
+  // A call's tokens may outnumber 32 bits: those past `total` are dropped.
+  int64_t before = 0;
+  int b = -1, start = 0, end = 0, group = 0;
+  int groups = 0;
+  for (int base = 0; base < a.batch && b < 0; base += 64) {
     int s = 0, e = 0;
-    if (base + lane <= b) {
+    if (base + lane < a.batch) {
       e = clamp_len(g, a.ends[base + lane]);
       s = a.starts[base + lane];
       s = s < 0 ? 0 : s > e ? e : s;
     }
-    int n = base + lane < b ? e - s : 0;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-    before += n;
-    if (base + 64 > b) {
-      start = __shfl(s, b - base);
-      end = __shfl(e, b - base);
+    const int n = e > s ? (e + 15) / 16 - s / 16 : 0;
+    const int inc = wave_prefix(n, Sum()), rows = wave_prefix(e - s, Sum());
+    if (const uint64_t past = __ballot(groups + inc > want && n > 0)) {
+      const int l = __builtin_ctzll(past);
+      b = base + l;
+      start = __builtin_amdgcn_readlane(s, l);
+      end = __builtin_amdgcn_readlane(e, l);
+      group = want - groups - __builtin_amdgcn_readlane(inc - n, l);
+      before += __builtin_amdgcn_readlane(rows - (e - s), l);
+    } else {
+      groups += lane63(inc);
+      before += lane63(rows);
     }
   }
-  start = uniform(start);
-  end = uniform(end);
+  if (b < 0 || before >= a.total) return;
   const int nq = end >> g.page_log2 << g.page_log2;
-  for (int t0 = start / 16 * 16 + (int)(blockIdx.x / g.nkv) * 16; t0 < end;
-       t0 += (int)(gridDim.x / g.nkv) * 16) {
-    __syncthreads();
+  {
+    const int t0 = start / 16 * 16 + group * 16;
     const bool held = t0 >= nq;  // a group of 16 is in one page or in the tail
     const int in = t0 & (g.page - 1);
     float ks = 1.0f, vs = 1.0f;
@@ -342,11 +398,8 @@ hipError_t launch_read(const Geo& g, const Pool& p, const int32_t* starts, const
                        const int32_t* tables, int batch, int total, void* k, void* v, int type,
                        hipStream_t s) {
   const ReadArgs a = {p, starts, ends, tables, k, v, batch, total, type};
-  // enough wavefronts for one sequence to hold all the rows; the kernel loops past them
-  int groups = (total + 15) / 16 + 1;
-  const int cap = 4096 / (batch < 64 ? batch : 64) + 1;
-  groups = groups > cap ? cap : groups;
-  const dim3 grid((unsigned)g.nkv * groups, batch);
+  // a sequence's tokens touch at most one group of 16 more than a 16th of them, begun ones counted
+  const dim3 grid((unsigned)g.nkv * (total / 16 + 2 * batch));
 #define JACQ_READ(HD, E)                                                                 \
   hipLaunchKernelGGL((q8_read_kernel<HD, E>), grid, dim3(64), 0, s, g, a)
   if (g.hd == 128) {
