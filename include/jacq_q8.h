@@ -54,14 +54,14 @@ extern "C" {
 /* The most queries per sequence of a call that adds up block weights. */
 #define JACQ_Q8_MAX_WEIGHTED_QUERIES 64
 /* The widest block table. */
-#define JACQ_Q8_MAX_PAGES_PER_SEQ 32768
+#define JACQ_Q8_MAX_PAGES_PER_SEQ 16384
 
 typedef struct jacq_q8_geometry {
   int32_t num_heads;         /* NH */
   int32_t num_kv_heads;      /* NKV; NH % NKV == 0, NH / NKV <= 16 */
   int32_t head_dim;          /* HD: 64 or 128 */
   int32_t page_size;         /* P: 16, 32 or 64 */
-  int32_t max_pages_per_seq; /* block-table row width, 1 to 32768 */
+  int32_t max_pages_per_seq; /* block-table row width, 1 to 16384 */
   int32_t num_pages;         /* physical pages in the pool */
   int32_t codes;             /* JACQ_Q8_INT8 or JACQ_Q8_E4M3 */
 } jacq_q8_geometry;

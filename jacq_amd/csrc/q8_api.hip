@@ -54,7 +54,7 @@ int check_geometry(const jacq_q8_geometry* x) {
     return fail(JACQ_KIVI_EINVAL,
                 "page_size must be 16, 32 or 64, got " + std::to_string(x->page_size));
   if (x->max_pages_per_seq < 1 || x->max_pages_per_seq > JACQ_Q8_MAX_PAGES_PER_SEQ)
-    return fail(JACQ_KIVI_EINVAL, "max_pages_per_seq must be in [1, 32768], got " +
+    return fail(JACQ_KIVI_EINVAL, "max_pages_per_seq must be in [1, 16384], got " +
                                       std::to_string(x->max_pages_per_seq));
   if (x->num_pages < 1)
     return fail(JACQ_KIVI_EINVAL, "num_pages (page storage capacity) must be positive");

@@ -129,6 +129,7 @@ struct Sum {
 };
 struct SumF {  // of fp32 bits
   __device__ int operator()(int a, int b) const {
+#pragma clang fp contract(off)
     return __float_as_int(__int_as_float(a) + __int_as_float(b));
   }
 };

@@ -359,6 +359,7 @@ __device__ inline int slices_of(const Span& s, int size) { return (s.units + siz
 //    16384 254 against 228; one of 4096 32 against 14.
 //  - Else about 4 slices a CU, of 4 to 16 units where there is less work.
 __device__ inline int slice_units(const AttendArgs& a, float all, float segments, int longest) {
+#pragma clang fp contract(off)  // the decode and the join have to find the same size
   const float cus = 0.25f * (float)a.target;
   if ((float)longest <= 1.4f * all / cus + 16.0f &&
       (segments <= cus || all >= 0.75f * segments * (float)longest))
@@ -373,7 +374,8 @@ __device__ inline int slice_units(const AttendArgs& a, float all, float segments
 // of sequence `b`.  Over the lanes of each wavefront alike.
 template <int ROWS>
 __device__ inline Slices cut(const Geo& g, const AttendArgs& a, int lane, int want, int b) {
-  // the sums are fp32: they choose the size, alike in every wavefront, and no more
+#pragma clang fp contract(off)
+  // the sums are fp32: they choose the size, alike in every wavefront and kernel, and no more
   float total = 0.0f, segments = 0.0f;
   int q0, m, blocks = 0, longest = 1;
   Span sp;
@@ -579,32 +581,38 @@ __global__ __launch_bounds__(256) void q8_join_kernel(Geo g, AttendArgs a) {
   }
 }
 
-// Adds up the weight of every block: a thread per 16 tokens, over kv heads, row blocks and rows in
-// that order; then the 16s of a page.  blockIdx.y: sequence.
+// Adds up the weight of every block: a lane per 16 tokens, a wavefront every fourth kv head; their
+// four sums in order, then the 16s of a page.  blockIdx.y: sequence.
 template <int NB>
 __global__ __launch_bounds__(256) void q8_weights_kernel(Geo g, AttendArgs a) {
   constexpr int ROWS = 16 * NB;
-  const int b = blockIdx.y, grp = blockIdx.x * 256 + threadIdx.x;
+  __shared__ float part[4][64];
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int grp = blockIdx.x * 64 + lane;
   int q0, m, blocks;
   Span sp;
   sequence_span<ROWS>(g, a, b, &q0, &m, &sp, &blocks);
   const int t0 = grp * 16, tile = t0 / kTile;
   // groups that no unit covers were not written by this call
-  const bool there = t0 < sp.n && m > 0 && (t0 >= sp.nq || tile < sp.ns || tile >= sp.w0);
+  const bool there = t0 < sp.n && (t0 >= sp.nq || tile < sp.ns || tile >= sp.w0);
   float sum = 0.0f;
-  if (there) {
-    for (int h = 0; h < g.nkv; ++h)
-      for (int rb = 0; rb < blocks; ++rb) {
-        const int64_t seg = ((int64_t)b * g.nkv + h) * a.row_blocks + rb;
-        const float* src = a.group_lse + (seg * a.groups + grp) * a.rows;
-        const int left = m * g.gqa - rb * ROWS, rows = left < ROWS ? left : ROWS;
-        for (int r = 0; r < rows; ++r) {
-          const int x = rb * ROWS + r;
-          const float lse = a.row_lse[(int64_t)(q0 + x / g.gqa) * g.nh + h * g.gqa + x % g.gqa];
-          if (lse != kNegInf) sum += exp2_(src[r] - lse);
-        }
+  for (int h = wave; h < g.nkv; h += 4)
+    for (int rb = 0; rb < blocks; ++rb) {
+      const int64_t seg = ((int64_t)b * g.nkv + h) * a.row_blocks + rb;
+      const float* src = a.group_lse + (seg * a.groups + grp) * a.rows;
+      const int left = m * g.gqa - rb * ROWS, rows = left < ROWS ? left : ROWS;
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r) {
+        const int x = rb * ROWS + r;
+        const float lse = a.row_lse[(int64_t)(q0 + x / g.gqa) * g.nh + h * g.gqa + x % g.gqa];
+        const float got = there ? src[r] : kNegInf;
+        sum += lse == kNegInf ? 0.0f : exp2_(got - lse);
       }
-  }
+    }
+  part[wave][lane] = sum;
+  __syncthreads();
+  if (wave > 0) return;
+  sum = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
   const int per = g.page / 16;
   for (int d = 1; d < per; d <<= 1) sum += __shfl_xor(sum, d);
   const int page = grp / per;
@@ -628,8 +636,8 @@ static void decode_kernels(const Geo& g, const AttendArgs& a, hipStream_t s) {
       hipLaunchKernelGGL((q8_join_kernel<HD, NB, false>), dim3(segments), dim3(256), 0, s, g, a);
   }
   if (a.weights)
-    hipLaunchKernelGGL((q8_weights_kernel<NB>), dim3((a.groups + 255) / 256, a.batch), dim3(256), 0,
-                       s, g, a);
+    hipLaunchKernelGGL((q8_weights_kernel<NB>), dim3((a.groups + 63) / 64, a.batch), dim3(256), 0, s,
+                       g, a);
 }
 
 template <int HD, bool E4M3>

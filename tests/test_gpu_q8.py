@@ -510,7 +510,7 @@ def test_block_weights(q8, page, m, window, sinks):
     assert torch.equal(w, held + held)
 
 
-@pytest.mark.parametrize("page,width", [(16, 1), (16, 40), (32, 1500), (16, 5000), (64, 32768)])
+@pytest.mark.parametrize("page,width", [(16, 1), (16, 40), (32, 1500), (16, 5000), (64, 16384)])
 @pytest.mark.parametrize("place", ["new", "same"])
 def test_evict(q8, page, width, place):
     rng = random.Random(width)
@@ -714,6 +714,46 @@ def test_lengths_past_the_table_are_clamped(q8):
     got = cache.decode(q, ints(1 << 30, -9), tables)
     assert torch.equal(got[0], cache.decode(q, ints(160, 0), tables)[0])
     assert not got[1].any()
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_calls(q8, seed):
+    """Any mix of lengths, queries, windows and heads: cut and uncut, few rows and many."""
+    rng = random.Random(1000 + seed)
+    nh, nkv, hd = rng.choice(HEADS)
+    page, codes = rng.choice((16, 32, 64)), rng.choice(("int8", "e4m3"))
+    dtype = rng.choice((torch.float16, torch.bfloat16))
+    batch = rng.choice((1, 2, 5, 20, 70))
+    most = rng.choice((40, 300, 3000, 12000)) // (1 if batch < 20 else 4)
+    lens = [rng.randint(0, most) if rng.random() < 0.8 else rng.randint(0, 3) for _ in range(batch)]
+    width = None if rng.random() < 0.5 else -(-max(lens + [1]) // page) + rng.choice((1, 500))
+    cache, tables, seq = make(q8, nh, nkv, hd, page, codes, lens, seed=seed, dtype=dtype,
+                              width=width)
+    spoil(cache, tables, lens)
+    gen = torch.Generator("cuda").manual_seed(seed)
+    kw = {}
+    if rng.random() < 0.5:
+        kw = {"window": rng.randint(1, 2 * most), "sinks": rng.choice((0, 1, 5, 100))}
+    for top in (1, rng.randint(2, 9), rng.randint(10, 200)):
+        m = [min(n, rng.randint(0, top)) for n in lens] if top > 1 else [1] * batch
+        cu = [0]
+        for x in m:
+            cu.append(cu[-1] + x)
+        q = randn(gen, cu[-1], nh, hd, dtype=dtype, scale=1.5)
+        lse = torch.zeros((cu[-1], nh), device="cuda")
+        if top == 1:
+            out = cache.decode(q, seq, tables, lse=lse, **kw)
+        else:
+            out = cache.prefill(q, ints(*cu), max(m + [1]), seq, tables, lse=lse, **kw)
+        check_attention(cache, tables, lens, q, cu, out, lse, **kw)
+        if top <= 9:
+            w = torch.full((batch, cache.geo.max_pages_per_seq), 3.0, device="cuda")
+            if top == 1:
+                again = cache.decode(q, seq, tables, weights=w, decay=0.0, **kw)
+            else:
+                again = cache.prefill(q, ints(*cu), max(m + [1]), seq, tables, weights=w,
+                                      decay=0.0, **kw)
+            check_attention(cache, tables, lens, q, cu, again, weights=w, **kw)
 
 
 def test_many_sequences(q8):

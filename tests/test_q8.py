@@ -29,7 +29,7 @@ def test_version_and_exports():
     (dict(num_heads=9), "multiple"), (dict(num_kv_heads=0), "multiple"),
     (dict(num_heads=34), "<= 16"), (dict(head_dim=96), "head_dim"), (dict(page_size=8), "page_size"),
     (dict(page_size=128), "page_size"), (dict(max_pages_per_seq=0), "max_pages"),
-    (dict(max_pages_per_seq=32769), "max_pages"), (dict(num_pages=0), "num_pages"),
+    (dict(max_pages_per_seq=16385), "max_pages"), (dict(num_pages=0), "num_pages"),
     (dict(codes="int4"), "codes")])
 def test_geometry_refusals(change, text):
     with pytest.raises(kivi.KiviCheckError, match=text):
