@@ -285,6 +285,7 @@ class PagedQ8Cache:
         fits = (self._index >= 0 and self._fits_rows(new_k, self._kv_row)
                 and self._fits_rows(new_v, self._kv_row) and new_v.shape[0] == total
                 and new_v.dtype is new_k.dtype and self._fits(start_lens, block_tables))
+        contiguous = fits
         if not fits:
             self._rows(new_k, nkv, "NEW_K")
             self._rows(new_v, nkv, "NEW_V")
@@ -304,10 +305,13 @@ class PagedQ8Cache:
         if not fits:
             self._here(("NEW_K", new_k), ("NEW_V", new_v), ("START_LENS", start_lens),
                        ("BLOCK_TABLES", block_tables), ("CU_NEW", cu_new))
+        if contiguous:
+            k_stride = v_stride = nkv * self.geo.head_dim
+        else:
+            k_stride, v_stride = self._stride(new_k, nkv), self._stride(new_v, nkv)
         self._call(_lib.jacq_q8_append, self.geo.ref, self._pool, new_k.data_ptr(),
-                   new_v.data_ptr(), DTYPES[new_k.dtype], self._stride(new_k, nkv),
-                   self._stride(new_v, nkv), _ptr(cu_new), start_lens.data_ptr(),
-                   block_tables.data_ptr(), total, max_new, self.batch)
+                   new_v.data_ptr(), DTYPES[new_k.dtype], k_stride, v_stride, _ptr(cu_new),
+                   start_lens.data_ptr(), block_tables.data_ptr(), total, max_new, self.batch)
 
     def _attend(self, q, cu_q, max_q, seq_lens, block_tables, window, sinks, scale, weights, decay,
                 out, lse, workspace) -> torch.Tensor:
@@ -319,6 +323,7 @@ class PagedQ8Cache:
             self._rows(q, nh, "Q")
             self._tables(seq_lens, block_tables)
         total = q.shape[0]
+        contiguous = fits
         if window is None:
             window = 0
         else:
@@ -333,8 +338,9 @@ class PagedQ8Cache:
             _check(max_q <= MAX_WEIGHTED_QUERIES, "WEIGHTS take at most ", MAX_WEIGHTED_QUERIES,
                    " queries per sequence, got ", max_q)
             _check(0.0 <= decay < math.inf, "DECAY must be finite and not negative")
-        if out is None:
-            out = torch.empty((total, nh, hd), dtype=q.dtype, device=q.device)
+        if out is None:  # empty_like is the quicker one, for a q that is contiguous
+            out = (torch.empty_like(q) if contiguous else
+                   torch.empty((total, nh, hd), dtype=q.dtype, device=q.device))
         else:
             check_shape(out, (total, nh, hd), "O")
             _check(out.dtype in (q.dtype, torch.float32) and out.is_contiguous(),
@@ -361,7 +367,8 @@ class PagedQ8Cache:
             _check(workspace.is_contiguous(), "workspace must be contiguous")
             size = workspace.numel() * workspace.element_size()
         args = _ATTEND.pack(q.data_ptr(), _ptr(cu_q), seq_lens.data_ptr(), block_tables.data_ptr(),
-                            out.data_ptr(), _ptr(lse), _ptr(weights), self._stride(q, nh),
+                            out.data_ptr(), _ptr(lse), _ptr(weights),
+                            nh * hd if contiguous else self._stride(q, nh),
                             DTYPES[q.dtype], DTYPES[out.dtype], self.batch, total, max_q,
                             min(window, 1 << 30), min(sinks, 1 << 30), scale, decay)
         self._call(_lib.jacq_q8_attend, g.ref, self._pool, args, _ptr(workspace), size)
