@@ -367,7 +367,15 @@ __device__ inline int slice_units(const AttendArgs& a, float all, float segments
   const int fair = (int)(all / cus) + 1;  // one slice a CU
   const int few = fair < 4 ? 4 : fair > 16 ? 16 : fair;
   const int many = (int)(all / (float)a.target) + 1;
-  return many > few ? many : few;
+  // whole rounds of the workgroup's wavefronts
+  return ((many > few ? many : few) + kWaves - 1) / kWaves * kWaves;
+}
+
+// Units of each of the n slices but the last: equal, in whole rounds of the wavefronts too (never
+// more than the size they were counted by, so the last has some left).
+__device__ inline int even_units(const Span& s, int n) {
+  const int u = (s.units + n - 1) / n;
+  return n == 1 ? u : (u + kWaves - 1) / kWaves * kWaves;
 }
 
 // The cut, and the sequence that has slice `want` (b >= batch: none), or, with want < 0, the place
@@ -437,8 +445,9 @@ __global__ __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) void q8_decode_kernel
     x /= g.nkv;
     s.rb = uniform(x % blocks);
     const int z = uniform(x / blocks), n = uniform(slices_of(s.span, c.size));
-    u0 = uniform((int)((int64_t)s.span.units * z / n));
-    u1 = uniform((int)((int64_t)s.span.units * (z + 1) / n));
+    const int each = uniform(even_units(s.span, n));
+    u0 = z * each;
+    u1 = u0 + each < s.span.units ? u0 + each : s.span.units;
     whole = n == 1;
   } else {
     s.b = blockIdx.x / (g.nkv * a.row_blocks);
