@@ -191,6 +191,13 @@ struct Wave {
            (a.window > 0 && t0 <= last - a.window && t0 + kTile > a.sinks);
   }
 
+  // No row sees the 16 tokens from t on, as their windows begin later: their page may be any, and
+  // its e4m3 codes NaN, which a weight of 0 would not take out.
+  __device__ bool before_window(const Segment& s, int t) const {
+    const int first = s.span.n - s.m + s.rb * 16 * NB / g.gqa;
+    return t + 15 <= first - a.window && t >= a.sinks;
+  }
+
   __device__ void scores(const Codes& c, f4 (&sc)[NB][4]) const {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -287,6 +294,9 @@ struct Wave {
         f4 sc[NB][4];
         scores(c, sc);
         const float ks = c.there ? c.ks : __builtin_nanf(""), vs = c.vs;
+        if (E4M3 && masked && a.window > 0 && before_window(s, t0 + kq * 16))
+#pragma unroll
+          for (int d = 0; d < DT; ++d) c.v[d] = u4{0, 0, 0, 0};
         if (next >= 0) load_k(s, next, nk, nv, c);
         h8 p[NB][2];
 #pragma unroll

@@ -227,6 +227,12 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
     uint16_t* dst = &lds.v[u & 1][0][0];
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
+      if (E4M3 && a.window > 0) {
+        // A page before every row's window may be any, and its e4m3 codes NaN, which a weight of 0
+        // would not take out.
+        const int t = tile_at(u) + vt[i];
+        if (t + g.page - 1 <= pfirst - a.window && t >= a.sinks) vc[i] = u4{0, 0, 0, 0};
+      }
       *(h8*)(dst + vs0[i]) = codes8<E4M3>(vc[i].x, vc[i].y);
       *(h8*)(dst + vs1[i]) = codes8<E4M3>(vc[i].z, vc[i].w);
     }

@@ -269,6 +269,14 @@ class PagedQ8Cache:
         if rc != 0:
             raise KiviLaunchError(last_error())
 
+    def _workspace_size(self, key: tuple) -> int:
+        if len(self._sizes) > 4096:
+            self._sizes.clear()
+        with torch.cuda.device(self._index):  # the size goes by its compute units
+            size = self._sizes[key] = _lib.jacq_q8_attend_workspace_size(
+                self.geo.ref, self.batch, *key)
+        return size
+
     # ---- calls ----
 
     def append(self, new_k: torch.Tensor, new_v: torch.Tensor, block_tables: torch.Tensor,
@@ -299,8 +307,8 @@ class PagedQ8Cache:
             max_new = 1
         else:
             self._ints(cu_new, self.batch + 1, "CU_NEW")
-            max_new = total if max_new is None else max_new
-            _check(max_new >= 0, "MAX_NEW must not be negative")
+            _check(max_new is None or max_new >= 0, "MAX_NEW must not be negative")
+            max_new = total if max_new is None else min(int(max_new), total)
             fits = fits and cu_new.get_device() == self._index
         if not fits:
             self._here(("NEW_K", new_k), ("NEW_V", new_v), ("START_LENS", start_lens),
@@ -324,6 +332,12 @@ class PagedQ8Cache:
             self._tables(seq_lens, block_tables)
         total = q.shape[0]
         contiguous = fits
+        if weights is not None:
+            self._weights(weights)
+            _check(max_q <= MAX_WEIGHTED_QUERIES, "WEIGHTS take at most ", MAX_WEIGHTED_QUERIES,
+                   " queries per sequence, got ", max_q)
+            _check(0.0 <= decay < math.inf, "DECAY must be finite and not negative")
+        max_q = min(max_q, total)
         if window is None:
             window = 0
         else:
@@ -333,11 +347,6 @@ class PagedQ8Cache:
         _check(0.0 < scale < math.inf, "SCALE must be positive and finite")
         if cu_q is not None:
             self._ints(cu_q, self.batch + 1, "CU_Q")
-        if weights is not None:
-            self._weights(weights)
-            _check(max_q <= MAX_WEIGHTED_QUERIES, "WEIGHTS take at most ", MAX_WEIGHTED_QUERIES,
-                   " queries per sequence, got ", max_q)
-            _check(0.0 <= decay < math.inf, "DECAY must be finite and not negative")
         if out is None:  # empty_like is the quicker one, for a q that is contiguous
             out = (torch.empty_like(q) if contiguous else
                    torch.empty((total, nh, hd), dtype=q.dtype, device=q.device))
@@ -357,10 +366,7 @@ class PagedQ8Cache:
             key = (total, max_q, weights is not None)
             size = self._sizes.get(key)
             if size is None:
-                if len(self._sizes) > 4096:
-                    self._sizes.clear()
-                size = self._sizes[key] = _lib.jacq_q8_attend_workspace_size(
-                    g.ref, self.batch, total, max_q, weights is not None)
+                size = self._workspace_size(key)
             if size:
                 workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         else:
@@ -448,6 +454,8 @@ class PagedQ8Cache:
             self._weights(weights)
         _check(sink_pages >= 0 and recent_pages >= 0 and sink_pages + recent_pages <= keep,
                "KEEP must be at least SINK_PAGES + RECENT_PAGES, neither negative")
+        if keep >= self.geo.max_pages_per_seq:  # no sequence has more
+            keep, sink_pages, recent_pages = self.geo.max_pages_per_seq, 0, 0
         if out is None:
             out = (torch.empty_like(block_tables), torch.empty_like(seq_lens),
                    torch.empty_like(weights), torch.empty_like(seq_lens))
@@ -462,7 +470,6 @@ class PagedQ8Cache:
             self._here(("WEIGHTS", weights), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
                        *(("an output", t) for t in out))
         self._call(_lib.jacq_q8_evict, self.geo.ref, weights.data_ptr(), seq_lens.data_ptr(),
-                   block_tables.data_ptr(), self.batch, min(int(keep), (1 << 31) - 1),
-                   int(sink_pages), int(recent_pages), tables_out.data_ptr(), lens_out.data_ptr(),
+                   block_tables.data_ptr(), self.batch, keep, sink_pages, recent_pages, tables_out.data_ptr(), lens_out.data_ptr(),
                    weights_out.data_ptr(), evicted.data_ptr())
         return out

@@ -280,6 +280,47 @@ def test_decode_window_and_sinks(q8, window, sinks, page):
                     sinks=sinks)
 
 
+@pytest.mark.parametrize("given_back", [False, True])
+@pytest.mark.parametrize("m", [1, 3, 50])
+@pytest.mark.parametrize("page", [16, 32])
+def test_pages_before_the_window_may_hold_anything(q8, page, m, given_back):
+    # and their entries may name no page
+    lens, window, sinks = [333, 700, 1000, 65], 100, 10
+    cache, tables, n = make(q8, 40, 8, 128, page, "e4m3", lens, seed=page)
+    gen = torch.Generator("cuda").manual_seed(m)
+    q = randn(gen, len(lens) * m, 40, 128)
+    cu = [b * m for b in range(len(lens) + 1)]
+    names = dict(window=window, sinks=sinks)
+
+    def attend(t):
+        if m == 1:
+            return cache.decode(q, n, t, **names)
+        return cache.prefill(q, ints(*cu), m, n, t, **names)
+
+    want = attend(tables)
+    seen = torch.zeros(cache.geo.num_pages, dtype=torch.bool, device="cuda")
+    bare = torch.full_like(tables, -1)
+    for b, k in enumerate(lens):
+        for p in range(k // page):
+            if p * page < sinks or (p + 1) * page > k - m + 1 - window:
+                seen[int(tables[b, p])] = True
+                bare[b, p] = tables[b, p]
+    assert int((~seen).sum()) > 4
+    cache.k_code[~seen], cache.v_code[~seen] = 0x7F, 0xFF
+    cache.k_scale[~seen], cache.v_scale[~seen] = float("inf"), float("nan")
+    if given_back:
+        # such an entry is read as page 0's codes, which are spoiled too
+        spare = int((~seen).nonzero()[-1])
+        for x in (cache.k_code, cache.v_code, cache.k_scale, cache.v_scale):
+            x[spare] = x[0]
+        for x in (cache.k_code, cache.v_code):
+            x[0] = 0x7F
+        bare[bare == 0] = spare
+    assert torch.equal(attend(bare if given_back else tables), want)
+    if not given_back:
+        check_attention(cache, tables, lens, q, cu, want, **names)
+
+
 @pytest.mark.parametrize("lens", [[20001], [3, 9000, 1, 0, 12345], [700] * 70 + [5000]])
 @pytest.mark.parametrize("codes", ["int8", "e4m3"])
 def test_decode_split_over_workgroups(q8, lens, codes):
@@ -705,6 +746,25 @@ def test_offsets_past_32_bits(q8):
     check_attention(cache, tables, [n], q, [0, n], got)
     got = cache.decode(q[-1:], ints(n), tables)
     check_attention(cache, tables, [n], q[-1:], [0, 1], got)
+
+
+def test_bounds_past_32_bits(q8):
+    big = 1 << 33
+    lens, gen = [70, 3], torch.Generator("cuda").manual_seed(0)
+    cache, tables, n = make(q8, 4, 2, 64, 16, "int8", lens)
+    other = q8.PagedQ8Cache(cache.geo, 2)
+    k, v = randn(gen, 7, 2, 64), randn(gen, 7, 2, 64)
+    for c in (cache, other):
+        c.append(k, v, tables, torch.zeros_like(n), cu_new=ints(0, 5, 7),
+                 max_new=big if c is cache else 5)
+    assert torch.equal(cache.k_tail[0, :, :5], other.k_tail[0, :, :5])
+    n, q = ints(5, 2), randn(gen, 7, 4, 64)
+    assert torch.equal(cache.prefill(q, ints(0, 5, 7), big, n, tables, window=big, sinks=big),
+                       other.prefill(q, ints(0, 5, 7), 5, n, tables))
+    w = torch.ones(2, cache.geo.max_pages_per_seq, device="cuda")
+    n = ints(*lens)
+    got = cache.evict(w, n, tables, keep=2 * big, sink_pages=big, recent_pages=big)
+    assert all(torch.equal(a, b) for a, b in zip(got, (tables, n, w, torch.zeros_like(n))))
 
 
 def test_lengths_past_the_table_are_clamped(q8):
