@@ -131,13 +131,16 @@ int device_cus() {
 // ---- how an attention call runs ----
 // The decode kernel reads the cache once per 32 rows of a kv head and splits it freely; the
 // prefill kernel shares it among 128 rows.  The first is used up to 32 rows, and for so few rows
-// in all that the second leaves most of the chip idle: 40/8 heads of 128, 16384 tokens, one
-// sequence: 8 queries 29 us against 36, 16 queries 41 against 38; four sequences: 8 queries 62
-// against 55; 14/2 heads of 64: 64 queries 35 against 33.
+// in all that the second leaves most of the chip idle.  40/8 heads of 128, 16384 tokens, one
+// sequence (us, first against second): 8 queries 30 against 36, 16 42 against 39, 32 60 against 48;
+// four sequences: 6 queries 50 against 51, 7 86 against 57.  One sequence of 2048: 16 queries 19
+// against 25, 32 20 against 27; 14/2 heads of 64, 8192 tokens: 64 queries 22 against 27, 128 27
+// against 29; 16 sequences of 4096, 40/8 heads: 6 queries 57 against 47, 8 60 against 54.
 constexpr int kFewRows = 32;
 constexpr int kFewHeads = 1024;  // queries x query heads of the call
-// Units up to which the decode kernel does not cut a segment (slice_units would not either): no
-// plan, no join.  The table's width bounds them, so a narrow table saves about 4 us.
+// Units up to which the decode kernel does not cut a segment: no plan, no join.  The table's width
+// bounds them.  40/8 heads of 128, without against with (us): one sequence of 700 tokens 14.5
+// against 15.8, 16 of 500 14.6 against 18.1, 64 of 500 22.9 against 27.0.
 constexpr int kWholeUnits = 16;
 constexpr int kSliceUnits = 8; // units of a prefill's slice at least, by the table's width
 

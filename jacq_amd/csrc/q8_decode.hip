@@ -363,21 +363,22 @@ __device__ inline int slices_of(const Span& s, int size) { return (s.units + siz
 
 // Units of a slice, from the call's units, its segments and the longest one's units.
 //  - Uncut, if that takes no longer: a workgroup alone on a CU needs about 0.4 us a unit (HD 128),
-//    the memory 0.8 us a unit and CU, a cut call about 6 us more; and where segments outnumber CUs
-//    only if they are about equally long.  40/8 heads of 128, uncut against cut (us): 64 sequences
-//    of 2048 tokens 47 against 52, of 4096 99 against 107; 16 of 4096 37 against 32; 64 of 1024 to
-//    16384 254 against 228; one of 4096 32 against 14.
-//  - Else about 4 slices a CU, of 4 to 16 units where there is less work.
+//    the memory 0.8 us a unit and CU, a cut call about 2 us more; and where segments outnumber CUs
+//    only if they are about equally long.  40/8 heads of 128, uncut against cut (us): 32 sequences
+//    of 2048 tokens 29.7 against 31.1, 64 49.7 against 51.1, 64 of 4096 106 against 110; 16 of 1000
+//    22.3 against 18.1, of 2000 30.2 against 25.7, of 4096 41.6 against 31.7; 64 of 1024 to 16384
+//    267 against 235; one of 4096 35.3 against 12.6.
+//  - Else about 4 slices a CU (2 to 8 differ by 10 % at most), of 4 to 16 units where there is less
+//    work, and whole rounds of the workgroup's wavefronts.
 __device__ inline int slice_units(const AttendArgs& a, float all, float segments, int longest) {
 #pragma clang fp contract(off)  // the decode and the join have to find the same size
   const float cus = 0.25f * (float)a.target;
-  if ((float)longest <= 1.4f * all / cus + 16.0f &&
+  if ((float)longest <= 1.4f * all / cus + 4.0f &&
       (segments <= cus || all >= 0.75f * segments * (float)longest))
     return longest;
   const int fair = (int)(all / cus) + 1;  // one slice a CU
   const int few = fair < 4 ? 4 : fair > 16 ? 16 : fair;
   const int many = (int)(all / (float)a.target) + 1;
-  // whole rounds of the workgroup's wavefronts
   return ((many > few ? many : few) + kWaves - 1) / kWaves * kWaves;
 }
 
