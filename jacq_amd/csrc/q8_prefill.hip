@@ -2,13 +2,24 @@
 //
 // A workgroup has 128 query rows of one kv head (row = query token x head of
 // the group), 32 for each of 4 wavefronts, and goes through the tiles of 64
-// tokens that any of its rows sees, or through one of several slices of them.  A tile's codes are converted to fp16 once
-// and shared through the LDS.  S^T = K Q^T and O^T += V^T P^T on
-// v_mfma_f32_32x32x16_f16; a lane's column is a query row, so its maximum, sum
-// and rescaling are the lane's own (and its partner's, 32 lanes on), and the
-// order in which K's rows enter makes P the next operand as it stands.
-// The scales of 16 tokens are the wavefront's: t = s (ks q) + log2(vs), as in
-// q8_decode.hip, where the reason is.
+// tokens that any of its rows sees, or through one of several slices of them.
+// A tile's codes are converted to fp16 once and shared through the LDS.
+// S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_f16; a lane's column is
+// a query row, so its maximum, sum and rescaling are the lane's own (and its
+// partner's, 32 lanes on), and the order in which K's rows enter makes P the
+// next operand as it stands.  The scales of 16 tokens are the wavefront's:
+// t = s (ks q) + log2(vs), as in q8_decode.hip, where the reason is.
+//
+// Bound by the matrix cores, the LDS and the vector units together.  A prompt of
+// 8191 tokens (40/8 heads of 128, int8): 780 to 820 us, 840 to 880 TFLOP/s, where
+// the library's product of 8192^3 runs at 1145.  Of the CUs' cycles the matrix
+// cores are busy for 40 %, the vector units for 56 %, the LDS for 53 %.  Without the
+// staging it takes 586 us, without the softmax 629, the products with their
+// LDS reads alone 526: an operand feeds one product, since 64 rows a wavefront
+// (two products each) do not fit the registers at HD 128 (spills, 1061 us).
+// Two workgroups a CU, not in step: one's products run beside the other's
+// softmax.  The softmax of a half tile among the next half's products, in one
+// wavefront's order, was as fast (HD 128: 820 us; HD 64: 204 against 213).
 #include <type_traits>
 
 #include "q8_common.h"
