@@ -430,7 +430,8 @@ class PagedQ8Cache:
         _check(total >= 0, "TOTAL must not be negative")
         if not fits:
             self._here(("STARTS", starts), ("ENDS", ends), ("BLOCK_TABLES", block_tables))
-        k, v = torch.empty((2, total, g.num_kv_heads, g.head_dim), dtype=dtype, device=self.device)
+        k = torch.empty((total, g.num_kv_heads, g.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         self._call(_lib.jacq_q8_read, g.ref, self._pool, starts.data_ptr(), ends.data_ptr(),
                    block_tables.data_ptr(), self.batch, total, k.data_ptr(), v.data_ptr(),
                    DTYPES[dtype])

@@ -692,6 +692,68 @@ def test_graph_replays(q8):
         assert torch.equal(x, y)
 
 
+def test_replays_of_a_prompt_in_slices(q8):
+    """Captured once, replayed with other lengths, offsets and queries; the rows behind the last
+    sequence, and queries past max_q, are left as they are."""
+    lens, m = [9000, 4000, 300], 60
+    cache, tables, seq = make(q8, 40, 8, 128, 32, "int8", lens, seed=125)
+    gen = torch.Generator("cuda").manual_seed(126)
+    q = randn(gen, 3 * m + 7, 40, 128)
+    cu = ints(0, m, 2 * m, 3 * m)
+    size = q8.lib().jacq_q8_attend_workspace_size(cache.geo.ref, 3, 3 * m + 7, m, 0)
+    assert size > 0  # slices
+    out = torch.full((3 * m + 7, 40, 128), 7.0, dtype=torch.float16, device="cuda")
+    cache.prefill(q, cu, m, seq, tables, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.prefill(q, cu, m, seq, tables, out=out)
+    for now, at in ((lens, [0, m, 2 * m, 3 * m]), ([8000, 65, 300], [0, 10, 70, 71]),
+                    ([0, 4000, 1], [5, 5, 66, 67]), (lens, [0, m + 4, m + 5, 3 * m])):
+        q.copy_(randn(gen, *q.shape))
+        seq.copy_(ints(*now))
+        cu.copy_(ints(*at))
+        out.fill_(7.0)
+        graph.replay()
+        want = torch.full_like(out, 7.0)
+        cache.prefill(q, cu, m, seq, tables, out=want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert bool((out[:at[0]] == 7.0).all()) and bool((out[at[3]:] == 7.0).all())
+        for b in range(3):  # a query past max_q is left alone, and the others count from the end
+            count = at[b + 1] - at[b]
+            assert bool((out[at[b] + min(count, m):at[b + 1]] == 7.0).all())
+            if count <= m and now[b]:
+                rows = slice(at[b], at[b + 1])
+                check_attention(cache.sequence_view(b), tables[b:b + 1], now[b:b + 1], q[rows],
+                                [0, count], out[rows])
+
+
+def test_calls_of_several_threads(q8):
+    import threading
+    lens = [3000, 5000]
+    cache, tables, seq = make(q8, 8, 2, 128, 32, "int8", lens, seed=127)
+    gen = torch.Generator("cuda").manual_seed(128)
+    q = [randn(gen, 2, 8, 128) for _ in range(4)]
+    want = [cache.decode(x, seq, tables) for x in q]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = cache.decode(q[i], seq, tables)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_another_stream_and_a_shared_workspace(q8):
     lens = [4000, 9000]
     cache, tables, seq = make(q8, 8, 2, 128, 32, "int8", lens, seed=120)
