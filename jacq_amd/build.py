@@ -47,7 +47,7 @@ def hipcc() -> str:
 # Kernels that must not spill: a spill makes the kernel need scratch memory,
 # which cost the decode about 17 us (13%) when a 12-byte spill crept in.
 NO_SCRATCH = ("kivi_decode_stream_kernel", "kivi_decode_chunk_kernel", "kivi_append_kernel",
-              "q8_append_kernel", "q8_read_kernel", "q8_decode_kernel", "q8_join_kernel",
+              "q8_append_kernel", "q8_read_kernel", "q8_plan_kernel", "q8_decode_kernel", "q8_join_kernel",
               "q8_weights_kernel", "q8_prefill_kernel", "q8_merge_kernel", "q8_evict_kernel")
 
 

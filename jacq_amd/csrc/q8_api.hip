@@ -129,25 +129,32 @@ int device_cus() {
 }
 
 // ---- how an attention call runs ----
-// The decode kernel reads the cache once per 32 rows of a kv head and splits it freely; the
-// prefill kernel shares it among 128 rows.  The first is used up to 32 rows, and for so few rows
-// in all that the second leaves most of the chip idle.  40/8 heads of 128, 16384 tokens, one
-// sequence (us, first against second): 8 queries 30 against 36, 16 42 against 39, 32 60 against 48;
-// four sequences: 6 queries 50 against 51, 7 86 against 57.  One sequence of 2048: 16 queries 19
-// against 25, 32 20 against 27; 14/2 heads of 64, 8192 tokens: 64 queries 22 against 27, 128 27
-// against 29; 16 sequences of 4096, 40/8 heads: 6 queries 57 against 47, 8 60 against 54.
-constexpr int kFewRows = 32;
-constexpr int kFewHeads = 1024;  // queries x query heads of the call
+// The decode kernel reads the cache once per 32 rows of a kv head (a second time mostly from a
+// cache nearer by) and splits it freely; the prefill kernel shares it among 128 rows.  The first is
+// used up to 64 rows, and for so few rows in all that the second leaves most of the chip idle.
+// Decode against prefill, us (heads of 128 unless said otherwise):
+//   40 to 64 rows  32 sequences, 64/8 heads, 8 queries: of 500 tokens 26 against 29, 2000 48
+//                  against 58, 12000 222 against 279; 4 of 16384, 40/8 heads, 12 queries: 61
+//                  against 59; 64 of 500, 32/8 heads, 16 queries: 45 against 37
+//   70, 80 rows    4 of 16384, 40/8 heads, 16 queries: 76 against 64; 16 of 4096, 14/2 heads of 64,
+//                  14 queries: 34 against 27
+//   one sequence   40/8 heads, 32 queries: of 2048 tokens 20 against 27, 16384 45 against 49; 8/1
+//                  heads, 16384 tokens: 128 queries 34 against 41, 200 53 against 49
+constexpr int kFewRows = 64;
+constexpr int kFewHeads = 2048;  // queries x query heads of the call
 // Units up to which the decode kernel does not cut a segment: no plan, no join.  The table's width
 // bounds them.  40/8 heads of 128, without against with (us): one sequence of 700 tokens 14.5
 // against 15.8, 16 of 500 14.6 against 18.1, 64 of 500 22.9 against 27.0.
 constexpr int kWholeUnits = 16;
-constexpr int kSliceUnits = 8; // units of a prefill's slice at least, by the table's width
+// Sequences up to which every workgroup finds the cut by itself (a lane each); more have a kernel
+// for it.  32/8 heads of 128, by itself against by the kernel (us): 80 sequences of 100 to 4000
+// tokens 99 against 97, 256 of 100 to 1000 99 against 86, 512 of 100 to 500 187 against 123.
+constexpr int kCutBatch = 64;
 
 struct Plan {
-  bool prefill;
+  bool prefill, planned;
   int slices, nb, rows, row_blocks, target, groups;
-  size_t ml, acc, group_lse, row_lse, bytes;  // offsets into the workspace, and its size
+  size_t ml, acc, plan, group_lse, row_lse, bytes;  // offsets into the workspace, and its size
 };
 
 // Workgroups that share the tokens of a prefill's row tile.  A workgroup alone on a CU takes about
@@ -159,7 +166,7 @@ struct Plan {
 // 493 in one, 443 in 2, 446 in 4; a prompt of 8191 825 in one, 907 in 2.
 int plan_slices(double groups, int64_t tokens) {
   const double load = groups / device_cus();
-  const int most = (int)std::min<int64_t>(32, tokens / (kSliceUnits * jacq::q8::kTile));
+  const int most = (int)std::min<int64_t>(32, tokens / (jacq::q8::kSliceUnits * jacq::q8::kTile));
   int best = 1;
   double least = 0;
   for (int s = 1; s <= std::max(1, most); ++s) {
@@ -204,6 +211,8 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
   const size_t parts = p.target ? (size_t)p.target + segments : 0;
   p.ml = take(parts * p.rows * 2 * sizeof(float));
   p.acc = take(parts * p.rows * g.hd * sizeof(float));
+  p.planned = p.target && batch > kCutBatch;
+  p.plan = take(p.planned ? ((size_t)batch + 2) * sizeof(int32_t) : 0);
   p.group_lse = take(weighted ? (size_t)segments * p.groups * p.rows * sizeof(float) : 0);
   p.row_lse = take(weighted ? (size_t)total_q * g.nh * sizeof(float) : 0);
   p.bytes = at;
@@ -339,6 +348,7 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.slices = p.slices;
     if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, stream), "prefill");
     a.target = p.target;
+    a.plan = p.planned ? (int32_t*)(ws + p.plan) : nullptr;
     a.rows = p.rows;
     a.row_blocks = p.row_blocks;
     a.groups = p.groups;

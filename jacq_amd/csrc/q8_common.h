@@ -19,6 +19,8 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kFloor = 0x1p-24f;   // a block's largest magnitude counts as at least this
 constexpr float kHalfMax = 65504.0f;
 constexpr int kTile = 64;            // tokens per step of the attention kernels
+constexpr int kPrefillRows = 128;    // query rows of a workgroup of the prefill kernel
+constexpr int kSliceUnits = 8;       // tiles of one of its slices at least
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Geo {
@@ -65,6 +67,7 @@ struct AttendArgs {
   float* part_acc;        // the same [HD]
   float* group_lse;       // [batch][nkv][row blocks][groups][rows]
   float* row_lse;         // [total_q][nh], base 2
+  int32_t* plan;          // decode of many sequences: [batch + 1] first slices, then their size
   int target;             // decode: slices to aim at, 4 a CU; 0: segments stay whole
   int rows;               // rows of a segment at most (<= 16 NB)
   int row_blocks;         // row blocks of a sequence at most
@@ -155,6 +158,18 @@ __device__ inline void queries_of(const AttendArgs& a, int b, int* q0, int* m) {
   hi = hi < lo ? lo : hi > a.total_q ? a.total_q : hi;
   *q0 = lo;
   *m = hi - lo > a.max_q ? a.max_q : hi - lo;
+}
+
+// A prefill's slices of a sequence of n tokens: at most a.slices, and none of fewer than kSliceUnits
+// tiles, by what a row tile may see.
+__device__ inline int prefill_slices(const AttendArgs& a, int n) {
+  int tiles = (n + kTile - 1) / kTile;
+  if (a.window > 0) {  // its rows are at most kPrefillRows tokens
+    const int64_t most = ((int64_t)a.window + a.sinks + kPrefillRows) / kTile + 3;
+    tiles = tiles < most ? tiles : (int)most;
+  }
+  const int s = (tiles + kSliceUnits - 1) / kSliceUnits;
+  return s < 1 ? 1 : s < a.slices ? s : a.slices;
 }
 
 // The tiles of kTile tokens that the queries of a sequence of n tokens may see, in order: the

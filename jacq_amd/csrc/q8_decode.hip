@@ -21,8 +21,10 @@
 // runs at 4.96; 4 queries of each of 32 sequences of 1500 to 6007 (32/8 heads, bf16) 51 + 7 us.
 // One sequence of 512 tokens (32/4 heads of 64) is latency: 5.5 us, four dependent rounds of
 // memory (length, table, codes, and the fold through the LDS).
-// Two wavefronts a SIMD (16 rows): the codes of a unit in flight take 48 registers; at three a
-// SIMD the kernel spilled 12 bytes and was slower.
+// Wavefronts a SIMD at HD 128: three of 16 rows, two of 32; the codes of a unit in flight are 64
+// registers.  With two and one, 1024 sequences of 100 to 500 tokens took 212 us instead of 178,
+// with 8 queries each 489 instead of 288 (32/8 heads); one sequence of 500000 tokens, 4 queries,
+// 238 instead of 200 (40/8 heads).
 #include "q8_common.h"
 
 namespace jacq {
@@ -54,6 +56,7 @@ struct Wave {
   int pos[NB];     // the row's position; below 0 where there is no row
   f4 acc[NB][DT];
   float m[NB], l[NB];
+  float group[NB];  // the last tile's, of this lane's 16 tokens
 
   struct Codes {
     u4 k[4][KL];
@@ -120,32 +123,34 @@ struct Wave {
     return a.tables[(int64_t)s.b * g.max_pages + (t >> g.page_log2)];
   }
   __device__ bool exists(int page) const { return page >= 0 && page < g.num_pages; }
-  __device__ int64_t slot_of(const Segment& s, int page) const {
-    return (int64_t)(exists(page) ? page : 0) * g.nkv + s.h;
-  }
+  __device__ uint32_t held(int page) const { return exists(page) ? page : 0; }
 
   __device__ void pages(const Segment& s, int tile, int& pk, int& pv) const {
     pk = page_of(s, tile * kTile + n16 / 4 * 16);
     pv = page_of(s, tile * kTile + kq * 16);
   }
 
-  // A quantised tile's K codes with the scales, and its V codes.
-  __device__ void load_k(const Segment& s, int tile, int pk, int pv, Codes& c) const {
-    const int tk = (tile * kTile + n16 / 4 * 16) & (g.page - 1);
-    const int64_t sk = slot_of(s, pk), sv = slot_of(s, pv);
-    const uint8_t* k = a.pool.k_code + (sk * g.page + tk + (n16 & 3)) * HD + kq * 16;
+  // A quantised tile's K codes, its scales and its V codes.  A tile begins a page or lies in one, so
+  // where a lane reads in its page is the same for all.
+  __device__ void load_k(const Segment& s, int pk, Codes& c) const {
+    uint32_t in = (s.h * g.page + (n16 / 4 * 16 & (g.page - 1)) + (n16 & 3)) * HD + kq * 16;
+    asm volatile("" : "+v"(in));  // one register over the loop, not a pointer's two
+    const uint8_t* k = a.pool.k_code + ((uint64_t)held(pk) * (uint32_t)(g.nkv * g.page * HD) + in);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int j = 0; j < KL; ++j) c.k[t][j] = *(const u4*)(k + t * 4 * HD + j * 64);
-    c.ks = a.pool.k_scale[sv];
-    c.there = exists(pv);
-    c.vs = a.pool.v_scale[sv];
   }
-  __device__ void load_v(const Segment& s, int tile, int pv, Codes& c) const {
-    const int tv = (tile * kTile + kq * 16) & (g.page - 1);
-    const int64_t sv = slot_of(s, pv);
-    const uint8_t* v = a.pool.v_code + (sv * HD + n16) * g.page + tv;
+  __device__ void load_scales(const Segment& s, int pv, Codes& c) const {
+    const uint64_t slot = (uint64_t)held(pv) * (uint32_t)g.nkv + (uint32_t)s.h;
+    c.ks = a.pool.k_scale[slot];
+    c.there = exists(pv);
+    c.vs = a.pool.v_scale[slot];
+  }
+  __device__ void load_v(const Segment& s, int pv, Codes& c) const {
+    uint32_t in = (s.h * HD + n16) * g.page + (kq * 16 & (g.page - 1));
+    asm volatile("" : "+v"(in));
+    const uint8_t* v = a.pool.v_code + ((uint64_t)held(pv) * (uint32_t)(g.nkv * g.page * HD) + in);
 #pragma unroll
     for (int d = 0; d < DT; ++d) c.v[d] = *(const u4*)(v + d * 16 * g.page);
   }
@@ -153,7 +158,7 @@ struct Wave {
   // Scores -> weights -> O^T.  sc: raw scores of this lane's 16 tokens, t0 their first one;
   // tokens from `end` on are not there.  Returns through pv_step the fp16 weights.
   __device__ void soften(const Segment& s, int nb, f4 (&sc)[4], int t0, int end, float ks, float vs,
-                         bool masked, bool weigh, h8& p0, h8& p1) {
+                         bool masked, h8& p0, h8& p1) {
     const float av = qs[nb] * ks, bv = log2_(vs), ivs = 1.0f / vs;
     float t[16];
     float mx = kNegInf;
@@ -185,10 +190,17 @@ struct Wave {
     }
     const float part = sum == 0.0f ? 0.0f : sum * ivs;  // a scale that nothing sees may be any
     l[nb] += part;
-    if (weigh && t0 < end && nb * 16 + n16 < s.nrows) {
-      const int64_t seg = ((int64_t)s.b * g.nkv + s.h) * a.row_blocks + s.rb;
-      a.group_lse[(seg * a.groups + (t0 >> 4)) * a.rows + nb * 16 + n16] = base + log2_(part);
-    }
+    group[nb] = base + log2_(part);
+  }
+
+  // The base-2 logarithms of the weight of this lane's 16 tokens from t0 on, for the block weights.
+  __device__ void store_group(const Segment& s, int t0, int end) const {
+    if (!a.weights || t0 >= end) return;
+    const int64_t seg = ((int64_t)s.b * g.nkv + s.h) * a.row_blocks + s.rb;
+    float* dst = a.group_lse + (seg * a.groups + (t0 >> 4)) * a.rows;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      if (nb * 16 + n16 < s.nrows) dst[nb * 16 + n16] = group[nb];
   }
 
   __device__ bool needs_mask(const Segment& s, int t0, int end) const {
@@ -260,8 +272,9 @@ struct Wave {
     h8 p[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
-      soften(s, nb, sc[nb], s.span.nq + kq * 16, s.span.n, 1.0f, 1.0f, true, a.weights != nullptr,
-             p[nb][0], p[nb][1]);
+      soften(s, nb, sc[nb], s.span.nq + kq * 16, s.span.n, 1.0f, 1.0f, true, p[nb][0],
+             p[nb][1]);
+    store_group(s, s.span.nq + kq * 16, s.span.n);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       h8 vv[2];
@@ -277,7 +290,7 @@ struct Wave {
         acc[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[0], p[nb][0], acc[nb][d], 0, 0, 0);
         acc[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[1], p[nb][1], acc[nb][d], 0, 0, 0);
       }
-      if (d & 1) __builtin_amdgcn_sched_barrier(0);  // two channel tiles' loads at a time
+      if (NB == 2 || d & 1) __builtin_amdgcn_sched_barrier(0);  // few loads at a time: registers
     }
   }
 
@@ -292,8 +305,9 @@ struct Wave {
       Codes c;
       int pk, pv, nk = 0, nv = 0, tile = sp.tile_of(u0);
       pages(s, tile, pk, pv);
-      load_k(s, tile, pk, pv, c);
-      load_v(s, tile, pv, c);
+      load_k(s, pk, c);
+      load_scales(s, pv, c);
+      load_v(s, pv, c);
       if (u0 + kWaves < e) pages(s, sp.tile_of(u0 + kWaves), nk, nv);
       for (;;) {
         const int next = u0 + kWaves < e ? sp.tile_of(u0 + kWaves) : -1;
@@ -305,19 +319,23 @@ struct Wave {
         if (E4M3 && masked && a.window > 0 && before_window(s, t0 + kq * 16))
 #pragma unroll
           for (int d = 0; d < DT; ++d) c.v[d] = u4{0, 0, 0, 0};
-        if (next >= 0) load_k(s, next, nk, nv, c);
+        if (next >= 0) load_k(s, nk, c);
         h8 p[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          soften(s, nb, sc[nb], t0 + kq * 16, sp.nq, ks, vs, masked, a.weights != nullptr,
-                 p[nb][0], p[nb][1]);
+          soften(s, nb, sc[nb], t0 + kq * 16, sp.nq, ks, vs, masked, p[nb][0], p[nb][1]);
         values(c, p);
         u0 += kWaves;
         if (next < 0) break;
-        load_v(s, next, nv, c);
+        load_scales(s, nv, c);
+        load_v(s, nv, c);
+        // behind the loads: what is loaded behind a store waits for it too (256 sequences of 100 to
+        // 4000 tokens, 32/8 heads of 128: 241 us against 246)
+        store_group(s, t0 + kq * 16, sp.nq);
         if (u0 + kWaves < e) pages(s, sp.tile_of(u0 + kWaves), nk, nv);
         tile = next;
       }
+      store_group(s, tile * kTile + kq * 16, sp.nq);
     }
     if (u0 < u1) tail(s);  // the unit behind the quantised ones
   }
@@ -397,53 +415,113 @@ __device__ inline int even_units(const Span& s, int n) {
   return n == 1 ? u : (u + kWaves - 1) / kWaves * kWaves;
 }
 
+// The same of a cut that q8_plan_kernel left: 64 places a step.
+__device__ inline Slices planned(const AttendArgs& a, int lane, int want, int b) {
+  const int size = uniform(a.plan[a.batch + 1]);
+  if (want < 0) return {size, b, uniform(a.plan[b])};
+  if (want >= uniform(a.plan[a.batch])) return {size, a.batch, 0};
+  // the last sequence whose first slice is not behind `want`: one without slices is not the last
+  int at = 0;
+  for (int n = a.batch; n > 1;) {
+    const int step = (n + 63) / 64, i = lane * step;
+    const uint64_t upto = __ballot(i < n && a.plan[at + (i < n ? i : 0)] <= want);
+    const int skip = (__popcll(upto) - 1) * step;
+    at += skip;
+    n = step < n - skip ? step : n - skip;
+  }
+  return {size, at, uniform(a.plan[at])};
+}
+
 // The cut, and the sequence that has slice `want` (b >= batch: none), or, with want < 0, the place
-// of sequence `b`.  Over the lanes of each wavefront alike.
+// of sequence `b`.  Over the lanes of each wavefront alike, a sequence each.
 template <int ROWS>
 __device__ inline Slices cut(const Geo& g, const AttendArgs& a, int lane, int want, int b) {
 #pragma clang fp contract(off)
+  if (a.plan) return planned(a, lane, want, b);
   // the sums are fp32: they choose the size, alike in every wavefront and kernel, and no more
-  float total = 0.0f, segments = 0.0f;
-  int q0, m, blocks = 0, longest = 1;
+  float u = 0.0f, n = 0.0f;
+  int q0, m, blocks = 0, most = 1;
   Span sp;
-  for (int base = 0; base < a.batch; base += 64) {
-    float u = 0.0f, n = 0.0f;
-    int most = 0;
-    if (base + lane < a.batch) {
-      sequence_span<ROWS>(g, a, base + lane, &q0, &m, &sp, &blocks);
-      n = (float)(blocks * g.nkv);
-      u = (float)sp.units * n;
-      most = blocks ? sp.units : 0;
-    }
-    total += __int_as_float(lane63(wave_prefix(__float_as_int(u), SumF())));
-    segments += __int_as_float(lane63(wave_prefix(__float_as_int(n), SumF())));
-    most = lane63(wave_prefix(most, Max()));
-    longest = most > longest ? most : longest;
+  if (lane < a.batch) {
+    sequence_span<ROWS>(g, a, lane, &q0, &m, &sp, &blocks);
+    n = (float)(blocks * g.nkv);
+    u = (float)sp.units * n;
+    most = blocks ? sp.units : 1;
   }
-  const int size = uniform(slice_units(a, total, segments, longest));
-  int sum = 0;
-  for (int base = 0; base < a.batch; base += 64) {
-    int n = 0;
-    if (base + lane < a.batch) {
-      if (a.batch > 64) sequence_span<ROWS>(g, a, base + lane, &q0, &m, &sp, &blocks);
-      n = slices_of(sp, size) * blocks * g.nkv;
-    }
-    const int inc = wave_prefix(n, Sum());
-    if (want < 0) {
-      if (b < base + 64) return {size, b, sum + __builtin_amdgcn_readlane(inc - n, uniform(b - base))};
-    } else if (const uint64_t past = __ballot(sum + inc > want && n > 0)) {
-      const int l = __builtin_ctzll(past);
-      return {size, base + l, sum + __builtin_amdgcn_readlane(inc - n, l)};
-    }
-    sum += lane63(inc);
+  const float total = __int_as_float(lane63(wave_prefix(__float_as_int(u), SumF())));
+  const float segments = __int_as_float(lane63(wave_prefix(__float_as_int(n), SumF())));
+  const int size = uniform(slice_units(a, total, segments, lane63(wave_prefix(most, Max()))));
+  const int count = lane < a.batch ? slices_of(sp, size) * blocks * g.nkv : 0;
+  const int inc = wave_prefix(count, Sum());
+  if (want < 0) return {size, b, __builtin_amdgcn_readlane(inc - count, uniform(b))};
+  if (const uint64_t past = __ballot(inc > want && count > 0)) {
+    const int l = __builtin_ctzll(past);
+    return {size, l, __builtin_amdgcn_readlane(inc - count, l)};
   }
   return {size, a.batch, 0};
+}
+
+// The cut of many sequences, once for the call.  One workgroup.
+template <int NB>
+__global__ __launch_bounds__(1024) void q8_plan_kernel(Geo g, AttendArgs a) {
+  constexpr int ROWS = 16 * NB;
+  __shared__ float units[16], segments[16];
+  __shared__ int longest[16], sums[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  int q0, m, blocks;
+  Span sp;
+  float u = 0.0f, n = 0.0f;
+  int most = 1;
+  for (int b = tid; b < a.batch; b += 1024) {
+    sequence_span<ROWS>(g, a, b, &q0, &m, &sp, &blocks);
+    n += (float)(blocks * g.nkv);
+    u += (float)sp.units * (float)(blocks * g.nkv);
+    most = blocks && sp.units > most ? sp.units : most;
+  }
+  u = __int_as_float(lane63(wave_prefix(__float_as_int(u), SumF())));
+  n = __int_as_float(lane63(wave_prefix(__float_as_int(n), SumF())));
+  most = lane63(wave_prefix(most, Max()));
+  if (lane == 0) {
+    units[wave] = u;
+    segments[wave] = n;
+    longest[wave] = most;
+  }
+  __syncthreads();
+  u = n = 0.0f;
+  for (int i = 0; i < 16; ++i) {
+    u += units[i];
+    n += segments[i];
+    most = longest[i] > most ? longest[i] : most;
+  }
+  const int size = uniform(slice_units(a, u, n, most));
+  int before = 0;
+  for (int base = 0, turn = 0; base < a.batch; base += 1024, turn ^= 1) {
+    const int b = base + tid;
+    int count = 0;
+    if (b < a.batch) {
+      sequence_span<ROWS>(g, a, b, &q0, &m, &sp, &blocks);
+      count = slices_of(sp, size) * blocks * g.nkv;
+    }
+    const int inc = wave_prefix(count, Sum());
+    if (lane == 63) sums[turn][wave] = inc;
+    __syncthreads();  // the other turn's sums have been read by all
+    int here = before + inc - count;
+    for (int i = 0; i < 16; ++i) {
+      here += i < wave ? sums[turn][i] : 0;
+      before += sums[turn][i];
+    }
+    if (b < a.batch) a.plan[b] = here;
+  }
+  if (tid == 0) {
+    a.plan[a.batch] = before;
+    a.plan[a.batch + 1] = size;
+  }
 }
 
 // A workgroup of kWaves wavefronts has a slice of a segment.  target > 0: slice blockIdx.x of the
 // cut; else the segment blockIdx.x = (sequence, row block, kv head) whole.
 template <int HD, bool E4M3, int NB>
-__global__ __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) void q8_decode_kernel(Geo g,
+__global__ __launch_bounds__(64 * kWaves, NB == 1 ? 3 : 2) void q8_decode_kernel(Geo g,
                                                                                  AttendArgs a) {
   constexpr int ROWS = 16 * NB;
   constexpr int LD = HD + 4;
@@ -625,7 +703,7 @@ __global__ __launch_bounds__(256) void q8_weights_kernel(Geo g, AttendArgs a) {
   // groups that no unit covers were not written by this call
   const bool there = t0 < sp.n && (t0 >= sp.nq || tile < sp.ns || tile >= sp.w0);
   float sum = 0.0f;
-  for (int h = wave; h < g.nkv; h += 4)
+  for (int h = __ballot(there) ? wave : g.nkv; h < g.nkv; h += 4)
     for (int rb = 0; rb < blocks; ++rb) {
       const int64_t seg = ((int64_t)b * g.nkv + h) * a.row_blocks + rb;
       const float* src = a.group_lse + (seg * a.groups + grp) * a.rows;
@@ -655,6 +733,7 @@ template <int HD, bool E4M3, int NB>
 static void decode_kernels(const Geo& g, const AttendArgs& a, hipStream_t s) {
   const int segments = a.batch * g.nkv * a.row_blocks;
   const unsigned blocks = a.target ? a.target + segments : segments;
+  if (a.plan) hipLaunchKernelGGL((q8_plan_kernel<NB>), dim3(1), dim3(1024), 0, s, g, a);
   hipLaunchKernelGGL((q8_decode_kernel<HD, E4M3, NB>), dim3(blocks), dim3(64 * kWaves), 0, s, g, a);
   if (a.target) {
     // from about 8 slices a segment on, a workgroup per row: its threads share the slices

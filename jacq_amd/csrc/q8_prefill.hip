@@ -31,7 +31,8 @@ namespace q8 {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;
+constexpr int kRows = kPrefillRows;
+static_assert(kRows == 32 * kWaves, "32 a wavefront");
 constexpr float kSlack = 8.0f;  // the running maximum moves only by more than this (base 2)
 constexpr float kNegInf = -__builtin_inff();
 
@@ -99,6 +100,8 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   const int rows = m * g.gqa;
   if (rt * kRows >= rows) return;
   const int n = uniform(clamp_len(g, a.lens[b]));
+  const int slices = uniform(prefill_slices(a, n));
+  if (slice >= slices) return;
   // positions of the workgroup's and the wavefront's rows
   const int end_row = rows < (rt + 1) * kRows ? rows : (rt + 1) * kRows;
   const int pfirst = uniform(n - m + rt * kRows / g.gqa);
@@ -152,8 +155,8 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   int top = plast < 0 ? 0 : (plast >> 6) + 1;
   top = top > sp.tiles ? sp.tiles : top;
   const int every = plast < 0 ? 0 : sp.ns + (top > sp.w0 ? top - sp.w0 : 0);
-  const int from = uniform((int)((int64_t)every * slice / a.slices));
-  const int quant = uniform((int)((int64_t)every * (slice + 1) / a.slices)) - from;
+  const int from = uniform((int)((int64_t)every * slice / slices));
+  const int quant = uniform((int)((int64_t)every * (slice + 1) / slices)) - from;
 
   // ---- staging: a thread has KC chunks of K and of V ----
   // K chunk i: 16 codes (kcc) of row kr + i 64 / KC.  V chunk i: 16 tokens (group vg) of channel
@@ -414,7 +417,7 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
       turn();
     }
   }
-  if (plast >= sp.nq && n > sp.nq && slice == a.slices - 1) {
+  if (plast >= sp.nq && n > sp.nq && slice == slices - 1) {
     stage_tail();
     turn();
     if (wlast >= sp.nq) {
@@ -427,7 +430,7 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   l += other_half(l);
   if (!ok) return;
   const int64_t at = (int64_t)(q0 + tok) * g.nh + head;
-  if (a.slices > 1) {  // q8_merge_kernel joins the slices
+  if (slices > 1) {  // q8_merge_kernel joins the slices
     const int64_t part = (int64_t)slice * a.total_q * g.nh + at;
     if (hh == 0) {
       a.part_ml[2 * part] = mx;
@@ -456,13 +459,15 @@ template <int HD>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Geo g, AttendArgs a) {
   int q0, m;
   queries_of(a, blockIdx.y, &q0, &m);
+  const int slices = prefill_slices(a, clamp_len(g, a.lens[blockIdx.y]));
+  if (slices == 1) return;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int ch = (int)(i % (HD / 4)) * 4;
   if (i / (HD / 4) >= (int64_t)m * g.nh) return;
   const int64_t at = (int64_t)q0 * g.nh + i / (HD / 4), rows = (int64_t)a.total_q * g.nh;
   float mx = kNegInf, l = 0.0f;
   f4 acc = {0, 0, 0, 0};
-  for (int s = 0; s < a.slices; ++s) {
+  for (int s = 0; s < slices; ++s) {
     const float pm = a.part_ml[2 * (s * rows + at)], pl = a.part_ml[2 * (s * rows + at) + 1];
     const f4 pa = *(const f4*)(a.part_acc + (s * rows + at) * HD + ch);
     const float to = fmaxf(mx, pm);

@@ -886,3 +886,28 @@ def test_many_sequences(q8):
     q = randn(gen, 700, 4, 64)
     got = cache.decode(q, seq, tables)
     check_attention(cache, tables, lens, q, list(range(701)), got)
+
+
+@pytest.mark.parametrize("batch,heads", [(65, (10, 2, 128)), (1100, (4, 2, 64)), (2500, (8, 1, 64))])
+def test_many_sequences_under_a_wide_table(q8, batch, heads):
+    """A cut that a kernel of its own plans: one round of 1024 sequences and more."""
+    rng = random.Random(batch)
+    lens = [rng.choice((0, 1, 30, 64, 200)) for _ in range(batch)]
+    lens[batch // 2], lens[-1] = 9000, 3001
+    cache, tables, seq = make(q8, *heads, 32, "int8", lens, seed=151)
+    gen = torch.Generator("cuda").manual_seed(152)
+    for m in (1, 2):
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + min(n, m) if m > 1 else cu[-1] + 1)
+        q = randn(gen, cu[-1], heads[0], heads[2])
+        w = torch.ones((batch, cache.geo.max_pages_per_seq), device="cuda")
+        for window, sinks in ((None, 0), (70, 5)):
+            names = dict(window=window, sinks=sinks)
+            got = (cache.decode(q, seq, tables, weights=w, decay=0.0, **names) if m == 1 else
+                   cache.prefill(q, ints(*cu), m, seq, tables, weights=w, decay=0.0, **names))
+            some = sorted(rng.sample(range(batch), 60) + [0, batch // 2, batch - 1])
+            for b in some:
+                rows = slice(cu[b], cu[b + 1])
+                check_attention(cache.sequence_view(b), tables[b:b + 1], lens[b:b + 1], q[rows],
+                                [0, cu[b + 1] - cu[b]], got[rows], weights=w[b:b + 1], **names)
