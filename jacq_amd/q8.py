@@ -255,8 +255,9 @@ class PagedQ8Cache:
                 and lens.get_device() == self._index == tables.get_device())
 
     def _fits_rows(self, t: torch.Tensor, row: tuple) -> bool:
-        return (t.dim() == 3 and t.shape[1:] == row and t.is_contiguous()
-                and (t.dtype is torch.float16 or t.dtype is torch.bfloat16)
+        shape, dtype = t.shape, t.dtype
+        return (len(shape) == 3 and shape[1] == row[0] and shape[2] == row[1]
+                and t.is_contiguous() and (dtype is torch.float16 or dtype is torch.bfloat16)
                 and t.get_device() == self._index)
 
     def _call(self, fn, *args) -> None:
@@ -291,8 +292,9 @@ class PagedQ8Cache:
         nkv = self.geo.num_kv_heads
         total = new_k.shape[0] if new_k.dim() else 0
         fits = (self._index >= 0 and self._fits_rows(new_k, self._kv_row)
-                and self._fits_rows(new_v, self._kv_row) and new_v.shape[0] == total
-                and new_v.dtype is new_k.dtype and self._fits(start_lens, block_tables))
+                and new_v.shape == new_k.shape and new_v.is_contiguous()
+                and new_v.dtype is new_k.dtype and new_v.get_device() == self._index
+                and self._fits(start_lens, block_tables))
         contiguous = fits
         if not fits:
             self._rows(new_k, nkv, "NEW_K")
@@ -422,7 +424,8 @@ class PagedQ8Cache:
         are dropped, rows that none fills undefined."""
         g = self.geo
         fits = (self._index >= 0 and self._fits(ends, block_tables)
-                and self._fits(starts, block_tables))
+                and starts.shape == self._lens_shape and starts.dtype is torch.int32
+                and starts.is_contiguous() and starts.get_device() == self._index)
         if not fits:
             self._tables(ends, block_tables, "ENDS")
             self._ints(starts, self.batch, "STARTS")
