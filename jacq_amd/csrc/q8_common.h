@@ -21,6 +21,9 @@ constexpr float kHalfMax = 65504.0f;
 constexpr int kTile = 64;            // tokens per step of the attention kernels
 constexpr int kPrefillRows = 128;    // query rows of a workgroup of the prefill kernel
 constexpr int kSliceUnits = 8;       // tiles of one of its slices at least
+// Workgroups of the decode kernel that a CU holds (a wavefront of each a SIMD), by what its
+// registers allow.
+constexpr int decode_groups(int hd, int nb) { return (hd == 128 ? 4 : 5) - nb; }
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Geo {
@@ -68,7 +71,8 @@ struct AttendArgs {
   float* group_lse;       // [batch][nkv][row blocks][groups][rows]
   float* row_lse;         // [total_q][nh], base 2
   int32_t* plan;          // decode of many sequences: [batch + 1] first slices, then their size
-  int target;             // decode: slices to aim at, 4 a CU; 0: segments stay whole
+  int target;             // decode: slices to aim at; 0: segments stay whole
+  int cus;                // compute units
   int rows;               // rows of a segment at most (<= 16 NB)
   int row_blocks;         // row blocks of a sequence at most
   int groups;             // 16-token groups a table addresses

@@ -394,17 +394,21 @@ __device__ inline int slices_of(const Span& s, int size) { return (s.units + siz
 //    of 2048 tokens 29.7 against 31.1, 64 49.7 against 51.1, 64 of 4096 106 against 110; 16 of 1000
 //    22.3 against 18.1, of 2000 30.2 against 25.7, of 4096 41.6 against 31.7; 64 of 1024 to 16384
 //    267 against 235; one of 4096 35.3 against 12.6.
-//  - Else about 4 slices a CU (2 to 8 differ by 10 % at most), of 4 to 16 units where there is less
-//    work, and whole rounds of the workgroup's wavefronts.
+//  - Else as many slices as the chip holds workgroups, once or twice (a.target), where a segment's
+//    last slice counts half, so that few are left for another round; of 4 to 16 units where there is
+//    less work, and whole rounds of the workgroup's wavefronts.  A fixed 4 a CU took, us: 3 sequences
+//    of 20001 to 65535, 64/8 heads 58 against 53; 24 of 4096 to 12289, 40/8 heads, with block weights
+//    106 against 100; 16 of 1000 to 8000, 32/32 heads 117 against 110.
 __device__ inline int slice_units(const AttendArgs& a, float all, float segments, int longest) {
 #pragma clang fp contract(off)  // the decode and the join have to find the same size
-  const float cus = 0.25f * (float)a.target;
+  const float cus = (float)a.cus;
   if ((float)longest <= 1.4f * all / cus + 4.0f &&
       (segments <= cus || all >= 0.75f * segments * (float)longest))
     return longest;
   const int fair = (int)(all / cus) + 1;  // one slice a CU
   const int few = fair < 4 ? 4 : fair > 16 ? 16 : fair;
-  const int many = (int)(all / (float)a.target) + 1;
+  const float fit = (float)a.target - 0.5f * segments, half = 0.5f * (float)a.target;
+  const int many = (int)(all / (fit > half ? fit : half)) + 1;
   return ((many > few ? many : few) + kWaves - 1) / kWaves * kWaves;
 }
 
@@ -521,7 +525,7 @@ __global__ __launch_bounds__(1024) void q8_plan_kernel(Geo g, AttendArgs a) {
 // A workgroup of kWaves wavefronts has a slice of a segment.  target > 0: slice blockIdx.x of the
 // cut; else the segment blockIdx.x = (sequence, row block, kv head) whole.
 template <int HD, bool E4M3, int NB>
-__global__ __launch_bounds__(64 * kWaves, NB == 1 ? 3 : 2) void q8_decode_kernel(Geo g,
+__global__ __launch_bounds__(64 * kWaves, decode_groups(HD, NB)) void q8_decode_kernel(Geo g,
                                                                                  AttendArgs a) {
   constexpr int ROWS = 16 * NB;
   constexpr int LD = HD + 4;
@@ -736,8 +740,9 @@ static void decode_kernels(const Geo& g, const AttendArgs& a, hipStream_t s) {
   if (a.plan) hipLaunchKernelGGL((q8_plan_kernel<NB>), dim3(1), dim3(1024), 0, s, g, a);
   hipLaunchKernelGGL((q8_decode_kernel<HD, E4M3, NB>), dim3(blocks), dim3(64 * kWaves), 0, s, g, a);
   if (a.target) {
-    // from about 8 slices a segment on, a workgroup per row: its threads share the slices
-    if (a.target >= 8 * segments)
+    // from about 16 slices a segment on, a workgroup per row: its threads share the slices (at 8
+    // to 16, 8 sequences of 100 to 3000 tokens, 16/16 heads of 64, 4 queries: 16.0 us against 14.6)
+    if (a.target >= 16 * segments)
       hipLaunchKernelGGL((q8_join_kernel<HD, NB, true>), dim3(segments, a.rows), dim3(256), 0, s, g,
                          a);
     else
