@@ -17,9 +17,9 @@
 // (fp16 holds w to 2^-12; bf16 would hold it to 2^-9.)
 //
 // Bound by memory.  Measured (40/8 heads of 128, int8, page 32): 64 sequences of 1024 to 16384
-// tokens, one query each, 1.16 GB: 220 us and 5 us for the join, 5.2 TB/s, where a copy of 2 GiB
-// runs at 4.96; 4 queries of each of 32 sequences of 1500 to 6007 (32/8 heads, bf16) 49 + 7 us.
-// One sequence of 512 tokens (32/4 heads of 64) is latency: 5.4 us, four dependent rounds of
+// tokens, one query each, 1.16 GB: 215 us and 5 us for the join, 5.3 TB/s, where a copy of 2 GiB
+// runs at 4.96; 4 queries of each of 32 sequences of 1500 to 6007 (32/8 heads, bf16) 47 + 6 us.
+// One sequence of 512 tokens (32/4 heads of 64) is latency: 5.5 us, four dependent rounds of
 // memory (length, table, codes, and the fold through the LDS).
 // Wavefronts a SIMD at HD 128: three of 16 rows, two of 32; the codes of a unit in flight are 64
 // registers.  With two and one, 1024 sequences of 100 to 500 tokens took 212 us instead of 178,
