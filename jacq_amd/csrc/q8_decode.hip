@@ -390,10 +390,12 @@ __device__ inline int slices_of(const Span& s, int size) { return (s.units + siz
 // Units of a slice, from the call's units, its segments and the longest one's units.
 //  - Uncut, if that takes no longer: a workgroup alone on a CU needs about 0.4 us a unit (HD 128),
 //    the memory 0.8 us a unit and CU, a cut call about 2 us more; and where segments outnumber CUs
-//    only if they are about equally long.  40/8 heads of 128, uncut against cut (us): 32 sequences
-//    of 2048 tokens 29.7 against 31.1, 64 49.7 against 51.1, 64 of 4096 106 against 110; 16 of 1000
-//    22.3 against 18.1, of 2000 30.2 against 25.7, of 4096 41.6 against 31.7; 64 of 1024 to 16384
-//    267 against 235; one of 4096 35.3 against 12.6.
+//    only if they are about equally long and, with up to 16 rows, fill the CUs about evenly.  40/8
+//    heads of 128, uncut against cut (us): 32 sequences of 2048 tokens 27.8 against 29.5, 64 48.2
+//    against 50.3, 64 of 4096 103 against 110; 16 of 1000 22.3 against 18.1, of 2000 30.2 against
+//    25.7, of 4096 41.6 against 31.7; 64 of 1024 to 16384 267 against 235; one of 4096 35.3 against
+//    12.6; 48 with windows of 4096, 32/8 heads, 91 against 87; 4 queries of 48 of 3000 to 3500 77
+//    against 91.
 //  - Else as many slices as the chip holds workgroups, once or twice (a.target), where a segment's
 //    last slice counts half, so that few are left for another round; of 4 to 16 units where there is
 //    less work, and whole rounds of the workgroup's wavefronts.  A fixed 4 a CU took, us: 3 sequences
@@ -402,8 +404,9 @@ __device__ inline int slices_of(const Span& s, int size) { return (s.units + siz
 __device__ inline int slice_units(const AttendArgs& a, float all, float segments, int longest) {
 #pragma clang fp contract(off)  // the decode and the join have to find the same size
   const float cus = (float)a.cus;
+  const bool even = a.rows > 16 || segments >= 0.8f * cus * __builtin_ceilf(segments / cus);
   if ((float)longest <= 1.4f * all / cus + 4.0f &&
-      (segments <= cus || all >= 0.75f * segments * (float)longest))
+      (segments <= cus || (even && all >= 0.75f * segments * (float)longest)))
     return longest;
   const int fair = (int)(all / cus) + 1;  // one slice a CU
   const int few = fair < 4 ? 4 : fair > 16 ? 16 : fair;
