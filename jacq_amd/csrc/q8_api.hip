@@ -153,30 +153,21 @@ constexpr int kCutBatch = 64;
 
 struct Plan {
   bool prefill, planned;
+  float load;
   int slices, nb, rows, row_blocks, target, groups;
   size_t ml, acc, plan, group_lse, row_lse, bytes;  // offsets into the workspace, and its size
 };
 
-// Workgroups that share the tokens of a prefill's row tile.  A workgroup alone on a CU takes about
-// 1.7 us a tile of 64 tokens, two 2.5 us (HD 128): `groups` row tiles in S slices take about
-// c(groups S / CUs) / S, c(x) = 1 up to one per CU and 3/4 for each begun one from there, with an
-// end that is not full; the slices' partial sums and their join cost about S 400 / tokens of the
-// whole.  The table's width stands for the tokens.  Measured (us, 40/8 heads of 128): 32 queries
-// over 16384 tokens 430 in one slice, 47 in 16; 511 queries of each of 4 sequences of up to 16001
-// 493 in one, 443 in 2, 446 in 4; a prompt of 8191 825 in one, 907 in 2.
-int plan_slices(double groups, int64_t tokens) {
-  const double load = groups / device_cus();
-  const int most = (int)std::min<int64_t>(32, tokens / (jacq::q8::kSliceUnits * jacq::q8::kTile));
+// A prefill's slices, for as many tokens as the table addresses: the kernels use fewer for
+// sequences of fewer (slices_cost, which has the reasons).
+int plan_slices(float load, int64_t tokens) {
+  const int most =
+      (int)std::min<int64_t>(jacq::q8::kMaxSlices, tokens / (jacq::q8::kSliceUnits * jacq::q8::kTile));
   int best = 1;
-  double least = 0;
-  for (int s = 1; s <= std::max(1, most); ++s) {
-    const double c = load * s <= 1 ? 1.0 : 0.75 * std::ceil(load * s);
-    const double t = (c + 0.3) / s + (s > 1 ? 0.75 * load * s * 400.0 / (double)tokens : 0.0);
-    if (s == 1 || t < least) {
+  for (int s = 2; s <= most; ++s)
+    if (jacq::q8::slices_cost(load, s, (float)tokens) <
+        jacq::q8::slices_cost(load, best, (float)tokens))
       best = s;
-      least = t;
-    }
-  }
   return best;
 }
 
@@ -191,8 +182,9 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
     return here;
   };
   if (p.prefill) {
-    p.slices = plan_slices((double)jacq::q8::prefill_tiles(g, max_q) * g.nkv * batch,
-                           (int64_t)g.max_pages * g.page);
+    p.load = (float)jacq::q8::prefill_tiles(g, max_q) * (float)g.nkv * (float)batch /
+             (float)device_cus();
+    p.slices = plan_slices(p.load, (int64_t)g.max_pages * g.page);
     if (p.slices > 1) {
       const size_t rows_all = (size_t)p.slices * total_q * g.nh;
       p.ml = take(rows_all * 2 * sizeof(float));
@@ -351,6 +343,7 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.group_lse = a.weights ? (float*)(ws + p.group_lse) : nullptr;
     a.row_lse = a.weights ? (float*)(ws + p.row_lse) : nullptr;
     a.slices = p.slices;
+    a.load = p.load;
     if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, stream), "prefill");
     a.target = p.target;
     a.cus = device_cus();

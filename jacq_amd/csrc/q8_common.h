@@ -21,6 +21,7 @@ constexpr float kHalfMax = 65504.0f;
 constexpr int kTile = 64;            // tokens per step of the attention kernels
 constexpr int kPrefillRows = 128;    // query rows of a workgroup of the prefill kernel
 constexpr int kSliceUnits = 8;       // tiles of one of its slices at least
+constexpr int kMaxSlices = 32;       // of its slices at most
 // Workgroups of the decode kernel that a CU holds (a wavefront of each a SIMD), by what its
 // registers allow.
 constexpr int decode_groups(int hd, int nb) { return (hd == 128 ? 4 : 5) - nb; }
@@ -76,7 +77,8 @@ struct AttendArgs {
   int rows;               // rows of a segment at most (<= 16 NB)
   int row_blocks;         // row blocks of a sequence at most
   int groups;             // 16-token groups a table addresses
-  int slices;             // prefill: workgroups that share a row tile's tokens
+  int slices;             // prefill: workgroups that share a row tile's tokens, at most
+  float load;             // row tiles a CU
 };
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -164,16 +166,35 @@ __device__ inline void queries_of(const AttendArgs& a, int b, int* q0, int* m) {
   *m = hi - lo > a.max_q ? a.max_q : hi - lo;
 }
 
-// A prefill's slices of a sequence of n tokens: at most a.slices, and none of fewer than kSliceUnits
-// tiles, by what a row tile may see.
+// Workgroups that share the tokens of a prefill's row tile.  A workgroup alone on a CU takes about
+// 1.7 us a tile of 64 tokens, two 2.5 us (HD 128): `load` row tiles a CU in s slices take about
+// c(load s) / s, c(x) = 1 up to one per CU and 3/4 for each begun one from there, with an end that
+// is not full; the slices' partial sums and their join cost about s 400 / tokens of the whole.
+// Measured (us, 40/8 heads of 128): 32 queries over 16384 tokens 430 in one slice, 47 in 16; 511
+// queries of each of 4 sequences of up to 16001 493 in one, 443 in 2, 446 in 4; a prompt of 8191 825
+// in one, 907 in 2.  Order-preserving as bits: it is positive.
+__host__ __device__ inline float slices_cost(float load, int s, float tokens) {
+#pragma clang fp contract(off)  // every kernel has to choose alike
+  const float x = load * (float)s, c = x <= 1.0f ? 1.0f : 0.75f * __builtin_ceilf(x);
+  return (c + 0.3f) / (float)s + (s > 1 ? 300.0f * x / tokens : 0.0f);
+}
+
+// The slices of a sequence of n tokens: the best number up to a.slices (the best for as many tokens
+// as the table addresses) by what its row tiles may see, none of fewer than kSliceUnits tiles.  Over
+// the lanes of a wavefront, a number each.
 __device__ inline int prefill_slices(const AttendArgs& a, int n) {
+  if (a.slices == 1) return 1;
   int tiles = (n + kTile - 1) / kTile;
-  if (a.window > 0) {  // its rows are at most kPrefillRows tokens
+  if (a.window > 0) {  // a tile's rows are at most kPrefillRows tokens
     const int64_t most = ((int64_t)a.window + a.sinks + kPrefillRows) / kTile + 3;
     tiles = tiles < most ? tiles : (int)most;
   }
-  const int s = (tiles + kSliceUnits - 1) / kSliceUnits;
-  return s < 1 ? 1 : s < a.slices ? s : a.slices;
+  const int top = (tiles + kSliceUnits - 1) / kSliceUnits;
+  const int s = (int)(threadIdx.x & 31) + 1;
+  // the cost's upper bits and the number, the less the better
+  int key = (__float_as_int(slices_cost(a.load, s, (float)(tiles * kTile))) & ~31) | (s - 1);
+  key = s == 1 || (s <= a.slices && s <= top) ? 0x7fffffff - key : 0;
+  return ((0x7fffffff - lane63(wave_prefix(key, Max()))) & 31) + 1;
 }
 
 // The tiles of kTile tokens that the queries of a sequence of n tokens may see, in order: the
