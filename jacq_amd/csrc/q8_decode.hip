@@ -316,7 +316,8 @@ struct Wave {
         f4 sc[NB][4];
         scores(c, sc);
         const float ks = c.there ? c.ks : __builtin_nanf(""), vs = c.vs;
-        if (E4M3 && masked && a.window > 0 && before_window(s, t0 + kq * 16))
+        // a page outside the pool reads as page 0, whose e4m3 codes may be NaN: as before a window
+        if (E4M3 && masked && (!c.there || (a.window > 0 && before_window(s, t0 + kq * 16))))
 #pragma unroll
           for (int d = 0; d < DT; ++d) c.v[d] = u4{0, 0, 0, 0};
         if (next >= 0) load_k(s, nk, c);

@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   auto exists = [&](int page) { return page >= 0 && page < g.num_pages; };
   u4 kc[KC], vc[KC];
   float scale_k = 0, scale_v = 0;
-  bool no_page = false;
+  bool no_page = false, no_v[KC];
   int pk[KC], pv[KC], ps = 0;
   auto pages_k = [&](int u) {
     const int t0 = tile_at(u);
@@ -223,6 +223,7 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
       const int page = uniform(pv[i]);
+      no_v[i] = !exists(page);
       vc[i] = *(const u4*)(a.pool.v_code + (exists(page) ? page : 0) * stride + v_off[i]);
     }
   };
@@ -243,11 +244,12 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
     uint16_t* dst = &lds.v[u & 1][0][0];
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      if (E4M3 && a.window > 0) {
+      if (E4M3) {
         // A page before every row's window may be any, and its e4m3 codes NaN, which a weight of 0
-        // would not take out.
+        // would not take out; so may page 0, read for an entry outside the pool, for rows before it.
         const int t = tile_at(u) + vt[i];
-        if (t + g.page - 1 <= pfirst - a.window && t >= a.sinks) vc[i] = u4{0, 0, 0, 0};
+        if (no_v[i] || (a.window > 0 && t + g.page - 1 <= pfirst - a.window && t >= a.sinks))
+          vc[i] = u4{0, 0, 0, 0};
       }
       *(h8*)(dst + vs0[i]) = codes8<E4M3>(vc[i].x, vc[i].y);
       *(h8*)(dst + vs1[i]) = codes8<E4M3>(vc[i].z, vc[i].w);

@@ -1,0 +1,68 @@
+"""Edges of the 8-bit paged cache's calls, through both attention kernels: the decode's takes few
+rows or few heads, the prompts' the rest, so each size here says which one it is for."""
+from __future__ import annotations
+
+import dataclasses
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import q8_ref as ref  # noqa: E402
+from tests.test_gpu_q8 import I32, check_attention, ints, make, q8, randn, spoil  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+
+def offsets(m):
+    cu = [0]
+    for x in m:
+        cu.append(cu[-1] + x)
+    return cu
+
+
+def runs_prefill(q8, cache, total, max_q):  # noqa: F811
+    """Whether a call without block weights goes to the prompts' kernel: the other one's workspace
+    is as much smaller without them as what they take (under a table so wide that its calls are
+    cut; the choice does not go by the table)."""
+    g = dataclasses.replace(cache.geo, max_pages_per_seq=16384)
+    rows = max_q * g.gqa
+    block = 16 if rows <= 16 else 32
+    weights = (cache.batch * g.num_kv_heads * -(-rows // block) * g.max_pages_per_seq
+               * (g.page_size // 16) * min(rows, block), total * g.num_heads)
+    size = [q8.lib().jacq_q8_attend_workspace_size(g.ref, cache.batch, total, max_q, w)
+            for w in (0, 1)]
+    return size[1] - size[0] != sum(-(-4 * n // 256) * 256 for n in weights)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("heads,m,prompt", [((4, 2, 64), 40, False), ((4, 1, 128), 45, False),
+                                            ((32, 8, 128), 40, True), ((14, 2, 64), 60, True)])
+def test_a_page_outside_the_pool_reaches_no_query_before_it(q8, codes, page, heads, m, prompt):  # noqa: F811
+    """The codes read in its place are page 0's, which may be memory that was never written."""
+    nh, nkv, hd = heads
+    lens = [160 + page + 3, 224 + page + 5, 200]
+    cache, tables, seq = make(q8, nh, nkv, hd, page, codes, lens, seed=page + m)
+    assert runs_prefill(q8, cache, 3 * m, m) == prompt
+    spare = (set(range(cache.geo.num_pages)) - set(tables[tables >= 0].tolist())).pop()
+    for x in (cache.k_code, cache.v_code, cache.k_scale, cache.v_scale):
+        x[spare] = x[0]
+    tables[tables == 0] = spare
+    gen = torch.Generator("cuda").manual_seed(m)
+    q = randn(gen, 3 * m, nh, hd)
+    cu = offsets([m] * 3)
+    clean = cache.prefill(q, ints(*cu), m, seq, tables)
+    check_attention(cache, tables, lens, q, cu, clean)
+    cache.k_code[0], cache.v_code[0] = 0x7F, 0xFF
+    cache.k_scale[0], cache.v_scale[0] = float("inf"), float("nan")
+    # pages in the midst of 64-token tiles, with queries before them in the same tile
+    bad = tables.clone()
+    bad[0, 160 // page], bad[1, 224 // page] = 1 << 30, -7
+    got = cache.prefill(q, ints(*cu), m, seq, bad)
+    for b, first in ((0, 160), (1, 224), (2, lens[2])):
+        sees = torch.arange(lens[b] - m, lens[b], device="cuda") >= first
+        assert b == 2 or 0 < int(sees.sum()) < m
+        rows = slice(cu[b], cu[b + 1])
+        assert bool(got[rows][sees].isnan().all())
+        assert torch.equal(got[rows][~sees], clean[rows][~sees]), b
