@@ -26,6 +26,14 @@ constexpr int kMaxSlices = 32;       // of its slices at most
 // registers allow.
 constexpr int decode_groups(int hd, int nb) { return (hd == 128 ? 4 : 5) - nb; }
 constexpr float kLog2e = 1.4426950408889634f;
+// The weights 2^(t - m) that are rounded to fp16, the type that the matrix cores take at full rate
+// with the most bits: m moves to kLift below a row's largest t, and only where that has passed m by
+// kSlack more.  So they end at 2^15, the largest so far is at least 2^7, and the others keep 11 bits
+// (half a step: 2^-11 of them) down to 2^-14, and are off by at most 2^-25 below.  O loses at most n
+// 2^-32 of the largest |v| in the heaviest's block to that; the sum that divides it is of the
+// unrounded weights, in fp32.
+constexpr float kLift = 7.0f;
+constexpr float kSlack = 8.0f;
 
 struct Geo {
   int nh, nkv, hd, page, page_log2, max_pages, num_pages, gqa, codes;

@@ -12,9 +12,10 @@
 //
 // The V scale is constant over a lane's 16 tokens and enters the exponent:
 //   t = s (ks scale log2e) + log2(vs),  w = 2^(t - m),  O = sum(w v) / sum(w / vs)
-// so the P that is rounded to fp16 is at most 2^kSlack, however the scales
-// differ between blocks, and no accumulator needs a scale of its own.
-// (fp16 holds w to 2^-12; bf16 would hold it to 2^-9.)
+// so no accumulator needs a scale of its own, and the P that is rounded to fp16
+// (kLift has its range; bf16 would be off by 2^-8 of it, fp16 by 2^-11) is at most
+// 2^15.  What it may lose is small next to the block of the largest w, so beside a
+// block of far larger V scale, not next to the values of a smaller one.
 //
 // Bound by memory.  Measured (40/8 heads of 128, int8, page 32): 64 sequences of 1024 to 16384
 // tokens, one query each, 1.16 GB: 215 us and 5 us for the join, 5.3 TB/s, where a copy of 2 GiB
@@ -31,7 +32,6 @@ namespace jacq {
 namespace q8 {
 
 constexpr int kWaves = 4;         // wavefronts of a workgroup: they share a slice, unit by unit
-constexpr float kSlack = 8.0f;    // the running maximum moves only by more than this (base 2)
 constexpr float kNegInf = -__builtin_inff();
 
 // One segment's place: sequence, kv head, row block, and its units' span.
@@ -171,8 +171,8 @@ struct Wave {
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16));
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    if (__ballot(mx > m[nb] + kSlack)) {  // also where m is -inf and mx is not
-      const float to = mx > m[nb] + kSlack ? mx : m[nb];
+    if (__ballot(mx > m[nb] + (kLift + kSlack))) {  // also where m is -inf and mx is not
+      const float to = mx > m[nb] + (kLift + kSlack) ? mx - kLift : m[nb];
       const float f = to > m[nb] ? exp2_(m[nb] - to) : 1.0f;
       m[nb] = to;
       l[nb] *= f;

@@ -33,7 +33,6 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kRows = kPrefillRows;
 static_assert(kRows == 32 * kWaves, "32 a wavefront");
-constexpr float kSlack = 8.0f;  // the running maximum moves only by more than this (base 2)
 constexpr float kNegInf = -__builtin_inff();
 
 template <int HD>
@@ -349,8 +348,8 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
       top = fmaxf(top, __builtin_fmaf(x, ga[k], gb[k]));
     }
     top = fmaxf(top, other_half(top));
-    if (__ballot(top > mx + kSlack)) {
-      const float to = top > mx + kSlack ? top : mx;
+    if (__ballot(top > mx + (kLift + kSlack))) {
+      const float to = top > mx + (kLift + kSlack) ? top - kLift : mx;
       const float f = to > mx ? exp2_(mx - to) : 1.0f;
       mx = to;
       l *= f;

@@ -66,3 +66,38 @@ def test_a_page_outside_the_pool_reaches_no_query_before_it(q8, codes, page, hea
         rows = slice(cu[b], cu[b + 1])
         assert bool(got[rows][sees].isnan().all())
         assert torch.equal(got[rows][~sees], clean[rows][~sees]), b
+
+
+@pytest.mark.parametrize("heads,batch,m", [((4, 1, 64), 512, 1), ((10, 1, 128), 512, 3),
+                                           ((32, 2, 64), 20, 9), ((8, 1, 128), 20, 17)])
+def test_many_light_tokens_weigh_beside_a_heavy_one(q8, heads, batch, m):  # noqa: F811
+    """A first token of 96 % of the weight, in a block of 32 times the others' V scale, and 65536
+    tokens of 2^-20.5 of its weight each: next to the heaviest they are 2^-25.5, and 4 % together.
+    As many sequences of the same pages as leave each to few wavefronts."""
+    nh, nkv, hd = heads
+    page, n = 32, 65536 + 32
+    k = torch.zeros((n, nkv, hd), dtype=torch.float16, device="cuda")
+    k[0, :, 0] = 1.0
+    v = torch.ones((n, nkv, hd), dtype=torch.float16, device="cuda")
+    v[:page] = 0.0
+    v[0, :, 3] = 32.0
+    width = n // page
+    tables = torch.arange(width, **I32).repeat(batch, 1)
+    cache = q8.PagedQ8Cache(q8.Q8Geometry(nh, nkv, hd, page, width, width), batch)
+    cache.sequence_view(0).append(k, v, tables[:1], ints(0), cu_new=ints(0, n))
+    assert runs_prefill(q8, cache, m * batch, m) == (m > 3)
+    q = torch.zeros((m * batch, nh, hd), dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 20.5 * 0.6931471805599453 * hd ** 0.5
+    o = torch.empty((m * batch, nh, hd), device="cuda")
+    lse = torch.empty((m * batch, nh), device="cuda")
+    cache.prefill(q, ints(*offsets([m] * batch)), m, ints(*[n] * batch), tables, out=o, lse=lse)
+    r = ref.attend(q[:m], *ref.held_values(cache, tables, 0, n), n)
+    assert 0.035 < float(r["o"][0, 0, 0]) < 0.05
+    err = ref.score_error(r, hd)
+    # half a step of the weights, relative; 2^-32 of the heaviest's block each; the scores' error
+    tol = (2.0 ** -24 * r["o"].abs() + (2.0 ** -11 + err[..., None]) * r["abs"]
+           + n * 2.0 ** -32 * r["vmax"])
+    for b in range(batch):
+        rows = slice(b * m, b * m + m)
+        ref.assert_within(o[rows], r["o"], tol)
+        ref.assert_within(lse[rows], r["lse"], err + 2.0 ** -22 * (1 + r["lse"].abs()))
