@@ -107,7 +107,9 @@ int jacq_q8_append(const jacq_q8_geometry* geo, const jacq_q8_pool* pool, const 
  *            times what it held (decay 0 overwrites) plus the softmax weight
  *            of its tokens summed over the sequence's queries and heads;
  *            at most JACQ_Q8_MAX_WEIGHTED_QUERIES queries per sequence
- *   max_q    no sequence has more queries than this (more are left alone)
+ *   max_q    no sequence has more queries than this (of one that has, the
+ *            first max_q are computed, at their own positions; the others are
+ *            left alone)
  * Rows of Q and O outside every sequence's queries are not touched.  The
  * workspace needs no particular contents; calls that can run at the same time
  * must not share one. */

@@ -160,17 +160,19 @@ __device__ inline int clamp_len(const Geo& g, int n) {
   return n < 0 ? 0 : n > cap ? cap : n;
 }
 
-// Queries of sequence b: rows [q0, q0 + m) of Q, whatever the table of offsets holds.
-__device__ inline void queries_of(const AttendArgs& a, int b, int* q0, int* m) {
+// Queries of sequence b: rows [q0, q0 + m) of Q, whatever the table of offsets holds.  m is at most
+// max_q; `all` are the sequence's own, which its last tokens are.
+__device__ inline void queries_of(const AttendArgs& a, int b, int* q0, int* m, int* all) {
   if (!a.cu) {
     *q0 = b;
-    *m = 1;
+    *m = *all = 1;
     return;
   }
   int lo = a.cu[b], hi = a.cu[b + 1];
   lo = lo < 0 ? 0 : lo > a.total_q ? a.total_q : lo;
   hi = hi < lo ? lo : hi > a.total_q ? a.total_q : hi;
   *q0 = lo;
+  *all = hi - lo;
   *m = hi - lo > a.max_q ? a.max_q : hi - lo;
 }
 
@@ -209,15 +211,16 @@ __device__ inline int prefill_slices(const AttendArgs& a, int n) {
 // sinks' tiles, the window's, then the tail (fp16) as a unit of its own.
 struct Span {
   int n;        // tokens
+  int first;    // the lowest position of a query (may be negative)
   int nq;       // of them quantised
   int w0;       // first tile of the window
   int ns;       // tiles of the sinks before it
   int tiles;    // quantised tiles in all
   int units;    // units of a segment, at least 1 (a segment without tokens still writes its zeros)
   __device__ Span() {}
-  // first: the lowest position of a query (may be negative)
-  __device__ Span(const Geo& g, int n_, int first, int window, int sinks) {
+  __device__ Span(const Geo& g, int n_, int first_, int window, int sinks) {
     n = n_;
+    first = first_;
     nq = n >> g.page_log2 << g.page_log2;
     tiles = (nq + kTile - 1) / kTile;
     w0 = ns = 0;

@@ -74,7 +74,7 @@ struct Wave {
       const int row = s.rb * 16 * NB + nb * 16 + n16;
       const int tok = row / g.gqa, head = s.h * g.gqa + row % g.gqa;
       const bool ok = tok < s.m;
-      pos[nb] = ok ? s.span.n - s.m + tok : -1;
+      pos[nb] = ok ? s.span.first + tok : -1;
       m[nb] = kNegInf;
       l[nb] = 0.0f;
 #pragma unroll
@@ -205,8 +205,8 @@ struct Wave {
 
   __device__ bool needs_mask(const Segment& s, int t0, int end) const {
     // uniform: the tile's 64 tokens are all there and every row sees them
-    const int first = s.span.n - s.m + s.rb * 16 * NB / g.gqa;
-    const int last = s.span.n - s.m + (s.rb * 16 * NB + s.nrows - 1) / g.gqa;
+    const int first = s.span.first + s.rb * 16 * NB / g.gqa;
+    const int last = s.span.first + (s.rb * 16 * NB + s.nrows - 1) / g.gqa;
     return t0 + kTile > end || t0 + kTile - 1 > first ||
            (a.window > 0 && t0 <= last - a.window && t0 + kTile > a.sinks);
   }
@@ -214,7 +214,7 @@ struct Wave {
   // No row sees the 16 tokens from t on, as their windows begin later: their page may be any, and
   // its e4m3 codes NaN, which a weight of 0 would not take out.
   __device__ bool before_window(const Segment& s, int t) const {
-    const int first = s.span.n - s.m + s.rb * 16 * NB / g.gqa;
+    const int first = s.span.first + s.rb * 16 * NB / g.gqa;
     return t + 15 <= first - a.window && t >= a.sinks;
   }
 
@@ -371,9 +371,10 @@ __device__ inline void finish_row(const Geo& g, const AttendArgs& a, const Segme
 template <int ROWS>
 __device__ inline void sequence_span(const Geo& g, const AttendArgs& a, int b, int* q0, int* m,
                                      Span* span, int* blocks) {
-  queries_of(a, b, q0, m);
+  int all;
+  queries_of(a, b, q0, m, &all);
   const int n = clamp_len(g, a.lens[b]);
-  *span = Span(g, n, n - *m, a.window, a.sinks);
+  *span = Span(g, n, n - all, a.window, a.sinks);
   *blocks = (*m * g.gqa + ROWS - 1) / ROWS;
 }
 

@@ -92,8 +92,8 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   const int b = blockIdx.y, h = blockIdx.x % g.nkv;
   const int rt = tiles - 1 - (int)blockIdx.x / g.nkv;  // the longest first
   const int slice = blockIdx.z;
-  int q0, m;
-  queries_of(a, b, &q0, &m);
+  int q0, m, all;
+  queries_of(a, b, &q0, &m, &all);
   q0 = uniform(q0);
   m = uniform(m);
   const int rows = m * g.gqa;
@@ -101,19 +101,20 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   const int n = uniform(clamp_len(g, a.lens[b]));
   const int slices = uniform(prefill_slices(a, n));
   if (slice >= slices) return;
-  // positions of the workgroup's and the wavefront's rows
+  // positions: the first query's, then the workgroup's and the wavefront's rows
+  const int p0 = n - uniform(all);
   const int end_row = rows < (rt + 1) * kRows ? rows : (rt + 1) * kRows;
-  const int pfirst = uniform(n - m + rt * kRows / g.gqa);
-  const int plast = uniform(n - m + (end_row - 1) / g.gqa);
+  const int pfirst = uniform(p0 + rt * kRows / g.gqa);
+  const int plast = uniform(p0 + (end_row - 1) / g.gqa);
   const int wr0 = rt * kRows + wave * 32;
   const int wr1 = wr0 + 32 < rows ? wr0 + 32 : rows;
-  const int wfirst = uniform(n - m + wr0 / g.gqa);
-  const int wlast = uniform(wr0 < rows ? n - m + (wr1 - 1) / g.gqa : -1);
+  const int wfirst = uniform(p0 + wr0 / g.gqa);
+  const int wlast = uniform(wr0 < rows ? p0 + (wr1 - 1) / g.gqa : -1);
 
   const int row = wr0 + n32;
   const bool ok = row < rows;
   const int tok = ok ? row / g.gqa : 0, head = h * g.gqa + row % g.gqa;
-  const int pos = ok ? n - m + tok : -1;
+  const int pos = ok ? p0 + tok : -1;
   h8 q[KS];
   float qs = a.scale, mx = kNegInf, l = 0.0f;
   f16v acc[DT];
@@ -458,8 +459,8 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
 // Joins the slices of every row, in their order: a thread per 4 channels.  blockIdx.y: sequence.
 template <int HD>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Geo g, AttendArgs a) {
-  int q0, m;
-  queries_of(a, blockIdx.y, &q0, &m);
+  int q0, m, all;
+  queries_of(a, blockIdx.y, &q0, &m, &all);
   const int slices = prefill_slices(a, clamp_len(g, a.lens[blockIdx.y]));
   if (slices == 1) return;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

@@ -409,9 +409,10 @@ class PagedQ8Cache:
         """q [tokens, NH, HD]: rows cu_q[b] to cu_q[b + 1] (cu_q [batch + 1] int32) are the last
         tokens of sequence b, whose seq_lens[b] tokens are all in the cache; each sees the
         tokens up to its own, or the window and sinks of ``decode``.  No sequence has more than
-        max_q.  Rows outside every sequence are left as they are (undefined in a fresh
-        output).  weights, as in ``decode``, take at most 64 queries per sequence: the last
-        ones of a prompt, in a call of their own."""
+        max_q: of one that has, the rows after its first max_q are left as they are, and so
+        are rows outside every sequence (undefined in a fresh output).  weights, as in
+        ``decode``, take at most 64 queries per sequence: the last ones of a prompt, in a call
+        of their own."""
         _check(cu_q is not None, "CU_Q must be given")
         _check(max_q >= 0, "MAX_Q must not be negative")
         return self._attend(q, cu_q, int(max_q), seq_lens, block_tables, window, sinks, scale,

@@ -101,3 +101,36 @@ def test_many_light_tokens_weigh_beside_a_heavy_one(q8, heads, batch, m):  # noq
         rows = slice(b * m, b * m + m)
         ref.assert_within(o[rows], r["o"], tol)
         ref.assert_within(lse[rows], r["lse"], err + 2.0 ** -22 * (1 + r["lse"].abs()))
+
+
+@pytest.mark.parametrize("heads,most", [((10, 2, 128), 3), ((8, 2, 64), 20), ((32, 8, 128), 70),
+                                        ((14, 2, 64), 80)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (50, 3)])
+def test_queries_past_max_q_leave_the_others_where_they_stand(q8, heads, most, window, sinks):  # noqa: F811
+    nh, nkv, hd = heads
+    lens, ms = [300, 40, 1000], [most + 50, 1, most]
+    cache, tables, seq = make(q8, nh, nkv, hd, 32, "e4m3", lens, seed=most)
+    spoil(cache, tables, lens)
+    gen = torch.Generator("cuda").manual_seed(most + 1)
+    cu = offsets(ms)
+    q = randn(gen, cu[-1], nh, hd)
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((cu[-1], nh), 7.0, device="cuda")
+    names = dict(window=window, sinks=sinks)
+    assert runs_prefill(q8, cache, cu[-1], most) == (most >= 70)
+    cache.prefill(q, ints(*cu), most, seq, tables, out=out, lse=lse, **names)
+    want = cache.prefill(q, ints(*cu), max(ms), seq, tables, **names)
+    check_attention(cache, tables, lens, q, cu, want, **names)
+    assert bool((out[most:cu[1]] == 7).all()) and bool((lse[most:cu[1]] == 7).all())
+    out[most:cu[1]] = want[most:cu[1]]
+    k, v = ref.held_values(cache, tables, 0, 300)
+    lse[most:cu[1]] = ref.attend(q[:cu[1]], k, v, 300, window, sinks)["lse"][most:].float()
+    check_attention(cache, tables, lens, q, cu, out, lse, **names)
+    if most <= 64:
+        w = torch.empty((3, cache.geo.max_pages_per_seq), device="cuda")
+        cache.prefill(q, ints(*cu), most, seq, tables, weights=w, decay=0.0, **names)
+        r = ref.attend(q[:cu[1]], k, v, 300, window, sinks)
+        sums = r["p"][:, :most].sum((0, 1, 2))
+        sums = torch.cat((sums, sums.new_zeros(20))).view(-1, 32).sum(1)
+        ref.assert_within(w[0, :10], sums, (float(ref.score_error(r, hd).max()) + 2.0 ** -14) * sums
+                          + 2.0 ** -100)
