@@ -302,8 +302,10 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
                                         std::to_string(x->max_q));
     const int64_t row = (int64_t)geo->num_heads * geo->head_dim;
     if (int e = check_stride(x->q_stride, row, "Q")) return e;
-    if (x->batch == 0 || x->total_q == 0 || x->max_q == 0) return JACQ_KIVI_OK;
-    if (!x->Q || !x->O || !x->SEQ_LENS || !x->BLOCK_TABLES)
+    if (x->batch == 0) return JACQ_KIVI_OK;
+    const bool none = x->total_q == 0 || x->max_q == 0;  // then there are offsets, not one query each
+    if (none && !x->WEIGHTS) return JACQ_KIVI_OK;
+    if (!x->SEQ_LENS || (!none && (!x->Q || !x->O || !x->BLOCK_TABLES)))
       return fail(JACQ_KIVI_EINVAL, "a tensor pointer is null");
     if (!aligned({x->Q, x->O, workspace}, 16) ||
         !aligned({x->CU_Q, x->SEQ_LENS, x->BLOCK_TABLES, x->LSE, x->WEIGHTS}, 4))
@@ -329,6 +331,10 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.sinks = std::min(x->sinks, 1 << 30);
     a.scale = x->scale * jacq::q8::kLog2e;
     a.decay = x->decay;
+    if (none) {
+      a.groups = g.max_pages * (g.page / 16);
+      return launched(jacq::q8::launch_decay(g, a, stream), "decay");
+    }
     const Plan p = plan_attend(g, a.batch, a.total_q, a.max_q, a.weights != nullptr);
     if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 ||
         (int64_t)a.batch * g.nkv * std::max(1, p.row_blocks) > INT32_MAX)

@@ -246,6 +246,7 @@ hipError_t launch_read(const Geo& g, const Pool& p, const int32_t* starts, const
                        const int32_t* tables, int batch, int total, void* k, void* v, int type,
                        hipStream_t s);
 hipError_t launch_decode(const Geo& g, const AttendArgs& a, int nb, hipStream_t s);
+hipError_t launch_decay(const Geo& g, const AttendArgs& a, hipStream_t s);  // of a call of no queries
 hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s);
 int prefill_tiles(const Geo& g, int max_q);  // workgroups of a kv head and slice
 hipError_t launch_evict(const Geo& g, const float* w, const int32_t* lens, const int32_t* tables,

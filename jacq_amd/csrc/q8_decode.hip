@@ -758,6 +758,13 @@ static void decode_kernels(const Geo& g, const AttendArgs& a, hipStream_t s) {
                        g, a);
 }
 
+// A call of no queries: max_q is 0, so no segment adds anything and the weights decay.
+hipError_t launch_decay(const Geo& g, const AttendArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((q8_weights_kernel<1>), dim3((a.groups + 63) / 64, a.batch), dim3(256), 0, s, g,
+                     a);
+  return hipGetLastError();
+}
+
 template <int HD, bool E4M3>
 static void decode_rows(const Geo& g, const AttendArgs& a, int nb, hipStream_t s) {
   if (nb == 1) decode_kernels<HD, E4M3, 1>(g, a, s);

@@ -134,3 +134,23 @@ def test_queries_past_max_q_leave_the_others_where_they_stand(q8, heads, most, w
         sums = torch.cat((sums, sums.new_zeros(20))).view(-1, 32).sum(1)
         ref.assert_within(w[0, :10], sums, (float(ref.score_error(r, hd).max()) + 2.0 ** -14) * sums
                           + 2.0 ** -100)
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.5, 1.0])
+def test_weights_decay_in_a_call_of_no_queries(q8, decay):  # noqa: F811
+    """As those of a sequence without queries do beside one that has some."""
+    cache, tables, seq = make(q8, 10, 2, 64, 32, "int8", [300, 40], seed=3)
+    gen = torch.Generator("cuda").manual_seed(4)
+    held = torch.rand((2, cache.geo.max_pages_per_seq), generator=gen, device="cuda")
+    q = randn(gen, 2, 10, 64)
+    want = held.clone()
+    cache.prefill(q, ints(0, 0, 2), 2, seq, tables, weights=want, decay=decay)
+    want[1] = decay * held[1]
+    for rows, most in ((q[:0], 5), (q[:0], 0), (q, 0)):
+        w = held.clone()
+        if decay == 0.0:
+            w[0, 0] = float("nan")
+        out = torch.full((rows.shape[0], 10, 64), 7.0, dtype=torch.float16, device="cuda")
+        cache.prefill(rows, ints(0, 0, rows.shape[0]), most, seq, tables, weights=w, decay=decay,
+                      out=out)
+        assert torch.equal(w, want) and bool((out == 7).all())
