@@ -190,8 +190,8 @@ class PagedQ8Cache:
             check_shape(t[n], shape, n)
             _check(t[n].dtype == dtype and t[n].is_contiguous(), n, " must be contiguous ", dtype)
             _check(t[n].device == t["k_code"].device, n, " must be on the device of k_code")
-            setattr(self, n, t[n])
-        self.geo, self.batch, self.device = geo, batch, t["k_code"].device
+        vars(self).update({n: t[n] for n in POOL}, geo=geo)
+        self.batch, self.device = batch, t["k_code"].device
         self._index = self.device.index if self.device.type == "cuda" else -1
         self._record = _Pool(*(t[n].data_ptr() for n in POOL))
         self._pool = ctypes.byref(self._record)
@@ -199,6 +199,19 @@ class PagedQ8Cache:
         self._q_row, self._kv_row = (g.num_heads, g.head_dim), (g.num_kv_heads, g.head_dim)
         self._lens_shape, self._table_shape = (batch,), (batch, g.max_pages_per_seq)
         self._sizes = {}
+
+    def __setattr__(self, name: str, value) -> None:
+        """Another tensor in a tensor's place, or another geometry: checked, and what the calls
+        hold goes by it."""
+        if (name in POOL or name == "geo") and name in vars(self):
+            t = {n: getattr(self, n) for n in POOL}
+            if name == "geo":
+                value.check()
+                self._set(value, t)
+            else:
+                self._set(self.geo, {**t, name: value})
+        else:
+            object.__setattr__(self, name, value)
 
     def sequence_view(self, b: int) -> "PagedQ8Cache":
         """A one-sequence cache sharing this cache's pool and sequence b's tail."""

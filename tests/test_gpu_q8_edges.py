@@ -154,3 +154,20 @@ def test_weights_decay_in_a_call_of_no_queries(q8, decay):  # noqa: F811
         cache.prefill(rows, ints(0, 0, rows.shape[0]), most, seq, tables, weights=w, decay=decay,
                       out=out)
         assert torch.equal(w, want) and bool((out == 7).all())
+
+
+def test_a_tensor_put_in_the_place_of_another_is_the_one_used(q8):  # noqa: F811
+    cache, tables, seq = make(q8, 4, 2, 64, 16, "int8", [37, 20], seed=8)
+    gen = torch.Generator("cuda").manual_seed(9)
+    k, v, q = randn(gen, 2, 2, 64), randn(gen, 2, 2, 64), randn(gen, 2, 4, 64)
+    before = cache.decode(q, seq, tables)
+    for name in ("k_tail", "v_tail", "k_code"):
+        old = getattr(cache, name)
+        keep = old.clone()
+        setattr(cache, name, keep)
+        old.fill_(1)  # nothing reads it any more
+    assert torch.equal(cache.decode(q, seq, tables), before)
+    cache.append(k, v, tables, seq)
+    assert torch.equal(cache.k_tail[0, :, 5], k[0]) and torch.equal(cache.v_tail[1, :, 4], v[1])
+    got = cache.decode(q, seq + 1, tables)
+    check_attention(cache, tables, [38, 21], q, [0, 1, 2], got)

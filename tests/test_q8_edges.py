@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from jacq_amd import kivi, q8  # noqa: E402,F401
-from tests.test_q8 import EINVAL, Record, error  # noqa: E402
+from tests.test_q8 import EINVAL, GOOD, Record, error  # noqa: E402
 
 
 def test_a_call_of_no_queries_with_weights_is_checked():
@@ -14,3 +14,30 @@ def test_a_call_of_no_queries_with_weights_is_checked():
         error(Record().attend(WEIGHTS=0x60000, SEQ_LENS=0, **kw), EINVAL, "null")
         error(Record().attend(WEIGHTS=0x60002, Q=0, O=0, **kw), EINVAL, "4-byte")
         assert Record().attend(Q=0, O=0, SEQ_LENS=0, **kw) == 0
+
+
+@pytest.fixture
+def cache():
+    return q8.PagedQ8Cache(q8.Q8Geometry(**GOOD), 3, device="cpu")
+
+
+def held(c):
+    """The addresses that a call of this cache passes."""
+    return tuple(getattr(c._record, n) for n in q8.POOL)
+
+
+def test_calls_take_the_tensors_that_a_cache_holds_now(cache):
+    for name in q8.POOL:
+        new = getattr(cache, name).clone()
+        setattr(cache, name, new)
+        assert getattr(cache, name) is new
+        assert held(cache) == tuple(t.data_ptr() for t in cache.pool())
+        for bad in (new[:, :1], new.to(torch.float64)):
+            with pytest.raises(kivi.KiviCheckError, match=name):
+                setattr(cache, name, bad)
+        assert getattr(cache, name) is new  # as it was
+        assert held(cache) == tuple(t.data_ptr() for t in cache.pool())
+    with pytest.raises(kivi.KiviCheckError, match="k_code"):
+        cache.geo = q8.Q8Geometry(**{**GOOD, "num_pages": 17})
+    cache.geo = q8.Q8Geometry(**{**GOOD, "max_pages_per_seq": 9})
+    assert cache._table_shape == (3, 9)
