@@ -213,6 +213,13 @@ class PagedQ8Cache:
         else:
             object.__setattr__(self, name, value)
 
+    def __getstate__(self):  # copies and pickles carry the tensors, not their addresses
+        return {n: getattr(self, n) for n in ("geo", *POOL)}
+
+    def __setstate__(self, state: dict) -> None:
+        state["geo"].check()
+        self._set(state["geo"], state)
+
     def sequence_view(self, b: int) -> "PagedQ8Cache":
         """A one-sequence cache sharing this cache's pool and sequence b's tail."""
         t = {n: getattr(self, n) for n in POOL}

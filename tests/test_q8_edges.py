@@ -1,6 +1,9 @@
 """Edges of the 8-bit cache's host side, without a GPU."""
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -41,3 +44,16 @@ def test_calls_take_the_tensors_that_a_cache_holds_now(cache):
         cache.geo = q8.Q8Geometry(**{**GOOD, "num_pages": 17})
     cache.geo = q8.Q8Geometry(**{**GOOD, "max_pages_per_seq": 9})
     assert cache._table_shape == (3, 9)
+
+
+def test_copies_and_pickles_hold_tensors_of_their_own(cache):
+    cache.k_code.random_(0, 255)
+    for make, shared in ((copy.copy, True), (copy.deepcopy, False),
+                         (lambda c: pickle.loads(pickle.dumps(c)), False)):
+        other = make(cache)
+        assert other.geo == cache.geo and other.batch == 3
+        assert all(torch.equal(a, b) for a, b in zip(other.pool(), cache.pool()))
+        assert held(other) == tuple(t.data_ptr() for t in other.pool())
+        assert (held(other) == held(cache)) == shared
+    view = copy.deepcopy(cache.sequence_view(1))
+    assert view.batch == 1 and held(view)[0] != held(cache)[0]
