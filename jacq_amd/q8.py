@@ -180,6 +180,7 @@ class PagedQ8Cache:
     def _set(self, geo: Q8Geometry, t: dict) -> None:
         g = geo
         batch = t["k_tail"].shape[0]
+        _check(batch >= 1, "batch must be positive")
         codes = (g.num_pages, g.num_kv_heads)
         want = {"k_code": ((*codes, g.page_size, g.head_dim), torch.uint8),
                 "v_code": ((*codes, g.head_dim, g.page_size), torch.uint8),
@@ -222,6 +223,7 @@ class PagedQ8Cache:
 
     def sequence_view(self, b: int) -> "PagedQ8Cache":
         """A one-sequence cache sharing this cache's pool and sequence b's tail."""
+        _check(0 <= b < self.batch, "a sequence must be in [0, ", self.batch, "), got ", b)
         t = {n: getattr(self, n) for n in POOL}
         t["k_tail"], t["v_tail"] = self.k_tail[b:b + 1], self.v_tail[b:b + 1]
         return PagedQ8Cache.from_tensors(self.geo, t)

@@ -57,3 +57,13 @@ def test_copies_and_pickles_hold_tensors_of_their_own(cache):
         assert (held(other) == held(cache)) == shared
     view = copy.deepcopy(cache.sequence_view(1))
     assert view.batch == 1 and held(view)[0] != held(cache)[0]
+
+
+def test_a_view_of_no_sequence_is_refused(cache):
+    for b in (-1, 3, 1 << 40):
+        with pytest.raises(kivi.KiviCheckError, match="sequence must be in"):
+            cache.sequence_view(b)
+    t = dict(zip(q8.POOL, cache.pool()))
+    with pytest.raises(kivi.KiviCheckError, match="batch"):
+        q8.PagedQ8Cache.from_tensors(cache.geo, {**t, "k_tail": t["k_tail"][:0],
+                                                 "v_tail": t["v_tail"][:0]})
