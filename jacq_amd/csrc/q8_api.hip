@@ -159,22 +159,33 @@ struct Plan {
 };
 
 // A prefill's slices, for as many tokens as the table addresses: the kernels use fewer for
-// sequences of fewer (slices_cost, which has the reasons).
+// sequences of fewer (slices_cost, which has the reasons).  One, unless more promise 3 % at least:
+// where a CU has many row tiles the promise is no more than a fuller last round, and the slices that
+// are not used and the merge cost more (64 prompts of 100 to 500 tokens under a table of 65536, 32/8
+// heads of 128, 18.8 tiles a CU: 227 us in up to 4 slices, 190 in one).
 int plan_slices(float load, int64_t tokens) {
   const int most =
       (int)std::min<int64_t>(jacq::q8::kMaxSlices, tokens / (jacq::q8::kSliceUnits * jacq::q8::kTile));
+  auto cost = [&](int s) { return jacq::q8::slices_cost(load, s, (float)tokens); };
   int best = 1;
   for (int s = 2; s <= most; ++s)
-    if (jacq::q8::slices_cost(load, s, (float)tokens) <
-        jacq::q8::slices_cost(load, best, (float)tokens))
-      best = s;
-  return best;
+    if (cost(s) < cost(best)) best = s;
+  return cost(best) < 0.97f * cost(1) ? best : 1;
 }
 
 Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted) {
   Plan p = {};
   const int64_t rows = (int64_t)max_q * g.gqa;
-  p.prefill = !weighted && rows > kFewRows && (int64_t)batch * max_q * g.nh > kFewHeads;
+  // The call's queries, not max_q for every sequence: of a cache's sequences some may have none.
+  const int64_t queries = std::min<int64_t>((int64_t)batch * max_q, total_q);
+  // Their row tiles, or blocks of so many rows: of as few sequences as they can be of, and a begun
+  // one more for each but the first, as most calls of several are ragged.
+  auto blocks = [&](int64_t block) {
+    const int64_t each = (rows + block - 1) / block, full = queries / max_q, rest = queries % max_q;
+    return std::min(batch * each, full * each + (rest * g.gqa + block - 1) / block +
+                                      full + (rest > 0) - 1);
+  };
+  p.prefill = !weighted && rows > kFewRows && queries * g.nh > kFewHeads;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -182,8 +193,7 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
     return here;
   };
   if (p.prefill) {
-    p.load = (float)jacq::q8::prefill_tiles(g, max_q) * (float)g.nkv * (float)batch /
-             (float)device_cus();
+    p.load = (float)(blocks(jacq::q8::kPrefillRows) * g.nkv) / (float)device_cus();
     p.slices = plan_slices(p.load, (int64_t)g.max_pages * g.page);
     if (p.slices > 1) {
       const size_t rows_all = (size_t)p.slices * total_q * g.nh;
@@ -203,7 +213,7 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
     const int64_t slots = (int64_t)jacq::q8::decode_groups(g.hd, p.nb) * device_cus();
     // one round of workgroups where the segments' last slices are at most a sixth of it, else two:
     // with one, 16 sequences of 1000 to 8000, 32/32 heads of 128, take 116 us instead of 111
-    p.target = (int)(3 * segments <= slots ? slots : 2 * slots);
+    p.target = (int)(3 * blocks(16 * p.nb) * g.nkv <= slots ? slots : 2 * slots);
   }
   const size_t parts = p.target ? (size_t)p.target + segments : 0;
   p.ml = take(parts * p.rows * 2 * sizeof(float));
@@ -214,6 +224,13 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
   p.row_lse = take(weighted ? (size_t)total_q * g.nh * sizeof(float) : 0);
   p.bytes = at;
   return p;
+}
+
+// As many units as Place may give to the call's queries.
+int64_t place_units(const AttendArgs& a, int per, int log2) {
+  const int64_t of_all = ((int64_t)a.total_q * per >> log2) + a.batch;
+  const int64_t each = ((int64_t)a.max_q * per + (1 << log2) - 1) >> log2;
+  return a.batch <= jacq::q8::kCounted ? std::min(of_all, a.batch * each) : of_all;
 }
 
 }  // namespace
@@ -350,6 +367,13 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.row_lse = a.weights ? (float*)(ws + p.row_lse) : nullptr;
     a.slices = p.slices;
     a.load = p.load;
+    const int64_t tiles = place_units(a, g.gqa, jacq::q8::kRowsLog2);
+    const int64_t merges = p.slices > 1 ? place_units(a, g.nh, jacq::q8::merge_log2(g.hd)) : 0;
+    // a launch has fewer than 2^32 threads
+    if (p.prefill && std::max(tiles * g.nkv, merges) >= 1 << 24)
+      return fail(JACQ_KIVI_EINVAL, "too many query rows in one call");
+    a.tiles = (unsigned)tiles;
+    a.merges = (unsigned)merges;
     if (p.prefill) return launched(jacq::q8::launch_prefill(g, a, stream), "prefill");
     a.target = p.target;
     a.cus = device_cus();

@@ -19,7 +19,8 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kFloor = 0x1p-24f;   // a block's largest magnitude counts as at least this
 constexpr float kHalfMax = 65504.0f;
 constexpr int kTile = 64;            // tokens per step of the attention kernels
-constexpr int kPrefillRows = 128;    // query rows of a workgroup of the prefill kernel
+constexpr int kRowsLog2 = 7;
+constexpr int kPrefillRows = 1 << kRowsLog2;  // query rows of a workgroup of the prefill kernel
 constexpr int kSliceUnits = 8;       // tiles of one of its slices at least
 constexpr int kMaxSlices = 32;       // of its slices at most
 // Workgroups of the decode kernel that a CU holds (a wavefront of each a SIMD), by what its
@@ -87,6 +88,7 @@ struct AttendArgs {
   int groups;             // 16-token groups a table addresses
   int slices;             // prefill: workgroups that share a row tile's tokens, at most
   float load;             // row tiles a CU
+  unsigned tiles, merges; // prefill: its units of row tiles, and its merge's (Place)
 };
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -176,6 +178,60 @@ __device__ inline void queries_of(const AttendArgs& a, int b, int* q0, int* m, i
   *m = hi - lo > a.max_q ? a.max_q : hi - lo;
 }
 
+// Where a prefill's workgroup, or one of its merge, works.  A unit is 2^log2 rows of a sequence, `per`
+// a query; the sequences' units follow each other, so a call's go by its queries and not by its
+// sequences times max_q.  A unit of no rows is little work, but such units between the others leave
+// those to few of a chiplet's engines (300 sequences of 1000 tokens with a query each, 40/8 heads of
+// 128, under max_q 26 and 100, so with 1 and 3 empty ones each: 361 and 697 us, 217 and 237 without).
+// Over the lanes of a wavefront alike, a sequence each.  Up to 64 sequences every one's units are
+// counted; of more, one's units begin at (cu[b] per >> log2) + b, which leaves it as many as its rows
+// begin or one more, and its sequence is found in every 64th offset first.
+constexpr int kCounted = 64;
+struct Place {
+  int b, q0, m, all;  // sequence, and queries_of it
+  int n;              // its tokens
+  int at;             // which of its units; below 0: none
+};
+__device__ inline Place place_of(const Geo& g, const AttendArgs& a, int unit, int per, int log2) {
+  const int lane = threadIdx.x & 63;
+  auto offset = [&](int b) {
+    const int x = a.cu[b];
+    return x < 0 ? 0 : x > a.total_q ? a.total_q : x;
+  };
+  auto first = [&](int b, int q) { return ((int64_t)q * per >> log2) + b; };
+  int at = 0, n = a.batch;
+  while (n > 64) {
+    const int step = (n + 63) / 64, i = lane * step;
+    const int past = __popcll(__ballot(i < n && first(at + i, offset(at + (i < n ? i : 0))) <= unit));
+    const int skip = past > 0 ? (past - 1) * step : 0;
+    at += skip;
+    n = step < n - skip ? step : n - skip;
+  }
+  const int b = at + (lane < n ? lane : n - 1), lo = offset(b), len = clamp_len(g, a.lens[b]);
+  int hi = offset(b + 1);
+  hi = hi < lo ? lo : hi;
+  const int m = hi - lo > a.max_q ? a.max_q : hi - lo;
+  int begin;
+  uint64_t here;  // the last lane of these has the unit
+  if (a.batch <= kCounted) {
+    const int units = lane < n ? (int)(((int64_t)m * per + (1 << log2) - 1) >> log2) : 0;
+    begin = wave_prefix(units, Sum()) - units;
+    here = __ballot(unit >= begin && unit - begin < units);
+  } else {
+    begin = (int)first(b, lo);
+    here = __ballot(lane < n && begin <= unit);
+  }
+  const int l = here ? 63 - __builtin_clzll(here) : 0;
+  Place p;
+  p.b = uniform(at + l);
+  p.q0 = __builtin_amdgcn_readlane(lo, l);
+  p.all = __builtin_amdgcn_readlane(hi, l) - p.q0;
+  p.m = __builtin_amdgcn_readlane(m, l);
+  p.n = __builtin_amdgcn_readlane(len, l);
+  p.at = here ? unit - __builtin_amdgcn_readlane(begin, l) : -1;
+  return p;
+}
+
 // Workgroups that share the tokens of a prefill's row tile.  A workgroup alone on a CU takes about
 // 1.7 us a tile of 64 tokens, two 2.5 us (HD 128): `load` row tiles a CU in s slices take about
 // c(load s) / s, c(x) = 1 up to one per CU and 3/4 for each begun one from there, with an end that
@@ -248,7 +304,8 @@ hipError_t launch_read(const Geo& g, const Pool& p, const int32_t* starts, const
 hipError_t launch_decode(const Geo& g, const AttendArgs& a, int nb, hipStream_t s);
 hipError_t launch_decay(const Geo& g, const AttendArgs& a, hipStream_t s);  // of a call of no queries
 hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s);
-int prefill_tiles(const Geo& g, int max_q);  // workgroups of a kv head and slice
+// (query, head) rows of a workgroup of the prefill's merge: a thread per 4 channels, 256 threads
+constexpr int merge_log2(int hd) { return hd == 128 ? 3 : 4; }
 hipError_t launch_evict(const Geo& g, const float* w, const int32_t* lens, const int32_t* tables,
                         int batch, int keep, int sink, int recent, int32_t* tables_out,
                         int32_t* lens_out, float* w_out, int32_t* evicted, hipStream_t s);

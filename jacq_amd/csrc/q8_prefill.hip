@@ -81,7 +81,7 @@ __device__ inline uint64_t low_bits(int n) {
 }
 
 template <int HD, bool E4M3>
-__global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendArgs a, int tiles) {
+__global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendArgs a) {
   constexpr int KS = HD / 16;                        // k-steps of S^T
   constexpr int DT = HD / 32;                        // channel tiles
   constexpr int KC = kTile * HD / 16 / kThreads;     // 16-code chunks of K (and of V) a thread stages
@@ -89,20 +89,16 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
   Lds<HD>& lds = *(Lds<HD>*)shared_bytes;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int n32 = lane & 31, hh = lane >> 5;
-  const int b = blockIdx.y, h = blockIdx.x % g.nkv;
-  const int rt = tiles - 1 - (int)blockIdx.x / g.nkv;  // the longest first
-  const int slice = blockIdx.z;
-  int q0, m, all;
-  queries_of(a, b, &q0, &m, &all);
-  q0 = uniform(q0);
-  m = uniform(m);
-  const int rows = m * g.gqa;
-  if (rt * kRows >= rows) return;
-  const int n = uniform(clamp_len(g, a.lens[b]));
+  const int h = blockIdx.x % g.nkv, slice = blockIdx.y;
+  const Place place = place_of(g, a, blockIdx.x / g.nkv, g.gqa, kRowsLog2);
+  const int b = place.b, q0 = place.q0, n = place.n;
+  const int rows = place.m * g.gqa;
+  const int rt = (rows + kRows - 1) / kRows - 1 - place.at;  // the longest first
+  if (rt < 0 || place.at < 0) return;
   const int slices = uniform(prefill_slices(a, n));
   if (slice >= slices) return;
   // positions: the first query's, then the workgroup's and the wavefront's rows
-  const int p0 = n - uniform(all);
+  const int p0 = n - place.all;
   const int end_row = rows < (rt + 1) * kRows ? rows : (rt + 1) * kRows;
   const int pfirst = uniform(p0 + rt * kRows / g.gqa);
   const int plast = uniform(p0 + (end_row - 1) / g.gqa);
@@ -456,17 +452,17 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
              f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]} * inv);
 }
 
-// Joins the slices of every row, in their order: a thread per 4 channels.  blockIdx.y: sequence.
+// Joins the slices of every row, in their order: a thread per 4 channels.
 template <int HD>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Geo g, AttendArgs a) {
-  int q0, m, all;
-  queries_of(a, blockIdx.y, &q0, &m, &all);
-  const int slices = prefill_slices(a, clamp_len(g, a.lens[blockIdx.y]));
-  if (slices == 1) return;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  static_assert(256 / (HD / 4) == 1 << merge_log2(HD), "rows of a workgroup");
+  const Place p = place_of(g, a, blockIdx.x, g.nh, merge_log2(HD));
+  const int slices = prefill_slices(a, p.n);
+  if (slices == 1 || p.at < 0) return;
+  const int64_t i = (int64_t)p.at * 256 + threadIdx.x;
   const int ch = (int)(i % (HD / 4)) * 4;
-  if (i / (HD / 4) >= (int64_t)m * g.nh) return;
-  const int64_t at = (int64_t)q0 * g.nh + i / (HD / 4), rows = (int64_t)a.total_q * g.nh;
+  if (i / (HD / 4) >= (int64_t)p.m * g.nh) return;
+  const int64_t at = (int64_t)p.q0 * g.nh + i / (HD / 4), rows = (int64_t)a.total_q * g.nh;
   float mx = kNegInf, l = 0.0f;
   f4 acc = {0, 0, 0, 0};
   for (int s = 0; s < slices; ++s) {
@@ -487,26 +483,16 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Geo g, AttendArgs a) {
 
 template <int HD, bool E4M3>
 static hipError_t prefill_codes(const Geo& g, const AttendArgs& a, hipStream_t s) {
-  const int tiles = prefill_tiles(g, a.max_q);
-  const dim3 grid((unsigned)tiles * g.nkv, a.batch, a.slices);
+  const dim3 grid((unsigned)(a.tiles * g.nkv), a.slices);
   if (sizeof(Lds<HD>) > 65536) {  // past 64 KiB a kernel asks for its LDS
     const hipError_t e = hipFuncSetAttribute((const void*)q8_prefill_kernel<HD, E4M3>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)sizeof(Lds<HD>));
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((q8_prefill_kernel<HD, E4M3>), grid, dim3(kThreads), sizeof(Lds<HD>), s, g, a,
-                     tiles);
-  if (a.slices > 1) {
-    const int64_t threads = (int64_t)a.max_q * g.nh * (HD / 4);
-    hipLaunchKernelGGL((q8_merge_kernel<HD>), dim3((unsigned)((threads + 255) / 256), a.batch),
-                       dim3(256), 0, s, g, a);
-  }
+  hipLaunchKernelGGL((q8_prefill_kernel<HD, E4M3>), grid, dim3(kThreads), sizeof(Lds<HD>), s, g, a);
+  if (a.slices > 1) hipLaunchKernelGGL((q8_merge_kernel<HD>), dim3(a.merges), dim3(256), 0, s, g, a);
   return hipGetLastError();
-}
-
-int prefill_tiles(const Geo& g, int max_q) {
-  return (int)(((int64_t)max_q * g.gqa + kRows - 1) / kRows);
 }
 
 hipError_t launch_prefill(const Geo& g, const AttendArgs& a, hipStream_t s) {

@@ -3,6 +3,7 @@ rows or few heads, the prompts' the rest, so each size here says which one it is
 from __future__ import annotations
 
 import dataclasses
+import random
 
 import pytest
 
@@ -171,3 +172,39 @@ def test_a_tensor_put_in_the_place_of_another_is_the_one_used(q8):  # noqa: F811
     assert torch.equal(cache.k_tail[0, :, 5], k[0]) and torch.equal(cache.v_tail[1, :, 4], v[1])
     got = cache.decode(q, seq + 1, tables)
     check_attention(cache, tables, [38, 21], q, [0, 1, 2], got)
+
+
+@pytest.mark.parametrize("heads,batch", [((32, 8, 128), 64), ((14, 2, 64), 65), ((16, 1, 64), 300),
+                                         ((8, 1, 128), 5000)])
+def test_prompts_of_few_among_many_sequences(q8, heads, batch):  # noqa: F811
+    """Most sequences have no query, some one, few as many as a prompt has; one is long, so that
+    its row tiles are cut and merged.  Rows before, between and behind them stay."""
+    rng = random.Random(batch)
+    nh, nkv, hd = heads
+    lens = [rng.choice((0, 1, 17, 64, 200)) for _ in range(batch)]
+    ms = [rng.choice((0, 0, 0, 0, 0, 0, 0, 0, 0, 1)) if n else 0 for n in lens]
+    for b, n, m in ((0, 300, 40), (batch // 3, 9000, 130), (batch // 3 + 1, 40, 40),
+                    (batch // 2, 700, 33), (batch - 1, 150, 150)):
+        lens[b], ms[b] = n, m
+    cache, tables, seq = make(q8, nh, nkv, hd, 32, "int8", lens, seed=batch)
+    spoil(cache, tables, lens)
+    cu = [3 + x for x in offsets(ms)]
+    total, most = cu[-1] + 50, 150
+    assert runs_prefill(q8, cache, total, most)
+    size = q8.lib().jacq_q8_attend_workspace_size(cache.geo.ref, batch, total, most, 0)
+    assert size >= 2 * total * nh * (hd + 2) * 4  # slices
+    gen = torch.Generator("cuda").manual_seed(batch)
+    q = randn(gen, total, nh, hd)
+    some = [b for b in range(batch) if ms[b] > 1] + rng.sample([b for b in range(batch) if ms[b] == 1],
+                                                               min(20, ms.count(1)))
+    for window, sinks in ((None, 0), (100, 3)):
+        names = dict(window=window, sinks=sinks)
+        out, lse = torch.full_like(q, 7.0), torch.full((total, nh), 7.0, device="cuda")
+        cache.prefill(q, ints(*cu), most, seq, tables, out=out, lse=lse, **names)
+        for b in some:
+            rows = slice(cu[b], cu[b + 1])
+            check_attention(cache.sequence_view(b), tables[b:b + 1], lens[b:b + 1], q[rows],
+                            [0, ms[b]], out[rows], lse[rows], **names)
+        assert not bool((lse[3:cu[-1]] == 7).any())  # every row has been written
+        for x in (out, lse):
+            assert bool((x[:3] == 7).all()) and bool((x[cu[-1]:] == 7).all())

@@ -67,3 +67,30 @@ def test_a_view_of_no_sequence_is_refused(cache):
     with pytest.raises(kivi.KiviCheckError, match="batch"):
         q8.PagedQ8Cache.from_tensors(cache.geo, {**t, "k_tail": t["k_tail"][:0],
                                                  "v_tail": t["v_tail"][:0]})
+
+
+def workspace(batch, total, max_q, weighted=0, **geo):
+    g = q8.Q8Geometry(**{**dict(num_heads=40, num_kv_heads=8, head_dim=128, page_size=32,
+                                max_pages_per_seq=512, num_pages=512), **geo})
+    return q8.lib().jacq_q8_attend_workspace_size(g.ref, batch, total, max_q, weighted)
+
+
+@pytest.mark.parametrize("heads", [(40, 8, 128), (14, 2, 64)])
+def test_a_call_is_planned_by_its_queries_not_by_the_caches_sequences(heads):
+    geo = dict(zip(("num_heads", "num_kv_heads", "head_dim"), heads))
+    # queries of one sequence: as many slices of its tokens in a cache of one sequence and of many
+    for queries in (200, 512, 2000):
+        alone = workspace(1, queries, queries, **geo)
+        assert alone > 0
+        for batch in (2, 64, 1000):
+            assert workspace(batch, queries, queries, **geo) == alone
+    # so few that the decode's kernel has them alone, whose workspace is the smaller by what block
+    # weights take: their sums of 1024 groups of 16 tokens and rows, and the rows' own
+    queries = 20
+    g = heads[0] // heads[1]
+    blocks = -(-queries * g // 32)
+    for batch in (1, 64):
+        sums = batch * heads[1] * blocks * 1024 * 32 * 4
+        rows = -(-queries * heads[0] * 4 // 256) * 256
+        assert (workspace(batch, queries, queries, 1, **geo)
+                - workspace(batch, queries, queries, **geo)) == sums + rows
