@@ -208,3 +208,188 @@ def test_prompts_of_few_among_many_sequences(q8, heads, batch):  # noqa: F811
         assert not bool((lse[3:cu[-1]] == 7).any())  # every row has been written
         for x in (out, lse):
             assert bool((x[:3] == 7).all()) and bool((x[cu[-1]:] == 7).all())
+
+
+# The decode's kernel takes up to 64 rows (queries x heads of a kv head) or 2048 (query, head) rows of
+# a call: a few heads stay in it, 32/8 heads of 40 queries and more do not.
+BOTH = pytest.mark.parametrize("heads,m,prompt", [((4, 2, 64), 40, False), ((10, 2, 128), 12, False),
+                                                  ((32, 8, 128), 70, True), ((28, 4, 64), 90, True)])
+
+
+@BOTH
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("where", ["block", "tail"])
+def test_a_nan_key_reaches_the_queries_that_see_it(q8, heads, m, prompt, codes, where):  # noqa: F811
+    """One kv head of one token, in K or V; windows that end before it."""
+    nh, nkv, hd = heads
+    g, page, n = nh // nkv, 16, 16 * 20 + 9
+    gen = torch.Generator("cuda").manual_seed(m)
+    k, v = randn(gen, n, nkv, hd), randn(gen, n, nkv, hd)
+    at = n - 9 - max(page, m // 2) if where == "block" else n - 4
+    (k if codes == "int8" else v)[at, 1, 7] = float("nan")
+    cache = q8.PagedQ8Cache(q8.Q8Geometry(nh, nkv, hd, page, 32, 32, codes), 1)
+    tables = torch.randperm(32, generator=gen, device="cuda").to(torch.int32).view(1, 32)
+    cache.append(k, v, tables, ints(0), cu_new=ints(0, n))
+    assert runs_prefill(q8, cache, m, m) == prompt
+    q = randn(gen, m, nh, hd)
+    pos = torch.arange(n - m, n, device="cuda")
+    first = at // page * page if where == "block" else at  # a block quantised with it is NaN whole
+    last = (at // page + 1) * page - 1 if where == "block" else at
+    for window, sinks in ((None, 0), (7, 0), (5, 3)):
+        lse = torch.empty((m, nh), device="cuda")
+        got = cache.prefill(q, ints(0, m), m, ints(n), tables, window=window, sinks=sinks, lse=lse)
+        sees = pos >= first
+        if window is not None:
+            sees &= pos - window < last
+        assert 0 < int(sees.sum()) <= m - (m > 40 or where == "tail")
+        head = torch.arange(nh, device="cuda") // g == 1
+        want = sees[:, None] & head[None]
+        assert torch.equal(got.isnan().all(-1), want) and torch.equal(got.isnan().any(-1), want)
+        assert torch.equal(lse.isnan(), want)
+        check = [h for h in range(nh) if h // g != 1]
+        kk, vv = ref.held_values(cache, tables, 0, n)
+        r = ref.attend(q, kk.nan_to_num(0), vv, n, window, sinks)
+        tol = ref.tolerance(r, hd, torch.float16)
+        ref.assert_within(got[:, check], r["o"][:, check], tol[:, check])
+        ref.assert_within(got[~sees], r["o"][~sees], tol[~sees])
+
+
+@BOTH
+def test_queries_of_any_size_through_both_kernels(q8, heads, m, prompt):  # noqa: F811
+    """bf16 queries past fp16's range and below it, a row of zeros, NaN and infinity, beside keys of
+    a zero block; causal, so that tiles are masked in part."""
+    nh, nkv, hd = heads
+    page, n = 32, 300
+    gen = torch.Generator("cuda").manual_seed(m)
+    k = randn(gen, n, nkv, hd)
+    v = randn(gen, n, nkv, hd)
+    k[256:288] = 0  # its scale of K is 2^-24 / 127
+    cache = q8.PagedQ8Cache(q8.Q8Geometry(nh, nkv, hd, page, 10, 10, "int8"), 1)
+    tables = torch.arange(10, **I32).flip(0).contiguous().view(1, 10)
+    cache.append(k, v, tables, ints(0), cu_new=ints(0, n))
+    assert runs_prefill(q8, cache, m, m) == prompt
+    q = randn(gen, m, nh, hd, dtype=torch.bfloat16)
+    sizes = torch.tensor([1e8, 1e-8, 1.0, 1e-30, 0.0, 1e5, 1e-36], device="cuda")
+    f = sizes[torch.arange(m * nh, device="cuda") % 7].view(m, nh, 1)
+    q = (q.float() * f).bfloat16()
+    for scale in (1e-7, 0.1):
+        rows = torch.ones((m, nh), dtype=torch.bool, device="cuda")
+        if scale == 0.1:
+            # scores of 1e6 and more are one key's alone: their error is past any weight's
+            rows = f[..., 0] < 1e4
+        o = torch.empty((m, nh, hd), device="cuda")
+        lse = torch.empty((m, nh), device="cuda")
+        cache.prefill(q, ints(0, m), m, ints(n), tables, scale=scale, out=o, lse=lse)
+        r = ref.attend(q, *ref.held_values(cache, tables, 0, n), n, scale=scale)
+        tol = ref.tolerance(r, hd, torch.float32)
+        ref.assert_within(o[rows], r["o"][rows], tol[rows])
+        err = ref.score_error(r, hd) + 2.0 ** -22 * (1 + r["lse"].abs())
+        ref.assert_within(lse[rows], r["lse"][rows], err[rows])
+    clean = cache.prefill(q, ints(0, m), m, ints(n), tables, scale=1e-7)
+    q[m - 3, 1, 5], q[m // 2, nh - 1, 9] = float("nan"), float("inf")
+    got = cache.prefill(q, ints(0, m), m, ints(n), tables, scale=1e-7)
+    bad = torch.zeros((m, nh), dtype=torch.bool, device="cuda")
+    bad[m - 3, 1] = bad[m // 2, nh - 1] = True
+    assert bool(got[bad].isnan().all()) and torch.equal(got[~bad], clean[~bad])
+
+
+@BOTH
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_blocks_whose_scales_differ_by_far_through_both_kernels(q8, heads, m, prompt, codes):  # noqa: F811
+    """V of the blocks differs by factors of up to 2^20; the blocks of the largest are as good as
+    unseen, so what O is made of is small beside them."""
+    nh, nkv, hd = heads
+    page, n = 16, 16 * 12 + 7
+    gen = torch.Generator("cuda").manual_seed(m)
+    k, v = randn(gen, n, nkv, hd, scale=0.1), randn(gen, n, nkv, hd)
+    f = torch.tensor([1.0, 2.0 ** -10, 2.0 ** 10, 2.0 ** -14, 0.0, 3.0], device="cuda").repeat(3)
+    v = (v * f.repeat_interleave(page)[:n].view(n, 1, 1)).half()
+    for block in (2, 8):
+        k[block * page:(block + 1) * page] = -8.0
+    cache = q8.PagedQ8Cache(q8.Q8Geometry(nh, nkv, hd, page, 13, 13, codes), 1)
+    tables = torch.arange(13, **I32).view(1, 13)
+    cache.append(k, v, tables, ints(0), cu_new=ints(0, n))
+    assert runs_prefill(q8, cache, m, m) == prompt
+    q = torch.full((m, nh, hd), 0.7, dtype=torch.float16, device="cuda")
+    q += randn(gen, m, nh, hd, scale=0.05)
+    o = torch.empty((m, nh, hd), device="cuda")
+    cache.prefill(q, ints(0, m), m, ints(n), tables, out=o)
+    kk, vv = ref.held_values(cache, tables, 0, n)
+    r = ref.attend(q, kk, vv, n)
+    # what fp16 weights lose, 2^-32 of the heaviest's block a token, is of what weighs anything
+    seen = r["p"].amax((0, 1, 2)) > 2.0 ** -30
+    assert not bool(seen[32:48].any()) and bool(seen[16:32].all())
+    r["vmax"] = vv[:, seen].abs().amax()
+    ref.assert_within(o, r["o"], ref.tolerance(r, hd, torch.float32))
+
+
+@pytest.mark.parametrize("heads", [(32, 8, 128), (14, 2, 64), (16, 1, 64)])
+@pytest.mark.parametrize("step", [-1, 0, 1])
+def test_either_side_of_the_rule_between_the_kernels(q8, heads, step):  # noqa: F811
+    """64 rows of a kv head, and 2048 (query, head) rows of a call: the last of the one kernel, the
+    first of the other, and all of both batches against the definition."""
+    nh, nkv, hd = heads
+    for batch, m in ((2048 // (64 // (nh // nkv) * nh) + 3, 64 // (nh // nkv) + step),
+                     (1, 2048 // nh + step)):
+        if m < 1:
+            continue
+        lens = [m + 70 * b + 5 for b in range(batch)]
+        cache, tables, seq = make(q8, nh, nkv, hd, 32, "int8", lens, seed=m + batch)
+        spoil(cache, tables, lens)
+        cu = offsets([m] * batch)
+        gen = torch.Generator("cuda").manual_seed(m)
+        q = randn(gen, cu[-1], nh, hd, dtype=torch.bfloat16)
+        assert (runs_prefill(q8, cache, cu[-1], m)
+                == (m * (nh // nkv) > 64 and cu[-1] * nh > 2048))
+        lse = torch.empty((cu[-1], nh), device="cuda")
+        got = cache.prefill(q, ints(*cu), m, seq, tables, lse=lse)
+        check_attention(cache, tables, lens, q, cu, got, lse)
+
+
+@pytest.mark.parametrize("heads", [(32, 8, 128), (12, 6, 64), (30, 10, 64), (5, 5, 128)])
+@pytest.mark.parametrize("m", [1, 7])
+def test_block_weights_of_more_kv_heads_than_wavefronts(q8, heads, m):  # noqa: F811
+    nh, nkv, hd = heads
+    lens = [m, 100, 1003]
+    cache, tables, seq = make(q8, nh, nkv, hd, 32, "int8", lens, seed=nkv)
+    spoil(cache, tables, lens)
+    gen = torch.Generator("cuda").manual_seed(nkv + 1)
+    cu = offsets([m] * 3)
+    q = randn(gen, cu[-1], nh, hd)
+    w = torch.full((3, cache.geo.max_pages_per_seq), float("nan"), device="cuda")
+    for window, sinks in ((None, 0), (50, 3)):
+        names = dict(window=window, sinks=sinks, weights=w, decay=0.0)
+        got = (cache.decode(q, seq, tables, **names) if m == 1 else
+               cache.prefill(q, ints(*cu), m, seq, tables, **names))
+        check_attention(cache, tables, lens, q, cu, got, weights=w, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("why", ["key", "page"])
+def test_weights_of_a_poisoned_sequence_evict_as_nan(q8, why):  # noqa: F811
+    """Its weights are NaN, which is lightest: all alike, so the earlier blocks stay.  The others'
+    weights are as if it were not there."""
+    page, nh, nkv, hd = 16, 16, 8, 64
+    lens = [160 + 5, 160 + 5]
+    gen = torch.Generator("cuda").manual_seed(11)
+    k, v = randn(gen, 2 * 165, nkv, hd), randn(gen, 2 * 165, nkv, hd)
+    tables = torch.randperm(22, generator=gen, device="cuda").to(torch.int32).view(2, 11)
+    cache = q8.PagedQ8Cache(q8.Q8Geometry(nh, nkv, hd, page, 11, 22, "e4m3"), 2)
+    if why == "key":
+        k[40, 5, 3] = float("nan")
+    cache.append(k, v, tables, ints(0, 0), cu_new=ints(0, 165, 330))
+    seen = tables.clone()
+    if why == "page":
+        seen[0, 2] = -1
+    q = randn(gen, 2, nh, hd)
+    w = torch.empty((2, 11), device="cuda")
+    got = cache.decode(q, ints(*lens), seen, weights=w, decay=0.0)
+    assert bool(w[0].isnan().all()) and not bool(w[1].isnan().any())
+    check_attention(cache.sequence_view(1), tables[1:], lens[1:], q[1:], [0, 1], got[1:],
+                    weights=w[1:])
+    names = dict(sink_pages=0, recent_pages=1)
+    out = cache.evict(w, ints(*lens), tables, 4, **names)
+    want = ref.evict(w.cpu(), lens, tables.cpu(), page, 4, 0, 1)
+    for a, b in zip(out, want):
+        assert torch.equal(a.cpu().nan_to_num(-5.0) if a.is_floating_point() else a.cpu(),
+                           b.nan_to_num(-5.0) if b.is_floating_point() else b)
+    assert out[0][0, :4].tolist() == [*tables[0, :3].tolist(), int(tables[0, 9])]
