@@ -28,7 +28,9 @@
  *   K/V_TAIL      fp16   [batch, NKV, P, HD]: tokens len / P * P ... len - 1
  *   BLOCK_TABLES  int32  [batch, max_pages_per_seq]
  *   weights       fp32   [batch, max_pages_per_seq]
- * Lengths are clamped on the device to [0, max_pages_per_seq * P].  A table
+ * Lengths are clamped on the device to [0, max_pages_per_seq * P]; of a
+ * sequence whose length before an append is outside [0, that) all new tokens
+ * are dropped.  A table
  * entry outside [0, num_pages) is never dereferenced: a read of it gives NaN,
  * a write to it is dropped.
  */
@@ -106,7 +108,11 @@ int jacq_q8_append(const jacq_q8_geometry* geo, const jacq_q8_pool* pool, const 
  *   WEIGHTS  NULL or [batch, max_pages_per_seq] fp32: of every block, decay
  *            times what it held (decay 0 overwrites) plus the softmax weight
  *            of its tokens summed over the sequence's queries and heads;
- *            at most JACQ_Q8_MAX_WEIGHTED_QUERIES queries per sequence
+ *            at most JACQ_Q8_MAX_WEIGHTED_QUERIES queries per sequence.  The
+ *            workspace then holds a float for every row (query x head) of
+ *            every 16 tokens that the table addresses, the rows of a kv head
+ *            in 16s or 32s: batch x NKV x max_pages_per_seq x P / 4 x rows
+ *            bytes, whatever the lengths are
  *   max_q    no sequence has more queries than this (of one that has, the
  *            first max_q are computed, at their own positions; the others are
  *            left alone)

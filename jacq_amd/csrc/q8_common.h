@@ -17,11 +17,10 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kFloor = 0x1p-24f;   // a block's largest magnitude counts as at least this
-constexpr float kHalfMax = 65504.0f;
 constexpr int kTile = 64;            // tokens per step of the attention kernels
 constexpr int kRowsLog2 = 7;
 constexpr int kPrefillRows = 1 << kRowsLog2;  // query rows of a workgroup of the prefill kernel
-constexpr int kSliceUnits = 8;       // tiles of one of its slices at least
+constexpr int kSliceUnits = 8;       // tiles of one of its slices, about, at least (prefill_slices)
 constexpr int kMaxSlices = 32;       // of its slices at most
 // Workgroups of the decode kernel that a CU holds (a wavefront of each a SIMD), by what its
 // registers allow.
@@ -94,7 +93,6 @@ struct AttendArgs {
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float log2_(float x) { return __builtin_amdgcn_logf(x); }
-__device__ inline float bf2f(uint32_t h) { return __uint_as_float(h << 16); }
 __device__ inline uint16_t f2bf(float f) {  // round to nearest even; NaN stays NaN
   return __builtin_bit_cast(uint16_t, (__bf16)f);
 }
@@ -233,9 +231,10 @@ __device__ inline Place place_of(const Geo& g, const AttendArgs& a, int unit, in
 }
 
 // Workgroups that share the tokens of a prefill's row tile.  A workgroup alone on a CU takes about
-// 1.7 us a tile of 64 tokens, two 2.5 us (HD 128): `load` row tiles a CU in s slices take about
-// c(load s) / s, c(x) = 1 up to one per CU and 3/4 for each begun one from there, with an end that
-// is not full; the slices' partial sums and their join cost about s 400 / tokens of the whole.
+// 1.7 us a tile of 64 tokens, two 2.5 us (HD 128; the rule is HD 64's too, where a tile takes half
+// and three share a CU): `load` row tiles a CU in s slices take about c(load s) / s, c(x) = 1 up to
+// one per CU and 3/4 for each begun one from there, with an end that is not full; the slices'
+// partial sums and their join cost about 300 load s / tokens of that.
 // Measured (us, 40/8 heads of 128): 32 queries over 16384 tokens 430 in one slice, 47 in 16; 511
 // queries of each of 4 sequences of up to 16001 493 in one, 443 in 2, 446 in 4; a prompt of 8191 825
 // in one, 907 in 2.  Order-preserving as bits: it is positive.
@@ -246,8 +245,9 @@ __host__ __device__ inline float slices_cost(float load, int s, float tokens) {
 }
 
 // The slices of a sequence of n tokens: the best number up to a.slices (the best for as many tokens
-// as the table addresses) by what its row tiles may see, none of fewer than kSliceUnits tiles.  Over
-// the lanes of a wavefront, a number each.
+// as the table addresses) by what its last row tile may see, one for each kSliceUnits tiles begun
+// at most: so of 9 tiles there may be slices of 4 and 5, and of a row tile that sees less, empty
+// ones.  Over the lanes of a wavefront, a number each.
 __device__ inline int prefill_slices(const AttendArgs& a, int n) {
   if (a.slices == 1) return 1;
   int tiles = (n + kTile - 1) / kTile;

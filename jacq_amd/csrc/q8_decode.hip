@@ -156,8 +156,8 @@ struct Wave {
   }
 
   // Scores -> weights -> O^T.  sc: raw scores of this lane's 16 tokens, t0 their first one;
-  // tokens from `end` on are not there.  Returns through pv_step the fp16 weights.
-  __device__ void soften(const Segment& s, int nb, f4 (&sc)[4], int t0, int end, float ks, float vs,
+  // tokens from `end` on are not there.  p0, p1: the weights in fp16.
+  __device__ void soften(int nb, f4 (&sc)[4], int t0, int end, float ks, float vs,
                          bool masked, h8& p0, h8& p1) {
     const float av = qs[nb] * ks, bv = log2_(vs), ivs = 1.0f / vs;
     float t[16];
@@ -194,6 +194,9 @@ struct Wave {
   }
 
   // The base-2 logarithms of the weight of this lane's 16 tokens from t0 on, for the block weights.
+  // In fp32, as the row's own that the weights kernel takes from them: the weight is of the row's
+  // whole sum, which is not known yet, and a logarithm needs no rescaling when the maximum moves.  Of
+  // a magnitude of up to 2^8, it leaves a weight within 2^-15 of itself.
   __device__ void store_group(const Segment& s, int t0, int end) const {
     if (!a.weights || t0 >= end) return;
     const int64_t seg = ((int64_t)s.b * g.nkv + s.h) * a.row_blocks + s.rb;
@@ -272,8 +275,7 @@ struct Wave {
     h8 p[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
-      soften(s, nb, sc[nb], s.span.nq + kq * 16, s.span.n, 1.0f, 1.0f, true, p[nb][0],
-             p[nb][1]);
+      soften(nb, sc[nb], s.span.nq + kq * 16, s.span.n, 1.0f, 1.0f, true, p[nb][0], p[nb][1]);
     store_group(s, s.span.nq + kq * 16, s.span.n);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -324,7 +326,7 @@ struct Wave {
         h8 p[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          soften(s, nb, sc[nb], t0 + kq * 16, sp.nq, ks, vs, masked, p[nb][0], p[nb][1]);
+          soften(nb, sc[nb], t0 + kq * 16, sp.nq, ks, vs, masked, p[nb][0], p[nb][1]);
         values(c, p);
         u0 += kWaves;
         if (next < 0) break;
@@ -390,9 +392,10 @@ struct Slices {
 __device__ inline int slices_of(const Span& s, int size) { return (s.units + size - 1) / size; }
 
 // Units of a slice, from the call's units, its segments and the longest one's units.
-//  - Uncut, if that takes no longer: a workgroup alone on a CU needs about 0.4 us a unit (HD 128),
-//    the memory 0.8 us a unit and CU, a cut call about 2 us more; and where segments outnumber CUs
-//    only if they are about equally long and, with up to 16 rows, fill the CUs about evenly.  40/8
+//  - Uncut, if that takes no longer: a workgroup alone on a CU needs about 0.4 us a unit (HD 128,
+//    whose rule is HD 64's too), the memory 0.8 us a unit and CU, a cut call about 2 us more; and
+//    where segments outnumber CUs only if they are about equally long and, with up to 16 rows, fill
+//    the CUs about evenly.  40/8
 //    heads of 128, uncut against cut (us): 32 sequences of 2048 tokens 27.8 against 29.5, 64 48.2
 //    against 50.3, 64 of 4096 103 against 110; 16 of 1000 22.3 against 18.1, of 2000 30.2 against
 //    25.7, of 4096 41.6 against 31.7; 64 of 1024 to 16384 267 against 235; one of 4096 35.3 against

@@ -415,7 +415,9 @@ class PagedQ8Cache:
         window: a query sees the last ``window`` tokens, itself among them, and the first
         ``sinks`` of the sequence; None: all.  weights [batch, max_pages_per_seq] fp32 becomes
         decay * weights + the softmax weight of each block's tokens, summed over the heads;
-        decay 0 overwrites.  lse [batch, NH] fp32 takes the log of the sum of exponentials.
+        decay 0 overwrites; the call's workspace then takes, whatever the lengths are, 4 bytes
+        for every head and every 16 tokens of the table's width (``prefill``: and query, the
+        rows of a kv head rounded up).  lse [batch, NH] fp32 takes the log of the sum of exponentials.
         A sequence of no tokens gives 0 (lse -inf)."""
         _check(q.dim() == 3 and q.shape[0] == self.batch, "Q must have one token per sequence (",
                self.batch, "), got ", tuple(q.shape))
@@ -497,6 +499,7 @@ class PagedQ8Cache:
             self._here(("WEIGHTS", weights), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
                        *(("an output", t) for t in out))
         self._call(_lib.jacq_q8_evict, self.geo.ref, weights.data_ptr(), seq_lens.data_ptr(),
-                   block_tables.data_ptr(), self.batch, keep, sink_pages, recent_pages, tables_out.data_ptr(), lens_out.data_ptr(),
-                   weights_out.data_ptr(), evicted.data_ptr())
+                   block_tables.data_ptr(), self.batch, keep, sink_pages, recent_pages,
+                   tables_out.data_ptr(), lens_out.data_ptr(), weights_out.data_ptr(),
+                   evicted.data_ptr())
         return out
