@@ -10,15 +10,16 @@
 // next operand as it stands.  The scales of 16 tokens are the wavefront's:
 // t = s (ks q) + log2(vs), as in q8_decode.hip, where the reason is.
 //
-// Bound by the matrix cores, the LDS and the vector units together.  A prompt of
+// Bound by the matrix cores, the LDS and the vector units taking turns.  A prompt of
 // 8191 tokens (40/8 heads of 128, int8): 780 to 820 us, 840 to 880 TFLOP/s, where
-// the library's product of 8192^3 runs at 1145.  Of the CUs' cycles the matrix
+// the library's product of 8192^3 runs at 1145 to 1242.  Of the CUs' cycles the matrix
 // cores are busy for 40 %, the vector units for 56 %, the LDS for 53 %.  Without the
 // staging it takes 586 us, without the softmax 629, the products with their
 // LDS reads alone 526: an operand feeds one product, since 64 rows a wavefront
 // (two products each) do not fit the registers at HD 128 (spills, 1061 us).
-// On zeros the same prompt takes 702 us against 854 on random values (one card):
-// the chip slows down under this load, so moving work about changes little.
+// On zeros the same prompt takes 702 us against 854 on random values (one card), the
+// matrix instructions alone 310 and 435: what they do not account for, about 400 us,
+// is the other work that does not run beside them.
 // Two workgroups a CU, not in step: one's products run beside the other's
 // softmax.  The softmax of a half tile among the next half's products, in one
 // wavefront's order, was as fast (HD 128: 820 us; HD 64: 204 against 213).
