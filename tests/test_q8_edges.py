@@ -94,3 +94,8 @@ def test_a_call_is_planned_by_its_queries_not_by_the_caches_sequences(heads):
         rows = -(-queries * heads[0] * 4 // 256) * 256
         assert (workspace(batch, queries, queries, 1, **geo)
                 - workspace(batch, queries, queries, **geo)) == sums + rows
+
+
+def test_more_row_tiles_than_a_launch_has_are_refused():
+    r = Record(max_pages_per_seq=4)
+    error(r.attend(batch=100, total_q=2 ** 31 - 1, max_q=100), EINVAL, "too many query rows")
