@@ -417,8 +417,8 @@ class PagedQ8Cache:
         decay * weights + the softmax weight of each block's tokens, summed over the heads;
         decay 0 overwrites; the call's workspace then takes, whatever the lengths are, 4 bytes
         for every head and every 16 tokens of the table's width (``prefill``: and query, the
-        rows of a kv head rounded up).  lse [batch, NH] fp32 takes the log of the sum of exponentials.
-        A sequence of no tokens gives 0 (lse -inf)."""
+        rows of a kv head rounded up).  lse [batch, NH] fp32 takes the log of the sum of
+        exponentials.  A sequence of no tokens gives 0 (lse -inf)."""
         _check(q.dim() == 3 and q.shape[0] == self.batch, "Q must have one token per sequence (",
                self.batch, "), got ", tuple(q.shape))
         return self._attend(q, None, 1, seq_lens, block_tables, window, sinks, scale, weights,
