@@ -211,7 +211,7 @@ def test_prompts_of_few_among_many_sequences(q8, heads, batch):  # noqa: F811
 
 
 # The decode's kernel takes up to 64 rows (queries x heads of a kv head) or 2048 (query, head) rows of
-# a call: a few heads stay in it, 32/8 heads of 40 queries and more do not.
+# a call: a few heads stay in it, 70 queries of 32/8 heads do not.
 BOTH = pytest.mark.parametrize("heads,m,prompt", [((4, 2, 64), 40, False), ((10, 2, 128), 12, False),
                                                   ((32, 8, 128), 70, True), ((28, 4, 64), 90, True)])
 
