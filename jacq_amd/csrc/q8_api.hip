@@ -165,8 +165,8 @@ struct Plan {
 // heads of 128, 18.8 tiles a CU: 227 us in up to 4 slices, 190 in one).
 int plan_slices(float load, int64_t tokens) {
   const int most =
-      (int)std::min<int64_t>(jacq::q8::kMaxSlices, tokens / (jacq::q8::kSliceUnits * jacq::q8::kTile));
-  auto cost = [&](int s) { return jacq::q8::slices_cost(load, s, (float)tokens); };
+      (int)std::min<int64_t>(jacq::kMaxSlices, tokens / (jacq::kSliceUnits * jacq::kTile));
+  auto cost = [&](int s) { return jacq::slices_cost(load, s, (float)tokens); };
   int best = 1;
   for (int s = 2; s <= most; ++s)
     if (cost(s) < cost(best)) best = s;
@@ -193,7 +193,7 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
     return here;
   };
   if (p.prefill) {
-    p.load = (float)(blocks(jacq::q8::kPrefillRows) * g.nkv) / (float)device_cus();
+    p.load = (float)(blocks(jacq::kPrefillRows) * g.nkv) / (float)device_cus();
     p.slices = plan_slices(p.load, (int64_t)g.max_pages * g.page);
     if (p.slices > 1) {
       const size_t rows_all = (size_t)p.slices * total_q * g.nh;
@@ -230,7 +230,7 @@ Plan plan_attend(const Geo& g, int batch, int total_q, int max_q, bool weighted)
 int64_t place_units(const AttendArgs& a, int per, int log2) {
   const int64_t of_all = ((int64_t)a.total_q * per >> log2) + a.batch;
   const int64_t each = ((int64_t)a.max_q * per + (1 << log2) - 1) >> log2;
-  return a.batch <= jacq::q8::kCounted ? std::min(of_all, a.batch * each) : of_all;
+  return a.batch <= jacq::kCounted ? std::min(of_all, a.batch * each) : of_all;
 }
 
 }  // namespace
@@ -346,7 +346,7 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.max_q = std::min(x->max_q, x->total_q);
     a.window = std::min(x->window, 1 << 30);
     a.sinks = std::min(x->sinks, 1 << 30);
-    a.scale = x->scale * jacq::q8::kLog2e;
+    a.scale = x->scale * jacq::kLog2e;
     a.decay = x->decay;
     if (none) {
       a.groups = g.max_pages * (g.page / 16);
@@ -367,8 +367,8 @@ int jacq_q8_attend(const jacq_q8_geometry* geo, const jacq_q8_pool* pool,
     a.row_lse = a.weights ? (float*)(ws + p.row_lse) : nullptr;
     a.slices = p.slices;
     a.load = p.load;
-    const int64_t tiles = place_units(a, g.gqa, jacq::q8::kRowsLog2);
-    const int64_t merges = p.slices > 1 ? place_units(a, g.nh, jacq::q8::merge_log2(g.hd)) : 0;
+    const int64_t tiles = place_units(a, g.gqa, jacq::kRowsLog2);
+    const int64_t merges = p.slices > 1 ? place_units(a, g.nh, jacq::merge_log2(g.hd)) : 0;
     // a launch has fewer than 2^32 threads
     if (p.prefill && std::max(tiles * g.nkv, merges) >= 1 << 24)
       return fail(JACQ_KIVI_EINVAL, "too many query rows in one call");

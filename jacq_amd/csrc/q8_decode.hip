@@ -31,17 +31,6 @@
 namespace jacq {
 namespace q8 {
 
-constexpr int kWaves = 4;         // wavefronts of a workgroup: they share a slice, unit by unit
-constexpr float kNegInf = -__builtin_inff();
-
-// One segment's place: sequence, kv head, row block, and its units' span.
-struct Segment {
-  int b, h, rb;
-  int q0, m;      // its sequence's first query and number of queries
-  int nrows;      // of this block
-  Span span;
-};
-
 template <int HD, bool E4M3, int NB>
 struct Wave {
   static constexpr int KS = HD / 32;  // k-steps of S^T
@@ -68,7 +57,7 @@ struct Wave {
   __device__ Wave(const Geo& g_, const AttendArgs& a_, int lane_)
       : g(g_), a(a_), lane(lane_), n16(lane_ & 15), kq(lane_ >> 4) {}
 
-  __device__ void start(const Segment& s) {
+  __device__ void start(const Segment<Geo>& s) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int row = s.rb * 16 * NB + nb * 16 + n16;
@@ -117,7 +106,7 @@ struct Wave {
 
   // The table's entry for the 16 tokens from t on; it is looked at when its page is loaded, so
   // that nothing waits for it before.
-  __device__ int page_of(const Segment& s, int t) const {
+  __device__ int page_of(const Segment<Geo>& s, int t) const {
     const int last = s.span.nq - 16;  // never past the sequence's own entries
     t = t < last ? t : last;
     return a.tables[(int64_t)s.b * g.max_pages + (t >> g.page_log2)];
@@ -125,14 +114,14 @@ struct Wave {
   __device__ bool exists(int page) const { return page >= 0 && page < g.num_pages; }
   __device__ uint32_t held(int page) const { return exists(page) ? page : 0; }
 
-  __device__ void pages(const Segment& s, int tile, int& pk, int& pv) const {
+  __device__ void pages(const Segment<Geo>& s, int tile, int& pk, int& pv) const {
     pk = page_of(s, tile * kTile + n16 / 4 * 16);
     pv = page_of(s, tile * kTile + kq * 16);
   }
 
   // A quantised tile's K codes, its scales and its V codes.  A tile begins a page or lies in one, so
   // where a lane reads in its page is the same for all.
-  __device__ void load_k(const Segment& s, int pk, Codes& c) const {
+  __device__ void load_k(const Segment<Geo>& s, int pk, Codes& c) const {
     uint32_t in = (s.h * g.page + (n16 / 4 * 16 & (g.page - 1)) + (n16 & 3)) * HD + kq * 16;
     asm volatile("" : "+v"(in));  // one register over the loop, not a pointer's two
     const uint8_t* k = a.pool.k_code + ((uint64_t)held(pk) * (uint32_t)(g.nkv * g.page * HD) + in);
@@ -141,13 +130,13 @@ struct Wave {
 #pragma unroll
       for (int j = 0; j < KL; ++j) c.k[t][j] = *(const u4*)(k + t * 4 * HD + j * 64);
   }
-  __device__ void load_scales(const Segment& s, int pv, Codes& c) const {
+  __device__ void load_scales(const Segment<Geo>& s, int pv, Codes& c) const {
     const uint64_t slot = (uint64_t)held(pv) * (uint32_t)g.nkv + (uint32_t)s.h;
     c.ks = a.pool.k_scale[slot];
     c.there = exists(pv);
     c.vs = a.pool.v_scale[slot];
   }
-  __device__ void load_v(const Segment& s, int pv, Codes& c) const {
+  __device__ void load_v(const Segment<Geo>& s, int pv, Codes& c) const {
     uint32_t in = (s.h * HD + n16) * g.page + (kq * 16 & (g.page - 1));
     asm volatile("" : "+v"(in));
     const uint8_t* v = a.pool.v_code + ((uint64_t)held(pv) * (uint32_t)(g.nkv * g.page * HD) + in);
@@ -197,7 +186,7 @@ struct Wave {
   // In fp32, as the row's own that the weights kernel takes from them: the weight is of the row's
   // whole sum, which is not known yet, and a logarithm needs no rescaling when the maximum moves.  Of
   // a magnitude of up to 2^8, it leaves a weight within 2^-15 of itself.
-  __device__ void store_group(const Segment& s, int t0, int end) const {
+  __device__ void store_group(const Segment<Geo>& s, int t0, int end) const {
     if (!a.weights || t0 >= end) return;
     const int64_t seg = ((int64_t)s.b * g.nkv + s.h) * a.row_blocks + s.rb;
     float* dst = a.group_lse + (seg * a.groups + (t0 >> 4)) * a.rows;
@@ -206,7 +195,7 @@ struct Wave {
       if (nb * 16 + n16 < s.nrows) dst[nb * 16 + n16] = group[nb];
   }
 
-  __device__ bool needs_mask(const Segment& s, int t0, int end) const {
+  __device__ bool needs_mask(const Segment<Geo>& s, int t0, int end) const {
     // uniform: the tile's 64 tokens are all there and every row sees them
     const int first = s.span.first + s.rb * 16 * NB / g.gqa;
     const int last = s.span.first + (s.rb * 16 * NB + s.nrows - 1) / g.gqa;
@@ -216,7 +205,7 @@ struct Wave {
 
   // No row sees the 16 tokens from t on, as their windows begin later: their page may be any, and
   // its e4m3 codes NaN, which a weight of 0 would not take out.
-  __device__ bool before_window(const Segment& s, int t) const {
+  __device__ bool before_window(const Segment<Geo>& s, int t) const {
     const int first = s.span.first + s.rb * 16 * NB / g.gqa;
     return t + 15 <= first - a.window && t >= a.sinks;
   }
@@ -251,7 +240,7 @@ struct Wave {
 
   // The tail: fp16 rows [nq, n), at most P of them.  Once per segment; V is gathered value by
   // value.
-  __device__ void tail(const Segment& s) {
+  __device__ void tail(const Segment<Geo>& s) {
     const int rows = s.span.n - s.span.nq;
     if (rows <= 0) return;
     const int64_t base = ((int64_t)s.b * g.nkv + s.h) * g.page * HD;
@@ -296,9 +285,9 @@ struct Wave {
     }
   }
 
-  // Units u0, u0 + kWaves, ... below u1.  One set of code registers: the next tile's K is
+  // Units u0, u0 + kSliceWaves, ... below u1.  One set of code registers: the next tile's K is
   // loaded when this one's scores are done, its V when this one's is used up.
-  __device__ void units(const Segment& s, int u0, int u1) {
+  __device__ void units(const Segment<Geo>& s, int u0, int u1) {
     if (u0 >= u1) return;
     const Span& sp = s.span;
     const int quant = sp.ns + sp.tiles - sp.w0;  // units of quantised tiles
@@ -310,9 +299,9 @@ struct Wave {
       load_k(s, pk, c);
       load_scales(s, pv, c);
       load_v(s, pv, c);
-      if (u0 + kWaves < e) pages(s, sp.tile_of(u0 + kWaves), nk, nv);
+      if (u0 + kSliceWaves < e) pages(s, sp.tile_of(u0 + kSliceWaves), nk, nv);
       for (;;) {
-        const int next = u0 + kWaves < e ? sp.tile_of(u0 + kWaves) : -1;
+        const int next = u0 + kSliceWaves < e ? sp.tile_of(u0 + kSliceWaves) : -1;
         const int t0 = tile * kTile;
         const bool masked = needs_mask(s, t0, sp.nq);
         f4 sc[NB][4];
@@ -328,14 +317,14 @@ struct Wave {
         for (int nb = 0; nb < NB; ++nb)
           soften(nb, sc[nb], t0 + kq * 16, sp.nq, ks, vs, masked, p[nb][0], p[nb][1]);
         values(c, p);
-        u0 += kWaves;
+        u0 += kSliceWaves;
         if (next < 0) break;
         load_scales(s, nv, c);
         load_v(s, nv, c);
         // behind the loads: what is loaded behind a store waits for it too (256 sequences of 100 to
         // 4000 tokens, 32/8 heads of 128: 241 us against 246)
         store_group(s, t0 + kq * 16, sp.nq);
-        if (u0 + kWaves < e) pages(s, sp.tile_of(u0 + kWaves), nk, nv);
+        if (u0 + kSliceWaves < e) pages(s, sp.tile_of(u0 + kSliceWaves), nk, nv);
         tile = next;
       }
       store_group(s, tile * kTile + kq * 16, sp.nq);
@@ -343,53 +332,6 @@ struct Wave {
     if (u0 < u1) tail(s);  // the unit behind the quantised ones
   }
 };
-
-__device__ inline void store_row(const AttendArgs& a, int64_t at, const float* x, int n) {
-  if (a.o_type == JACQ_Q8_FP32) {
-    for (int i = 0; i < n; i += 4) *(f4*)((float*)a.o + at + i) = *(const f4*)(x + i);
-    return;
-  }
-  for (int i = 0; i < n; i += 2) {
-    const uint32_t lo = a.o_type == JACQ_Q8_BF16 ? f2bf(x[i]) : f2h_(x[i]);
-    const uint32_t hi = a.o_type == JACQ_Q8_BF16 ? f2bf(x[i + 1]) : f2h_(x[i + 1]);
-    *(uint32_t*)((uint16_t*)a.o + at + i) = lo | hi << 16;
-  }
-}
-
-// O and lse of a row from sum(w v), sum(w / vs) and the maximum that w refers to.
-__device__ inline void finish_row(const Geo& g, const AttendArgs& a, const Segment& s, int row,
-                                  int hd, int ch, float* x, int n, float l, float m) {
-  const int r = s.rb * a.rows + row, tok = s.q0 + r / g.gqa, head = s.h * g.gqa + r % g.gqa;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int i = 0; i < n; ++i) x[i] *= inv;
-  store_row(a, ((int64_t)tok * g.nh + head) * hd + ch, x, n);
-  if (ch == 0) {
-    const float lse = l == 0.0f ? kNegInf : m + log2_(l);
-    if (a.lse) a.lse[(int64_t)tok * g.nh + head] = lse / kLog2e;
-    if (a.row_lse) a.row_lse[(int64_t)tok * g.nh + head] = lse;
-  }
-}
-
-template <int ROWS>
-__device__ inline void sequence_span(const Geo& g, const AttendArgs& a, int b, int* q0, int* m,
-                                     Span* span, int* blocks) {
-  int all;
-  queries_of(a, b, q0, m, &all);
-  const int n = clamp_len(g, a.lens[b]);
-  *span = Span(g, n, n - all, a.window, a.sinks);
-  *blocks = (*m * g.gqa + ROWS - 1) / ROWS;
-}
-
-// How the call's segments are cut: into slices of about `size` units each, at most a.target of
-// them more than there are segments.  A sequence's slices are numbered from `before` on, kv head
-// by kv head fastest, then row block, then slice.
-struct Slices {
-  int size;
-  int b;
-  int before;
-};
-
-__device__ inline int slices_of(const Span& s, int size) { return (s.units + size - 1) / size; }
 
 // Units of a slice, from the call's units, its segments and the longest one's units.
 //  - Uncut, if that takes no longer: a workgroup alone on a CU needs about 0.4 us a unit (HD 128,
@@ -417,131 +359,26 @@ __device__ inline int slice_units(const AttendArgs& a, float all, float segments
   const int few = fair < 4 ? 4 : fair > 16 ? 16 : fair;
   const float fit = (float)a.target - 0.5f * segments, half = 0.5f * (float)a.target;
   const int many = (int)(all / (fit > half ? fit : half)) + 1;
-  return ((many > few ? many : few) + kWaves - 1) / kWaves * kWaves;
+  return ((many > few ? many : few) + kSliceWaves - 1) / kSliceWaves * kSliceWaves;
 }
 
-// Units of each of the n slices but the last: equal, in whole rounds of the wavefronts too (never
-// more than the size they were counted by, so the last has some left).
-__device__ inline int even_units(const Span& s, int n) {
-  const int u = (s.units + n - 1) / n;
-  return n == 1 ? u : (u + kWaves - 1) / kWaves * kWaves;
-}
-
-// The same of a cut that q8_plan_kernel left: 64 places a step.
-__device__ inline Slices planned(const AttendArgs& a, int lane, int want, int b) {
-  const int size = uniform(a.plan[a.batch + 1]);
-  if (want < 0) return {size, b, uniform(a.plan[b])};
-  if (want >= uniform(a.plan[a.batch])) return {size, a.batch, 0};
-  // the last sequence whose first slice is not behind `want`: one without slices is not the last
-  int at = 0;
-  for (int n = a.batch; n > 1;) {
-    const int step = (n + 63) / 64, i = lane * step;
-    const uint64_t upto = __ballot(i < n && a.plan[at + (i < n ? i : 0)] <= want);
-    const int skip = (__popcll(upto) - 1) * step;
-    at += skip;
-    n = step < n - skip ? step : n - skip;
-  }
-  return {size, at, uniform(a.plan[at])};
-}
-
-// The cut, and the sequence that has slice `want` (b >= batch: none), or, with want < 0, the place
-// of sequence `b`.  Over the lanes of each wavefront alike, a sequence each.
-template <int ROWS>
-__device__ inline Slices cut(const Geo& g, const AttendArgs& a, int lane, int want, int b) {
-#pragma clang fp contract(off)
-  if (a.plan) return planned(a, lane, want, b);
-  // the sums are fp32: they choose the size, alike in every wavefront and kernel, and no more
-  float u = 0.0f, n = 0.0f;
-  int q0, m, blocks = 0, most = 1;
-  Span sp;
-  if (lane < a.batch) {
-    sequence_span<ROWS>(g, a, lane, &q0, &m, &sp, &blocks);
-    n = (float)(blocks * g.nkv);
-    u = (float)sp.units * n;
-    most = blocks ? sp.units : 1;
-  }
-  const float total = __int_as_float(lane63(wave_prefix(__float_as_int(u), SumF())));
-  const float segments = __int_as_float(lane63(wave_prefix(__float_as_int(n), SumF())));
-  const int size = uniform(slice_units(a, total, segments, lane63(wave_prefix(most, Max()))));
-  const int count = lane < a.batch ? slices_of(sp, size) * blocks * g.nkv : 0;
-  const int inc = wave_prefix(count, Sum());
-  if (want < 0) return {size, b, __builtin_amdgcn_readlane(inc - count, uniform(b))};
-  if (const uint64_t past = __ballot(inc > want && count > 0)) {
-    const int l = __builtin_ctzll(past);
-    return {size, l, __builtin_amdgcn_readlane(inc - count, l)};
-  }
-  return {size, a.batch, 0};
-}
-
-// The cut of many sequences, once for the call.  One workgroup.
 template <int NB>
 __global__ __launch_bounds__(1024) void q8_plan_kernel(Geo g, AttendArgs a) {
-  constexpr int ROWS = 16 * NB;
-  __shared__ float units[16], segments[16];
-  __shared__ int longest[16], sums[2][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  int q0, m, blocks;
-  Span sp;
-  float u = 0.0f, n = 0.0f;
-  int most = 1;
-  for (int b = tid; b < a.batch; b += 1024) {
-    sequence_span<ROWS>(g, a, b, &q0, &m, &sp, &blocks);
-    n += (float)(blocks * g.nkv);
-    u += (float)sp.units * (float)(blocks * g.nkv);
-    most = blocks && sp.units > most ? sp.units : most;
-  }
-  u = __int_as_float(lane63(wave_prefix(__float_as_int(u), SumF())));
-  n = __int_as_float(lane63(wave_prefix(__float_as_int(n), SumF())));
-  most = lane63(wave_prefix(most, Max()));
-  if (lane == 0) {
-    units[wave] = u;
-    segments[wave] = n;
-    longest[wave] = most;
-  }
-  __syncthreads();
-  u = n = 0.0f;
-  for (int i = 0; i < 16; ++i) {
-    u += units[i];
-    n += segments[i];
-    most = longest[i] > most ? longest[i] : most;
-  }
-  const int size = uniform(slice_units(a, u, n, most));
-  int before = 0;
-  for (int base = 0, turn = 0; base < a.batch; base += 1024, turn ^= 1) {
-    const int b = base + tid;
-    int count = 0;
-    if (b < a.batch) {
-      sequence_span<ROWS>(g, a, b, &q0, &m, &sp, &blocks);
-      count = slices_of(sp, size) * blocks * g.nkv;
-    }
-    const int inc = wave_prefix(count, Sum());
-    if (lane == 63) sums[turn][wave] = inc;
-    __syncthreads();  // the other turn's sums have been read by all
-    int here = before + inc - count;
-    for (int i = 0; i < 16; ++i) {
-      here += i < wave ? sums[turn][i] : 0;
-      before += sums[turn][i];
-    }
-    if (b < a.batch) a.plan[b] = here;
-  }
-  if (tid == 0) {
-    a.plan[a.batch] = before;
-    a.plan[a.batch + 1] = size;
-  }
+  plan_cut<16 * NB>(g, a);
 }
 
-// A workgroup of kWaves wavefronts has a slice of a segment.  target > 0: slice blockIdx.x of the
+// A workgroup of kSliceWaves wavefronts has a slice of a segment.  target > 0: slice blockIdx.x of the
 // cut; else the segment blockIdx.x = (sequence, row block, kv head) whole.
 template <int HD, bool E4M3, int NB>
-__global__ __launch_bounds__(64 * kWaves, decode_groups(HD, NB)) void q8_decode_kernel(Geo g,
+__global__ __launch_bounds__(64 * kSliceWaves, decode_groups(HD, NB)) void q8_decode_kernel(Geo g,
                                                                                  AttendArgs a) {
   constexpr int ROWS = 16 * NB;
   constexpr int LD = HD + 4;
-  __shared__ __align__(16) float red[kWaves][ROWS][LD];
-  __shared__ float ml[kWaves][ROWS][2];
+  __shared__ __align__(16) float red[kSliceWaves][ROWS][LD];
+  __shared__ float ml[kSliceWaves][ROWS][2];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   Wave<HD, E4M3, NB> w(g, a, lane);
-  Segment s;
+  Segment<Geo> s;
   int u0 = 0, u1, blocks;
   bool whole = true;
   if (a.target) {
@@ -587,16 +424,16 @@ __global__ __launch_bounds__(64 * kWaves, decode_groups(HD, NB)) void q8_decode_
   }
   __syncthreads();
   constexpr int PER = HD / 16;  // channels of a thread
-  for (int i = threadIdx.x; i < s.nrows * 16; i += 64 * kWaves) {
+  for (int i = threadIdx.x; i < s.nrows * 16; i += 64 * kSliceWaves) {
     const int row = i / 16, ch = i % 16 * PER;
     float mm = kNegInf, l = 0.0f;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, ml[v][row][0]);
+    for (int v = 0; v < kSliceWaves; ++v) mm = fmaxf(mm, ml[v][row][0]);
     float x[PER];
 #pragma unroll
     for (int c = 0; c < PER; ++c) x[c] = 0.0f;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
+    for (int v = 0; v < kSliceWaves; ++v) {
       // a part without a maximum saw nothing, or only NaN: l tells
       const float mv = ml[v][row][0];
       const float f = mv == kNegInf ? 1.0f : exp2_(mv - mm);
@@ -618,85 +455,9 @@ __global__ __launch_bounds__(64 * kWaves, decode_groups(HD, NB)) void q8_decode_
   }
 }
 
-// Joins a segment's slices, in their order.  blockIdx.x: segment.  MANY: of the row blockIdx.y, the
-// threads side by side share the slices; else they share the rows.
 template <int HD, int NB, bool MANY>
 __global__ __launch_bounds__(256) void q8_join_kernel(Geo g, AttendArgs a) {
-  constexpr int ROWS = 16 * NB;
-  constexpr int TC = HD / 4;      // threads of a row
-  constexpr int PG = 256 / TC;    // rows, or slices, at a time
-  const int lane = threadIdx.x & 63;
-  Segment s;
-  int blocks;
-  s.b = blockIdx.x / (g.nkv * a.row_blocks);
-  s.h = blockIdx.x % g.nkv;
-  s.rb = blockIdx.x / g.nkv % a.row_blocks;
-  sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
-  if (s.rb >= blocks) return;
-  const int left = s.m * g.gqa - s.rb * ROWS;
-  s.nrows = left < ROWS ? left : ROWS;
-  if (MANY && (int)blockIdx.y >= s.nrows) return;
-  const Slices c = cut<ROWS>(g, a, lane, -1, s.b);
-  const int n = uniform(slices_of(s.span, c.size));
-  if (n == 1) return;
-  const int64_t first = c.before + s.rb * g.nkv + s.h;
-  const int step = blocks * g.nkv;
-  const int grp = threadIdx.x / TC, ch = threadIdx.x % TC * 4;
-  auto add = [&](float pm, float pl, f4 pa, float& mm, float& l, f4& acc) {
-    const float to = fmaxf(mm, pm);
-    const float f0 = mm == kNegInf ? 1.0f : exp2_(mm - to);
-    const float f1 = pm == kNegInf ? 1.0f : exp2_(pm - to);
-    acc = acc * f0 + pa * f1;
-    l = l * f0 + pl * f1;
-    mm = to;
-  };
-  // slices z0, z0 + by, ... of a row, 4 in flight
-  auto sum = [&](int row, int z0, int by, float& mm, float& l, f4& acc) {
-    for (int z = z0; z < n; z += 4 * by) {
-      float pm[4], pl[4];
-      f4 pa[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int zz = z + i * by < n ? z + i * by : z;
-        const int64_t at = (first + (int64_t)zz * step) * a.rows + row;
-        pm[i] = a.part_ml[at * 2];
-        pl[i] = a.part_ml[at * 2 + 1];
-        pa[i] = *(const f4*)(a.part_acc + at * HD + ch);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (z + i * by < n) add(pm[i], pl[i], pa[i], mm, l, acc);
-    }
-  };
-  if constexpr (!MANY) {
-    for (int row = grp; row < s.nrows; row += PG) {
-      float mm = kNegInf, l = 0.0f;
-      f4 acc = {0, 0, 0, 0};
-      sum(row, 0, 1, mm, l, acc);
-      float o[4] = {acc.x, acc.y, acc.z, acc.w};
-      finish_row(g, a, s, row, HD, ch, o, 4, l, mm);
-    }
-  } else {
-    __shared__ __align__(16) float red[PG][HD];
-    __shared__ float ml[PG][2];
-    const int row = blockIdx.y;
-    float mm = kNegInf, l = 0.0f;
-    f4 acc = {0, 0, 0, 0};
-    sum(row, grp, PG, mm, l, acc);
-    *(f4*)&red[grp][ch] = acc;
-    if (ch == 0) {
-      ml[grp][0] = mm;
-      ml[grp][1] = l;
-    }
-    __syncthreads();
-    if (threadIdx.x >= TC) return;
-    mm = kNegInf;
-    l = 0.0f;
-    acc = f4{0, 0, 0, 0};
-    for (int i = 0; i < PG; ++i) add(ml[i][0], ml[i][1], *(const f4*)&red[i][ch], mm, l, acc);
-    float o[4] = {acc.x, acc.y, acc.z, acc.w};
-    finish_row(g, a, s, row, HD, ch, o, 4, l, mm);
-  }
+  join_slices<HD, 16 * NB, MANY>(g, a);
 }
 
 // Adds up the weight of every block: a lane per 16 tokens, a wavefront every fourth kv head; their
@@ -746,7 +507,7 @@ static void decode_kernels(const Geo& g, const AttendArgs& a, hipStream_t s) {
   const int segments = a.batch * g.nkv * a.row_blocks;
   const unsigned blocks = a.target ? a.target + segments : segments;
   if (a.plan) hipLaunchKernelGGL((q8_plan_kernel<NB>), dim3(1), dim3(1024), 0, s, g, a);
-  hipLaunchKernelGGL((q8_decode_kernel<HD, E4M3, NB>), dim3(blocks), dim3(64 * kWaves), 0, s, g, a);
+  hipLaunchKernelGGL((q8_decode_kernel<HD, E4M3, NB>), dim3(blocks), dim3(64 * kSliceWaves), 0, s, g, a);
   if (a.target) {
     // from about 16 slices a segment on, a workgroup per row: its threads share the slices (at 8
     // to 16, 8 sequences of 100 to 3000 tokens, 16/16 heads of 64, 4 queries: 16.0 us against 14.6)

@@ -34,7 +34,6 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kRows = kPrefillRows;
 static_assert(kRows == 32 * kWaves, "32 a wavefront");
-constexpr float kNegInf = -__builtin_inff();
 
 template <int HD>
 struct Lds {
@@ -43,43 +42,12 @@ struct Lds {
   float ks[4][4], lvs[4][4], ivs[4][4];  // per 16 tokens: K scale, log2 and inverse of V's
 };
 
-// LDS writes are done, loads from memory may be in flight.
-__device__ inline void turn() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // Where chunk c (8 values) of a row lies, so that 16 rows' same chunk covers all banks.
 template <int HD>
 __device__ inline int k_chunk(int row, int c) {
   return HD == 128 ? c ^ (row & 15) : c ^ (row >> 1 & 7);
 }
 __device__ inline int v_chunk(int d, int c) { return c ^ (d >> 1 & 7); }
-
-// The value of the lane 32 on (or back).
-__device__ inline float other_half(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
-}
-
-// 4 values of O, in its type.
-__device__ inline void store4(const AttendArgs& a, int64_t at, f4 x) {
-  if (a.o_type == JACQ_Q8_FP32) {
-    *(f4*)((float*)a.o + at) = x;
-    return;
-  }
-  const bool bf = a.o_type == JACQ_Q8_BF16;
-  const uint32_t x0 = bf ? f2bf(x.x) : f2h_(x.x), x1 = bf ? f2bf(x.y) : f2h_(x.y);
-  const uint32_t x2 = bf ? f2bf(x.z) : f2h_(x.z), x3 = bf ? f2bf(x.w) : f2h_(x.w);
-  *(u2*)((uint16_t*)a.o + at) = u2{x0 | x1 << 16, x2 | x3 << 16};
-}
-
-// Bits 0 to n - 1; n in any range.
-__device__ inline uint64_t low_bits(int n) {
-  return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
-}
 
 template <int HD, bool E4M3>
 __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendArgs a) {
@@ -453,33 +421,9 @@ __global__ __launch_bounds__(kThreads, 2) void q8_prefill_kernel(Geo g, AttendAr
              f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]} * inv);
 }
 
-// Joins the slices of every row, in their order: a thread per 4 channels.
 template <int HD>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Geo g, AttendArgs a) {
-  static_assert(256 / (HD / 4) == 1 << merge_log2(HD), "rows of a workgroup");
-  const Place p = place_of(g, a, blockIdx.x, g.nh, merge_log2(HD));
-  const int slices = prefill_slices(a, p.n);
-  if (slices == 1 || p.at < 0) return;
-  const int64_t i = (int64_t)p.at * 256 + threadIdx.x;
-  const int ch = (int)(i % (HD / 4)) * 4;
-  if (i / (HD / 4) >= (int64_t)p.m * g.nh) return;
-  const int64_t at = (int64_t)p.q0 * g.nh + i / (HD / 4), rows = (int64_t)a.total_q * g.nh;
-  float mx = kNegInf, l = 0.0f;
-  f4 acc = {0, 0, 0, 0};
-  for (int s = 0; s < slices; ++s) {
-    const float pm = a.part_ml[2 * (s * rows + at)], pl = a.part_ml[2 * (s * rows + at) + 1];
-    const f4 pa = *(const f4*)(a.part_acc + (s * rows + at) * HD + ch);
-    const float to = fmaxf(mx, pm);
-    // a part without a maximum saw nothing, or only NaN: l tells
-    const float f0 = mx == kNegInf ? 1.0f : exp2_(mx - to);
-    const float f1 = pm == kNegInf ? 1.0f : exp2_(pm - to);
-    acc = acc * f0 + pa * f1;
-    l = l * f0 + pl * f1;
-    mx = to;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  store4(a, at * HD + ch, acc * inv);
-  if (a.lse && ch == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
+  merge_slices<HD>(g, a);
 }
 
 template <int HD, bool E4M3>
