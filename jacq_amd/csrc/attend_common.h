@@ -370,6 +370,79 @@ __device__ inline Slices cut(const G& g, const A& a, int lane, int want, int b) 
   return {size, a.batch, 0};
 }
 
+// The segment of this workgroup, and its units of it: target > 0: slice blockIdx.x of the cut; else
+// the segment blockIdx.x = (sequence, row block, kv head) whole.  False: none.
+template <int ROWS, class G, class A>
+__device__ inline bool place_slice(const G& g, const A& a, int lane, Segment<G>& s, int& u0, int& u1,
+                                   bool& whole) {
+  int blocks;
+  u0 = 0;
+  whole = true;
+  if (a.target) {
+    const Slices c = cut<ROWS>(g, a, lane, blockIdx.x, 0);
+    if (c.b >= a.batch) return false;
+    s.b = c.b;
+    sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
+    int x = blockIdx.x - c.before;
+    s.h = uniform(x % g.nkv);
+    x /= g.nkv;
+    s.rb = uniform(x % blocks);
+    const int z = uniform(x / blocks), n = uniform(slices_of(s.span, c.size));
+    const int each = uniform(even_units(s.span, n));
+    u0 = z * each;
+    u1 = u0 + each < s.span.units ? u0 + each : s.span.units;
+    whole = n == 1;
+  } else {
+    s.b = blockIdx.x / (g.nkv * a.row_blocks);
+    s.h = blockIdx.x % g.nkv;
+    s.rb = blockIdx.x / g.nkv % a.row_blocks;
+    sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
+    if (s.rb >= blocks) return false;
+    u1 = s.span.units;
+  }
+  const int left = s.m * g.gqa - s.rb * ROWS;
+  s.nrows = left < ROWS ? left : ROWS;
+  return true;
+}
+
+// Joins the wavefronts' parts of a slice: sum(w v) in red[wave][row][channel] and, in ml, the maximum
+// that w refers to and the sum of w; to O, or to the slice's place in the workspace.
+template <int HD, class G, class A, int ROWS, int LD>
+__device__ inline void fold_parts(const G& g, const A& a, const Segment<G>& s, bool whole,
+                                  const float (&red)[kSliceWaves][ROWS][LD],
+                                  const float (&ml)[kSliceWaves][ROWS][2]) {
+  constexpr int PER = HD / 16;  // channels of a thread
+  for (int i = threadIdx.x; i < s.nrows * 16; i += 64 * kSliceWaves) {
+    const int row = i / 16, ch = i % 16 * PER;
+    float mm = kNegInf, l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kSliceWaves; ++v) mm = fmaxf(mm, ml[v][row][0]);
+    float x[PER];
+#pragma unroll
+    for (int c = 0; c < PER; ++c) x[c] = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kSliceWaves; ++v) {
+      // a part without a maximum saw nothing, or only NaN: l tells
+      const float mv = ml[v][row][0];
+      const float f = mv == kNegInf ? 1.0f : exp2_(mv - mm);
+      l += ml[v][row][1] * f;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) x[c] += red[v][row][ch + c] * f;
+    }
+    if (whole) {
+      finish_row(g, a, s, row, HD, ch, x, PER, l, mm);
+    } else {
+      const int64_t at = (int64_t)blockIdx.x * a.rows + row;
+#pragma unroll
+      for (int c = 0; c < PER; c += 4) *(f4*)(a.part_acc + at * HD + ch + c) = *(f4*)(x + c);
+      if (ch == 0) {
+        a.part_ml[at * 2] = mm;
+        a.part_ml[at * 2 + 1] = l;
+      }
+    }
+  }
+}
+
 // The cut of many sequences, once for the call.  One workgroup of 1024.
 template <int ROWS, class G, class A>
 __device__ inline void plan_cut(const G& g, const A& a) {

@@ -32,6 +32,12 @@ int fail(int code, const std::string& msg) {
   return code;
 }
 
+}  // namespace
+
+int jacq::set_last_error(int code, const std::string& msg) { return fail(code, msg); }
+
+namespace {
+
 // Reference geometries: source_patch.py:660-671 (NH/NKV/TP2 local, HD,
 // OLD_BLOCKS, BLOCK_SIZE, RESIDUAL).
 constexpr jacq_kivi_geometry kGlobal = {40, 8, 128, 32, 32, 128, 124, INT32_MAX};

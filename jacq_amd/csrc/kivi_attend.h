@@ -1,0 +1,193 @@
+// kivi_attend.h -- attention of chunks of queries over the int4 cache, and its read-back: arguments,
+// spans, dequantisation.
+#pragma once
+
+#include "attend_common.h"
+#include "kivi_common.h"
+
+namespace jacq {
+
+struct KiviPool {
+  const uint8_t* k_code;
+  const uint16_t* k_scale;
+  const uint16_t* k_zero;
+  const uint8_t* v_code;
+  const uint16_t* v_scale;
+  const uint16_t* v_zero;
+  const uint16_t* k_scr;
+  const uint16_t* v_scr;
+};
+
+struct KiviAttendArgs {
+  KiviPool pool;
+  const uint16_t* q;
+  const int32_t* cu;
+  const int32_t* lens;
+  const int32_t* tables;
+  void* o;
+  float* lse;             // null: not wanted
+  float* row_lse;         // null
+  int64_t q_stride;
+  int q_bf16, o_type;     // o_type: kFp16, kBf16, kFp32
+  int batch, total_q, max_q;
+  int window, sinks;      // window 0: none
+  int causal;             // 0: every query sees every token
+  float scale;            // log2(e) included
+  // split pieces
+  float* part_ml;         // few queries: [target + segments][rows][2]
+  float* part_acc;        // the same [HD]
+  int32_t* plan;          // calls of many sequences: [batch + 1] first slices, then their size
+  int target;             // slices to aim at; 0: segments stay whole
+  int cus;                // compute units
+  int rows;               // rows of a segment at most (<= 16 NB)
+  int row_blocks;         // row blocks of a sequence at most
+};
+
+__device__ inline int clamp_len(const KiviGeo& g, int n) {
+  const int cap = g.lq + g.residual;
+  return n < 0 ? 0 : n > cap ? cap : n;
+}
+
+// The units of kGroup tokens that the queries of a sequence of n tokens may see, in order: the
+// sinks', then the window's; int4 groups before `old`, fp16 rows of the residual window from there.
+struct KiviSpan {
+  int n;        // tokens
+  int first;    // the lowest position of a query (may be negative)
+  int old;      // tokens in int4
+  int w0;       // first unit of the window
+  int ns;       // units of the sinks before it
+  int units;    // of a segment, at least 1 (a segment without tokens still writes its zeros)
+  __device__ int tile_of(int u) const { return u < ns ? u : w0 + u - ns; }
+};
+
+__device__ inline KiviSpan make_span(const KiviGeo& g, const KiviAttendArgs& a, int n, int all) {
+  KiviSpan s;
+  int residual;
+  s.n = n;
+  s.first = a.causal ? n - all : n - 1;
+  decode_window(g, n, &s.old, &residual);
+  const int tiles = (n + kGroup - 1) / kGroup;
+  s.w0 = s.ns = 0;
+  if (a.window > 0 && s.first >= a.window) {
+    s.w0 = (s.first - a.window + 1) / kGroup;
+    const int sinks = a.sinks < n ? a.sinks : n;
+    s.ns = (sinks + kGroup - 1) / kGroup;
+    s.ns = s.ns > s.w0 ? s.w0 : s.ns;
+  }
+  s.units = s.ns + tiles - s.w0;
+  s.units = s.units < 1 ? 1 : s.units;
+  return s;
+}
+
+template <>
+struct SpanOf<KiviGeo> {
+  typedef KiviSpan type;
+};
+
+// ---- codes to fp16 ----
+// A code in a byte of its own is, as e4m3, code x 2^-9 (the format's steps from 0 to 16 x 2^-9 are
+// even), so the conversion instruction with scale 2^9 gives two codes as exact fp16.  A value is
+// code * scale + zero, rounded to fp16 once: off by at most half a step, 2^-11 of it.
+
+struct Nibbles {
+  uint32_t even, odd;  // a dword's codes 0, 2, 4, 6 and 1, 3, 5, 7, a byte each
+  __device__ Nibbles(uint32_t w) : even(w & 0x0f0f0f0fu), odd(w >> 4 & 0x0f0f0f0fu) {}
+};
+__device__ inline h2 codes_lo(uint32_t bytes) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)bytes, 512.0f, false);
+}
+__device__ inline h2 codes_hi(uint32_t bytes) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)bytes, 512.0f, true);
+}
+__device__ inline h2 fma2(h2 c, h2 s, h2 z) { return __builtin_elementwise_fma(c, s, z); }
+__device__ inline h2 pair(uint32_t x) { return __builtin_bit_cast(h2, x); }
+__device__ inline uint32_t bits(h2 x) { return __builtin_bit_cast(uint32_t, x); }
+
+// 8 channels of a token (one dword), scales and zeros as they lie: the channels in their order.
+__device__ inline h8 values8(uint32_t w, u4 s, u4 z) {
+  const Nibbles n(w);
+  const uint32_t lo = __builtin_amdgcn_perm(n.odd, n.even, 0x05010400u);  // codes 0, 1, 2, 3
+  const uint32_t hi = __builtin_amdgcn_perm(n.odd, n.even, 0x07030602u);  // 4, 5, 6, 7
+  h8 r;
+  r.s01 = fma2(codes_lo(lo), pair(s.x), pair(z.x));
+  r.s23 = fma2(codes_hi(lo), pair(s.y), pair(z.y));
+  r.s45 = fma2(codes_lo(hi), pair(s.z), pair(z.z));
+  r.s67 = fma2(codes_hi(hi), pair(s.w), pair(z.w));
+  return r;
+}
+
+// 8 channels of two tokens (a dword each), s and z the two tokens' of their 32 channels: out[c] is
+// channel c of both.
+__device__ inline void values8x2(uint32_t a, uint32_t b, h2 s, h2 z, h2 (&out)[8]) {
+  const Nibbles x(a), y(b);
+  const uint32_t e0 = __builtin_amdgcn_perm(y.even, x.even, 0x05010400u);  // channels 0 and 2
+  const uint32_t e1 = __builtin_amdgcn_perm(y.even, x.even, 0x07030602u);  // 4 and 6
+  const uint32_t o0 = __builtin_amdgcn_perm(y.odd, x.odd, 0x05010400u);    // 1 and 3
+  const uint32_t o1 = __builtin_amdgcn_perm(y.odd, x.odd, 0x07030602u);    // 5 and 7
+  out[0] = fma2(codes_lo(e0), s, z);
+  out[1] = fma2(codes_lo(o0), s, z);
+  out[2] = fma2(codes_hi(e0), s, z);
+  out[3] = fma2(codes_hi(o0), s, z);
+  out[4] = fma2(codes_lo(e1), s, z);
+  out[5] = fma2(codes_lo(o1), s, z);
+  out[6] = fma2(codes_hi(e1), s, z);
+  out[7] = fma2(codes_hi(o1), s, z);
+}
+
+// The same of 4 channels of two tokens: w has the first token's 16 bits, then the second's.
+__device__ inline void values4x2(uint32_t w, h2 s, h2 z, h2 (&out)[4]) {
+  const Nibbles x(w);
+  const uint32_t e = __builtin_amdgcn_perm(0u, x.even, 0x03010200u);  // channels 0 and 2
+  const uint32_t o = __builtin_amdgcn_perm(0u, x.odd, 0x03010200u);   // 1 and 3
+  out[0] = fma2(codes_lo(e), s, z);
+  out[1] = fma2(codes_lo(o), s, z);
+  out[2] = fma2(codes_hi(e), s, z);
+  out[3] = fma2(codes_hi(o), s, z);
+}
+
+// A query row's values for the matrix cores, 8 of them in each of N operands, from fp16 or bf16, and
+// the scale that goes with them.  fp16 has the bits of bf16 but not its range: a power of two brings
+// the row's largest magnitude (`most` joins it over the row's lanes) to 2^14, so values down to 2^-28
+// of it keep all their bits.
+template <int N, class F>
+__device__ inline float half_row(const u4 (&raw)[N], int bf16, float scale, h8 (&q)[N], F most) {
+  if (!bf16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = __builtin_bit_cast(h8, raw[i]);
+    return scale;
+  }
+  auto value = [&](int i, int c) {
+    return __uint_as_float(c & 1 ? raw[i][c / 2] & 0xffff0000u : raw[i][c / 2] << 16);
+  };
+  float big = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) big = fmaxf(big, __builtin_fabsf(value(i, c)));
+  big = most(big);
+  const bool plain = !(big > 0.0f && big < __builtin_inff());
+  const int e = plain ? 0 : 14 - __builtin_amdgcn_frexp_expf(big);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) q[i][c] = (_Float16)__builtin_amdgcn_ldexpf(value(i, c), e);
+  return __builtin_amdgcn_ldexpf(scale, -e);
+}
+
+// The largest magnitude of two sets of fp16 pairs as bits, in either half: 0x7c00 and more is no
+// finite value.
+__device__ inline uint32_t most_bits(uint32_t a, uint32_t b) {
+  typedef uint16_t s2 __attribute__((ext_vector_type(2)));
+  const s2 x = __builtin_bit_cast(s2, a & 0x7fff7fffu), y = __builtin_bit_cast(s2, b & 0x7fff7fffu);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
+}
+__device__ inline uint32_t either_half(uint32_t x) { return (x >> 16) > (x & 0xffffu) ? x >> 16 : x & 0xffffu; }
+
+hipError_t launch_attend_few(const KiviGeo& g, const KiviAttendArgs& a, int nb, hipStream_t s);
+hipError_t launch_kivi_read(const KiviGeo& g, const KiviPool& p, const int32_t* starts,
+                            const int32_t* ends, const int32_t* tables, int batch, int total, void* k,
+                            void* v, int type, hipStream_t s);
+// Workgroups of the few-query kernel that a CU holds.
+constexpr int few_groups(int hd, int nb) { return hd == 64 && nb == 1 ? 3 : 2; }
+
+}  // namespace jacq

@@ -1,0 +1,267 @@
+// kivi_attend_api.hip -- host side of the int4 cache's attention of chunks and of its read-back: the
+// C ABI of include/jacq_kivi_attend.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <initializer_list>
+#include <string>
+
+#include "jacq_kivi_attend.h"
+#include "kivi_attend.h"
+#include "kivi_kernels.h"
+
+namespace {
+
+using jacq::KiviAttendArgs;
+using jacq::KiviGeo;
+using jacq::KiviPool;
+
+static_assert(jacq::kFp16 == JACQ_KIVI_FP16 && jacq::kBf16 == JACQ_KIVI_BF16 &&
+                  jacq::kFp32 == JACQ_KIVI_FP32,
+              "types");
+
+int fail(const std::string& msg) { return jacq::set_last_error(JACQ_KIVI_EINVAL, msg); }
+
+// No C++ exception leaves a C entry.
+template <class F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (...) {
+    return JACQ_KIVI_ENOMEM;
+  }
+}
+
+int launched(hipError_t e, const char* what) {
+  if (e == hipSuccess) return JACQ_KIVI_OK;
+  return jacq::set_last_error(JACQ_KIVI_EHIP,
+                              std::string(what) + " launch failed: " + hipGetErrorString(e));
+}
+
+bool aligned(std::initializer_list<const void*> ps, uintptr_t to) {
+  uintptr_t bits = 0;
+  for (const void* p : ps) bits |= (uintptr_t)p;
+  return (bits & (to - 1)) == 0;
+}
+
+KiviGeo make_geo(const jacq_kivi_geometry& x) {
+  KiviGeo g;
+  g.nh = x.num_heads;
+  g.nkv = x.num_kv_heads;
+  g.hd = x.head_dim;
+  g.page = x.page_size;
+  g.residual = x.residual;
+  g.max_pages = x.max_pages_per_seq;
+  g.num_pages = x.num_pages;
+  g.gqa = x.num_heads / x.num_kv_heads;
+  g.rs = x.residual + jacq::kGroup;
+  g.lq = (int)(((int64_t)x.max_pages_per_seq * x.page_size / jacq::kGroup) * jacq::kGroup);
+  return g;
+}
+
+int check_geometry(const jacq_kivi_geometry* x) {
+  if (int e = jacq_kivi_check_geometry(x)) return e;
+  if (x->num_heads > 65536) return fail("num_heads must be <= 65536");
+  return JACQ_KIVI_OK;
+}
+
+int check_pool(const jacq_kivi_pool* p) {
+  if (!p || !p->k_code || !p->k_scale || !p->k_zero || !p->v_code || !p->v_scale || !p->v_zero ||
+      !p->k_scratch || !p->v_scratch)
+    return fail("a pool pointer is null");
+  if (!aligned({p->k_code, p->k_scale, p->k_zero, p->v_code, p->v_scale, p->v_zero, p->k_scratch,
+                p->v_scratch},
+               16))
+    return fail("pool pointers must be 16-byte aligned");
+  return JACQ_KIVI_OK;
+}
+
+int check_batch(int32_t batch) {
+  if (batch < 0 || batch > 65535)
+    return fail("batch must be in [0, 65535], got " + std::to_string(batch));
+  return JACQ_KIVI_OK;
+}
+
+KiviPool read_pool(const jacq_kivi_pool& p) {
+  return {p.k_code, p.k_scale, p.k_zero, p.v_code, p.v_scale, p.v_zero, p.k_scratch, p.v_scratch};
+}
+
+// Compute units of the current device, looked up once per device.
+int device_cus() {
+  constexpr int kMost = 64;
+  static std::atomic<int> known[kMost];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (dev >= 0 && dev < kMost)
+    if (const int c = known[dev].load(std::memory_order_relaxed)) return c;
+  int cus = 0;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+      cus < 1)
+    return 256;
+  if (dev >= 0 && dev < kMost) known[dev].store(cus, std::memory_order_relaxed);
+  return cus;
+}
+
+// ---- how an attention call runs ----
+// Units (of 32 tokens) up to which segments stay whole: no plan, no join.  The table's width bounds
+// them.
+constexpr int kWholeUnits = 24;
+// Sequences up to which every workgroup finds the cut by itself (a lane each); more have a kernel
+// for it.
+constexpr int kCutBatch = 64;
+
+struct Plan {
+  bool planned;
+  int nb, rows, row_blocks, target;
+  size_t ml, acc, plan, bytes;  // offsets into the workspace, and its size
+};
+
+Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
+  Plan p = {};
+  const int64_t rows = (int64_t)max_q * g.gqa;
+  // The call's queries, not max_q for every sequence: of a cache's sequences some may have none.
+  const int64_t queries = std::min<int64_t>((int64_t)batch * max_q, total_q);
+  // Their blocks of so many rows: of as few sequences as they can be of, and a begun one more for
+  // each but the first, as most calls of several are ragged.
+  auto blocks = [&](int64_t block) {
+    const int64_t each = (rows + block - 1) / block, full = queries / max_q, rest = queries % max_q;
+    return std::min(batch * each, full * each + (rest * g.gqa + block - 1) / block +
+                                      full + (rest > 0) - 1);
+  };
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  p.nb = rows <= 16 ? 1 : 2;
+  p.rows = (int)std::min<int64_t>(rows, 16 * p.nb);
+  p.row_blocks = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
+  const int64_t most = (g.lq + g.residual + jacq::kGroup - 1) / jacq::kGroup;  // units of a segment
+  const int64_t segments = (int64_t)batch * g.nkv * p.row_blocks;
+  if (most > kWholeUnits) {
+    const int64_t slots = (int64_t)jacq::few_groups(g.hd, p.nb) * device_cus();
+    p.target = (int)(3 * blocks(16 * p.nb) * g.nkv <= slots ? slots : 2 * slots);
+  }
+  const size_t parts = p.target ? (size_t)p.target + segments : 0;
+  p.ml = take(parts * p.rows * 2 * sizeof(float));
+  p.acc = take(parts * p.rows * g.hd * sizeof(float));
+  p.planned = p.target && batch > kCutBatch;
+  p.plan = take(p.planned ? ((size_t)batch + 2) * sizeof(int32_t) : 0);
+  p.bytes = at;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t jacq_kivi_attend_workspace_size(const jacq_kivi_geometry* geo, int32_t batch, int32_t total_q,
+                                       int32_t max_q) {
+  size_t bytes = 0;
+  guarded([&]() -> int {
+    if (int e = check_geometry(geo)) return e;
+    if (batch > 0 && total_q > 0 && max_q > 0)
+      bytes = plan_attend(make_geo(*geo), batch, total_q, std::min(max_q, total_q)).bytes;
+    return JACQ_KIVI_OK;
+  });
+  return bytes;
+}
+
+int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
+                     const jacq_kivi_attend_args* x, void* workspace, size_t workspace_bytes,
+                     hipStream_t stream) {
+  return guarded([&]() -> int {
+    if (int e = check_geometry(geo)) return e;
+    if (int e = check_pool(pool)) return e;
+    if (!x) return fail("argument record is null");
+    if (int e = check_batch(x->batch)) return e;
+    if (x->q_dtype != JACQ_KIVI_FP16 && x->q_dtype != JACQ_KIVI_BF16)
+      return fail("queries must be fp16 or bf16");
+    if (x->o_dtype != x->q_dtype && x->o_dtype != JACQ_KIVI_FP32)
+      return fail("the output is of the queries' type or fp32");
+    if (x->total_q < 0 || x->max_q < 0) return fail("negative number of queries");
+    if (!x->CU_Q && (x->total_q != x->batch || (x->batch && x->max_q != 1)))
+      return fail("without CU_Q every sequence has one query");
+    if (x->window < 0 || x->sinks < 0) return fail("window and sinks must not be negative");
+    if (x->causal != 0 && x->causal != 1) return fail("causal must be 0 or 1");
+    if (!x->causal && (x->window || x->sinks))
+      return fail("queries that see every token have no window and no sinks");
+    if (!std::isfinite(x->scale) || x->scale <= 0) return fail("scale must be positive and finite");
+    const int64_t row = (int64_t)geo->num_heads * geo->head_dim;
+    if (x->q_stride < row || x->q_stride % 8 != 0)
+      return fail("Q row stride must be a multiple of 8 and at least " + std::to_string(row) +
+                  ", got " + std::to_string(x->q_stride));
+    if (x->batch == 0 || x->total_q == 0 || x->max_q == 0) return JACQ_KIVI_OK;
+    if (!x->Q || !x->O || !x->SEQ_LENS || (!x->BLOCK_TABLES && geo->max_pages_per_seq > 0))
+      return fail("a tensor pointer is null");
+    if (!aligned({x->Q, x->O, workspace}, 16) ||
+        !aligned({x->CU_Q, x->SEQ_LENS, x->BLOCK_TABLES, x->LSE}, 4))
+      return fail("Q, O and workspace pointers must be 16-byte aligned, the others 4-byte");
+    const KiviGeo g = make_geo(*geo);
+    KiviAttendArgs a = {};
+    a.pool = read_pool(*pool);
+    a.q = (const uint16_t*)x->Q;
+    a.cu = x->CU_Q;
+    a.lens = x->SEQ_LENS;
+    a.tables = x->BLOCK_TABLES;
+    a.o = x->O;
+    a.lse = x->LSE;
+    a.q_stride = x->q_stride;
+    a.q_bf16 = x->q_dtype == JACQ_KIVI_BF16;
+    a.o_type = x->o_dtype;
+    a.batch = x->batch;
+    a.total_q = x->total_q;
+    a.max_q = std::min(x->max_q, x->total_q);
+    a.window = std::min(x->window, 1 << 30);
+    a.sinks = std::min(x->sinks, 1 << 30);
+    a.causal = x->causal;
+    a.scale = x->scale * jacq::kLog2e;
+    const Plan p = plan_attend(g, a.batch, a.total_q, a.max_q);
+    const int64_t segments = (int64_t)a.batch * g.nkv * p.row_blocks;
+    // a launch has fewer than 2^32 threads
+    if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 || segments + p.target >= 1 << 24)
+      return fail("too many query rows in one call");
+    if (p.bytes && (!workspace || workspace_bytes < p.bytes))
+      return jacq::set_last_error(JACQ_KIVI_ENOMEM,
+                                  "the workspace needs " + std::to_string(p.bytes) + " bytes, got " +
+                                      std::to_string(workspace ? workspace_bytes : 0));
+    uint8_t* ws = (uint8_t*)workspace;
+    a.part_ml = (float*)(ws + p.ml);
+    a.part_acc = (float*)(ws + p.acc);
+    a.target = p.target;
+    a.cus = device_cus();
+    a.plan = p.planned ? (int32_t*)(ws + p.plan) : nullptr;
+    a.rows = p.rows;
+    a.row_blocks = p.row_blocks;
+    return launched(jacq::launch_attend_few(g, a, p.nb, stream), "attention");
+  });
+}
+
+int jacq_kivi_read(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool, const int32_t* STARTS,
+                   const int32_t* ENDS, const int32_t* BLOCK_TABLES, int32_t batch, int32_t total,
+                   void* K, void* V, int32_t dtype, hipStream_t stream) {
+  return guarded([&]() -> int {
+    if (int e = check_geometry(geo)) return e;
+    if (int e = check_pool(pool)) return e;
+    if (int e = check_batch(batch)) return e;
+    if (dtype < JACQ_KIVI_FP16 || dtype > JACQ_KIVI_FP32)
+      return fail("values are read as fp16, bf16 or fp32");
+    if (total < 0) return fail("negative number of tokens");
+    if (batch == 0 || total == 0) return JACQ_KIVI_OK;
+    if (!STARTS || !ENDS || (!BLOCK_TABLES && geo->max_pages_per_seq > 0) || !K || !V)
+      return fail("a tensor pointer is null");
+    if (!aligned({K, V}, 16) || !aligned({STARTS, ENDS, BLOCK_TABLES}, 4))
+      return fail("K and V must be 16-byte aligned, tables 4-byte");
+    if ((int64_t)geo->num_kv_heads * (total / jacq::kGroup + 2 * batch) >= 1 << 24)
+      return fail("too many tokens in one read");
+    return launched(jacq::launch_kivi_read(make_geo(*geo), read_pool(*pool), STARTS, ENDS,
+                                           BLOCK_TABLES, batch, total, K, V, dtype, stream),
+                    "read");
+  });
+}
+
+}  // extern "C"

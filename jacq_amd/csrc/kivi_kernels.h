@@ -1,6 +1,8 @@
 // kivi_kernels.h -- argument blocks and launchers of the gfx950 KIVI kernels.
 #pragma once
 
+#include <string>
+
 #include "kivi_common.h"
 
 namespace jacq {
@@ -92,6 +94,9 @@ __host__ __device__ inline void window_of(const KiviGeo& g, int retained_pages, 
     *old_valid = pages * g.page / kGroup * kGroup;
   }
 }
+
+// Leaves `msg` for jacq_kivi_last_error; returns `code`.
+int set_last_error(int code, const std::string& msg);
 
 hipError_t launch_append(const KiviGeo& g, const AppendArgs& a, int batch, hipStream_t stream);
 // `between`, when not null, is recorded on the stream after the main kernel

@@ -379,32 +379,9 @@ __global__ __launch_bounds__(64 * kSliceWaves, decode_groups(HD, NB)) void q8_de
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   Wave<HD, E4M3, NB> w(g, a, lane);
   Segment<Geo> s;
-  int u0 = 0, u1, blocks;
-  bool whole = true;
-  if (a.target) {
-    const Slices c = cut<ROWS>(g, a, lane, blockIdx.x, 0);
-    if (c.b >= a.batch) return;
-    s.b = c.b;
-    sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
-    int x = blockIdx.x - c.before;
-    s.h = uniform(x % g.nkv);
-    x /= g.nkv;
-    s.rb = uniform(x % blocks);
-    const int z = uniform(x / blocks), n = uniform(slices_of(s.span, c.size));
-    const int each = uniform(even_units(s.span, n));
-    u0 = z * each;
-    u1 = u0 + each < s.span.units ? u0 + each : s.span.units;
-    whole = n == 1;
-  } else {
-    s.b = blockIdx.x / (g.nkv * a.row_blocks);
-    s.h = blockIdx.x % g.nkv;
-    s.rb = blockIdx.x / g.nkv % a.row_blocks;
-    sequence_span<ROWS>(g, a, s.b, &s.q0, &s.m, &s.span, &blocks);
-    if (s.rb >= blocks) return;
-    u1 = s.span.units;
-  }
-  const int left = s.m * g.gqa - s.rb * ROWS;
-  s.nrows = left < ROWS ? left : ROWS;
+  int u0, u1;
+  bool whole;
+  if (!place_slice<ROWS>(g, a, lane, s, u0, u1, whole)) return;
   w.start(s);
   w.units(s, u0 + wave, u1);
 
@@ -423,36 +400,7 @@ __global__ __launch_bounds__(64 * kSliceWaves, decode_groups(HD, NB)) void q8_de
       *(f4*)&red[wave][nb * 16 + w.n16][d * 16 + w.kq * 4] = w.acc[nb][d];
   }
   __syncthreads();
-  constexpr int PER = HD / 16;  // channels of a thread
-  for (int i = threadIdx.x; i < s.nrows * 16; i += 64 * kSliceWaves) {
-    const int row = i / 16, ch = i % 16 * PER;
-    float mm = kNegInf, l = 0.0f;
-#pragma unroll
-    for (int v = 0; v < kSliceWaves; ++v) mm = fmaxf(mm, ml[v][row][0]);
-    float x[PER];
-#pragma unroll
-    for (int c = 0; c < PER; ++c) x[c] = 0.0f;
-#pragma unroll
-    for (int v = 0; v < kSliceWaves; ++v) {
-      // a part without a maximum saw nothing, or only NaN: l tells
-      const float mv = ml[v][row][0];
-      const float f = mv == kNegInf ? 1.0f : exp2_(mv - mm);
-      l += ml[v][row][1] * f;
-#pragma unroll
-      for (int c = 0; c < PER; ++c) x[c] += red[v][row][ch + c] * f;
-    }
-    if (whole) {
-      finish_row(g, a, s, row, HD, ch, x, PER, l, mm);
-    } else {
-      const int64_t at = (int64_t)blockIdx.x * a.rows + row;
-#pragma unroll
-      for (int c = 0; c < PER; c += 4) *(f4*)(a.part_acc + at * HD + ch + c) = *(f4*)(x + c);
-      if (ch == 0) {
-        a.part_ml[at * 2] = mm;
-        a.part_ml[at * 2 + 1] = l;
-      }
-    }
-  }
+  fold_parts<HD>(g, a, s, whole, red, ml);
 }
 
 template <int HD, int NB, bool MANY>

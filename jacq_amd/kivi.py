@@ -18,7 +18,9 @@ layer raises ``NativeLibraryMissing``.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -142,6 +144,13 @@ def lib() -> ctypes.CDLL:
     L.jacq_kivi_cache_append.argtypes = [ctypes.POINTER(Geometry)] + [_vp] * 12 + [
         _i32, _i32, _vp]
     L.jacq_kivi_cache_append.restype = ctypes.c_int
+    geo = ctypes.POINTER(Geometry)
+    L.jacq_kivi_attend_workspace_size.argtypes = [geo, _i32, _i32, _i32]
+    L.jacq_kivi_attend_workspace_size.restype = ctypes.c_size_t
+    L.jacq_kivi_attend.argtypes = [geo, _vp, _vp, _vp, ctypes.c_size_t, _vp]  # records: packed bytes
+    L.jacq_kivi_attend.restype = ctypes.c_int
+    L.jacq_kivi_read.argtypes = [geo, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp]
+    L.jacq_kivi_read.restype = ctypes.c_int
     L.jacq_kivi_plan_batched_write.argtypes = [_i32, _i32, _i32, _i32, ctypes.POINTER(Subchunk),
                                                _i32]
     L.jacq_kivi_plan_batched_write.restype = _i32
@@ -475,6 +484,14 @@ def _raw_stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(index) if index >= 0 else _stream(t.device).value
 
 
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+# the records of jacq_kivi_attend.h packed at once: setting a structure's fields one by one takes as
+# long as a launch
+_POOL = struct.Struct("@8P")
+_ATTEND = struct.Struct("@6Pq8if4x")
+
+
 class PagedKiviCache:
     """Page pool + per-sequence fp16 residual scratch for ``batch`` sequences,
     allocated on one device.  Tensors use the v1 layouts (include/jacq_kivi.h)."""
@@ -653,3 +670,159 @@ class PagedKiviCache:
         if rc != 0:
             _raise(rc)
         return out
+
+    # ---- attention of chunks of queries, read-back (include/jacq_kivi_attend.h) ----
+
+    def _fits_pool(self, index: int) -> bool:
+        g = self.geo
+        codes = (g.num_pages, g.num_kv_heads, g.page_size, g.head_dim // 2)
+        k_scales = (g.num_pages, g.num_kv_heads, g.head_dim)
+        v_scales = (g.num_pages, g.num_kv_heads, g.page_size, g.head_dim // g.group_size)
+        scratch = (self.batch, g.num_kv_heads, g.scratch_rows, g.head_dim)
+        for t, shape, dtype in ((self.k_code, codes, torch.uint8), (self.v_code, codes, torch.uint8),
+                                (self.k_scale, k_scales, torch.float16),
+                                (self.k_zero, k_scales, torch.float16),
+                                (self.v_scale, v_scales, torch.float16),
+                                (self.v_zero, v_scales, torch.float16),
+                                (self.k_scr, scratch, torch.float16),
+                                (self.v_scr, scratch, torch.float16)):
+            if not (t.shape == shape and t.dtype is dtype and t.is_contiguous()
+                    and t.get_device() == index):
+                return False
+        return True
+
+    def _here(self, *named) -> int:
+        """The index of the cache's GPU, on which the pool and the named tensors have to be."""
+        dev = self.k_code.device
+        for name, t in named:
+            if t is not None:
+                _check(t.device == dev, name, " must be on the cache's device ", dev, ", got ",
+                       t.device)
+        _check(dev.type == "cuda", "the cache must be on a GPU device, got ", dev)
+        index = self.k_code.get_device()
+        _check(self._fits_pool(index), "the cache's tensors must have the layouts of its geometry, "
+               "contiguous, on one device")
+        return index
+
+    def _offsets(self, t: torch.Tensor, n: int, name: str) -> None:
+        check_shape(t, (n,), name)
+        _check(t.dtype == torch.int32 and t.is_contiguous(), name, " must be contiguous int32")
+
+    def _call(self, index: int, fn, *args) -> None:
+        """The call with the cache's device current, on its current stream."""
+        if torch._C._cuda_getDevice() == index:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc != 0:
+            _raise(rc)
+
+    def _attend(self, q, cu_q, max_q, seq_lens, block_tables, window, sinks, causal, scale, out, lse,
+                workspace) -> torch.Tensor:
+        g = self.geo
+        nh, hd = g.num_heads, g.head_dim
+        _check(q.dim() == 3 and q.shape[1:] == (nh, hd), "Q must be [tokens, ", nh, ", ", hd,
+               "], got ", tuple(q.shape))
+        _check(q.dtype in (torch.float16, torch.bfloat16), "Q must be fp16 or bf16")
+        total, stride = q.shape[0], nh * hd
+        if not q.is_contiguous():
+            _check(total == 0 or (q.stride(2) == 1 and q.stride(1) == hd),
+                   "Q must have its heads side by side")
+            if total > 1:
+                stride = q.stride(0)
+                _check(stride >= nh * hd, "Q must have a token's row after the one before")
+        if not self._fits(seq_lens, block_tables):
+            self._check_tables(seq_lens, block_tables)
+        _check(seq_lens.is_contiguous(), "SEQ_LENS must be contiguous")
+        if cu_q is None:
+            _check(total == self.batch, "without CU_Q there is one query per sequence: ", self.batch,
+                   ", got ", total)
+            _check(max_q is None or max_q == 1, "MAX_Q is for CU_Q")
+            max_q = 1
+        else:
+            self._offsets(cu_q, self.batch + 1, "CU_Q")
+            _check(max_q is None or max_q >= 0, "MAX_Q must not be negative")
+            max_q = total if max_q is None else min(int(max_q), total)
+        if window is None:
+            window = 0
+        else:
+            _check(window >= 1, "WINDOW must be positive, or None")
+        _check(sinks >= 0, "SINKS must not be negative")
+        scale = hd ** -0.5 if scale is None else float(scale)
+        _check(0.0 < scale < math.inf, "SCALE must be positive and finite")
+        if out is None:
+            out = torch.empty((total, nh, hd), dtype=q.dtype, device=q.device)
+        else:
+            check_shape(out, (total, nh, hd), "O")
+            _check(out.dtype in (q.dtype, torch.float32) and out.is_contiguous(),
+                   "O must be contiguous, of Q's type or fp32")
+        if lse is not None:
+            check_shape(lse, (total, nh), "LSE")
+            _check(lse.dtype == torch.float32 and lse.is_contiguous(), "LSE must be contiguous fp32")
+        index = self._here(("Q", q), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
+                           ("CU_Q", cu_q), ("O", out), ("LSE", lse), ("workspace", workspace))
+        if workspace is None:
+            with torch.cuda.device(index):  # the size goes by its compute units
+                size = lib().jacq_kivi_attend_workspace_size(g.ref, self.batch, total, max_q)
+            if size:
+                workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        else:
+            _check(workspace.is_contiguous(), "workspace must be contiguous")
+            size = workspace.numel() * workspace.element_size()
+        args = _ATTEND.pack(q.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+                            seq_lens.data_ptr(), block_tables.data_ptr(), out.data_ptr(),
+                            0 if lse is None else lse.data_ptr(), stride, DTYPES[q.dtype],
+                            DTYPES[out.dtype], self.batch, total, max_q, min(window, 1 << 30),
+                            min(sinks, 1 << 30), causal, scale)
+        self._call(index, lib().jacq_kivi_attend, g.ref, _POOL.pack(*self._pool_ptrs()), args,
+                   0 if workspace is None else workspace.data_ptr(), size)
+        return out
+
+    def prefill(self, q: torch.Tensor, cu_q: torch.Tensor | None, max_q: int | None,
+                seq_lens: torch.Tensor, block_tables: torch.Tensor, window: int | None = None,
+                sinks: int = 0, scale: float | None = None, out: torch.Tensor | None = None,
+                lse: torch.Tensor | None = None, workspace: torch.Tensor | None = None
+                ) -> torch.Tensor:
+        """q [tokens, NH, HD] fp16 or bf16, whose rows may lie apart (a slice of a fused
+        projection) -> O [tokens, NH, HD] of q's type (or of ``out``'s, q's or fp32).
+
+        Rows cu_q[b] to cu_q[b + 1] (cu_q [batch + 1] int32; None: one query per sequence) are
+        the last tokens of sequence b, whose seq_lens[b] tokens are all in the cache; each sees
+        the tokens up to its own, or the last ``window`` of them, itself among them, and the
+        first ``sinks`` of the sequence.  No sequence has more than max_q queries: of one that
+        has, the rows after its first max_q are left as they are, and so are rows outside every
+        sequence (undefined in a fresh output).  lse [tokens, NH] fp32 takes the log of the sum
+        of exponentials.  A query that sees nothing gives 0 (lse -inf)."""
+        return self._attend(q, cu_q, max_q, seq_lens, block_tables, window, sinks, 1, scale, out,
+                            lse, workspace)
+
+    def cross(self, q: torch.Tensor, cu_q: torch.Tensor | None, max_q: int | None,
+              seq_lens: torch.Tensor, block_tables: torch.Tensor, scale: float | None = None,
+              out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """``prefill`` with no order between queries and tokens: every query of sequence b sees
+        all of its seq_lens[b] tokens (the states of an encoder, say), of which there may be
+        fewer than queries, or none (O 0, lse -inf)."""
+        return self._attend(q, cu_q, max_q, seq_lens, block_tables, None, 0, 0, scale, out, lse,
+                            workspace)
+
+    def read(self, starts: torch.Tensor, ends: torch.Tensor, block_tables: torch.Tensor,
+             total: int, dtype: torch.dtype = torch.float16):
+        """The values of tokens starts[b] to ends[b] of each sequence, ends[b] its length, one
+        sequence after another: K, V [total, NKV, HD].  total is their number: tokens past it
+        are dropped, rows that none fills undefined."""
+        g = self.geo
+        if not self._fits(ends, block_tables):
+            self._check_tables(ends, block_tables)
+        _check(ends.is_contiguous(), "ENDS must be contiguous")
+        self._offsets(starts, self.batch, "STARTS")
+        _check(dtype in DTYPES, "values are read as fp16, bf16 or fp32, not ", dtype)
+        _check(total >= 0, "TOTAL must not be negative")
+        index = self._here(("STARTS", starts), ("ENDS", ends), ("BLOCK_TABLES", block_tables))
+        k = torch.empty((total, g.num_kv_heads, g.head_dim), dtype=dtype, device=ends.device)
+        v = torch.empty_like(k)
+        self._call(index, lib().jacq_kivi_read, g.ref, _POOL.pack(*self._pool_ptrs()),
+                   starts.data_ptr(), ends.data_ptr(), block_tables.data_ptr(), self.batch, total,
+                   k.data_ptr(), v.data_ptr(), DTYPES[dtype])
+        return k, v
