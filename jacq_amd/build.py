@@ -16,7 +16,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libjacq_kivi.so")
 TORCH_LIB = os.path.join(HERE, "libjacq_kivi_torch.so")
 SOURCES = ["kivi_api.hip", "kivi_writer.hip", "kivi_decode.hip", "kivi_decode_mfma.hip",
-           "kivi_attend_api.hip", "kivi_few.hip", "kivi_read.hip", "rotary.hip",
+           "kivi_attend_api.hip", "kivi_few.hip", "kivi_prompt.hip",
+           "kivi_read.hip", "rotary.hip",
            "q8_api.hip", "q8_writer.hip", "q8_decode.hip", "q8_prefill.hip", "q8_evict.hip"]
 ARCH = "gfx950"
 
@@ -48,7 +49,8 @@ def hipcc() -> str:
 # Kernels that must not spill: a spill makes the kernel need scratch memory,
 # which cost the decode about 17 us (13%) when a 12-byte spill crept in.
 NO_SCRATCH = ("kivi_decode_stream_kernel", "kivi_decode_chunk_kernel", "kivi_append_kernel",
-              "kivi_few_kernel", "kivi_few_plan_kernel", "kivi_few_join_kernel", "kivi_read_kernel",
+              "kivi_few_kernel", "kivi_few_plan_kernel", "kivi_few_join_kernel", "kivi_slots_kernel",
+              "kivi_lay_kernel", "kivi_prompt_kernel", "kivi_prompt_merge_kernel", "kivi_read_kernel",
               "rotary_kernel",
               "q8_append_kernel", "q8_read_kernel", "q8_plan_kernel", "q8_decode_kernel", "q8_join_kernel",
               "q8_weights_kernel", "q8_prefill_kernel", "q8_merge_kernel", "q8_evict_kernel")

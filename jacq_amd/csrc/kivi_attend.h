@@ -34,13 +34,21 @@ struct KiviAttendArgs {
   int causal;             // 0: every query sees every token
   float scale;            // log2(e) included
   // split pieces
-  float* part_ml;         // few queries: [target + segments][rows][2]
+  float* part_ml;         // few queries: [target + segments][rows][2]; prompts: [slices][total_q][nh][2]
   float* part_acc;        // the same [HD]
   int32_t* plan;          // calls of many sequences: [batch + 1] first slices, then their size
   int target;             // slices to aim at; 0: segments stay whole
   int cus;                // compute units
   int rows;               // rows of a segment at most (<= 16 NB)
   int row_blocks;         // row blocks of a sequence at most
+  // prompts
+  int slices;             // workgroups that share a row tile's tokens, at most
+  float load;             // row tiles a CU
+  unsigned tiles, merges; // units of row tiles, and of the merge's (Place)
+  int32_t* slots;         // [batch + 1] first tile image of each sequence, then their number
+  int per_pass;           // tile images of a pass; a sequence's begin in one and may end behind it
+  uint8_t* images;        // K [64][HD], then V [HD][64], fp16, as they lie in the LDS
+  uint64_t* poison;       // of each image: the tokens whose V is not finite or not there
 };
 
 __device__ inline int clamp_len(const KiviGeo& g, int n) {
@@ -78,6 +86,28 @@ __device__ inline KiviSpan make_span(const KiviGeo& g, const KiviAttendArgs& a, 
   s.units = s.units < 1 ? 1 : s.units;
   return s;
 }
+
+// The tiles of kTile tokens that any query of a sequence sees: the sinks', then the window's.
+struct KiviTiles {
+  int n, old;
+  int w0, ns, units;
+  __device__ KiviTiles(const KiviGeo& g, const KiviAttendArgs& a, int n_, int first) {
+    int residual;
+    n = n_;
+    decode_window(g, n, &old, &residual);
+    const int tiles = (n + kTile - 1) / kTile;
+    w0 = ns = 0;
+    if (a.window > 0 && first >= a.window) {
+      w0 = (first - a.window + 1) / kTile;
+      const int sinks = a.sinks < n ? a.sinks : n;
+      ns = (sinks + kTile - 1) / kTile;
+      ns = ns > w0 ? w0 : ns;
+    }
+    units = ns + tiles - w0;
+  }
+  __device__ int tile_of(int u) const { return u < ns ? u : w0 + u - ns; }
+  __device__ int unit_of(int tile) const { return tile < ns ? tile : tile - w0 + ns; }
+};
 
 template <>
 struct SpanOf<KiviGeo> {
@@ -184,6 +214,8 @@ __device__ inline uint32_t most_bits(uint32_t a, uint32_t b) {
 __device__ inline uint32_t either_half(uint32_t x) { return (x >> 16) > (x & 0xffffu) ? x >> 16 : x & 0xffffu; }
 
 hipError_t launch_attend_few(const KiviGeo& g, const KiviAttendArgs& a, int nb, hipStream_t s);
+// Prompts: `passes` times the images of some sequences and their row tiles, then the slices' merge.
+hipError_t launch_attend_prompt(const KiviGeo& g, const KiviAttendArgs& a, int passes, hipStream_t s);
 hipError_t launch_kivi_read(const KiviGeo& g, const KiviPool& p, const int32_t* starts,
                             const int32_t* ends, const int32_t* tables, int batch, int total, void* k,
                             void* v, int type, hipStream_t s);

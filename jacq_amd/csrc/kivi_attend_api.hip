@@ -113,11 +113,32 @@ constexpr int kWholeUnits = 24;
 // for it.
 constexpr int kCutBatch = 64;
 
+// Rows of a kv head from which a call is a prompt's: its tokens become fp16 once, in the workspace.
+constexpr int kPromptRows = 256;
+// Bytes of fp16 tiles that a pass lays in the workspace, about, and passes at most: a call of more
+// (many sequences under a wide table) is left to the few-query kernel.
+constexpr int64_t kPassBytes = (int64_t)1 << 31;
+constexpr int64_t kMostPasses = 16;
+
 struct Plan {
-  bool planned;
+  bool prompt, planned;
   int nb, rows, row_blocks, target;
-  size_t ml, acc, plan, bytes;  // offsets into the workspace, and its size
+  float load;
+  int slices, per_pass, passes;
+  size_t ml, acc, plan, slots, images, poison, bytes;  // offsets into the workspace, and its size
 };
+
+// A prompt's slices, for as many tokens as the table addresses: the kernels use fewer for sequences of
+// fewer (slices_cost, which has the reasons).  One, unless more promise 3 % at least.
+int plan_slices(float load, int64_t tokens) {
+  const int most =
+      (int)std::min<int64_t>(jacq::kMaxSlices, tokens / (jacq::kSliceUnits * jacq::kTile));
+  auto cost = [&](int s) { return jacq::slices_cost(load, s, (float)tokens); };
+  int best = 1;
+  for (int s = 2; s <= most; ++s)
+    if (cost(s) < cost(best)) best = s;
+  return cost(best) < 0.97f * cost(1) ? best : 1;
+}
 
 Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   Plan p = {};
@@ -137,6 +158,30 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  const int64_t tokens = (int64_t)g.lq + g.residual;
+  const int64_t cap = (tokens + jacq::kTile - 1) / jacq::kTile;  // images of a sequence and kv head
+  const int64_t image = (int64_t)4 * jacq::kTile * g.hd * g.nkv;
+  const int64_t images = std::min<int64_t>(batch, total_q) * cap;
+  p.per_pass = (int)std::max<int64_t>(1, std::min(images, kPassBytes / image));
+  const int64_t passes = (images + p.per_pass - 1) / p.per_pass;
+  p.prompt = rows >= kPromptRows && passes <= kMostPasses && images <= INT32_MAX - 1024;
+  if (p.prompt) {
+    p.passes = (int)passes;
+    p.load = (float)(blocks(jacq::kPrefillRows) * g.nkv) / (float)device_cus();
+    p.slices = plan_slices(p.load, tokens);
+    if (p.slices > 1) {
+      const size_t rows_all = (size_t)p.slices * total_q * g.nh;
+      p.ml = take(rows_all * 2 * sizeof(float));
+      p.acc = take(rows_all * g.hd * sizeof(float));
+    }
+    // a sequence's images may end behind the pass that they begin in
+    const size_t held = (size_t)(passes == 1 ? images : p.per_pass + cap) * g.nkv;
+    p.slots = take(((size_t)batch + 1) * sizeof(int32_t));
+    p.poison = take(held * sizeof(uint64_t));
+    p.images = take(held * 4 * jacq::kTile * g.hd);
+    p.bytes = at;
+    return p;
+  }
   p.nb = rows <= 16 ? 1 : 2;
   p.rows = (int)std::min<int64_t>(rows, 16 * p.nb);
   p.row_blocks = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
@@ -153,6 +198,13 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   p.plan = take(p.planned ? ((size_t)batch + 2) * sizeof(int32_t) : 0);
   p.bytes = at;
   return p;
+}
+
+// As many units as Place may give to the call's queries.
+int64_t place_units(const KiviAttendArgs& a, int per, int log2) {
+  const int64_t of_all = ((int64_t)a.total_q * per >> log2) + a.batch;
+  const int64_t each = ((int64_t)a.max_q * per + (1 << log2) - 1) >> log2;
+  return a.batch <= jacq::kCounted ? std::min(of_all, a.batch * each) : of_all;
 }
 
 }  // namespace
@@ -223,7 +275,10 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
     const Plan p = plan_attend(g, a.batch, a.total_q, a.max_q);
     const int64_t segments = (int64_t)a.batch * g.nkv * p.row_blocks;
     // a launch has fewer than 2^32 threads
-    if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 || segments + p.target >= 1 << 24)
+    const int64_t tiles = place_units(a, g.gqa, jacq::kRowsLog2);
+    const int64_t merges = p.slices > 1 ? place_units(a, g.nh, jacq::merge_log2(g.hd)) : 0;
+    if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 ||
+        (p.prompt ? std::max(tiles * g.nkv, merges) : segments + p.target) >= 1 << 24)
       return fail("too many query rows in one call");
     if (p.bytes && (!workspace || workspace_bytes < p.bytes))
       return jacq::set_last_error(JACQ_KIVI_ENOMEM,
@@ -232,6 +287,17 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
     uint8_t* ws = (uint8_t*)workspace;
     a.part_ml = (float*)(ws + p.ml);
     a.part_acc = (float*)(ws + p.acc);
+    if (p.prompt) {
+      a.slices = p.slices;
+      a.load = p.load;
+      a.tiles = (unsigned)tiles;
+      a.merges = (unsigned)merges;
+      a.slots = (int32_t*)(ws + p.slots);
+      a.per_pass = p.per_pass;
+      a.images = ws + p.images;
+      a.poison = (uint64_t*)(ws + p.poison);
+      return launched(jacq::launch_attend_prompt(g, a, p.passes, stream), "attention");
+    }
     a.target = p.target;
     a.cus = device_cus();
     a.plan = p.planned ? (int32_t*)(ws + p.plan) : nullptr;
