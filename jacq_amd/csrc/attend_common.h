@@ -406,13 +406,14 @@ __device__ inline bool place_slice(const G& g, const A& a, int lane, Segment<G>&
 }
 
 // Joins the wavefronts' parts of a slice: sum(w v) in red[wave][row][channel] and, in ml, the maximum
-// that w refers to and the sum of w; to O, or to the slice's place in the workspace.
+// that w refers to and the sum of w; to O, or to the slice's place in the workspace.  `rows` of the
+// segment's from row0 on.
 template <int HD, class G, class A, int ROWS, int LD>
 __device__ inline void fold_parts(const G& g, const A& a, const Segment<G>& s, bool whole,
                                   const float (&red)[kSliceWaves][ROWS][LD],
-                                  const float (&ml)[kSliceWaves][ROWS][2]) {
+                                  const float (&ml)[kSliceWaves][ROWS][2], int row0, int rows) {
   constexpr int PER = HD / 16;  // channels of a thread
-  for (int i = threadIdx.x; i < s.nrows * 16; i += 64 * kSliceWaves) {
+  for (int i = threadIdx.x; i < rows * 16; i += 64 * kSliceWaves) {
     const int row = i / 16, ch = i % 16 * PER;
     float mm = kNegInf, l = 0.0f;
 #pragma unroll
@@ -430,9 +431,9 @@ __device__ inline void fold_parts(const G& g, const A& a, const Segment<G>& s, b
       for (int c = 0; c < PER; ++c) x[c] += red[v][row][ch + c] * f;
     }
     if (whole) {
-      finish_row(g, a, s, row, HD, ch, x, PER, l, mm);
+      finish_row(g, a, s, row0 + row, HD, ch, x, PER, l, mm);
     } else {
-      const int64_t at = (int64_t)blockIdx.x * a.rows + row;
+      const int64_t at = (int64_t)blockIdx.x * a.rows + row0 + row;
 #pragma unroll
       for (int c = 0; c < PER; c += 4) *(f4*)(a.part_acc + at * HD + ch + c) = *(f4*)(x + c);
       if (ch == 0) {
@@ -500,7 +501,8 @@ __device__ inline void plan_cut(const G& g, const A& a) {
 }
 
 // Joins a segment's slices, in their order.  blockIdx.x: segment.  MANY: of the row blockIdx.y, the
-// threads side by side share the slices; else they share the rows.  256 threads.
+// threads side by side share the slices; else they share the rows, 1024 / HD at a time, with gridDim.y
+// workgroups.  256 threads.
 template <int HD, int ROWS, bool MANY, class G, class A>
 __device__ inline void join_slices(const G& g, const A& a) {
   constexpr int TC = HD / 4;      // threads of a row
@@ -549,7 +551,7 @@ __device__ inline void join_slices(const G& g, const A& a) {
     }
   };
   if constexpr (!MANY) {
-    for (int row = grp; row < s.nrows; row += PG) {
+    for (int row = grp + PG * blockIdx.y; row < s.nrows; row += PG * gridDim.y) {
       float mm = kNegInf, l = 0.0f;
       f4 acc = {0, 0, 0, 0};
       sum(row, 0, 1, mm, l, acc);

@@ -146,33 +146,24 @@ __device__ inline h8 values8(uint32_t w, u4 s, u4 z) {
   return r;
 }
 
-// 8 channels of two tokens (a dword each), s and z the two tokens' of their 32 channels: out[c] is
-// channel c of both.
-__device__ inline void values8x2(uint32_t a, uint32_t b, h2 s, h2 z, h2 (&out)[8]) {
-  const Nibbles x(a), y(b);
-  const uint32_t e0 = __builtin_amdgcn_perm(y.even, x.even, 0x05010400u);  // channels 0 and 2
-  const uint32_t e1 = __builtin_amdgcn_perm(y.even, x.even, 0x07030602u);  // 4 and 6
-  const uint32_t o0 = __builtin_amdgcn_perm(y.odd, x.odd, 0x05010400u);    // 1 and 3
-  const uint32_t o1 = __builtin_amdgcn_perm(y.odd, x.odd, 0x07030602u);    // 5 and 7
-  out[0] = fma2(codes_lo(e0), s, z);
-  out[1] = fma2(codes_lo(o0), s, z);
-  out[2] = fma2(codes_hi(e0), s, z);
-  out[3] = fma2(codes_hi(o0), s, z);
-  out[4] = fma2(codes_lo(e1), s, z);
-  out[5] = fma2(codes_lo(o1), s, z);
-  out[6] = fma2(codes_hi(e1), s, z);
-  out[7] = fma2(codes_hi(o1), s, z);
+// Of 8 channels of two tokens (a dword each) the even or the odd ones, s and z the two tokens' of their 32
+// channels: out[c] is channel 2 c + odd of both.
+__device__ inline void values8x2(uint32_t a, uint32_t b, int odd, h2 s, h2 z, h2 (&out)[4]) {
+  const uint32_t x = odd ? a >> 4 & 0x0f0f0f0fu : a & 0x0f0f0f0fu;
+  const uint32_t y = odd ? b >> 4 & 0x0f0f0f0fu : b & 0x0f0f0f0fu;
+  const uint32_t lo = __builtin_amdgcn_perm(y, x, 0x05010400u), hi = __builtin_amdgcn_perm(y, x, 0x07030602u);
+  out[0] = fma2(codes_lo(lo), s, z);
+  out[1] = fma2(codes_hi(lo), s, z);
+  out[2] = fma2(codes_lo(hi), s, z);
+  out[3] = fma2(codes_hi(hi), s, z);
 }
 
 // The same of 4 channels of two tokens: w has the first token's 16 bits, then the second's.
-__device__ inline void values4x2(uint32_t w, h2 s, h2 z, h2 (&out)[4]) {
-  const Nibbles x(w);
-  const uint32_t e = __builtin_amdgcn_perm(0u, x.even, 0x03010200u);  // channels 0 and 2
-  const uint32_t o = __builtin_amdgcn_perm(0u, x.odd, 0x03010200u);   // 1 and 3
-  out[0] = fma2(codes_lo(e), s, z);
-  out[1] = fma2(codes_lo(o), s, z);
-  out[2] = fma2(codes_hi(e), s, z);
-  out[3] = fma2(codes_hi(o), s, z);
+__device__ inline void values4x2(uint32_t w, int odd, h2 s, h2 z, h2 (&out)[2]) {
+  const uint32_t x = odd ? w >> 4 & 0x0f0f0f0fu : w & 0x0f0f0f0fu;
+  const uint32_t y = __builtin_amdgcn_perm(0u, x, 0x03010200u);
+  out[0] = fma2(codes_lo(y), s, z);
+  out[1] = fma2(codes_hi(y), s, z);
 }
 
 // A query row's values for the matrix cores, 8 of them in each of N operands, from fp16 or bf16, and
@@ -220,6 +211,6 @@ hipError_t launch_kivi_read(const KiviGeo& g, const KiviPool& p, const int32_t* 
                             const int32_t* ends, const int32_t* tables, int batch, int total, void* k,
                             void* v, int type, hipStream_t s);
 // Workgroups of the few-query kernel that a CU holds.
-constexpr int few_groups(int hd, int nb) { return hd == 64 && nb == 1 ? 3 : 2; }
+constexpr int few_groups(int hd, int nb) { return hd == 64 ? 5 - nb : 4 - nb; }
 
 }  // namespace jacq

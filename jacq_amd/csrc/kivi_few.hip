@@ -26,7 +26,7 @@ struct FewStage {
 
 // Stages of a wavefront's ring, by what the LDS holds for few_groups workgroups.
 template <int HD, int NB>
-constexpr int few_stages() { return HD == 64 ? 4 : 3; }
+constexpr int few_stages() { return HD == 64 ? 4 : NB == 1 ? 2 : 3; }
 
 __device__ inline int table_at(const int32_t* row, int i) {  // uniform: a scalar load
   return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(row + i);
@@ -78,76 +78,93 @@ struct Few {
     }
   }
 
-  // Whether rows of the block see anything of the unit; whether some do not see all of it.
+  // Whether some rows of the block do not see all of a unit.
   struct Seen {
     int first, last;  // positions of the block's first and last row
-    __device__ bool any(const KiviAttendArgs& a, int t0) const {
-      return t0 <= last && (a.window <= 0 || t0 + kGroup - 1 > first - a.window || t0 < a.sinks);
-    }
     __device__ bool part(const KiviAttendArgs& a, int t0) const {
       return t0 + kGroup - 1 > first ||
              (a.window > 0 && t0 <= last - a.window && t0 + kGroup > a.sinks);
     }
   };
 
-  // Scores -> weights, in fp16.  sc: raw scores of this lane's 8 tokens tok_v(kq, e) of the unit at t0;
-  // those of `poison` are NaN to the rows that see them.
-  __device__ void soften(int nb, const f4 (&sc)[2], int t0, bool masked, uint32_t poison, h8& p) {
-    float t[8];
+  // Both products of a unit.  This lane's 8 tokens are tok_v(kq, e) of the unit at t0; those of `poison`
+  // are NaN to the rows that see them.  All row blocks side by side, under one branch: their chains of
+  // dependent instructions fill each other's waits.  v(odd, x): the V operands of the even or odd
+  // channels of this lane, made when they are needed: registers are what limits the wavefronts a SIMD.
+  template <class V>
+  __device__ void unit(const h8 (&k)[2][KS], int t0, bool masked, bool weeds, uint32_t poison, V v) {
+    f4 sc[NB][2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = sc[e / 4][e & 3] * qs[nb];
-    if (poison) {
+    for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = poison >> e & 1 ? __builtin_nanf("") : t[e];
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          sc[nb][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[tt][i], q[nb][i],
+                                                              i ? sc[nb][tt] : f4{0, 0, 0, 0}, 0, 0, 0);
+    if (weeds) {  // uniform, as masked is
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          sc[nb][e / 4][e & 3] = poison >> e & 1 ? __builtin_nanf("") : sc[nb][e / 4][e & 3];
     }
     if (masked) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        t[e] = sees(t0 + tok_v(kq, e), pos[nb], a.window, a.sinks) ? t[e] : kNegInf;
-    }
-    float mx = max3f(max3f(max3f(t[0], t[1], t[2]), t[3], t[4]), max3f(t[5], t[6], t[7]), kNegInf);
-    mx = max_xor32(max_xor16(mx));
-    if (__ballot(mx > m[nb] + (kLift + kSlack))) {  // also where m is -inf and mx is not
-      const float to = mx > m[nb] + (kLift + kSlack) ? mx - kLift : m[nb];
-      const float f = to > m[nb] ? exp2_(m[nb] - to) : 1.0f;
-      m[nb] = to;
-      l[nb] *= f;
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int j = 0; j < CPL; ++j) acc[nb][j] *= f;
+        for (int e = 0; e < 8; ++e)
+          sc[nb][e / 4][e & 3] = sees(t0 + tok_v(kq, e), pos[nb], a.window, a.sinks)
+                                     ? sc[nb][e / 4][e & 3] : kNegInf;
     }
-    const float base = m[nb] == kNegInf ? 0.0f : m[nb];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float w = exp2_(t[e] - base);
-      l[nb] += w;
-      p[e] = (_Float16)w;
-    }
-  }
-
-  // Both products of a unit whose operands are ready.
-  __device__ void unit(const h8 (&k)[2][KS], const h8 (&v)[CPL], int t0, bool masked,
-                       uint32_t poison) {
+    float mx[NB];
+    bool grows = false;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      f4 sc[2];
+      const f4 x = sc[nb][0], y = sc[nb][1];
+      mx[nb] = max3f(max3f(x.x, x.y, x.z), max3f(x.w, y.x, y.y), max2f(y.z, y.w));
+      mx[nb] = max_xor32(max_xor16(mx[nb])) * qs[nb];
+      grows = grows || mx[nb] > m[nb] + (kLift + kSlack);
+    }
+    if (__ballot(grows)) {  // also where m is -inf and mx is not
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        sc[tt] = f4{0, 0, 0, 0};
+      for (int nb = 0; nb < NB; ++nb) {
+        const float to = mx[nb] > m[nb] + (kLift + kSlack) ? mx[nb] - kLift : m[nb];
+        const float f = to > m[nb] ? exp2_(m[nb] - to) : 1.0f;
+        m[nb] = to;
+        l[nb] *= f;
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
-          sc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[tt][i], q[nb][i], sc[tt], 0, 0, 0);
+        for (int j = 0; j < CPL; ++j) acc[nb][j] *= f;
       }
-      h8 p;
-      soften(nb, sc, t0, masked, poison, p);
+    }
+    h8 p[NB];
 #pragma unroll
-      for (int j = 0; j < CPL; ++j)
-        acc[nb][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[j], p, acc[nb][j], 0, 0, 0);
+    for (int nb = 0; nb < NB; ++nb) {
+      const float base = m[nb] == kNegInf ? 0.0f : -m[nb];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = exp2_(__builtin_fmaf(sc[nb][e / 4][e & 3], qs[nb], base));
+        l[nb] += w;
+        p[nb][e] = (_Float16)w;
+      }
+    }
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      h8 x[CPL / 2];
+      v(odd, x);
+#pragma unroll
+      for (int c = 0; c < CPL / 2; ++c)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          acc[nb][2 * c + odd] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[c], p[nb], acc[nb][2 * c + odd], 0,
+                                                                        0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
   // An int4 group in the LDS.  gone: bit i: its tokens 16 i on lie in a page outside the pool.
   __device__ void group(const FewStage<HD>* st, int t0, bool masked, int gone) {
-    h8 k[2][KS], v[CPL];
+    h8 k[2][KS];
     {
       kvec code[2];
 #pragma unroll
@@ -161,45 +178,41 @@ struct Few {
         for (int tt = 0; tt < 2; ++tt) k[tt][i] = values8(code[tt][i], s, z);
       }
     }
-    // V: scales and zeros of this lane's 8 tokens, two by two
+    // All scales and zeros of V, a few a lane: below 4096, 15 scale + |zero| is a finite fp16.
+    typedef uint32_t few_t __attribute__((ext_vector_type(HD / 64)));
+    const few_t some = *(const few_t*)(st->s + 4 * HD + lane * (HD / 16));
+    const uint32_t most = most_bits(some[0], some[HD / 64 - 1]);
+    // scales and zeros of this lane's 8 tokens, two by two
     const uint8_t* at = st->s + 4 * HD + 2 * (tok_v(kq, 0) * (HD / 32) + n16 * CPL / 32);
     constexpr int STEP = 2 * 2 * (HD / 32);  // two tokens on
-    uint32_t s[4], z[4], most = 0;
+    uint32_t s[4], z[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       s[p] = *(const uint16_t*)(at + 2 * p * STEP) | (uint32_t)*(const uint16_t*)(at + (2 * p + 1) * STEP) << 16;
       z[p] = *(const uint16_t*)(at + 2 * HD + 2 * p * STEP) |
              (uint32_t)*(const uint16_t*)(at + 2 * HD + (2 * p + 1) * STEP) << 16;
-      most = most_bits(most, most_bits(s[p], z[p]));
     }
-    // Below 4096, 15 scale + |zero| is a finite fp16.
     uint32_t poison = 0;
-    if (gone || __ballot(either_half(most) >= 0x6c00u)) poison = weed(s, z, gone);
+    const bool weeds = gone || __ballot(either_half(most) >= 0x6c00u);
+    if (weeds) poison = weed(s, z, gone);
     const uint8_t* vc = st->v + tok_v(kq, 0) * (HD / 2) + n16 * (CPL / 2);
+    typedef typename std::conditional<HD == 128, uint32_t, uint16_t>::type code_t;
+    code_t code[8];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      if constexpr (HD == 128) {
-        h2 x[8];
-        values8x2(*(const uint32_t*)(vc + 2 * p * HD), *(const uint32_t*)(vc + (2 * p + 1) * HD),
-                  pair(s[p]), pair(z[p]), x);
+    for (int e = 0; e < 8; ++e) code[e] = *(const code_t*)(vc + e * HD);
+    unit(k, t0, masked, weeds, poison, [&](int odd, h8 (&x)[CPL / 2]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j][2 * p] = x[j].x;
-          v[j][2 * p + 1] = x[j].y;
-        }
-      } else {
-        h2 x[4];
-        values4x2(*(const uint16_t*)(vc + 2 * p * HD) |
-                      (uint32_t)*(const uint16_t*)(vc + (2 * p + 1) * HD) << 16,
-                  pair(s[p]), pair(z[p]), x);
+      for (int p = 0; p < 4; ++p) {
+        h2 y[CPL / 2];
+        if constexpr (HD == 128) values8x2(code[2 * p], code[2 * p + 1], odd, pair(s[p]), pair(z[p]), y);
+        else values4x2(code[2 * p] | (uint32_t)code[2 * p + 1] << 16, odd, pair(s[p]), pair(z[p]), y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j][2 * p] = x[j].x;
-          v[j][2 * p + 1] = x[j].y;
+        for (int c = 0; c < CPL / 2; ++c) {
+          x[c][2 * p] = y[c].x;
+          x[c][2 * p + 1] = y[c].y;
         }
       }
-    }
-    unit(k, v, t0, masked, poison);
+    });
   }
 
   // A token's V that is not finite, or not there, must reach no row that does not see it, and a
@@ -228,19 +241,19 @@ struct Few {
     return bad;
   }
 
-  // 32 fp16 tokens from t0 on, at most; what lies behind the last one is not read.
+  // 32 fp16 tokens from t0 on, at most; what lies behind the last one is not read: the last one stands
+  // for it, and no row sees it.
   __device__ void recent(const Segment<KiviGeo>& s, int t0, bool masked) {
     const int64_t base = (((int64_t)s.b * g.nkv + s.h) * g.rs + (t0 - s.span.old)) * HD;
-    const int have = s.span.n - t0;
-    const uint16_t* ks = a.pool.k_scr + base + kq * (HD / 4);
-    const uint16_t* vs = a.pool.v_scr + base + n16 * CPL;
-    h8 k[2][KS], v[CPL];
+    const int last = s.span.n - t0 - 1;
+    const uint16_t *ks = a.pool.k_scr + base, *vs = a.pool.v_scr + base;
+    h8 k[2][KS];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       const int r = tok_k(tt, n16);
+      const uint32_t at = (r < last ? r : last) * HD + kq * (HD / 4);
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-        k[tt][i] = __builtin_bit_cast(h8, r < have ? *(const u4*)(ks + r * HD + 8 * i) : u4{0, 0, 0, 0});
+      for (int i = 0; i < KS; ++i) k[tt][i] = *(const h8*)(ks + at + 8 * i);
     }
     typedef uint32_t row_t __attribute__((ext_vector_type(CPL / 2)));
     row_t x[8];
@@ -248,14 +261,15 @@ struct Few {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int r = tok_v(kq, e);
-      x[e] = r < have ? *(const row_t*)(vs + r * HD) : row_t(0);
+      x[e] = *(const row_t*)(vs + (uint32_t)((r < last ? r : last) * HD + n16 * CPL));
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
       for (int c = 0; c < CPL / 2; ++c) most = most_bits(most, x[e][c]);
     uint32_t poison = 0;
-    if (__ballot(either_half(most) >= 0x7c00u)) {
+    const bool weeds = __ballot(either_half(most) >= 0x7c00u);
+    if (weeds) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         uint32_t mine = 0;
@@ -268,30 +282,34 @@ struct Few {
       }
       poison = any16(poison);
     }
+    unit(k, t0, masked, weeds, poison, [&](int odd, h8 (&v)[CPL / 2]) {
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
+      for (int p = 0; p < 4; ++p)
 #pragma unroll
-      for (int c = 0; c < CPL / 2; ++c) {
-        const h2 lo = pair(__builtin_amdgcn_perm(x[2 * p + 1][c], x[2 * p][c], 0x05040100u));
-        const h2 hi = pair(__builtin_amdgcn_perm(x[2 * p + 1][c], x[2 * p][c], 0x07060302u));
-        v[2 * c][2 * p] = lo.x;
-        v[2 * c][2 * p + 1] = lo.y;
-        v[2 * c + 1][2 * p] = hi.x;
-        v[2 * c + 1][2 * p + 1] = hi.y;
-      }
-    unit(k, v, t0, masked, poison);
+        for (int c = 0; c < CPL / 2; ++c) {
+          const h2 y = pair(__builtin_amdgcn_perm(x[2 * p + 1][c], x[2 * p][c],
+                                                  odd ? 0x07060302u : 0x05040100u));
+          v[c][2 * p] = y.x;
+          v[c][2 * p + 1] = y.y;
+        }
+    });
   }
 
-  // Units u0, u0 + kSliceWaves, ... below u1.
+  // Units u0, u0 + kSliceWaves, ... below u1, but those of which no row of this block sees anything:
+  // behind the last row, and between the sinks and the first row's window.
   __device__ void units(const Segment<KiviGeo>& s, FewStage<HD>* ring, int u0, int u1) {
     const KiviSpan& sp = s.span;
     Seen seen;
     seen.first = uniform(position(s, s.rb * 16 * NB));
     seen.last = uniform(position(s, s.rb * 16 * NB + s.nrows - 1));
-    // the next unit from u on of which rows of this block see anything
-    auto next = [&](int u) {
-      while (u < u1 && !seen.any(a, sp.tile_of(u) * kGroup)) u += kSliceWaves;
-      return u;
+    // the units of this block's window, [lo, hi)
+    const int hi = seen.last < 0 ? 0 : sp.ns + (seen.last / kGroup + 1 - sp.w0);
+    int lo = sp.ns;
+    if (a.window > 0 && seen.first >= a.window)
+      lo = sp.ns + ((seen.first - a.window + 1) / kGroup - sp.w0);
+    u1 = u1 < hi ? u1 : hi;
+    auto next = [&](int u) {  // u, or behind what lies between the sinks and lo
+      return u >= sp.ns && u < lo ? u + (lo - u + kSliceWaves - 1) / kSliceWaves * kSliceWaves : u;
     };
     const StageBases sb = stage_bases<HD, P>(a.pool, g.nkv, s.h, lane);
     const int32_t* table = a.tables + (int64_t)s.b * g.max_pages;
@@ -340,7 +358,6 @@ struct Few {
     }
     for (; at < u1; at = next(at + kSliceWaves)) {
       const int t0 = sp.tile_of(at) * kGroup;
-      if (t0 >= sp.n) break;  // a segment without tokens
       recent(s, t0, seen.part(a, t0));
     }
   }
@@ -366,10 +383,10 @@ __device__ inline int slice_units(const KiviAttendArgs& a, float all, float segm
 template <int HD, int P, int NB>
 __global__ __launch_bounds__(64 * kSliceWaves, few_groups(HD, NB)) void kivi_few_kernel(
     KiviGeo g, KiviAttendArgs a) {
-  constexpr int ROWS = 16 * NB, LD = HD + 4, S = few_stages<HD, NB>();
+  constexpr int LD = HD + 4, S = few_stages<HD, NB>();
   struct Parts {
-    float red[kSliceWaves][ROWS][LD];
-    float ml[kSliceWaves][ROWS][2];
+    float red[kSliceWaves][16][LD];
+    float ml[kSliceWaves][16][2];
   };
   constexpr size_t RING = sizeof(FewStage<HD>) * S * kSliceWaves;
   __shared__ __align__(16) uint8_t shared[RING > sizeof(Parts) ? RING : sizeof(Parts)];
@@ -377,33 +394,34 @@ __global__ __launch_bounds__(64 * kSliceWaves, few_groups(HD, NB)) void kivi_few
   Segment<KiviGeo> s;
   int u0, u1;
   bool whole;
-  if (!place_slice<ROWS>(g, a, lane, s, u0, u1, whole)) return;
+  if (!place_slice<16 * NB>(g, a, lane, s, u0, u1, whole)) return;
   Few<HD, P, NB> w(g, a, lane);
   w.start(s);
   w.units(s, (FewStage<HD>*)shared + wave * S, uniform(u0 + wave), uniform(u1));
 
-  // Fold the wavefronts' parts, which take the rings' place.
-  __syncthreads();
+  // Fold the wavefronts' parts, which take the rings' place: 16 rows at a time.
   Parts& parts = *(Parts*)shared;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
+    __syncthreads();
     float l = w.l[nb];
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (lane < 16) {
-      parts.ml[wave][nb * 16 + lane][0] = w.m[nb];
-      parts.ml[wave][nb * 16 + lane][1] = l;
+      parts.ml[wave][lane][0] = w.m[nb];
+      parts.ml[wave][lane][1] = l;
     }
     // O^T row 4 kq + r of operand j is channel CPL (4 kq + r) + j
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int j = 0; j < HD / 16; j += 4)
-        *(f4*)&parts.red[wave][nb * 16 + w.n16][(4 * w.kq + r) * (HD / 16) + j] =
+        *(f4*)&parts.red[wave][w.n16][(4 * w.kq + r) * (HD / 16) + j] =
             f4{w.acc[nb][j][r], w.acc[nb][j + 1][r], w.acc[nb][j + 2][r], w.acc[nb][j + 3][r]};
+    __syncthreads();
+    const int left = s.nrows - 16 * nb;
+    fold_parts<HD>(g, a, s, whole, parts.red, parts.ml, 16 * nb, left < 16 ? left : 16);
   }
-  __syncthreads();
-  fold_parts<HD>(g, a, s, whole, parts.red, parts.ml);
 }
 
 template <int NB>
@@ -427,7 +445,8 @@ static hipError_t few_kernels(const KiviGeo& g, const KiviAttendArgs& a, hipStre
       hipLaunchKernelGGL((kivi_few_join_kernel<HD, NB, true>), dim3(segments, a.rows), dim3(256), 0, s,
                          g, a);
     else
-      hipLaunchKernelGGL((kivi_few_join_kernel<HD, NB, false>), dim3(segments), dim3(256), 0, s, g, a);
+      hipLaunchKernelGGL((kivi_few_join_kernel<HD, NB, false>),
+                         dim3(segments, (a.rows * HD + 1023) / 1024), dim3(256), 0, s, g, a);
   }
   return hipGetLastError();
 }

@@ -160,8 +160,14 @@ __global__ __launch_bounds__(2 * HD) void kivi_lay_kernel(KiviGeo g, KiviAttendA
         }
 #pragma unroll
         for (int p = 0; p < 4; ++p)
-          values8x2(w[2 * p], w[2 * p + 1], pair(s[2 * p] | s[2 * p + 1] << 16),
-                    pair(z[2 * p] | z[2 * p + 1] << 16), x[p]);
+#pragma unroll
+          for (int odd = 0; odd < 2; ++odd) {
+            h2 y[4];
+            values8x2(w[2 * p], w[2 * p + 1], odd, pair(s[2 * p] | s[2 * p + 1] << 16),
+                      pair(z[2 * p] | z[2 * p + 1] << 16), y);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[p][2 * c + odd] = y[c];
+          }
       } else {
         u4 row[8];
 #pragma unroll

@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64 * kSliceWaves, decode_groups(HD, NB)) void q8_de
       *(f4*)&red[wave][nb * 16 + w.n16][d * 16 + w.kq * 4] = w.acc[nb][d];
   }
   __syncthreads();
-  fold_parts<HD>(g, a, s, whole, red, ml);
+  fold_parts<HD>(g, a, s, whole, red, ml, 0, s.nrows);
 }
 
 template <int HD, int NB, bool MANY>
