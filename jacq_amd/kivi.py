@@ -428,9 +428,9 @@ def plan_batched_write(start_seq_len: int, num_new_tokens: int, residual: int = 
 # ---------------------------------------------------------------------------
 
 class _WithRecord:
-    """A place for the argument record outside the geometry's own attributes, which
-    vars(), copies and pickles show."""
-    __slots__ = ("_ref",)
+    """A place for the argument record, and for the workspace sizes asked for so far,
+    outside the geometry's own attributes, which vars(), copies and pickles show."""
+    __slots__ = ("_ref", "_sizes")
 
 
 @dataclass(frozen=True)
@@ -673,36 +673,37 @@ class PagedKiviCache:
 
     # ---- attention of chunks of queries, read-back (include/jacq_kivi_attend.h) ----
 
-    def _fits_pool(self, index: int) -> bool:
-        g = self.geo
+    def __setattr__(self, name: str, value) -> None:
+        object.__setattr__(self, name, value)
+        vars(self).pop("_held", None)  # the record goes by what the cache holds now
+
+    def __getstate__(self):  # copies and pickles make their own record
+        return {n: v for n, v in vars(self).items() if n != "_held"}
+
+    def _record(self):
+        """The packed pool record and the GPU's index, once the cache's tensors are seen to have
+        the layouts of its geometry."""
+        lib()
+        g, dev = self.geo, self.k_code.device
         codes = (g.num_pages, g.num_kv_heads, g.page_size, g.head_dim // 2)
         k_scales = (g.num_pages, g.num_kv_heads, g.head_dim)
         v_scales = (g.num_pages, g.num_kv_heads, g.page_size, g.head_dim // g.group_size)
         scratch = (self.batch, g.num_kv_heads, g.scratch_rows, g.head_dim)
-        for t, shape, dtype in ((self.k_code, codes, torch.uint8), (self.v_code, codes, torch.uint8),
-                                (self.k_scale, k_scales, torch.float16),
-                                (self.k_zero, k_scales, torch.float16),
-                                (self.v_scale, v_scales, torch.float16),
-                                (self.v_zero, v_scales, torch.float16),
-                                (self.k_scr, scratch, torch.float16),
-                                (self.v_scr, scratch, torch.float16)):
-            if not (t.shape == shape and t.dtype is dtype and t.is_contiguous()
-                    and t.get_device() == index):
-                return False
-        return True
+        for t, shape, dtype, name in zip(
+                self.pool(), (codes, k_scales, k_scales, codes, v_scales, v_scales, scratch, scratch),
+                (torch.uint8, *[torch.float16] * 2) * 2 + (torch.float16,) * 2, POOL_NAMES):
+            _check(t.shape == shape and t.dtype == dtype and t.is_contiguous() and t.device == dev,
+                   name, " must be contiguous ", dtype, " ", shape, " on ", dev)
+        held = vars(self)["_held"] = (_POOL.pack(*self._pool_ptrs()), self.k_code.get_device())
+        return held
 
-    def _here(self, *named) -> int:
-        """The index of the cache's GPU, on which the pool and the named tensors have to be."""
+    def _here(self, index: int, *named) -> None:
         dev = self.k_code.device
         for name, t in named:
             if t is not None:
                 _check(t.device == dev, name, " must be on the cache's device ", dev, ", got ",
                        t.device)
-        _check(dev.type == "cuda", "the cache must be on a GPU device, got ", dev)
-        index = self.k_code.get_device()
-        _check(self._fits_pool(index), "the cache's tensors must have the layouts of its geometry, "
-               "contiguous, on one device")
-        return index
+        _check(index >= 0, "the cache must be on a GPU device, got ", dev)
 
     def _offsets(self, t: torch.Tensor, n: int, name: str) -> None:
         check_shape(t, (n,), name)
@@ -718,30 +719,55 @@ class PagedKiviCache:
         if rc != 0:
             _raise(rc)
 
+    def _workspace_size(self, key: tuple) -> int:
+        g = self.geo
+        with torch.cuda.device(key[0]):  # the size goes by its compute units
+            size = lib().jacq_kivi_attend_workspace_size(g.ref, *key[1:])
+        try:
+            sizes = g._sizes
+        except AttributeError:
+            sizes = {}
+            object.__setattr__(g, "_sizes", sizes)
+        if len(sizes) > 4096:
+            sizes.clear()
+        sizes[key] = size
+        return size
+
     def _attend(self, q, cu_q, max_q, seq_lens, block_tables, window, sinks, causal, scale, out, lse,
                 workspace) -> torch.Tensor:
-        g = self.geo
+        g, batch = self.geo, self.batch
         nh, hd = g.num_heads, g.head_dim
-        _check(q.dim() == 3 and q.shape[1:] == (nh, hd), "Q must be [tokens, ", nh, ", ", hd,
-               "], got ", tuple(q.shape))
-        _check(q.dtype in (torch.float16, torch.bfloat16), "Q must be fp16 or bf16")
-        total, stride = q.shape[0], nh * hd
-        if not q.is_contiguous():
-            _check(total == 0 or (q.stride(2) == 1 and q.stride(1) == hd),
-                   "Q must have its heads side by side")
-            if total > 1:
-                stride = q.stride(0)
-                _check(stride >= nh * hd, "Q must have a token's row after the one before")
-        if not self._fits(seq_lens, block_tables):
+        pool, index = vars(self).get("_held") or self._record()
+        shape, dtype = q.shape, q.dtype
+        contiguous = q.is_contiguous()
+        fits = (index >= 0 and len(shape) == 3 and shape[1] == nh and shape[2] == hd and contiguous
+                and (dtype is torch.float16 or dtype is torch.bfloat16)
+                and self._fits(seq_lens, block_tables) and seq_lens.is_contiguous()
+                and q.get_device() == index == seq_lens.get_device() == block_tables.get_device())
+        stride = nh * hd
+        if not fits:
+            _check(len(shape) == 3 and shape[1:] == (nh, hd), "Q must be [tokens, ", nh, ", ", hd,
+                   "], got ", tuple(shape))
+            _check(dtype in (torch.float16, torch.bfloat16), "Q must be fp16 or bf16")
+            if not contiguous:
+                _check(shape[0] == 0 or (q.stride(2) == 1 and q.stride(1) == hd),
+                       "Q must have its heads side by side")
+                if shape[0] > 1:
+                    stride = q.stride(0)
+                    _check(stride >= nh * hd, "Q must have a token's row after the one before")
             self._check_tables(seq_lens, block_tables)
-        _check(seq_lens.is_contiguous(), "SEQ_LENS must be contiguous")
+            _check(seq_lens.is_contiguous(), "SEQ_LENS must be contiguous")
+        total = shape[0]
         if cu_q is None:
-            _check(total == self.batch, "without CU_Q there is one query per sequence: ", self.batch,
-                   ", got ", total)
+            _check(total == batch, "without CU_Q there is one query per sequence: ", batch, ", got ",
+                   total)
             _check(max_q is None or max_q == 1, "MAX_Q is for CU_Q")
             max_q = 1
         else:
-            self._offsets(cu_q, self.batch + 1, "CU_Q")
+            if not (cu_q.shape == (batch + 1,) and cu_q.dtype is torch.int32
+                    and cu_q.is_contiguous() and cu_q.get_device() == index):
+                self._offsets(cu_q, batch + 1, "CU_Q")
+                fits = False
             _check(max_q is None or max_q >= 0, "MAX_Q must not be negative")
             max_q = total if max_q is None else min(int(max_q), total)
         if window is None:
@@ -751,20 +777,25 @@ class PagedKiviCache:
         _check(sinks >= 0, "SINKS must not be negative")
         scale = hd ** -0.5 if scale is None else float(scale)
         _check(0.0 < scale < math.inf, "SCALE must be positive and finite")
-        if out is None:
-            out = torch.empty((total, nh, hd), dtype=q.dtype, device=q.device)
-        else:
+        if out is not None:
             check_shape(out, (total, nh, hd), "O")
-            _check(out.dtype in (q.dtype, torch.float32) and out.is_contiguous(),
+            _check(out.dtype in (dtype, torch.float32) and out.is_contiguous(),
                    "O must be contiguous, of Q's type or fp32")
         if lse is not None:
             check_shape(lse, (total, nh), "LSE")
             _check(lse.dtype == torch.float32 and lse.is_contiguous(), "LSE must be contiguous fp32")
-        index = self._here(("Q", q), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
-                           ("CU_Q", cu_q), ("O", out), ("LSE", lse), ("workspace", workspace))
+        if not fits or out is not None or lse is not None or workspace is not None:
+            self._here(index, ("Q", q), ("SEQ_LENS", seq_lens), ("BLOCK_TABLES", block_tables),
+                       ("CU_Q", cu_q), ("O", out), ("LSE", lse), ("workspace", workspace))
+        if out is None:  # empty_like is the quicker one, for a q that is contiguous
+            out = (torch.empty_like(q) if contiguous else
+                   torch.empty((total, nh, hd), dtype=dtype, device=q.device))
         if workspace is None:
-            with torch.cuda.device(index):  # the size goes by its compute units
-                size = lib().jacq_kivi_attend_workspace_size(g.ref, self.batch, total, max_q)
+            key = (index, batch, total, max_q)
+            try:
+                size = g._sizes[key]
+            except (AttributeError, KeyError):
+                size = self._workspace_size(key)
             if size:
                 workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         else:
@@ -772,10 +803,10 @@ class PagedKiviCache:
             size = workspace.numel() * workspace.element_size()
         args = _ATTEND.pack(q.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
                             seq_lens.data_ptr(), block_tables.data_ptr(), out.data_ptr(),
-                            0 if lse is None else lse.data_ptr(), stride, DTYPES[q.dtype],
-                            DTYPES[out.dtype], self.batch, total, max_q, min(window, 1 << 30),
+                            0 if lse is None else lse.data_ptr(), stride, DTYPES[dtype],
+                            DTYPES[out.dtype], batch, total, max_q, min(window, 1 << 30),
                             min(sinks, 1 << 30), causal, scale)
-        self._call(index, lib().jacq_kivi_attend, g.ref, _POOL.pack(*self._pool_ptrs()), args,
+        self._call(index, _lib.jacq_kivi_attend, g.ref, pool, args,
                    0 if workspace is None else workspace.data_ptr(), size)
         return out
 
@@ -813,16 +844,20 @@ class PagedKiviCache:
         sequence after another: K, V [total, NKV, HD].  total is their number: tokens past it
         are dropped, rows that none fills undefined."""
         g = self.geo
-        if not self._fits(ends, block_tables):
-            self._check_tables(ends, block_tables)
-        _check(ends.is_contiguous(), "ENDS must be contiguous")
-        self._offsets(starts, self.batch, "STARTS")
+        pool, index = vars(self).get("_held") or self._record()
         _check(dtype in DTYPES, "values are read as fp16, bf16 or fp32, not ", dtype)
         _check(total >= 0, "TOTAL must not be negative")
-        index = self._here(("STARTS", starts), ("ENDS", ends), ("BLOCK_TABLES", block_tables))
+        if not (index >= 0 and self._fits(ends, block_tables) and ends.is_contiguous()
+                and starts.shape == (self.batch,) and starts.dtype is torch.int32
+                and starts.is_contiguous()
+                and starts.get_device() == index == ends.get_device() == block_tables.get_device()):
+            self._check_tables(ends, block_tables)
+            _check(ends.is_contiguous(), "ENDS must be contiguous")
+            self._offsets(starts, self.batch, "STARTS")
+            self._here(index, ("STARTS", starts), ("ENDS", ends), ("BLOCK_TABLES", block_tables))
         k = torch.empty((total, g.num_kv_heads, g.head_dim), dtype=dtype, device=ends.device)
         v = torch.empty_like(k)
-        self._call(index, lib().jacq_kivi_read, g.ref, _POOL.pack(*self._pool_ptrs()),
-                   starts.data_ptr(), ends.data_ptr(), block_tables.data_ptr(), self.batch, total,
-                   k.data_ptr(), v.data_ptr(), DTYPES[dtype])
+        self._call(index, _lib.jacq_kivi_read, g.ref, pool, starts.data_ptr(), ends.data_ptr(),
+                   block_tables.data_ptr(), self.batch, total, k.data_ptr(), v.data_ptr(),
+                   DTYPES[dtype])
         return k, v

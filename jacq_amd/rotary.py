@@ -151,6 +151,14 @@ class Rotary:
                " must have a token's row after the one before")
         return max(t.stride(0), shape[1] * hd)
 
+    def _quick(self, t: torch.Tensor, index: int) -> int:
+        """The elements between token rows, or 0 for the named checks to say what is wrong: they
+        take the host longer than a small call takes the GPU."""
+        shape, stride, hd = t.shape, t.stride(), self.head_dim
+        return (stride[0] if len(shape) == 3 and shape[2] == hd and stride[2] == 1 and stride[1] == hd
+                and stride[0] >= shape[1] * hd > 0 and t.dtype in DTYPES and t.get_device() == index
+                else 0)
+
     def rotate(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                inverse: bool = False, k_dtype: torch.dtype | None = None,
                q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
@@ -160,40 +168,54 @@ class Rotary:
         q_out, k_out, of any type, which may be q and k themselves and must overlap neither
         otherwise.  k may be None.  inverse: by the negative angles; with an amplitude of 1 the
         way back, with any the gradient of this rotation for the gradient of its outputs."""
-        tokens = q.shape[0] if q.dim() else 0
-        strides = [self._rows(q, tokens, None, "Q"), 0, 0, 0]
-        heads, kv_heads = q.shape[1], 0
+        shape, dtype, index = q.shape, q.dtype, q.get_device()
+        tokens = shape[0] if len(shape) else 0
+        q_stride, k_stride = self._quick(q, index), 0
+        fits = (q_stride and index >= 0 and positions.shape == (tokens,)
+                and (positions.dtype is torch.int32 or positions.dtype is torch.int64)
+                and positions.is_contiguous() and positions.get_device() == index)
         if k is not None:
-            strides[1] = self._rows(k, tokens, None, "K")
-            kv_heads = k.shape[1]
-            _check(k.dtype == q.dtype, "K must be of Q's type")
+            k_stride = self._quick(k, index)
+            fits = fits and k_stride and k.shape[0] == tokens and k.dtype is dtype
+        fits = fits and q_out is None and k_out is None and (k_dtype is None or k is not None)
+        if not fits:
+            q_stride = self._rows(q, tokens, None, "Q")
+            if k is not None:
+                k_stride = self._rows(k, tokens, None, "K")
+                _check(k.dtype == dtype, "K must be of Q's type")
+            else:
+                _check(k_out is None and k_dtype is None, "K_OUT and K_DTYPE are for K")
+            check_shape(positions, (tokens,), "POSITIONS")
+            _check(positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous(),
+                   "POSITIONS must be contiguous int32 or int64")
+        heads, kv_heads = shape[1], 0 if k is None else k.shape[1]
+        _check(k_dtype is None or k_dtype in DTYPES, "K_DTYPE must be fp16, bf16 or fp32")
+        strides = [q_stride, k_stride, heads * self.head_dim, kv_heads * self.head_dim]
+        if q_out is None:  # empty_like is the quicker one, where it gives rows side by side
+            q_out = (torch.empty_like(q) if fits else
+                     torch.empty((tokens, heads, self.head_dim), dtype=dtype, device=q.device))
         else:
-            _check(k_out is None and k_dtype is None, "K_OUT and K_DTYPE are for K")
-        check_shape(positions, (tokens,), "POSITIONS")
-        _check(positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous(),
-               "POSITIONS must be contiguous int32 or int64")
-        if q_out is None:
-            q_out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=q.device)
-        strides[2] = self._rows(q_out, tokens, heads, "Q_OUT")
+            strides[2] = self._rows(q_out, tokens, heads, "Q_OUT")
         if k is not None:
             if k_out is None:
-                _check(k_dtype is None or k_dtype in DTYPES, "K_DTYPE must be fp16, bf16 or fp32")
-                k_out = torch.empty((tokens, kv_heads, self.head_dim), dtype=k_dtype or k.dtype,
-                                    device=q.device)
-            _check(k_dtype is None or k_out.dtype == k_dtype, "K_OUT must be of K_DTYPE")
-            strides[3] = self._rows(k_out, tokens, kv_heads, "K_OUT")
-        index = q.get_device()
-        _check(index >= 0, "Q must be on a GPU device, got ", q.device)
-        for t, name in ((k, "K"), (positions, "POSITIONS"), (q_out, "Q_OUT"), (k_out, "K_OUT")):
-            _check(t is None or t.get_device() == index, name, " must be on Q's device")
-        for t, out, i, name in ((q, q_out, 0, "Q_OUT"), (k, k_out, 1, "K_OUT")):
-            if t is not None and t.data_ptr() == out.data_ptr() and t.numel():
-                _check(t.dtype == out.dtype and strides[i] == strides[i + 2], name,
-                       " at its input's place must be of its type and stride")
+                k_out = (torch.empty_like(k, dtype=k_dtype or dtype) if fits else
+                         torch.empty((tokens, kv_heads, self.head_dim), dtype=k_dtype or dtype,
+                                     device=q.device))
+            else:
+                strides[3] = self._rows(k_out, tokens, kv_heads, "K_OUT")
+                _check(k_dtype is None or k_out.dtype == k_dtype, "K_OUT must be of K_DTYPE")
+        if not fits:
+            _check(index >= 0, "Q must be on a GPU device, got ", q.device)
+            for t, name in ((k, "K"), (positions, "POSITIONS"), (q_out, "Q_OUT"), (k_out, "K_OUT")):
+                _check(t is None or t.get_device() == index, name, " must be on Q's device")
+            for t, out, i, name in ((q, q_out, 0, "Q_OUT"), (k, k_out, 1, "K_OUT")):
+                if t is not None and t.data_ptr() == out.data_ptr() and t.numel():
+                    _check(t.dtype == out.dtype and strides[i] == strides[i + 2], name,
+                           " at its input's place must be of its type and stride")
         args = _ARGS.pack(q.data_ptr(), 0 if k is None else k.data_ptr(), positions.data_ptr(),
                           q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
                           ctypes.addressof(self._turns), *strides, tokens, heads, kv_heads,
-                          self.head_dim, self.rotary_dim, LAYOUTS[self.layout], DTYPES[q.dtype],
+                          self.head_dim, self.rotary_dim, LAYOUTS[self.layout], DTYPES[dtype],
                           DTYPES[q_out.dtype], 0 if k is None else DTYPES[k_out.dtype],
                           positions.dtype == torch.int64, bool(inverse), self.amplitude)
         fn = lib().jacq_rotary

@@ -2,6 +2,9 @@
 GPU."""
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -153,15 +156,39 @@ def test_python_read_refusals(kw, text):
         cpu_cache().read(**args)
 
 
+POOL_ATTRS = ("k_code", "k_scale", "k_zero", "v_code", "v_scale", "v_zero", "k_scr", "v_scr")
+
+
 def test_a_cache_of_other_tensors_than_its_geometrys_is_not_taken():
-    good = cpu_cache()
-    assert good._fits_pool(-1)
-    for name in ("k_code", "k_scale", "k_zero", "v_code", "v_scale", "v_zero", "k_scr", "v_scr"):
-        t = getattr(good, name)
+    for name in POOL_ATTRS:
+        cache = cpu_cache()
+        t = getattr(cache, name)
+        cache._record()
         for other in (t[:-1], t.double(), torch.cat((t, t), -1)[..., :t.shape[-1]]):
-            bad = cpu_cache()
-            setattr(bad, name, other)
-            assert not bad._fits_pool(-1)
+            setattr(cache, name, other)
+            with pytest.raises(kivi.KiviCheckError, match="must be contiguous"):
+                cache.prefill(q(), CU, 2, LENS, TABLES)
+        setattr(cache, name, t)
+        cache._record()
+
+
+def test_calls_take_the_tensors_that_a_cache_holds_now():
+    cache = cpu_cache()
+
+    def held(c):
+        return kivi._POOL.unpack((vars(c).get("_held") or c._record())[0])
+
+    for name in POOL_ATTRS:
+        held(cache)
+        setattr(cache, name, getattr(cache, name).clone())
+        assert held(cache) == tuple(t.data_ptr() for t in cache.pool())
+    for make, shared in ((copy.copy, True), (copy.deepcopy, False),
+                         (lambda c: pickle.loads(pickle.dumps(c)), False)):
+        other = make(cache)
+        assert other.geo == cache.geo and other.batch == 2
+        assert held(other) == tuple(t.data_ptr() for t in other.pool())
+        assert (held(other) == held(cache)) == shared
+    assert held(cache.sequence_view(1))[6] == cache.k_scr[1].data_ptr()
 
 
 # ---- the reference itself ----
