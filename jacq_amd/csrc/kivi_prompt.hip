@@ -242,13 +242,13 @@ __global__ __launch_bounds__(2 * HD) void kivi_lay_kernel(KiviGeo g, KiviAttendA
 }
 
 template <int HD>
-__global__ __launch_bounds__(64 * kPromptWaves, 2) void kivi_prompt_kernel(KiviGeo g, KiviAttendArgs a,
+__global__ __launch_bounds__(64 * kPromptWaves, 3) void kivi_prompt_kernel(KiviGeo g, KiviAttendArgs a,
                                                                            int pass) {
   constexpr int KS = HD / 16;  // k-steps of S^T
   constexpr int DT = HD / 32;  // channel tiles
   struct Lds {
     uint16_t k[2][kTile][HD];
-    uint16_t v[2][HD][kTile];
+    uint16_t v[HD][kTile];
   };
   extern __shared__ __align__(16) uint8_t shared_bytes[];
   Lds& lds = *(Lds*)shared_bytes;
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kivi_prompt_kernel(KiviG
   };
   auto copy_v = [&](int u) {
     copy(images + (uint64_t)seq.unit_of(tile_at(u)) * sizeof(Image<HD>) + kTile * HD * 2,
-         lds_addr(&lds.v[u & 1][0][0]) + wave * PART);
+         lds_addr(&lds.v[0][0]) + wave * PART);
   };
 
   // K row of this lane in a tile of 32: the scores of a lane are then tokens 8 hh ... + 7 of either half
@@ -345,9 +345,6 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kivi_prompt_kernel(KiviG
   };
   // What a tile is to the wavefront's rows: nothing (behind them all, or before their windows), seen by
   // all of them, or in part.
-  auto nothing = [&](int t0) {
-    return t0 > wlast || (a.window > 0 && t0 + kTile - 1 <= wfirst - a.window && t0 >= a.sinks);
-  };
   auto whole = [&](int t0) {
     return t0 + kTile - 1 <= wfirst && (a.window <= 0 || t0 > wlast - a.window || t0 + kTile <= a.sinks);
   };
@@ -402,7 +399,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kivi_prompt_kernel(KiviG
       }
   };
   auto values = [&](int u) {
-    const uint16_t* vb = &lds.v[u & 1][0][0];
+    const uint16_t* vb = &lds.v[0][0];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -418,31 +415,31 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kivi_prompt_kernel(KiviG
 
   if (count > 0) {
     copy_k(0);
+    landed();
     copy_v(0);
     copy_k(1);
-    landed();
-    if (!nothing(tile_at(0) * kTile)) scores(0);
-    turn();
     for (int u = 0; u < count; ++u) {
-      // K of u + 2 takes the place of u's, whose scores are done; V of u + 1 that of u - 1
-      copy_k(u + 2);
-      copy_v(u + 1);
       const int t0 = tile_at(u) * kTile;
-      if (!nothing(t0)) {
-        soften(u, t0);
-        values(u);
-      }
-      if (u + 1 < count && !nothing(tile_at(u + 1) * kTile)) scores(u + 1);
-      landed();
+      scores(u);
+      soften(u, t0);
+      landed();     // V of u and K of u + 1; and K of u is done with
+      copy_k(u + 2);
+      values(u);
+      turn();       // V of u is done with
+      copy_v(u + 1);
     }
+    wait_vm<0>();
   }
 
   l += other_half(l);
-  if (!ok) return;
-  const int64_t at = (int64_t)(q0 + tok) * g.nh + head;
+  // the row once more, rather than in registers over the loop
+  const int end_lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+  const int out_row = wr0 + (end_lane & 31), hh_ = end_lane >> 5;
+  if (out_row >= rows) return;
+  const int64_t at = (int64_t)(q0 + out_row / g.gqa) * g.nh + h * g.gqa + out_row % g.gqa;
   if (slices > 1) {  // kivi_prompt_merge_kernel joins the slices
     const int64_t part = (int64_t)slice * a.total_q * g.nh + at;
-    if (hh == 0) {
+    if (hh_ == 0) {
       a.part_ml[2 * part] = mx;
       a.part_ml[2 * part + 1] = l;
     }
@@ -450,17 +447,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kivi_prompt_kernel(KiviG
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *(f4*)(a.part_acc + part * HD + d * 32 + i * 8 + hh * 4) =
+        *(f4*)(a.part_acc + part * HD + d * 32 + i * 8 + hh_ * 4) =
             f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
     return;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (a.lse && hh == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
+  if (a.lse && hh_ == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      store4(a, at * HD + d * 32 + i * 8 + hh * 4,
+      store4(a, at * HD + d * 32 + i * 8 + hh_ * 4,
              f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]} * inv);
 }
 
@@ -472,7 +469,7 @@ __global__ __launch_bounds__(256) void kivi_prompt_merge_kernel(KiviGeo g, KiviA
 template <int HD>
 static hipError_t prompt_kernels(const KiviGeo& g, const KiviAttendArgs& a, int passes, int64_t images,
                                  hipStream_t s) {
-  constexpr int LDS = 2 * sizeof(Image<HD>);
+  constexpr int LDS = (2 * kTile * HD + kTile * HD) * 2;
   if (LDS > 65536) {  // past 64 KiB a kernel asks for its LDS
     const hipError_t e = hipFuncSetAttribute((const void*)kivi_prompt_kernel<HD>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
