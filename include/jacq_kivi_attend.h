@@ -15,10 +15,12 @@
  * with K = code * scale + zero of its group and channel, V = code * scale +
  * zero of itself and its 32 channels; else it is row t - old of the scratch.
  * Values are rounded to fp16 once.  A token that a query does not see may hold
- * anything.  To a query that sees it, a V that is not finite counts as a NaN
- * key: all of the query's output is NaN.  A table entry outside
- * [0, num_pages) is never dereferenced: its tokens are NaN to the queries
- * that see them.  Lengths are clamped on the device to
+ * anything.  To a query that sees it, a V that is not finite (fp16 V; or zero
+ * or zero + 15 scale of 32 of its channels beyond fp16) counts as a NaN key:
+ * all of the query's output is NaN.  A table entry outside
+ * [0, num_pages) is never dereferenced: its tokens, and if it is a group's
+ * first, which holds the scales of K, the group's, are NaN to the queries
+ * that see them, and are read as NaN.  Lengths are clamped on the device to
  * [0, jacq_kivi_max_seq_len].
  */
 #ifndef JACQ_KIVI_ATTEND_H

@@ -222,12 +222,13 @@ __device__ inline uint64_t low_bits(int n) {
   return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
 }
 
-// Joins the slices of every row, in their order: a thread per 4 channels, 256 a workgroup.
+// Joins the slices of every row, in their order: a thread per 4 channels, 256 a workgroup.  row_slices is
+// the cache's own rule.
 template <int HD, class G, class A>
 __device__ inline void merge_slices(const G& g, const A& a) {
   static_assert(256 / (HD / 4) == 1 << merge_log2(HD), "rows of a workgroup");
   const Place p = place_of(g, a, blockIdx.x, g.nh, merge_log2(HD));
-  const int slices = prefill_slices(a, p.n);
+  const int slices = uniform(row_slices(g, a, p));
   if (slices == 1 || p.at < 0) return;
   const int64_t i = (int64_t)p.at * 256 + threadIdx.x;
   const int ch = (int)(i % (HD / 4)) * 4;

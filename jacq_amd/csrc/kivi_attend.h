@@ -43,9 +43,9 @@ struct KiviAttendArgs {
   int row_blocks;         // row blocks of a sequence at most
   // prompts
   int slices;             // workgroups that share a row tile's tokens, at most
-  float load;             // row tiles a CU
   unsigned tiles, merges; // units of row tiles, and of the merge's (Place)
-  int32_t* slots;         // [batch + 1] first tile image of each sequence, then their number
+  int32_t* slots;         // [batch + 1] first tile image of each sequence, then their number, then
+                          // (float) the tiles that are a slice's share
   int per_pass;           // tile images of a pass; a sequence's begin in one and may end behind it
   uint8_t* images;        // K [64][HD], then V [HD][64], fp16, as they lie in the LDS
   uint64_t* poison;       // of each image: the tokens whose V is not finite or not there
@@ -108,6 +108,30 @@ struct KiviTiles {
   __device__ int tile_of(int u) const { return u < ns ? u : w0 + u - ns; }
   __device__ int unit_of(int tile) const { return tile < ns ? tile : tile - w0 + ns; }
 };
+
+// Tiles that a row tile of a sequence goes through, about: half of its own queries' are behind its rows.
+__device__ inline float row_tiles_units(const KiviAttendArgs& a, const KiviTiles& t, int m, int all) {
+#pragma clang fp contract(off)  // every kernel has to find the same
+  float units = (float)t.units;
+  if (a.window > 0) {
+    const float most = ((float)a.window + (float)a.sinks + (float)kPrefillRows) / (float)kTile + 2.0f;
+    units = units < most ? units : most;
+  } else if (a.causal) {
+    units -= ((float)all - 0.5f * (float)m) / (float)kTile;
+  }
+  return units < 1.0f ? 1.0f : units;
+}
+
+// Workgroups that share the tokens of each of a sequence's row tiles.
+__device__ inline int kivi_slices(const KiviAttendArgs& a, const KiviTiles& t, int m, int all) {
+  if (a.slices == 1) return 1;
+  const float share = __int_as_float(a.slots[a.batch + 1]);
+  const int n = (int)__builtin_ceilf(row_tiles_units(a, t, m, all) / share);
+  return n < 1 ? 1 : n > a.slices ? a.slices : n;
+}
+__device__ inline int row_slices(const KiviGeo& g, const KiviAttendArgs& a, const Place& p) {
+  return kivi_slices(a, KiviTiles(g, a, p.n, a.causal ? p.n - p.all : p.n - 1), p.m, p.all);
+}
 
 template <>
 struct SpanOf<KiviGeo> {
@@ -195,6 +219,12 @@ __device__ inline float half_row(const u4 (&raw)[N], int bf16, float scale, h8 (
   return __builtin_amdgcn_ldexpf(scale, -e);
 }
 
+// Whether fp16 holds all values of a scale and a zero, the ends being 0 and 15 times the scale from it;
+// NaN does not pass, and 65520 is the least that rounds to infinity.
+__device__ inline bool holds(float scale, float zero) {
+  return __builtin_fabsf(zero) < 65520.0f && __builtin_fabsf(__builtin_fmaf(15.0f, scale, zero)) < 65520.0f;
+}
+
 // The largest magnitude of two sets of fp16 pairs as bits, in either half: 0x7c00 and more is no
 // finite value.
 __device__ inline uint32_t most_bits(uint32_t a, uint32_t b) {
@@ -210,6 +240,8 @@ hipError_t launch_attend_prompt(const KiviGeo& g, const KiviAttendArgs& a, int p
 hipError_t launch_kivi_read(const KiviGeo& g, const KiviPool& p, const int32_t* starts,
                             const int32_t* ends, const int32_t* tables, int batch, int total, void* k,
                             void* v, int type, hipStream_t s);
+// Workgroups of the prompts' kernel that a CU holds.
+constexpr int prompt_groups(int hd) { return hd == 128 ? 3 : 4; }
 // Workgroups of the few-query kernel that a CU holds.
 constexpr int few_groups(int hd, int nb) { return hd == 64 ? 5 - nb : 4 - nb; }
 

@@ -113,32 +113,34 @@ constexpr int kWholeUnits = 24;
 // for it.
 constexpr int kCutBatch = 64;
 
-// Rows of a kv head from which a call is a prompt's: its tokens become fp16 once, in the workspace.
-constexpr int kPromptRows = 256;
-// Bytes of fp16 tiles that a pass lays in the workspace, about, and passes at most: a call of more
-// (many sequences under a wide table) is left to the few-query kernel.
+// A call is a prompt's, whose tokens become fp16 once, in the workspace, from so many rows of a kv head
+// and (query, head) rows x tokens of the table on.  Few-query kernel against prompts', us a call:
+//   160 rows   8 sequences of 4000 to 8000, 40/8 heads of 128 121 against 138; 32 of 300 to 1500 77 and 92
+//   320 rows   the same 171 and 164, 131 and 117; one of 16384 62 and 69 (42 M rows x tokens), 16/16 heads
+//              of 64 83 and 69 (84 M)
+//   640 rows   one of 16384, 40/8 heads of 128 107 and 92 (84 M), of 700 19 and 28 (4 M); 8 of 4000 to
+//              8000, 14/2 heads of 64 91 and 57 (82 M), 32 of 300 to 1500 50 and 46 (61 M)
+//   1274 rows  one of 16384, 14/2 heads of 64 45 and 48 (42 M)
+constexpr int64_t kPromptRows = 320;
+constexpr int64_t kPromptWork = 50000000;
+// Bytes of fp16 tiles that a pass lays in the workspace, about, and passes at most, a few us each (of a
+// wide table's, most have nothing to do): a call of more is left to the few-query kernel.
 constexpr int64_t kPassBytes = (int64_t)1 << 31;
-constexpr int64_t kMostPasses = 16;
+constexpr int64_t kMostPasses = 64;
+// A prompt's workgroups a CU at most, slices counted: those that the lengths do not ask for end at once.
+constexpr int64_t kMostGroups = 8;
+// Bytes of parts for which the few-query kernel still cuts: a call of more has segments enough.
+constexpr int64_t kMostParts = (int64_t)1 << 30;
+
+// Test hook: not 0: the bytes of a pass on the calling thread.
+thread_local int64_t g_pass_bytes = 0;
 
 struct Plan {
   bool prompt, planned;
   int nb, rows, row_blocks, target;
-  float load;
   int slices, per_pass, passes;
   size_t ml, acc, plan, slots, images, poison, bytes;  // offsets into the workspace, and its size
 };
-
-// A prompt's slices, for as many tokens as the table addresses: the kernels use fewer for sequences of
-// fewer (slices_cost, which has the reasons).  One, unless more promise 3 % at least.
-int plan_slices(float load, int64_t tokens) {
-  const int most =
-      (int)std::min<int64_t>(jacq::kMaxSlices, tokens / (jacq::kSliceUnits * jacq::kTile));
-  auto cost = [&](int s) { return jacq::slices_cost(load, s, (float)tokens); };
-  int best = 1;
-  for (int s = 2; s <= most; ++s)
-    if (cost(s) < cost(best)) best = s;
-  return cost(best) < 0.97f * cost(1) ? best : 1;
-}
 
 Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   Plan p = {};
@@ -162,13 +164,19 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   const int64_t cap = (tokens + jacq::kTile - 1) / jacq::kTile;  // images of a sequence and kv head
   const int64_t image = (int64_t)4 * jacq::kTile * g.hd * g.nkv;
   const int64_t images = std::min<int64_t>(batch, total_q) * cap;
-  p.per_pass = (int)std::max<int64_t>(1, std::min(images, kPassBytes / image));
+  const int64_t pass_bytes = g_pass_bytes ? g_pass_bytes : kPassBytes;
+  p.per_pass = (int)std::max<int64_t>(1, std::min(images, pass_bytes / image));
   const int64_t passes = (images + p.per_pass - 1) / p.per_pass;
-  p.prompt = rows >= kPromptRows && passes <= kMostPasses && images <= INT32_MAX - 1024;
+  p.prompt = rows >= kPromptRows && queries * g.nh * tokens >= kPromptWork &&
+             passes <= kMostPasses && images <= INT32_MAX - 4096;
   if (p.prompt) {
     p.passes = (int)passes;
-    p.load = (float)(blocks(jacq::kPrefillRows) * g.nkv) / (float)device_cus();
-    p.slices = plan_slices(p.load, tokens);
+    // row tiles in so many slices that their workgroups are no more than kMostGroups a CU: the device
+    // uses as many as the lengths ask for (kivi_slots_kernel), the others end at once
+    const int64_t groups = std::max<int64_t>(1, blocks(jacq::kPrefillRows) * g.nkv);
+    p.slices = (int)std::max<int64_t>(
+        1, std::min<int64_t>({jacq::kMaxSlices, tokens / (jacq::kSliceUnits * jacq::kTile),
+                              kMostGroups * device_cus() / groups}));
     if (p.slices > 1) {
       const size_t rows_all = (size_t)p.slices * total_q * g.nh;
       p.ml = take(rows_all * 2 * sizeof(float));
@@ -176,7 +184,7 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
     }
     // a sequence's images may end behind the pass that they begin in
     const size_t held = (size_t)(passes == 1 ? images : p.per_pass + cap) * g.nkv;
-    p.slots = take(((size_t)batch + 1) * sizeof(int32_t));
+    p.slots = take(((size_t)batch + 2) * sizeof(int32_t));
     p.poison = take(held * sizeof(uint64_t));
     p.images = take(held * 4 * jacq::kTile * g.hd);
     p.bytes = at;
@@ -191,6 +199,7 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
     const int64_t slots = (int64_t)jacq::few_groups(g.hd, p.nb) * device_cus();
     p.target = (int)(3 * blocks(16 * p.nb) * g.nkv <= slots ? slots : 2 * slots);
   }
+  if ((p.target + segments) * p.rows * (g.hd + 2) * (int64_t)sizeof(float) > kMostParts) p.target = 0;
   const size_t parts = p.target ? (size_t)p.target + segments : 0;
   p.ml = take(parts * p.rows * 2 * sizeof(float));
   p.acc = take(parts * p.rows * g.hd * sizeof(float));
@@ -210,6 +219,14 @@ int64_t place_units(const KiviAttendArgs& a, int per, int log2) {
 }  // namespace
 
 extern "C" {
+
+// Test hooks outside the ABI: prompts of the calling thread lay about so many bytes of fp16 tiles a
+// pass (0: as many as ever); whether a call is a prompt's.
+void jacq_kivi_test_pass_bytes(int64_t bytes) { g_pass_bytes = bytes; }
+int32_t jacq_kivi_test_is_prompt(const jacq_kivi_geometry* geo, int32_t batch, int32_t total_q,
+                                 int32_t max_q) {
+  return plan_attend(make_geo(*geo), batch, total_q, std::min(max_q, total_q)).prompt;
+}
 
 size_t jacq_kivi_attend_workspace_size(const jacq_kivi_geometry* geo, int32_t batch, int32_t total_q,
                                        int32_t max_q) {
@@ -289,7 +306,7 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
     a.part_acc = (float*)(ws + p.acc);
     if (p.prompt) {
       a.slices = p.slices;
-      a.load = p.load;
+      a.cus = device_cus();
       a.tiles = (unsigned)tiles;
       a.merges = (unsigned)merges;
       a.slots = (int32_t*)(ws + p.slots);

@@ -223,8 +223,7 @@ struct Few {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float sc = h2f_((uint16_t)(s[e / 2] >> 16 * (e & 1))), ze = h2f_((uint16_t)(z[e / 2] >> 16 * (e & 1)));
-      // also for NaN; 65520 is the least that rounds to infinity
-      if (!(15.0f * __builtin_fabsf(sc) + __builtin_fabsf(ze) < 65520.0f)) bad |= 1u << e;
+      if (!holds(sc, ze)) bad |= 1u << e;
     }
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -308,8 +307,9 @@ struct Few {
     if (a.window > 0 && seen.first >= a.window)
       lo = sp.ns + ((seen.first - a.window + 1) / kGroup - sp.w0);
     u1 = u1 < hi ? u1 : hi;
+    const int sinks = a.window > 0 ? (int)(((int64_t)a.sinks + kGroup - 1) / kGroup) : 0;  // units of them
     auto next = [&](int u) {  // u, or behind what lies between the sinks and lo
-      return u >= sp.ns && u < lo ? u + (lo - u + kSliceWaves - 1) / kSliceWaves * kSliceWaves : u;
+      return u >= sinks && u < lo ? u + (lo - u + kSliceWaves - 1) / kSliceWaves * kSliceWaves : u;
     };
     const StageBases sb = stage_bases<HD, P>(a.pool, g.nkv, s.h, lane);
     const int32_t* table = a.tables + (int64_t)s.b * g.max_pages;

@@ -17,6 +17,7 @@ namespace jacq {
 namespace {
 
 constexpr int kPromptWaves = 4;
+constexpr float kRounds = 0.7f;
 static_assert(kPrefillRows == 32 * kPromptWaves, "32 rows a wavefront");
 
 // Where chunk c (8 values) of a row of an image lies, so that 16 rows' same chunk covers all banks.
@@ -52,11 +53,14 @@ __device__ inline bool images_of(const KiviGeo& g, const KiviAttendArgs& a, int 
 
 }  // namespace
 
-// The first image of every sequence.  One workgroup.
+// The first image of every sequence, and a slice's share of the tiles that row tiles go through.  One
+// workgroup.
 __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendArgs a) {
   __shared__ int sums[2][16];
+  __shared__ float work[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   int before = 0;
+  float w = 0.0f;
   for (int base = 0, turn = 0; base < a.batch; base += 1024, turn ^= 1) {
     const int b = base + tid;
     int units = 0;
@@ -64,7 +68,11 @@ __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendA
       int q0, m, all;
       queries_of(a, b, &q0, &m, &all);
       const int n = clamp_len(g, a.lens[b]);
-      if (m > 0) units = KiviTiles(g, a, n, a.causal ? n - all : n - 1).units;
+      if (m > 0) {
+        const KiviTiles tiles(g, a, n, a.causal ? n - all : n - 1);
+        units = tiles.units;
+        w += (float)((m * g.gqa + kPrefillRows - 1) / kPrefillRows) * row_tiles_units(a, tiles, m, all);
+      }
     }
     const int inc = wave_prefix(units, Sum());
     if (lane == 63) sums[turn][wave] = inc;
@@ -76,7 +84,16 @@ __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendA
     }
     if (b < a.batch) a.slots[b] = here;
   }
-  if (tid == 0) a.slots[a.batch] = before;
+  w = __int_as_float(lane63(wave_prefix(__float_as_int(w), SumF())));
+  if (lane == 0) work[wave] = w;
+  __syncthreads();
+  if (tid == 0) {
+    a.slots[a.batch] = before;
+    w = 0.0f;
+    for (int i = 0; i < 16; ++i) w += work[i];
+    const float share = w * (float)g.nkv / (kRounds * (float)(prompt_groups(g.hd) * a.cus));
+    a.slots[a.batch + 1] = __float_as_int(share > (float)kSliceUnits ? share : (float)kSliceUnits);
+  }
 }
 
 // The images of a pass, one at a time (blockIdx.y: kv head).  HD threads have V, a chunk of 8 channels of 8
@@ -152,10 +169,7 @@ __global__ __launch_bounds__(2 * HD) void kivi_lay_kernel(KiviGeo g, KiviAttendA
         if (!ok[0] || !ok[r0 >> 4]) mask = 255;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          // also for NaN; 65520 is the least that rounds to infinity
-          if (!(15.0f * __builtin_fabsf(h2f_((uint16_t)s[e])) + __builtin_fabsf(h2f_((uint16_t)z[e])) <
-                65520.0f))
-            mask |= 1u << e;
+          if (!holds(h2f_((uint16_t)s[e]), h2f_((uint16_t)z[e]))) mask |= 1u << e;
           if (mask >> e & 1) s[e] = z[e] = 0;
         }
 #pragma unroll
@@ -242,8 +256,8 @@ __global__ __launch_bounds__(2 * HD) void kivi_lay_kernel(KiviGeo g, KiviAttendA
 }
 
 template <int HD>
-__global__ __launch_bounds__(64 * kPromptWaves, 3) void kivi_prompt_kernel(KiviGeo g, KiviAttendArgs a,
-                                                                           int pass) {
+__global__ __launch_bounds__(64 * kPromptWaves, prompt_groups(HD)) void kivi_prompt_kernel(
+    KiviGeo g, KiviAttendArgs a, int pass) {
   constexpr int KS = HD / 16;  // k-steps of S^T
   constexpr int DT = HD / 32;  // channel tiles
   struct Lds {
@@ -260,13 +274,13 @@ __global__ __launch_bounds__(64 * kPromptWaves, 3) void kivi_prompt_kernel(KiviG
   const int rows = place.m * g.gqa;
   const int rt = (rows + kPrefillRows - 1) / kPrefillRows - 1 - place.at;  // the longest first
   if (rt < 0 || place.at < 0) return;
-  const int slices = uniform(prefill_slices(a, n));
-  if (slice >= slices) return;
   // positions: the first query's, then the workgroup's and the wavefront's rows; without an order every
   // row stands at the last token
   const int p0 = n - place.all;
   auto position = [&](int row) { return a.causal ? p0 + row / g.gqa : n - 1; };
   const KiviTiles seq(g, a, n, a.causal ? p0 : n - 1);
+  const int slices = uniform(kivi_slices(a, seq, place.m, place.all));
+  if (slice >= slices) return;
   int64_t image;
   if (!images_of(g, a, b, pass, seq.units, h, &image)) return;
   const int end_row = rows < (rt + 1) * kPrefillRows ? rows : (rt + 1) * kPrefillRows;
@@ -301,8 +315,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 3) void kivi_prompt_kernel(KiviG
   int top = plast < 0 ? 0 : (plast >> 6) + 1;
   top = top > end ? end : top;
   const int every = plast < 0 ? 0 : own.ns + (top > own.w0 ? top - own.w0 : 0);
-  const int from = uniform((int)((int64_t)every * slice / slices));
-  const int count = uniform((int)((int64_t)every * (slice + 1) / slices)) - from;
+  // every slice's tiles but the last one's are as many: below 2^12 tiles, at most 32 slices
+  const int share = slices == 1 ? every : (every + slices - 1) / slices;
+  const int from = slice * share;
+  const int count = uniform(every - from < share ? every - from : share);
   auto tile_at = [&](int u) { return own.tile_of(from + (u < count ? u : count - 1)); };
 
   // ---- staging: a wavefront copies its quarter of K's and of V's image ----
@@ -343,8 +359,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 3) void kivi_prompt_kernel(KiviG
         s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], i ? s[t] : f16v{}, 0, 0, 0);
       }
   };
-  // What a tile is to the wavefront's rows: nothing (behind them all, or before their windows), seen by
-  // all of them, or in part.
+  // Whether all of the wavefront's rows see all of a tile.
   auto whole = [&](int t0) {
     return t0 + kTile - 1 <= wfirst && (a.window <= 0 || t0 > wlast - a.window || t0 + kTile <= a.sinks);
   };
@@ -367,10 +382,13 @@ __global__ __launch_bounds__(64 * kPromptWaves, 3) void kivi_prompt_kernel(KiviG
       see >>= hh * 8;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t bits = (uint32_t)(see >> (16 * k)) & 255u;
+        const uint32_t bits = (uint32_t)(see >> (16 * k));
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          s[k / 2][(k & 1) * 8 + i] = bits >> i & 1 ? s[k / 2][(k & 1) * 8 + i] : kNegInf;
+        for (int i = 0; i < 8; ++i) {  // all ones where it is seen: two instructions each
+          const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
+          s[k / 2][(k & 1) * 8 + i] = __uint_as_float(
+              (__float_as_uint(s[k / 2][(k & 1) * 8 + i]) & keep) | (0xff800000u & ~keep));
+        }
       }
     }
     float top = kNegInf;
@@ -470,11 +488,6 @@ template <int HD>
 static hipError_t prompt_kernels(const KiviGeo& g, const KiviAttendArgs& a, int passes, int64_t images,
                                  hipStream_t s) {
   constexpr int LDS = (2 * kTile * HD + kTile * HD) * 2;
-  if (LDS > 65536) {  // past 64 KiB a kernel asks for its LDS
-    const hipError_t e = hipFuncSetAttribute((const void*)kivi_prompt_kernel<HD>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (e != hipSuccess) return e;
-  }
   hipLaunchKernelGGL(kivi_slots_kernel, dim3(1), dim3(1024), 0, s, g, a);
   const dim3 lay((unsigned)images, g.nkv), grid((unsigned)(a.tiles * g.nkv), a.slices);
   for (int pass = 0; pass < passes; ++pass) {

@@ -132,7 +132,8 @@ __global__ __launch_bounds__(256) void kivi_read_kernel(KiviGeo g, ReadArgs a) {
       }
     return;
   }
-  // A group lies in one page or two; its scales of K in the first.
+  // A group lies in one page or two; its scales of K in the first, without which its tokens of the
+  // second are not there either.
   const int32_t* table = a.tables + (int64_t)b * g.max_pages + t0 / g.page;
   int page[2];
   bool ok[2];
@@ -141,6 +142,7 @@ __global__ __launch_bounds__(256) void kivi_read_kernel(KiviGeo g, ReadArgs a) {
     page[i] = table[g.page == 16 ? i : 0];
     ok[i] = page[i] >= 0 && page[i] < g.num_pages;
     page[i] = ok[i] ? page[i] : 0;
+    ok[i] &= ok[0];
   }
   h2 ks[4], kz[4];
   {
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(256) void kivi_read_kernel(KiviGeo g, ReadArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ks[i] = pair(s[i]);
-      kz[i] = ok[0] ? pair(z[i]) : pair(0x7e007e00u);
+      kz[i] = pair(z[i]);
     }
   }
   uint32_t kc[N], vc[N], vs[N], vz[N];

@@ -140,6 +140,10 @@ inline __device__ Span make_span(const Geo& g, const AttendArgs& a, int n, int a
   return Span(g, n, n - all, a.window, a.sinks);
 }
 
+__device__ inline int row_slices(const Geo&, const AttendArgs& a, const Place& p) {
+  return prefill_slices(a, p.n);
+}
+
 hipError_t launch_append(const Geo& g, const AppendArgs& a, int batch, hipStream_t s);
 hipError_t launch_read(const Geo& g, const Pool& p, const int32_t* starts, const int32_t* ends,
                        const int32_t* tables, int batch, int total, void* k, void* v, int type,

@@ -123,12 +123,21 @@ def test_a_query_or_a_few_of_every_sequence(kivi, heads, page, dtype):
             check(cache, tables, lens, q, cu, got, causal=False)
 
 
+def is_prompt(kivi, cache, total, max_q):
+    """Whether the prompts' kernel runs a call, not the one for few queries."""
+    return bool(kivi.lib().jacq_kivi_test_is_prompt(cache.geo.ref, cache.batch, total, max_q))
+
+
 @pytest.mark.parametrize("heads", [(14, 2, 64), (40, 8, 128), (4, 4, 64), (8, 1, 128)])
 @pytest.mark.parametrize("page", [16, 32])
-def test_prompts_and_chunks(kivi, heads, page):
+@pytest.mark.parametrize("prompt", [False, True])
+def test_prompts_and_chunks(kivi, heads, page, prompt):
+    """Under a wide table these are prompts; under a narrow one of a few heads' they are not."""
     nh, nkv, hd = heads
     lens = [0, 1, 70, 333, 700, 1500]
-    cache, tables, seq = make(kivi, nh, nkv, hd, page, 64, lens, seed=hd)
+    width = 262080 // page if prompt else None
+    cache, tables, seq = make(kivi, nh, nkv, hd, page, 64, lens, seed=hd, width=width)
+    assert is_prompt(kivi, cache, sum(lens), 1500) == (prompt or nh > 8)
     gen = torch.Generator("cuda").manual_seed(page)
     for m in (lens, [0, 0, 0, 0, 0, 1500], [1, 1, 65, 200, 128, 513], [2, 130, 1, 0, 700, 64]):
         cu = offsets(m)
