@@ -71,7 +71,7 @@ __device__ inline void store8(void* p, int64_t at, u4 raw) {
 
 // blockIdx.x: 4 wavefronts' (group, kv head), kv heads fastest.
 template <int HD, int TYPE>
-__global__ __launch_bounds__(256) void kivi_read_kernel(KiviGeo g, ReadArgs a) {
+__global__ __launch_bounds__(256, 4) void kivi_read_kernel(KiviGeo g, ReadArgs a) {
   constexpr int CH = HD / 8;             // lanes of a token
   constexpr int STEP = 64 / CH;          // tokens at a time
   constexpr int N = kGroup / STEP;       // tokens of a lane
