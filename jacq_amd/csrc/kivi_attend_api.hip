@@ -106,11 +106,16 @@ int device_cus() {
 }
 
 // ---- how an attention call runs ----
-// Units (of 32 tokens) up to which segments stay whole: no plan, no join.  The table's width bounds
-// them.
-constexpr int kWholeUnits = 24;
+// Units (of 32 tokens) up to which segments stay whole: no plan, no join, a launch less.  The table's
+// width bounds them, the lengths are the device's.  us a call, whole against cut:
+//   kWholeUnits     one of 512 tokens, 2 queries, 32/4 heads of 64 8.8 and 12.3; of 700 (24 units), 4 queries,
+//                   40/8 heads of 128 14.6 and 14.0; of 1500 22.2 and 13.9
+//   kWholeFull      where every CU has two segments: 32 of 300 to 1500, 16/16 heads of 64 20.2 and 23.4; 256,
+//                   14/2 heads of 64 21.5 and 27.4; 64 of 1500 to 1900, 32/8 heads of 128 36 and 41; but one
+//                   of 1500 among 63 of 30 19.5 and 14.3
+constexpr int kWholeUnits = 24, kWholeFull = 64;
 // Sequences up to which every workgroup finds the cut by itself (a lane each); more have a kernel
-// for it.
+// for it, 2 us a call where both could.
 constexpr int kCutBatch = 64;
 
 // A call is a prompt's, whose tokens become fp16 once, in the workspace, from so many rows of a kv head
@@ -195,7 +200,7 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   p.row_blocks = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
   const int64_t most = (g.lq + g.residual + jacq::kGroup - 1) / jacq::kGroup;  // units of a segment
   const int64_t segments = (int64_t)batch * g.nkv * p.row_blocks;
-  if (most > kWholeUnits) {
+  if (most > (segments >= 2 * device_cus() ? kWholeFull : kWholeUnits)) {
     const int64_t slots = (int64_t)jacq::few_groups(g.hd, p.nb) * device_cus();
     p.target = (int)(3 * blocks(16 * p.nb) * g.nkv <= slots ? slots : 2 * slots);
   }

@@ -365,12 +365,16 @@ struct Few {
 
 }  // namespace
 
-// Units of a slice, from the call's units, its segments and the longest one's units.
+// Units of a slice, from the call's units, its segments and the longest one's units.  Segments stay whole
+// if none is much longer than a CU's share and they fill the CUs evenly: 32 of 1900 to 2100 tokens, 6
+// queries, 40/8 heads of 128, whole 34.6 us, cut 35.8; but 8 of 1000 to 4000, a query of 32/32 heads, 46 and
+// 32.  Else slices are a CU's share, so that few of them are joined, but 8 units at least (less is all
+// fixed cost) and 32 at most (16 us of a wavefront: the tail), and no more than there is room for.
 __device__ inline int slice_units(const KiviAttendArgs& a, float all, float segments, int longest) {
 #pragma clang fp contract(off)  // the kernel and its join have to find the same size
   const float cus = (float)a.cus;
   const bool even = a.rows > 16 || segments >= 0.8f * cus * __builtin_ceilf(segments / cus);
-  if ((float)longest <= 1.4f * all / cus + 8.0f &&
+  if ((float)longest <= 1.2f * all / cus + 8.0f &&
       (segments <= cus || (even && all >= 0.75f * segments * (float)longest)))
     return longest;
   const int fair = (int)(all / cus) + 1;  // one slice a CU
