@@ -47,6 +47,7 @@ struct KiviAttendArgs {
   int32_t* slots;         // [batch + 1] first tile image of each sequence, then their number, then
                           // (float) the tiles that are a slice's share
   int per_pass;           // tile images of a pass; a sequence's begin in one and may end behind it
+  int limit;              // images of a call of one pass, which end in it; else INT32_MAX
   uint8_t* images;        // K [64][HD], then V [HD][64], fp16, as they lie in the LDS
   uint64_t* poison;       // of each image: the tokens whose V is not finite or not there
 };

@@ -316,6 +316,7 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
       a.merges = (unsigned)merges;
       a.slots = (int32_t*)(ws + p.slots);
       a.per_pass = p.per_pass;
+      a.limit = p.passes == 1 ? p.per_pass : INT32_MAX;
       a.images = ws + p.images;
       a.poison = (uint64_t*)(ws + p.poison);
       return launched(jacq::launch_attend_prompt(g, a, p.passes, stream), "attention");

@@ -53,13 +53,16 @@ __device__ inline bool images_of(const KiviGeo& g, const KiviAttendArgs& a, int 
 
 }  // namespace
 
-// The first image of every sequence, and a slice's share of the tiles that row tiles go through.  One
-// workgroup.
+// The first image of every sequence, and a slice's share of the tiles that row tiles go through.  Offsets
+// that go back can give more sequences queries than there are queries, and more images than the workspace
+// has room for: those behind a.limit are left out.  One workgroup.
 __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendArgs a) {
   __shared__ int sums[2][16];
   __shared__ float work[16];
+  __shared__ int out;  // the first image that is left out
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   int before = 0;
+  if (tid == 0) out = INT32_MAX;
   float w = 0.0f;
   for (int base = 0, turn = 0; base < a.batch; base += 1024, turn ^= 1) {
     const int b = base + tid;
@@ -82,13 +85,17 @@ __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendA
       here += i < wave ? sums[turn][i] : 0;
       before += sums[turn][i];
     }
-    if (b < a.batch) a.slots[b] = here;
+    if (b < a.batch) {
+      const bool fits = here <= a.limit - units;
+      a.slots[b] = fits ? here : INT32_MAX;
+      if (!fits) atomicMin(&out, here);
+    }
   }
   w = __int_as_float(lane63(wave_prefix(__float_as_int(w), SumF())));
   if (lane == 0) work[wave] = w;
   __syncthreads();
   if (tid == 0) {
-    a.slots[a.batch] = before;
+    a.slots[a.batch] = before < out ? before : out;
     w = 0.0f;
     for (int i = 0; i < 16; ++i) w += work[i];
     const float share = w * (float)g.nkv / (kRounds * (float)(prompt_groups(g.hd) * a.cus));

@@ -308,6 +308,27 @@ def test_a_given_workspace_is_enough_and_may_hold_anything(kivi):  # noqa: F811
                 cache.prefill(q, ints(*cu), most, seq, tables, workspace=ws[:size - 1])
 
 
+def test_offsets_that_go_back_stay_in_the_workspace(kivi):  # noqa: F811
+    """More sequences have queries than there are queries: tiles for whose keys there is no room."""
+    nh, nkv, hd, total, most, batch = 128, 8, 64, 330, 320, 1000
+    geo = kivi.KiviGeometry(nh, nkv, hd, 16, 32, 32, 75, 75)
+    cache = kivi.PagedKiviCache(geo, batch)
+    for x in cache.pool():
+        x.zero_()
+    assert is_prompt(kivi, cache, total, most)
+    tables = torch.arange(75, **I32).repeat(batch, 1)
+    seq = torch.full((batch,), 1200, **I32)
+    q = torch.ones(total, nh, hd, dtype=torch.float16, device="cuda")
+    size = kivi.lib().jacq_kivi_attend_workspace_size(geo.ref, batch, total, most)
+    ws = torch.full((size + (1 << 24),), 0xFF, dtype=torch.uint8, device="cuda")
+    for cu in (torch.arange(batch + 1) % (total + 1), torch.arange(batch, -1, -1) % 320,
+               (torch.arange(batch + 1) % 2) * total):
+        got = cache.prefill(q, cu.to(**I32), most, seq, tables, workspace=ws[:size])
+        torch.cuda.synchronize()
+        assert bool((ws[size:] == 0xFF).all()), "written behind the workspace"
+    del got
+
+
 def test_pools_past_32_bits(kivi):  # noqa: F811
     """Pages whose codes lie behind the first 4 GiB."""
     nh, nkv, hd, pages = 40, 8, 128, 600_000
