@@ -675,14 +675,20 @@ class PagedKiviCache:
 
     def __setattr__(self, name: str, value) -> None:
         object.__setattr__(self, name, value)
-        vars(self).pop("_held", None)  # the record goes by what the cache holds now
+        vars(self).pop("_index", None)  # other tensors are looked at anew
 
-    def __getstate__(self):  # copies and pickles make their own record
-        return {n: v for n, v in vars(self).items() if n != "_held"}
+    def __getstate__(self):  # copies and pickles look at their own
+        return {n: v for n, v in vars(self).items() if n != "_index"}
 
     def _record(self):
-        """The packed pool record and the GPU's index, once the cache's tensors are seen to have
-        the layouts of its geometry."""
+        """The packed pool record and the GPU's index."""
+        index = vars(self).get("_index")
+        if index is None:
+            index = self._layouts()
+        return _POOL.pack(*self._pool_ptrs()), index
+
+    def _layouts(self) -> int:
+        """The GPU's index, once the cache's tensors are seen to have the layouts of its geometry."""
         lib()
         g, dev = self.geo, self.k_code.device
         codes = (g.num_pages, g.num_kv_heads, g.page_size, g.head_dim // 2)
@@ -694,8 +700,8 @@ class PagedKiviCache:
                 (torch.uint8, *[torch.float16] * 2) * 2 + (torch.float16,) * 2, POOL_NAMES):
             _check(t.shape == shape and t.dtype == dtype and t.is_contiguous() and t.device == dev,
                    name, " must be contiguous ", dtype, " ", shape, " on ", dev)
-        held = vars(self)["_held"] = (_POOL.pack(*self._pool_ptrs()), self.k_code.get_device())
-        return held
+        index = vars(self)["_index"] = self.k_code.get_device()
+        return index
 
     def _here(self, index: int, *named) -> None:
         dev = self.k_code.device
@@ -737,7 +743,7 @@ class PagedKiviCache:
                 workspace) -> torch.Tensor:
         g, batch = self.geo, self.batch
         nh, hd = g.num_heads, g.head_dim
-        pool, index = vars(self).get("_held") or self._record()
+        pool, index = self._record()
         shape, dtype = q.shape, q.dtype
         contiguous = q.is_contiguous()
         fits = (index >= 0 and len(shape) == 3 and shape[1] == nh and shape[2] == hd and contiguous
@@ -844,7 +850,7 @@ class PagedKiviCache:
         sequence after another: K, V [total, NKV, HD].  total is their number: tokens past it
         are dropped, rows that none fills undefined."""
         g = self.geo
-        pool, index = vars(self).get("_held") or self._record()
+        pool, index = self._record()
         _check(dtype in DTYPES, "values are read as fp16, bf16 or fp32, not ", dtype)
         _check(total >= 0, "TOTAL must not be negative")
         if not (index >= 0 and self._fits(ends, block_tables) and ends.is_contiguous()

@@ -176,11 +176,13 @@ def test_calls_take_the_tensors_that_a_cache_holds_now():
     cache = cpu_cache()
 
     def held(c):
-        return kivi._POOL.unpack((vars(c).get("_held") or c._record())[0])
+        return kivi._POOL.unpack(c._record()[0])
 
     for name in POOL_ATTRS:
         held(cache)
         setattr(cache, name, getattr(cache, name).clone())
+        assert held(cache) == tuple(t.data_ptr() for t in cache.pool())
+        getattr(cache, name).data = getattr(cache, name).clone()
         assert held(cache) == tuple(t.data_ptr() for t in cache.pool())
     for make, shared in ((copy.copy, True), (copy.deepcopy, False),
                          (lambda c: pickle.loads(pickle.dumps(c)), False)):
