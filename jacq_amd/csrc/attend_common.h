@@ -78,6 +78,12 @@ struct Max {  // of numbers that are not negative
 };
 __device__ inline int lane63(int x) { return __builtin_amdgcn_readlane(x, 63); }
 
+// How many of a sequence's m queries a launch takes: all, unless the cache's own overload says otherwise.
+template <class A>
+__device__ inline int taken(const A&, int m) {
+  return m;
+}
+
 // Queries of sequence b: rows [q0, q0 + m) of Q, whatever the table of offsets holds.  m is at most
 // max_q; `all` are the sequence's own, which its last tokens are.
 template <class A>
@@ -92,7 +98,7 @@ __device__ inline void queries_of(const A& a, int b, int* q0, int* m, int* all) 
   hi = hi < lo ? lo : hi > a.total_q ? a.total_q : hi;
   *q0 = lo;
   *all = hi - lo;
-  *m = hi - lo > a.max_q ? a.max_q : hi - lo;
+  *m = taken(a, hi - lo > a.max_q ? a.max_q : hi - lo);
 }
 
 // Where a prefill's workgroup, or one of its merge, works.  A unit is 2^log2 rows of a sequence, `per`
@@ -128,7 +134,7 @@ __device__ inline Place place_of(const G& g, const A& a, int unit, int per, int 
   const int b = at + (lane < n ? lane : n - 1), lo = offset(b), len = clamp_len(g, a.lens[b]);
   int hi = offset(b + 1);
   hi = hi < lo ? lo : hi;
-  const int m = hi - lo > a.max_q ? a.max_q : hi - lo;
+  const int m = taken(a, hi - lo > a.max_q ? a.max_q : hi - lo);
   int begin;
   uint64_t here;  // the last lane of these has the unit
   if (a.batch <= kCounted) {

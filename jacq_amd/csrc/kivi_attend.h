@@ -32,6 +32,7 @@ struct KiviAttendArgs {
   int batch, total_q, max_q;
   int window, sinks;      // window 0: none
   int causal;             // 0: every query sees every token
+  int above, upto;        // a launch takes the sequences of more queries than the one, at most the other
   float scale;            // log2(e) included
   // split pieces
   float* part_ml;         // few queries: [target + segments][rows][2]; prompts: [slices][total_q][nh][2]
@@ -51,6 +52,8 @@ struct KiviAttendArgs {
   uint8_t* images;        // K [64][HD], then V [HD][64], fp16, as they lie in the LDS
   uint64_t* poison;       // of each image: the tokens whose V is not finite or not there
 };
+
+__device__ inline int taken(const KiviAttendArgs& a, int m) { return m > a.above && m <= a.upto ? m : 0; }
 
 __device__ inline int clamp_len(const KiviGeo& g, int n) {
   const int cap = g.lq + g.residual;

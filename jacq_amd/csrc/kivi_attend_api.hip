@@ -128,6 +128,16 @@ constexpr int kCutBatch = 64;
 //   1274 rows  one of 16384, 14/2 heads of 64 45 and 48 (42 M)
 constexpr int64_t kPromptRows = 320;
 constexpr int64_t kPromptWork = 50000000;
+// Where a call has at most half the queries that max_q for every sequence would be, as with chunks of some
+// prompts between steps of other sequences, those of at most so many rows of a kv head are the few-query
+// kernel's, which lays nothing.  40/8 heads of 128, sequences of 4000 tokens, us with the split and without:
+// 512 queries of one of 32 143 and 345, of two of 64 212 and 635, of one of 3 93 and 86; 7 of 16 365 and 398.
+// 16 rows would do for single queries (136, 201, 92), not for four of them.
+constexpr int kSplitRows = 32;
+// Such a call is a prompt's from so many segments of the few-query kernel on, too, since most are empty:
+// 256 queries of one of 64 sequences of 1000 tokens (20480) 111 us there and 63 so, of one of 32 (10240) 66
+// and 58, of one of 16 (5120) 43 and 57; 100 of each of 4 of 100 of 200 tokens (10400) 36 and 43.
+constexpr int64_t kSplitSegments = 12000;
 // Bytes of fp16 tiles that a pass lays in the workspace, about, and passes at most, a few us each (of a
 // wide table's, most have nothing to do): a call of more is left to the few-query kernel.
 constexpr int64_t kPassBytes = (int64_t)1 << 31;
@@ -141,10 +151,13 @@ constexpr int64_t kMostParts = (int64_t)1 << 30;
 thread_local int64_t g_pass_bytes = 0;
 
 struct Plan {
-  bool prompt, planned;
+  bool prompt, few;       // which kernels run: both for sequences of many queries and of few
+  int split;              // then, the queries up to which a sequence is the few-query kernel's
+  bool planned;
   int nb, rows, row_blocks, target;
   int slices, per_pass, passes;
   size_t ml, acc, plan, slots, images, poison, bytes;  // offsets into the workspace, and its size
+  size_t few_ml, few_acc;
 };
 
 Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
@@ -168,12 +181,15 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   const int64_t tokens = (int64_t)g.lq + g.residual;
   const int64_t cap = (tokens + jacq::kTile - 1) / jacq::kTile;  // images of a sequence and kv head
   const int64_t image = (int64_t)4 * jacq::kTile * g.hd * g.nkv;
-  const int64_t images = std::min<int64_t>(batch, total_q) * cap;
   const int64_t pass_bytes = g_pass_bytes ? g_pass_bytes : kPassBytes;
+  if (2 * (int64_t)total_q <= (int64_t)batch * max_q) p.split = kSplitRows / g.gqa;
+  const int64_t images = std::min<int64_t>(batch, total_q / (p.split + 1)) * cap;
   p.per_pass = (int)std::max<int64_t>(1, std::min(images, pass_bytes / image));
   const int64_t passes = (images + p.per_pass - 1) / p.per_pass;
-  p.prompt = rows >= kPromptRows && queries * g.nh * tokens >= kPromptWork &&
-             passes <= kMostPasses && images <= INT32_MAX - 4096;
+  p.prompt = rows >= kPromptRows && images > 0 && passes <= kMostPasses && images <= INT32_MAX - 4096 &&
+             (queries * g.nh * tokens >= kPromptWork ||
+              (p.split && batch * g.nkv * ((rows + 31) / 32) >= kSplitSegments));
+  p.few = !p.prompt || p.split;
   if (p.prompt) {
     p.passes = (int)passes;
     // row tiles in so many slices that their workgroups are no more than kMostGroups a CU: the device
@@ -192,24 +208,26 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
     p.slots = take(((size_t)batch + 2) * sizeof(int32_t));
     p.poison = take(held * sizeof(uint64_t));
     p.images = take(held * 4 * jacq::kTile * g.hd);
-    p.bytes = at;
-    return p;
   }
-  p.nb = rows <= 16 ? 1 : 2;
-  p.rows = (int)std::min<int64_t>(rows, 16 * p.nb);
-  p.row_blocks = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
-  const int64_t most = (g.lq + g.residual + jacq::kGroup - 1) / jacq::kGroup;  // units of a segment
-  const int64_t segments = (int64_t)batch * g.nkv * p.row_blocks;
-  if (most > (segments >= 2 * device_cus() ? kWholeFull : kWholeUnits)) {
-    const int64_t slots = (int64_t)jacq::few_groups(g.hd, p.nb) * device_cus();
-    p.target = (int)(3 * blocks(16 * p.nb) * g.nkv <= slots ? slots : 2 * slots);
+  if (p.few) {
+    const int64_t most_rows = p.prompt ? p.split * g.gqa : rows;
+    p.nb = most_rows <= 16 ? 1 : 2;
+    p.rows = (int)std::min<int64_t>(most_rows, 16 * p.nb);
+    p.row_blocks = (int)((most_rows + 16 * p.nb - 1) / (16 * p.nb));
+    const int64_t most = (g.lq + g.residual + jacq::kGroup - 1) / jacq::kGroup;  // units of a segment
+    const int64_t segments = (int64_t)batch * g.nkv * p.row_blocks;
+    if (most > (segments >= 2 * device_cus() ? kWholeFull : kWholeUnits)) {
+      const int64_t slots = (int64_t)jacq::few_groups(g.hd, p.nb) * device_cus();
+      const int64_t filled = p.prompt ? segments : blocks(16 * p.nb) * g.nkv;
+      p.target = (int)(3 * filled <= slots ? slots : 2 * slots);
+    }
+    if ((p.target + segments) * p.rows * (g.hd + 2) * (int64_t)sizeof(float) > kMostParts) p.target = 0;
+    const size_t parts = p.target ? (size_t)p.target + segments : 0;
+    p.few_ml = take(parts * p.rows * 2 * sizeof(float));
+    p.few_acc = take(parts * p.rows * g.hd * sizeof(float));
+    p.planned = p.target && batch > kCutBatch;
+    p.plan = take(p.planned ? ((size_t)batch + 2) * sizeof(int32_t) : 0);
   }
-  if ((p.target + segments) * p.rows * (g.hd + 2) * (int64_t)sizeof(float) > kMostParts) p.target = 0;
-  const size_t parts = p.target ? (size_t)p.target + segments : 0;
-  p.ml = take(parts * p.rows * 2 * sizeof(float));
-  p.acc = take(parts * p.rows * g.hd * sizeof(float));
-  p.planned = p.target && batch > kCutBatch;
-  p.plan = take(p.planned ? ((size_t)batch + 2) * sizeof(int32_t) : 0);
   p.bytes = at;
   return p;
 }
@@ -300,18 +318,31 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
     const int64_t tiles = place_units(a, g.gqa, jacq::kRowsLog2);
     const int64_t merges = p.slices > 1 ? place_units(a, g.nh, jacq::merge_log2(g.hd)) : 0;
     if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 ||
-        (p.prompt ? std::max(tiles * g.nkv, merges) : segments + p.target) >= 1 << 24)
+        (p.prompt && std::max(tiles * g.nkv, merges) >= 1 << 24) || segments + p.target >= 1 << 24)
       return fail("too many query rows in one call");
     if (p.bytes && (!workspace || workspace_bytes < p.bytes))
       return jacq::set_last_error(JACQ_KIVI_ENOMEM,
                                   "the workspace needs " + std::to_string(p.bytes) + " bytes, got " +
                                       std::to_string(workspace ? workspace_bytes : 0));
     uint8_t* ws = (uint8_t*)workspace;
-    a.part_ml = (float*)(ws + p.ml);
-    a.part_acc = (float*)(ws + p.acc);
+    a.cus = device_cus();
+    a.upto = INT32_MAX;
+    if (p.few) {
+      KiviAttendArgs few = a;
+      if (p.prompt) few.upto = p.split;
+      few.part_ml = (float*)(ws + p.few_ml);
+      few.part_acc = (float*)(ws + p.few_acc);
+      few.target = p.target;
+      few.plan = p.planned ? (int32_t*)(ws + p.plan) : nullptr;
+      few.rows = p.rows;
+      few.row_blocks = p.row_blocks;
+      if (int e = launched(jacq::launch_attend_few(g, few, p.nb, stream), "attention")) return e;
+    }
     if (p.prompt) {
+      a.above = p.split;
+      a.part_ml = (float*)(ws + p.ml);
+      a.part_acc = (float*)(ws + p.acc);
       a.slices = p.slices;
-      a.cus = device_cus();
       a.tiles = (unsigned)tiles;
       a.merges = (unsigned)merges;
       a.slots = (int32_t*)(ws + p.slots);
@@ -321,12 +352,7 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
       a.poison = (uint64_t*)(ws + p.poison);
       return launched(jacq::launch_attend_prompt(g, a, p.passes, stream), "attention");
     }
-    a.target = p.target;
-    a.cus = device_cus();
-    a.plan = p.planned ? (int32_t*)(ws + p.plan) : nullptr;
-    a.rows = p.rows;
-    a.row_blocks = p.row_blocks;
-    return launched(jacq::launch_attend_few(g, a, p.nb, stream), "attention");
+    return JACQ_KIVI_OK;
   });
 }
 

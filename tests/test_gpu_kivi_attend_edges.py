@@ -188,6 +188,32 @@ def test_many_sequences(kivi, batch):  # noqa: F811
         check(cache, tables, lens, q, cu, got, causal=False)
 
 
+@pytest.mark.parametrize("batch", [6, 40, 90])
+@pytest.mark.parametrize("heads", [(40, 8, 128), (14, 2, 64), (16, 1, 64)])
+def test_steps_beside_prompts(kivi, heads, batch):  # noqa: F811
+    """A call of sequences for both kernels: none, one, a few queries, as many as the one takes and one
+    more, some hundreds."""
+    rng = random.Random(batch)
+    nh, nkv, hd = heads
+    split = 32 // (nh // nkv)
+    lens = [rng.choice((1, 100, 333, 900, 1600)) for _ in range(batch)]
+    lens[1], lens[2] = 2000, 1200
+    m = [rng.choice((0, 1, 1, 2, split, split + 1)) for _ in lens]
+    m[1], m[2] = 400, split + 1
+    cache, tables, seq = make(kivi, nh, nkv, hd, 16, 64, lens, seed=batch,
+                              width=(WIDE if batch < 9 else 20000) // 16)
+    cu = offsets(m)
+    assert 2 * cu[-1] <= batch * 400 and is_prompt(kivi, cache, cu[-1], 400)
+    gen = torch.Generator("cuda").manual_seed(batch)
+    q = randn(gen, cu[-1], nh, hd, dtype=torch.bfloat16)
+    for window, sinks in ((None, 0), (500, 40)):
+        lse = torch.empty(cu[-1], nh, device="cuda")
+        got = cache.prefill(q, ints(*cu), 400, seq, tables, window=window, sinks=sinks, lse=lse)
+        check(cache, tables, lens, q, cu, got, lse, window, sinks)
+    got = cache.cross(q, ints(*cu), 400, seq, tables)
+    check(cache, tables, lens, q, cu, got, causal=False)
+
+
 @pytest.mark.parametrize("batch,longest,prompt", [(7, 200, False), (7, 2100, True), (70, 200, True)])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_prompts_in_passes(kivi, batch, longest, prompt, hd):  # noqa: F811
