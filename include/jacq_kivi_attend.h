@@ -60,7 +60,8 @@ typedef struct jacq_kivi_pool {
  * the products.
  *   Q    [total_q, NH, HD] of q_dtype (fp16 or bf16), token rows q_stride
  *        elements apart
- *   O    [total_q, NH, HD] of o_dtype (q_dtype or fp32), contiguous
+ *   O    [total_q, NH, HD] of o_dtype (q_dtype or fp32), contiguous; may be Q
+ *        where that has its type and stride
  *   LSE  NULL or [total_q, NH] fp32: log of the sum of exp(scaled scores)
  *   max_q  no sequence has more queries than this (of one that has, the first
  *        max_q are computed, at their own positions; the others are left alone)

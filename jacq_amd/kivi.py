@@ -822,7 +822,8 @@ class PagedKiviCache:
                 lse: torch.Tensor | None = None, workspace: torch.Tensor | None = None
                 ) -> torch.Tensor:
         """q [tokens, NH, HD] fp16 or bf16, whose rows may lie apart (a slice of a fused
-        projection) -> O [tokens, NH, HD] of q's type (or of ``out``'s, q's or fp32).
+        projection) -> O [tokens, NH, HD] of q's type (or of ``out``'s, q's or fp32; it may be a
+        contiguous q itself).
 
         Rows cu_q[b] to cu_q[b + 1] (cu_q [batch + 1] int32; None: one query per sequence) are
         the last tokens of sequence b, whose seq_lens[b] tokens are all in the cache; each sees

@@ -214,6 +214,70 @@ def test_steps_beside_prompts(kivi, heads, batch):  # noqa: F811
     check(cache, tables, lens, q, cu, got, causal=False)
 
 
+def test_steps_beside_a_prompt_captured(kivi):  # noqa: F811
+    """With other queries, offsets (so other sequences for each kernel) and lengths copied in."""
+    nh, nkv, hd, batch = 16, 2, 128, 12
+    lens = [700 + 31 * b for b in range(batch)]
+    cache, tables, seq = make(kivi, nh, nkv, hd, 32, 32, lens, seed=1, width=WIDE // 32)
+    gen = torch.Generator("cuda").manual_seed(3)
+    q, where = randn(gen, 420, nh, hd), torch.zeros(batch + 1, **I32)
+    assert is_prompt(kivi, cache, 420, 300)
+    out = torch.empty_like(q)
+
+    def call():
+        cache.prefill(q, where, 300, seq, tables, window=400, sinks=2, out=out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    rng = random.Random(4)
+    for i in range(4):
+        m = [rng.choice((0, 1, 4, 5)) for _ in lens]
+        m[rng.randrange(batch)] = 300
+        m[rng.randrange(batch)] = 40
+        q.copy_(randn(gen, *q.shape))
+        where.copy_(ints(*offsets(m)))
+        out.fill_(7.0)
+        graph.replay()
+        check(cache, tables, lens, q, offsets(m), out, window=400, sinks=2)
+        assert bool((out[sum(m):] == 7.0).all())
+        got = out.clone()
+        out.fill_(7.0)
+        call()
+        assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("heads,m,prompt", SIZES)
+def test_lengths_are_clamped(kivi, heads, m, prompt):  # noqa: F811
+    nh, nkv, hd = heads
+    lens = [0, 200, 64 + 320]
+    cache, tables, seq, q, cu, most = call(kivi, *heads, 16, lens, m, prompt, seed=8)
+    cap = cache.geo.max_pages_per_seq * 16 // 32 * 32 + 64
+    wild = ints(-2 ** 31, 200, 2 ** 31 - 1 if not prompt else 384)
+    if not prompt:
+        assert lens[2] == cap
+    assert torch.equal(cache.prefill(q, ints(*cu), most, wild, tables),
+                       cache.prefill(q, ints(*cu), most, seq, tables))
+    assert torch.equal(cache.cross(q, ints(*cu), most, wild, tables),
+                       cache.cross(q, ints(*cu), most, seq, tables))
+    for a, b in zip(cache.read(ints(5, -9, 100), wild, tables, 484),
+                    cache.read(ints(0, 0, 100), seq, tables, 484)):
+        assert torch.equal(a, b) and bool(a.isfinite().all())
+
+
+@pytest.mark.parametrize("heads,m,prompt", SIZES)
+def test_the_output_may_be_the_queries(kivi, heads, m, prompt):  # noqa: F811
+    cache, tables, seq, q, cu, most = call(kivi, *heads, 32, [2000, 300, 77], m, prompt, seed=2)
+    want = cache.prefill(q, ints(*cu), most, seq, tables)
+    assert cache.prefill(q, ints(*cu), most, seq, tables, out=q) is q
+    assert torch.equal(q, want)
+
+
 @pytest.mark.parametrize("batch,longest,prompt", [(7, 200, False), (7, 2100, True), (70, 200, True)])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_prompts_in_passes(kivi, batch, longest, prompt, hd):  # noqa: F811
