@@ -288,6 +288,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, prompt_groups(HD)) void kivi_pro
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int n32 = lane & 31, hh = lane >> 5;
   const int h = blockIdx.x % g.nkv, slice = blockIdx.y;
+  if (pass > 0 && (int64_t)pass * a.per_pass >= uniform(a.slots[a.batch])) return;  // of a wide table's
   const Place place = place_of(g, a, blockIdx.x / g.nkv, g.gqa, kRowsLog2);
   const int b = place.b, q0 = place.q0, n = place.n;
   const int rows = place.m * g.gqa;
