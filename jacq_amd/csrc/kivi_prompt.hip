@@ -63,9 +63,27 @@ __device__ inline bool images_of(const KiviGeo& g, const KiviAttendArgs& a, int 
   return true;
 }
 
+// A sequence's images, and the tiles that its row tiles go through.
+__device__ inline int images_and_work(const KiviGeo& g, const KiviAttendArgs& a, int b, float& work) {
+  int q0, m, all;
+  queries_of(a, b, &q0, &m, &all);
+  work = 0.0f;
+  if (m == 0) return 0;
+  const KiviTiles tiles(g, a, clamp_len(g, a.lens[b]), a.causal ? clamp_len(g, a.lens[b]) - all
+                                                                : clamp_len(g, a.lens[b]) - 1);
+  work = (float)((m * g.gqa + kPrefillRows - 1) / kPrefillRows) * row_tiles_units(a, tiles, m, all);
+  return tiles.units;
+}
+
+__device__ inline float slice_share(const KiviGeo& g, const KiviAttendArgs& a, float work) {
+  const float share = work * (float)g.nkv / (kRounds * (float)(prompt_groups(g.hd) * a.cus));
+  return share > (float)kSliceUnits ? share : (float)kSliceUnits;
+}
+
 }  // namespace
 
-// The first image of every sequence, and a slice's share of the tiles that row tiles go through.  Offsets
+// The first image of every sequence, and a slice's share of the tiles that row tiles go through, of more
+// than kCounted sequences (kivi_lay_kernel finds those of fewer by itself, a launch and 2 to 4 us less).  Offsets
 // that go back can give more sequences queries than there are queries, and more images than the workspace
 // has room for: those behind a.limit are left out.  One workgroup.
 __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendArgs a) {
@@ -78,17 +96,9 @@ __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendA
   float w = 0.0f;
   for (int base = 0, turn = 0; base < a.batch; base += 1024, turn ^= 1) {
     const int b = base + tid;
-    int units = 0;
-    if (b < a.batch) {
-      int q0, m, all;
-      queries_of(a, b, &q0, &m, &all);
-      const int n = clamp_len(g, a.lens[b]);
-      if (m > 0) {
-        const KiviTiles tiles(g, a, n, a.causal ? n - all : n - 1);
-        units = tiles.units;
-        w += (float)((m * g.gqa + kPrefillRows - 1) / kPrefillRows) * row_tiles_units(a, tiles, m, all);
-      }
-    }
+    float own = 0.0f;
+    const int units = b < a.batch ? images_and_work(g, a, b, own) : 0;
+    w += own;
     const int inc = wave_prefix(units, Sum());
     if (lane == 63) sums[turn][wave] = inc;
     __syncthreads();  // the other turn's sums have been read by all
@@ -110,8 +120,7 @@ __global__ __launch_bounds__(1024) void kivi_slots_kernel(KiviGeo g, KiviAttendA
     a.slots[a.batch] = before < out ? before : out;
     w = 0.0f;
     for (int i = 0; i < 16; ++i) w += work[i];
-    const float share = w * (float)g.nkv / (kRounds * (float)(prompt_groups(g.hd) * a.cus));
-    a.slots[a.batch + 1] = __float_as_int(share > (float)kSliceUnits ? share : (float)kSliceUnits);
+    a.slots[a.batch + 1] = __float_as_int(slice_share(g, a, w));
   }
 }
 
@@ -126,13 +135,37 @@ __global__ __launch_bounds__(2 * HD) void kivi_lay_kernel(KiviGeo g, KiviAttendA
   const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
   const bool is_v = uniform(tid / HD) == 0;
   const int chunk = tid % HD % CH, part = tid % HD / CH;  // part: V: 8 tokens; K: 4 of a group's rows
-  const int64_t begin = (int64_t)pass * a.per_pass, total = uniform(a.slots[a.batch]);
+  const int64_t begin = (int64_t)pass * a.per_pass;
+  const bool few = a.batch <= kCounted;
+  int mine = 0, total;  // few: the first image of the lane's sequence
+  if (few) {
+    float w = 0.0f;
+    const int units = lane < a.batch ? images_and_work(g, a, lane, w) : 0;
+    const int inc = wave_prefix(units, Sum());
+    const bool fits = inc <= a.limit;
+    mine = fits ? inc - units : INT32_MAX;
+    // the images before the first one that does not fit
+    const uint64_t not_ = __ballot(!fits);
+    total = not_ ? __builtin_amdgcn_readlane(inc - units, __builtin_ctzll(not_)) : lane63(inc);
+    w = __int_as_float(lane63(wave_prefix(__float_as_int(w), SumF())));
+    if (pass == 0 && blockIdx.x == 0 && h == 0 && tid < 64) {  // for the kernels behind this one
+      if (lane < a.batch) a.slots[lane] = mine;
+      if (lane == 0) {
+        a.slots[a.batch] = total;
+        a.slots[a.batch + 1] = __float_as_int(slice_share(g, a, w));
+      }
+    }
+  } else {
+    total = uniform(a.slots[a.batch]);
+  }
   // up to the first sequence of the next pass
   int b = 0;
   for (int64_t slot = begin + blockIdx.x;; slot += gridDim.x) {
     if (slot >= total) return;
     // its sequence: the last one whose first image is not behind it (one without images is not the last)
-    {
+    if (few) {
+      b = 63 - __builtin_clzll(__ballot(lane < a.batch && mine <= slot));
+    } else {
       int at = 0;
       for (int n = a.batch; n > 1;) {
         const int step = (n + 63) / 64, i = lane * step;
@@ -143,7 +176,7 @@ __global__ __launch_bounds__(2 * HD) void kivi_lay_kernel(KiviGeo g, KiviAttendA
       }
       b = uniform(at);
     }
-    const int first = uniform(a.slots[b]);
+    const int first = few ? __builtin_amdgcn_readlane(mine, b) : uniform(a.slots[b]);
     if (first / a.per_pass != pass) {
       if (first >= begin) return;  // the next pass's
       continue;                    // the end of the last pass's
@@ -508,7 +541,7 @@ template <int HD>
 static hipError_t prompt_kernels(const KiviGeo& g, const KiviAttendArgs& a, int passes, int64_t images,
                                  hipStream_t s) {
   constexpr int LDS = (2 * kTile * HD + kTile * HD) * 2;
-  hipLaunchKernelGGL(kivi_slots_kernel, dim3(1), dim3(1024), 0, s, g, a);
+  if (a.batch > kCounted) hipLaunchKernelGGL(kivi_slots_kernel, dim3(1), dim3(1024), 0, s, g, a);
   const dim3 lay((unsigned)images, g.nkv), grid((unsigned)(a.tiles * g.nkv), a.slices);
   for (int pass = 0; pass < passes; ++pass) {
     if (g.page == 16)
