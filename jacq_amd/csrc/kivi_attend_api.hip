@@ -126,8 +126,13 @@ constexpr int kCutBatch = 64;
 //   640 rows   one of 16384, 40/8 heads of 128 107 and 92 (84 M), of 700 19 and 28 (4 M); 8 of 4000 to
 //              8000, 14/2 heads of 64 91 and 57 (82 M), 32 of 300 to 1500 50 and 46 (61 M)
 //   1274 rows  one of 16384, 14/2 heads of 64 45 and 48 (42 M)
+// or from so many full rounds of the few-query kernel's workgroups on, each of which pays its start and end:
+// prompts of 16 sequences of 200 tokens, 32/8 heads of 128 (3200 workgroups, 6 rounds), 57 and 39 us, of 8 of
+// 300 (2432) 50 and 36, of 4 of 300 to 600 46 and 35; but 128 queries of each of 8 of 500 to 1000, 40/8 heads
+// (1280), 49 and 55, a prompt of 1000 (1256) 43 and 49.
 constexpr int64_t kPromptRows = 320;
 constexpr int64_t kPromptWork = 50000000;
+constexpr int64_t kPromptRounds = 3;
 // Where a call has at most half the queries that max_q for every sequence would be, as with chunks of some
 // prompts between steps of other sequences, those of at most so many rows of a kv head are the few-query
 // kernel's, which lays nothing.  40/8 heads of 128, sequences of 4000 tokens, us with the split and without:
@@ -188,6 +193,7 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   const int64_t passes = (images + p.per_pass - 1) / p.per_pass;
   p.prompt = rows >= kPromptRows && images > 0 && passes <= kMostPasses && images <= INT32_MAX - 4096 &&
              (queries * g.nh * tokens >= kPromptWork ||
+              blocks(32) * g.nkv >= kPromptRounds * jacq::few_groups(g.hd, 2) * device_cus() ||
               (p.split && batch * g.nkv * ((rows + 31) / 32) >= kSplitSegments));
   p.few = !p.prompt || p.split;
   if (p.prompt) {
