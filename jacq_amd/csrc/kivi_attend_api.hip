@@ -152,6 +152,9 @@ constexpr int64_t kMostGroups = 8;
 // Bytes of parts for which the few-query kernel still cuts: a call of more has segments enough.
 constexpr int64_t kMostParts = (int64_t)1 << 30;
 
+// Workgroups of a launch, which has fewer than 2^32 threads.
+constexpr int64_t kMostSegments = 1 << 24;
+
 // Test hook: not 0: the bytes of a pass on the calling thread.
 thread_local int64_t g_pass_bytes = 0;
 
@@ -194,7 +197,7 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   p.prompt = rows >= kPromptRows && images > 0 && passes <= kMostPasses && images <= INT32_MAX - 4096 &&
              (queries * g.nh * tokens >= kPromptWork ||
               blocks(32) * g.nkv >= kPromptRounds * jacq::few_groups(g.hd, 2) * device_cus() ||
-              (p.split && batch * g.nkv * ((rows + 31) / 32) >= kSplitSegments));
+              (p.split && (int64_t)batch * g.nkv * ((rows + 31) / 32) >= kSplitSegments));
   p.few = !p.prompt || p.split;
   if (p.prompt) {
     p.passes = (int)passes;
@@ -227,7 +230,9 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
       const int64_t filled = p.prompt ? segments : blocks(16 * p.nb) * g.nkv;
       p.target = (int)(3 * filled <= slots ? slots : 2 * slots);
     }
-    if ((p.target + segments) * p.rows * (g.hd + 2) * (int64_t)sizeof(float) > kMostParts) p.target = 0;
+    if (segments >= kMostSegments ||  // a call that is refused
+        (p.target + segments) * p.rows * (g.hd + 2) * (int64_t)sizeof(float) > kMostParts)
+      p.target = 0;
     const size_t parts = p.target ? (size_t)p.target + segments : 0;
     p.few_ml = take(parts * p.rows * 2 * sizeof(float));
     p.few_acc = take(parts * p.rows * g.hd * sizeof(float));
@@ -320,11 +325,10 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
     a.scale = x->scale * jacq::kLog2e;
     const Plan p = plan_attend(g, a.batch, a.total_q, a.max_q);
     const int64_t segments = (int64_t)a.batch * g.nkv * p.row_blocks;
-    // a launch has fewer than 2^32 threads
     const int64_t tiles = place_units(a, g.gqa, jacq::kRowsLog2);
     const int64_t merges = p.slices > 1 ? place_units(a, g.nh, jacq::merge_log2(g.hd)) : 0;
     if ((int64_t)a.max_q * g.gqa > INT32_MAX / 2 ||
-        (p.prompt && std::max(tiles * g.nkv, merges) >= 1 << 24) || segments + p.target >= 1 << 24)
+        (p.prompt && std::max(tiles * g.nkv, merges) >= kMostSegments) || segments + p.target >= kMostSegments)
       return fail("too many query rows in one call");
     if (p.bytes && (!workspace || workspace_bytes < p.bytes))
       return jacq::set_last_error(JACQ_KIVI_ENOMEM,

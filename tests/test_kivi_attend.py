@@ -193,6 +193,19 @@ def test_calls_take_the_tensors_that_a_cache_holds_now():
     assert held(cache.sequence_view(1))[6] == cache.k_scr[1].data_ptr()
 
 
+@pytest.mark.parametrize("batch,total,most", [
+    (65535, 2 ** 31 - 1, 2 ** 31 - 1), (65535, 2 ** 31 - 1, 10), (1, 2 ** 31 - 1, 2 ** 31 - 1),
+    (65535, 100000, 50000), (300, 100000, 20000)])
+def test_workspaces_of_the_largest_calls_have_a_size(batch, total, most):
+    """Whether the call is refused or not: no product of its sizes passes 64 bits."""
+    for heads in ((65536, 65536, 128), (65536, 4096, 128), (40, 8, 128), (16, 1, 64)):
+        for pages in (0, 8000, 16000):
+            geo = kivi.KiviGeometry(*heads, 16, 32, 32, pages, 100)
+            size = kivi.lib().jacq_kivi_attend_workspace_size(geo.ref, batch, total, most)
+            # parts of 1 GiB, the tiles of a pass of 2 GiB and, behind it, of a sequence's end
+            assert size <= 2 ** 32 + 4096 * 64 * heads[2] * 4 * heads[1]
+
+
 # ---- the reference itself ----
 
 def test_the_reference_is_the_caches_definition():
