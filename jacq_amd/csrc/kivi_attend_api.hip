@@ -228,7 +228,11 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
     if (most > (segments >= 2 * device_cus() ? kWholeFull : kWholeUnits)) {
       const int64_t slots = (int64_t)jacq::few_groups(g.hd, p.nb) * device_cus();
       const int64_t filled = p.prompt ? segments : blocks(16 * p.nb) * g.nkv;
-      p.target = (int)(3 * filled <= slots ? slots : 2 * slots);
+      // One round of workgroups, or two where one would have fewer than two slices of a segment.  us with a
+      // third as the border, and with a half: 24, 28 and 32 sequences of 1500 to 6007, 4 queries, 40/8 heads
+      // of 128, 53 and 45, 54 and 49, 58 and 56 (all of 4000: 45 and 50, 54 and 54, 55 and 56); 144 of 1000
+      // to 4000, 14/2 heads of 64, 40 and 37.  With one round always, 64 of the first take 104 and not 95.
+      p.target = (int)(2 * filled <= slots ? slots : 2 * slots);
     }
     if (segments >= kMostSegments ||  // a call that is refused
         (p.target + segments) * p.rows * (g.hd + 2) * (int64_t)sizeof(float) > kMostParts)
