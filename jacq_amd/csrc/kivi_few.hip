@@ -11,9 +11,9 @@
 //
 // A group's codes, scales and zeros (40 HD bytes) come by LDS DMA, a ring of units ahead.
 //
-// Bound by issue, not by memory: of HD 128 a unit is about 425 vector instructions for 32 rows, 320
+// Bound by issue, not by memory: of HD 128 a unit is about 380 vector instructions for 32 rows, 320
 // for 16 (200 of them codes to fp16, which every row shares), for 5 KB.  32 sequences of 1500 to 6007 tokens, 40/8 heads
-// of 128, 4 queries: 56 us where the bytes alone take 35; 64 of 1024 to 16384 under a window of 4096, 32/8
+// of 128, 4 queries: 53 us where the bytes alone take 35; 64 of 1024 to 16384 under a window of 4096, 32/8
 // heads, one query: 70 us, as long as the bytes.  A sliced call has 13 us of its own: two launches, the cut,
 // the join.
 #include "kivi_attend.h"
