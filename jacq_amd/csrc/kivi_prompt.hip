@@ -55,8 +55,14 @@ __device__ inline void copy16(uint64_t base, uint32_t lane16, uint32_t dst) {
 }
 
 // Where a sequence's images are: those of kv head h from first + h units on, if they are of this pass.
+// A sequence without tokens has none, and is the first pass's: its place, the next one's first image, may be
+// behind the last pass.
 __device__ inline bool images_of(const KiviGeo& g, const KiviAttendArgs& a, int b, int pass, int units,
                                  int h, int64_t* at) {
+  if (units == 0) {
+    *at = 0;
+    return pass == 0;
+  }
   const int slot = uniform(a.slots[b]);
   if (slot / a.per_pass != pass) return false;
   *at = (int64_t)(slot % a.per_pass) * g.nkv + (int64_t)h * units;

@@ -1,0 +1,42 @@
+"""Extremes of the int4 cache's attention of chunks: sequences without tokens at a pass's end."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_kivi_attend import check, ints, is_prompt, kivi, make, offsets, randn  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def pass_bytes(kivi):  # noqa: F811
+    fn = kivi.lib().jacq_kivi_test_pass_bytes
+    fn.argtypes, fn.restype = [ctypes.c_int64], None
+    yield fn
+    fn(0)
+
+
+@pytest.mark.parametrize("batch,per_pass", [(6, 10), (6, 20), (6, 40), (70, 20), (70, 40)])
+def test_sequences_without_tokens_at_the_end_of_a_pass(kivi, pass_bytes, batch, per_pass):  # noqa: F811
+    """They have no tiles, so their place among the tiles is the next sequence's, or behind the last pass."""
+    nh, nkv, hd, m = 40, 8, 128, 400
+    lens = [640, 0, 640, 640, 640] + [0] * (batch - 5)
+    cache, tables, seq = make(kivi, nh, nkv, hd, 32, 32, lens, seed=batch, width=608 // 32)
+    cu = offsets([m] * 5 + [7] * (batch - 5))  # 7: more than what the kernel for few queries takes
+    gen = torch.Generator("cuda").manual_seed(per_pass)
+    q = randn(gen, cu[-1], nh, hd)
+    pass_bytes(per_pass * 4 * 64 * hd * nkv)  # 10 tiles a sequence: the last pass is full
+    assert is_prompt(kivi, cache, cu[-1], m)
+    for causal in (True, False):
+        out = torch.full((cu[-1], nh, hd), 7.0, dtype=torch.float16, device="cuda")
+        lse = torch.full((cu[-1], nh), 7.0, device="cuda")
+        (cache.prefill if causal else cache.cross)(q, ints(*cu), m, seq, tables, out=out, lse=lse)
+        check(cache, tables, lens, q, cu, out, lse, causal=causal)
+        for b, n in enumerate(lens):
+            if n == 0:
+                assert not out[cu[b]:cu[b + 1]].any(), f"sequence {b}"
+                assert bool((lse[cu[b]:cu[b + 1]] == -torch.inf).all()), f"sequence {b}"
