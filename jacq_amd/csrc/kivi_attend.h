@@ -197,7 +197,9 @@ __device__ inline void values4x2(uint32_t w, int odd, h2 s, h2 z, h2 (&out)[2]) 
 // A query row's values for the matrix cores, 8 of them in each of N operands, from fp16 or bf16, and
 // the scale that goes with them.  fp16 has the bits of bf16 but not its range: a power of two brings
 // the row's largest magnitude (`most` joins it over the row's lanes) to 2^14, so values down to 2^-28
-// of it keep all their bits.
+// of it keep all their bits.  The scale stays a normal number: for a row of subnormals it may lie below
+// fp32's range, and 0 times a masked score's -inf, or what is above it times a score of 0, is NaN.  A finite
+// score is below 2^38 before the scale, so at 2^-126 all weights are the 1 that they should be.
 template <int N, class F>
 __device__ inline float half_row(const u4 (&raw)[N], int bf16, float scale, h8 (&q)[N], F most) {
   if (!bf16) {
@@ -220,7 +222,7 @@ __device__ inline float half_row(const u4 (&raw)[N], int bf16, float scale, h8 (
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int c = 0; c < 8; ++c) q[i][c] = (_Float16)__builtin_amdgcn_ldexpf(value(i, c), e);
-  return __builtin_amdgcn_ldexpf(scale, -e);
+  return fminf(fmaxf(__builtin_amdgcn_ldexpf(scale, -e), 0x1p-126f), 0x1.fffffep127f);
 }
 
 // Whether fp16 holds all values of a scale and a zero, the ends being 0 and 15 times the scale from it;

@@ -1,4 +1,5 @@
-"""Extremes of the int4 cache's attention of chunks: sequences without tokens at a pass's end."""
+"""Extremes of the int4 cache's attention of chunks, through both of its kernels: sequences without tokens
+at a pass's end, queries and scales near the ends of their types."""
 from __future__ import annotations
 
 import ctypes
@@ -8,6 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from tests.test_gpu_kivi_attend import check, ints, is_prompt, kivi, make, offsets, randn  # noqa: E402,F401
+from tests.test_gpu_kivi_attend_edges import SIZES, call  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +42,35 @@ def test_sequences_without_tokens_at_the_end_of_a_pass(kivi, pass_bytes, batch, 
             if n == 0:
                 assert not out[cu[b]:cu[b + 1]].any(), f"sequence {b}"
                 assert bool((lse[cu[b]:cu[b + 1]] == -torch.inf).all()), f"sequence {b}"
+
+
+@pytest.mark.parametrize("heads,m,prompt", SIZES)
+def test_subnormal_queries_and_scales(kivi, heads, m, prompt):  # noqa: F811
+    """All scores are next to 0, so the output is a mean of the values that a query sees."""
+    nh, nkv, hd = heads
+    lens = [300, 222]
+    cache, tables, seq, q, cu, most = call(kivi, *heads, 16, lens, m, prompt, seed=11)
+    gen = torch.Generator("cuda").manual_seed(5)
+    bits = torch.randint(1, 4, q.shape, generator=gen, device="cuda", dtype=torch.int16)  # x 2^-133
+    bits[..., ::2] |= -2 ** 15  # negative ones
+    tiny = bits.view(torch.bfloat16)
+    one = torch.ones_like(tiny)
+    for x, scale in ((tiny, 1 / 128), (tiny, 2.0 ** -60), (one, 1e-42), (one * 2.0 ** 100, 1e-42),
+                     (q, 1e-42), (q.to(torch.bfloat16), 2.0 ** -149)):
+        for window, sinks in ((None, 0), (40, 3)):
+            got = cache.prefill(x, ints(*cu), most, seq, tables, window=window, sinks=sinks, scale=scale)
+            check(cache, tables, lens, x, cu, got, None, window, sinks, scale=scale)
+        got = cache.cross(x, ints(*cu), most, seq, tables, scale=scale)
+        check(cache, tables, lens, x, cu, got, causal=False, scale=scale)
+
+
+@pytest.mark.parametrize("heads,m,prompt", SIZES)
+def test_keys_of_0_under_a_scale_beyond_fp32(kivi, heads, m, prompt):  # noqa: F811
+    """The row's magnitude x the scale is no fp32 number, but the scores are 0."""
+    lens = [60, 50]
+    cache, tables, seq, q, cu, most = call(kivi, *heads, 16, lens, m, prompt, seed=14)
+    x = q.to(torch.bfloat16) * 2.0 ** 100
+    for b, n in enumerate(lens):
+        cache.k_scr[b, :, :n] = 0.0
+    got = cache.prefill(x, ints(*cu), most, seq, tables, scale=2.0 ** 60)
+    check(cache, tables, lens, x, cu, got, scale=2.0 ** 60)
