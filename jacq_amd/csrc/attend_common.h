@@ -223,6 +223,20 @@ __device__ inline void store4(const A& a, int64_t at, f4 x) {
   *(u2*)((uint16_t*)a.o + at) = u2{x0 | x1 << 16, x2 | x3 << 16};
 }
 
+// Whether query `tok` of a sequence of n tokens, whose first one stands at position `first`, sees any: then
+// weights whose sum is 0 are of scores that all are -inf.  Of a cache without a rule of its own they are
+// taken as a row's that sees nothing.
+template <class G, class A>
+__device__ inline bool sees_any(const G&, const A&, int /*n*/, int /*first*/, int /*tok*/) {
+  return false;
+}
+
+// What a row's weighted sums are multiplied by: 1 / l; where the row sees nothing 0, and where all that it
+// sees weighs nothing NaN, as 0 / 0.
+__device__ inline float over_sum(float l, bool sees) {
+  return l != 0.0f ? 1.0f / l : sees ? __builtin_nanf("") : 0.0f;
+}
+
 // Bits 0 to n - 1; n in any range.
 __device__ inline uint64_t low_bits(int n) {
   return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
@@ -253,7 +267,7 @@ __device__ inline void merge_slices(const G& g, const A& a) {
     l = l * f0 + pl * f1;
     mx = to;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = over_sum(l, sees_any(g, a, p.n, p.n - p.all, (int)(i / (HD / 4)) / g.nh));
   store4(a, at * HD + ch, acc * inv);
   if (a.lse && ch == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
 }
@@ -290,7 +304,7 @@ __device__ inline void store_row(const A& a, int64_t at, const float* x, int n) 
 template <class G, class A>
 __device__ inline void finish_row(const G& g, const A& a, const Segment<G>& s, int row, int hd, int ch, float* x, int n, float l, float m) {
   const int r = s.rb * a.rows + row, tok = s.q0 + r / g.gqa, head = s.h * g.gqa + r % g.gqa;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = over_sum(l, sees_any(g, a, s.span.n, s.span.first, r / g.gqa));
   for (int i = 0; i < n; ++i) x[i] *= inv;
   store_row(a, ((int64_t)tok * g.nh + head) * hd + ch, x, n);
   if (ch == 0) {

@@ -137,6 +137,11 @@ __device__ inline int row_slices(const KiviGeo& g, const KiviAttendArgs& a, cons
   return kivi_slices(a, KiviTiles(g, a, p.n, a.causal ? p.n - p.all : p.n - 1), p.m, p.all);
 }
 
+// A query sees its own token at least, or in no order all of them.
+__device__ inline bool sees_any(const KiviGeo&, const KiviAttendArgs& a, int n, int first, int tok) {
+  return (a.causal ? first + tok : n - 1) >= 0;
+}
+
 template <>
 struct SpanOf<KiviGeo> {
   typedef KiviSpan type;

@@ -528,7 +528,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, prompt_groups(HD)) void kivi_pro
             f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
     return;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = over_sum(l, sees_any(g, a, n, p0, out_row / g.gqa));
   if (a.lse && hh_ == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
 #pragma unroll
   for (int d = 0; d < DT; ++d)

@@ -831,7 +831,8 @@ class PagedKiviCache:
         first ``sinks`` of the sequence.  No sequence has more than max_q queries: of one that
         has, the rows after its first max_q are left as they are, and so are rows outside every
         sequence (undefined in a fresh output).  lse [tokens, NH] fp32 takes the log of the sum
-        of exponentials.  A query that sees nothing gives 0 (lse -inf)."""
+        of exponentials.  A query that sees nothing gives 0 (lse -inf); one whose scores all are
+        -inf, as keys with infinities give them, NaN."""
         return self._attend(q, cu_q, max_q, seq_lens, block_tables, window, sinks, 1, scale, out,
                             lse, workspace)
 

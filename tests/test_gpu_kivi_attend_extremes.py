@@ -1,5 +1,5 @@
 """Extremes of the int4 cache's attention of chunks, through both of its kernels: sequences without tokens
-at a pass's end, queries and scales near the ends of their types."""
+at a pass's end, queries and scales near the ends of their types, scores that are not finite."""
 from __future__ import annotations
 
 import ctypes
@@ -8,6 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from tests import kivi_attend_ref as ref  # noqa: E402
 from tests.test_gpu_kivi_attend import check, ints, is_prompt, kivi, make, offsets, randn  # noqa: E402,F401
 from tests.test_gpu_kivi_attend_edges import SIZES, call  # noqa: E402
 
@@ -74,3 +75,38 @@ def test_keys_of_0_under_a_scale_beyond_fp32(kivi, heads, m, prompt):  # noqa: F
         cache.k_scr[b, :, :n] = 0.0
     got = cache.prefill(x, ints(*cu), most, seq, tables, scale=2.0 ** 60)
     check(cache, tables, lens, x, cu, got, scale=2.0 ** 60)
+
+
+@pytest.mark.parametrize("heads,m,prompt", SIZES)
+def test_rows_whose_scores_are_all_minus_infinity(kivi, heads, m, prompt):  # noqa: F811
+    """0 / 0 by the definition, so NaN, with lse -inf; only a query that sees nothing gives 0."""
+    nh, nkv, hd = heads
+    lens = [3000, 300, 57, 1]  # cut into slices, whole
+    cache, tables, seq, q, cu, most = call(kivi, *heads, 16, lens, m, prompt, seed=12)
+    q[..., 5] = 1.0
+    assert bool((seq[3] < most).all())  # queries of the last that see nothing
+    last = [lens[0], 290, 50, 1]  # tokens of each, from the first on, whose keys have an infinity
+    for b, n in enumerate(lens):
+        old = ref.old_tokens(cache.geo, n)
+        for t in range(0, min(old, last[b]), ref.GROUP):
+            cache.k_zero[tables[b, t // 16].long(), :, 5] = -torch.inf
+        cache.k_scr[b, :, :max(0, last[b] - old), 5] = -torch.inf
+    for causal, window, sinks in ((True, None, 0), (True, 4, 0), (True, 4, 40), (False, None, 0)):
+        lse = torch.empty(cu[-1], nh, device="cuda")
+        if causal:
+            got = cache.prefill(q, ints(*cu), most, seq, tables, window=window, sinks=sinks, lse=lse)
+        else:
+            got = cache.cross(q, ints(*cu), most, seq, tables, lse=lse)
+        for b, n in enumerate(lens):
+            what = f"sequence {b}, causal {causal}, window {window}, sinks {sinks}"
+            lack = max(0, m - n) if causal else 0
+            rows = slice(cu[b] + lack, cu[b + 1])
+            assert not got[cu[b]:cu[b] + lack].any(), what
+            assert bool((lse[cu[b]:cu[b] + lack] == -torch.inf).all()), what
+            r = ref.attend(q[rows], *ref.held_values(cache, tables, b, n), window, sinks, causal)
+            none = r["lse"] == -torch.inf
+            assert bool(none.any()) if b in (0, 3) else bool((~none).any()), what
+            want = torch.where(none[..., None], torch.nan, r["o"])
+            r["size"] = torch.where(r["size"].isinf(), 30.0, r["size"])  # of the scores that are finite
+            ref.assert_within(got[rows], want, ref.tolerance(r, hd, got.dtype), what)
+            assert torch.equal(lse[rows] == -torch.inf, none), what
