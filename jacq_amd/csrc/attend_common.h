@@ -237,6 +237,12 @@ __device__ inline float over_sum(float l, bool sees) {
   return l != 0.0f ? 1.0f / l : sees ? __builtin_nanf("") : 0.0f;
 }
 
+// What a value of O is bounded by before it becomes fp16; a cache without a rule of its own has no bound.
+template <class G, class A>
+__device__ inline float bounded(const G&, const A&, float x) {
+  return x;
+}
+
 // Bits 0 to n - 1; n in any range.
 __device__ inline uint64_t low_bits(int n) {
   return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
@@ -268,7 +274,10 @@ __device__ inline void merge_slices(const G& g, const A& a) {
     mx = to;
   }
   const float inv = over_sum(l, sees_any(g, a, p.n, p.n - p.all, (int)(i / (HD / 4)) / g.nh));
-  store4(a, at * HD + ch, acc * inv);
+  acc *= inv;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) acc[c] = bounded(g, a, acc[c]);
+  store4(a, at * HD + ch, acc);
   if (a.lse && ch == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
 }
 
@@ -305,7 +314,7 @@ template <class G, class A>
 __device__ inline void finish_row(const G& g, const A& a, const Segment<G>& s, int row, int hd, int ch, float* x, int n, float l, float m) {
   const int r = s.rb * a.rows + row, tok = s.q0 + r / g.gqa, head = s.h * g.gqa + r % g.gqa;
   const float inv = over_sum(l, sees_any(g, a, s.span.n, s.span.first, r / g.gqa));
-  for (int i = 0; i < n; ++i) x[i] *= inv;
+  for (int i = 0; i < n; ++i) x[i] = bounded(g, a, x[i] * inv);
   store_row(a, ((int64_t)tok * g.nh + head) * hd + ch, x, n);
   if (ch == 0) {
     const float lse = l == 0.0f ? kNegInf : m + log2_(l);

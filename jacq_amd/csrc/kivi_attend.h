@@ -142,6 +142,13 @@ __device__ inline bool sees_any(const KiviGeo&, const KiviAttendArgs& a, int n, 
   return (a.causal ? first + tok : n - 1) >= 0;
 }
 
+// A mean of fp16 values is one, but the sum of the weights that they are multiplied by, each rounded to
+// fp16, may be a 2^-11th above the sum that divides it: beside 65504 that is beyond fp16.  NaN stays.
+__device__ inline float bounded(const KiviGeo&, const KiviAttendArgs& a, float x) {
+  if (a.o_type != kFp16) return x;
+  return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+}
+
 template <>
 struct SpanOf<KiviGeo> {
   typedef KiviSpan type;

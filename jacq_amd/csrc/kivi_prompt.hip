@@ -533,9 +533,12 @@ __global__ __launch_bounds__(64 * kPromptWaves, prompt_groups(HD)) void kivi_pro
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      store4(a, at * HD + d * 32 + i * 8 + hh_ * 4,
-             f4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]} * inv);
+    for (int i = 0; i < 4; ++i) {
+      f4 x;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = bounded(g, a, acc[d][4 * i + c] * inv);
+      store4(a, at * HD + d * 32 + i * 8 + hh_ * 4, x);
+    }
 }
 
 template <int HD>

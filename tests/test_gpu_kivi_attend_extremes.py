@@ -1,5 +1,6 @@
 """Extremes of the int4 cache's attention of chunks, through both of its kernels: sequences without tokens
-at a pass's end, queries and scales near the ends of their types, scores that are not finite."""
+at a pass's end, queries and scales near the ends of their types, scores that are not finite,
+values as large as fp16's."""
 from __future__ import annotations
 
 import ctypes
@@ -110,3 +111,33 @@ def test_rows_whose_scores_are_all_minus_infinity(kivi, heads, m, prompt):  # no
             r["size"] = torch.where(r["size"].isinf(), 30.0, r["size"])  # of the scores that are finite
             ref.assert_within(got[rows], want, ref.tolerance(r, hd, got.dtype), what)
             assert torch.equal(lse[rows] == -torch.inf, none), what
+
+
+@pytest.mark.parametrize("heads,m,prompt", SIZES)
+def test_a_mean_of_the_largest_values_is_finite(kivi, heads, m, prompt):  # noqa: F811
+    """The weights of 30 tokens are rounded up by a 2^-11th, the first's not, so their sum is more than the
+    rounded ones' is divided by; what it gives may not pass fp16, as no mean of fp16 values does."""
+    nh, nkv, hd = heads
+    for lens, groups in (([31], 0), ([31 + 2048], 64)):  # in the residual window; and behind groups that
+        cache, tables, seq, q, cu, most = call(kivi, *heads, 16, lens, m, prompt, seed=13)  # weigh nothing
+        old = ref.old_tokens(cache.geo, lens[0])
+        if groups:
+            for t in range(0, old, ref.GROUP):
+                at = tables[0, t // 16].long()
+                cache.k_scale[at], cache.k_zero[at] = 0.0, 0.0
+                cache.k_zero[at, :, 1] = -30000.0
+        left = lens[0] - old
+        k = torch.zeros(nkv, left, hd, dtype=torch.float16, device="cuda")
+        k[:, :-31, 1] = -30000.0
+        k[:, -31, 0] = 1.0
+        cache.k_scr[0, :, :left] = k
+        q.zero_()
+        q[..., :2] = 1.0
+        # weights 2^7 and 2^6.00079 = 64.035, which rounds to 64.0625
+        for sign in (1, -1):
+            cache.v_scr[0, :, :left] = sign * 65504.0
+            got = cache.cross(q, ints(*cu), most, seq, tables, scale=0.6926)
+            assert bool((got == sign * 65504.0).all())
+            got = cache.cross(q, ints(*cu), most, seq, tables, scale=0.6926,
+                              out=torch.empty(q.shape, device="cuda"))
+            assert bool(((got * sign - 65504.0).abs() <= 65504.0 * 2.0 ** -11).all())
