@@ -57,8 +57,8 @@ typedef struct jacq_kivi_pool {
  *             window is 0)
  *   causal 0  every query sees all SEQ_LENS[b] tokens; no window
  * A query that sees nothing gives 0 (lse -inf), one whose scores all are -inf
- * NaN (lse -inf), as the definition's 0 / 0.  Scores are scale (> 0) times the
- * products.
+ * NaN (lse -inf), as the definition's 0 / 0.  Scores are scale (> 0, finite
+ * times log2(e)) times the products.
  *   Q    [total_q, NH, HD] of q_dtype (fp16 or bf16), token rows q_stride
  *        elements apart
  *   O    [total_q, NH, HD] of o_dtype (q_dtype or fp32), contiguous; may be Q

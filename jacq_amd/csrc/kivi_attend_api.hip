@@ -297,7 +297,8 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
     if (x->causal != 0 && x->causal != 1) return fail("causal must be 0 or 1");
     if (!x->causal && (x->window || x->sinks))
       return fail("queries that see every token have no window and no sinks");
-    if (!std::isfinite(x->scale) || x->scale <= 0) return fail("scale must be positive and finite");
+    if (!std::isfinite(x->scale * jacq::kLog2e) || x->scale <= 0)
+      return fail("scale must be positive and finite, times log2(e) too");
     const int64_t row = (int64_t)geo->num_heads * geo->head_dim;
     if (x->q_stride < row || x->q_stride % 8 != 0)
       return fail("Q row stride must be a multiple of 8 and at least " + std::to_string(row) +

@@ -18,7 +18,6 @@ layer raises ``NativeLibraryMissing``.
 from __future__ import annotations
 
 import ctypes
-import math
 import os
 import struct
 from dataclasses import dataclass
@@ -485,6 +484,7 @@ def _raw_stream(t: torch.Tensor) -> int:
 
 
 DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+FLOAT_MAX = torch.finfo(torch.float32).max  # records hold floats
 
 # the records of jacq_kivi_attend.h packed at once: setting a structure's fields one by one takes as
 # long as a launch
@@ -782,7 +782,7 @@ class PagedKiviCache:
             _check(window >= 1, "WINDOW must be positive, or None")
         _check(sinks >= 0, "SINKS must not be negative")
         scale = hd ** -0.5 if scale is None else float(scale)
-        _check(0.0 < scale < math.inf, "SCALE must be positive and finite")
+        _check(0.0 < scale <= FLOAT_MAX, "SCALE must be positive and finite in fp32")
         if out is not None:
             check_shape(out, (total, nh, hd), "O")
             _check(out.dtype in (dtype, torch.float32) and out.is_contiguous(),

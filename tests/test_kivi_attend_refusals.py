@@ -1,0 +1,21 @@
+"""More refusals of the int4 cache's attention, without a GPU: arguments near the ends of their ranges."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from jacq_amd import kivi  # noqa: E402
+from tests.test_kivi_attend import CU, EINVAL, LENS, TABLES, attend, cpu_cache, error, q  # noqa: E402
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_a_scale_that_is_infinite_in_base_two_is_refused(scale):
+    """Scores are taken to base two, by scale x log2(e) in fp32."""
+    error(attend(scale=scale), EINVAL, "finite")
+
+
+@pytest.mark.parametrize("call", ["prefill", "cross"])
+def test_a_scale_beyond_fp32_is_refused(call):
+    with pytest.raises(kivi.KiviCheckError, match="SCALE"):
+        getattr(cpu_cache(), call)(q(), CU, 2, LENS, TABLES, scale=1e39)
