@@ -756,7 +756,7 @@ class PagedKiviCache:
                    "], got ", tuple(shape))
             _check(dtype in (torch.float16, torch.bfloat16), "Q must be fp16 or bf16")
             if not contiguous:
-                _check(shape[0] == 0 or (q.stride(2) == 1 and q.stride(1) == hd),
+                _check(shape[0] == 0 or (q.stride(2) == 1 and (nh == 1 or q.stride(1) == hd)),
                        "Q must have its heads side by side")
                 if shape[0] > 1:
                     stride = q.stride(0)

@@ -141,3 +141,14 @@ def test_a_mean_of_the_largest_values_is_finite(kivi, heads, m, prompt):  # noqa
             got = cache.cross(q, ints(*cu), most, seq, tables, scale=0.6926,
                               out=torch.empty(q.shape, device="cuda"))
             assert bool(((got * sign - 65504.0).abs() <= 65504.0 * 2.0 ** -11).all())
+
+
+def test_the_queries_of_one_head_may_lie_apart(kivi):  # noqa: F811
+    cache, tables, seq, q, cu, most = call(kivi, 1, 1, 64, 16, [300, 77], 5, False, seed=15)
+    wide = torch.full((cu[-1], 96), float("nan"), dtype=torch.float16, device="cuda")
+    x = wide[:, None, :64]
+    x.copy_(q)
+    assert not x.is_contiguous()
+    got = cache.prefill(x, ints(*cu), most, seq, tables)
+    assert torch.equal(got, cache.prefill(q, ints(*cu), most, seq, tables))
+    check(cache, tables, [300, 77], q, cu, got)

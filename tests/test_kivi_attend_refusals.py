@@ -19,3 +19,15 @@ def test_a_scale_that_is_infinite_in_base_two_is_refused(scale):
 def test_a_scale_beyond_fp32_is_refused(call):
     with pytest.raises(kivi.KiviCheckError, match="SCALE"):
         getattr(cpu_cache(), call)(q(), CU, 2, LENS, TABLES, scale=1e39)
+
+
+@pytest.mark.parametrize("call", ["prefill", "cross"])
+def test_the_queries_of_one_head_may_lie_apart(call):
+    """Heads of which there is one lie side by side whatever their stride is."""
+    geo = kivi.KiviGeometry(1, 1, 64, 16, 32, 64, 8, 16)
+    cache = kivi.PagedKiviCache(geo, 2, device="cpu")
+    wide = torch.zeros((3, 96), dtype=torch.float16)
+    for x in (wide[:, None, :64], wide[:, :64].unflatten(1, (1, 64)), wide[None, :, :64].transpose(0, 1)):
+        assert x.shape == (3, 1, 64) and not x.is_contiguous()
+        with pytest.raises(kivi.KiviCheckError, match="GPU device"):  # and nothing else is wrong
+            getattr(cache, call)(x, CU, 2, LENS, TABLES)
