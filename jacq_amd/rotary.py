@@ -21,7 +21,7 @@ from fractions import Fraction
 import torch
 
 from jacq_amd import kivi as _kivi
-from jacq_amd.kivi import DTYPES, KiviLaunchError, _check, check_shape
+from jacq_amd.kivi import DTYPES, FLOAT_MAX, KiviLaunchError, _check, check_shape
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 MAX_DIM = 256  # channels of a head that turn
@@ -122,7 +122,7 @@ class Rotary:
                    rotary_dim // 2, " numbers, got ", len(speeds))
             _check(all(math.isfinite(x) for x in speeds), "speeds must be finite")
         amplitude = own if amplitude is None else float(amplitude)
-        _check(math.isfinite(amplitude), "amplitude must be finite")
+        _check(abs(amplitude) <= FLOAT_MAX, "amplitude must be finite in fp32")
         self.head_dim, self.rotary_dim, self.layout = head_dim, rotary_dim, layout
         self.speeds, self.amplitude = tuple(speeds), amplitude
         self._turns = (ctypes.c_uint64 * len(speeds))(*[_turns(x) for x in speeds])
