@@ -71,7 +71,11 @@ class Scaling:
 def frequencies(rotary_dim: int, base: float = 10000.0, scaling: Scaling | None = None):
     """Radians a position of each pair, and the amplitude of cosine and sine."""
     if scaling is not None and scaling.kind == "base":
-        base *= scaling.factor ** (rotary_dim / max(1, rotary_dim - 2))
+        try:
+            base *= scaling.factor ** (rotary_dim / max(1, rotary_dim - 2))
+        except OverflowError:
+            base = math.inf
+        _check(base < math.inf, "the scaled base must be finite")
     f = [base ** (-2 * i / rotary_dim) for i in range(rotary_dim // 2)]
     if scaling is None or scaling.kind == "base":
         return f, 1.0
