@@ -143,13 +143,27 @@ constexpr int kSplitRows = 32;
 // 256 queries of one of 64 sequences of 1000 tokens (20480) 111 us there and 63 so, of one of 32 (10240) 66
 // and 58, of one of 16 (5120) 43 and 57; 100 of each of 4 of 100 of 200 tokens (10400) 36 and 43.
 constexpr int64_t kSplitSegments = 12000;
-// Bytes of fp16 tiles that a pass lays in the workspace, about, and passes at most, a few us each (of a
-// wide table's, most have nothing to do): a call of more is left to the few-query kernel.
+// Bytes of fp16 tiles that a pass lays in the workspace, about.
 constexpr int64_t kPassBytes = (int64_t)1 << 31;
+// Passes up to which a call is a prompt's: the table's width tells how many there may be, and one with nothing
+// to do still takes 9 to 12 us.  256 sequences, 40/8 heads of 128, us in the few-query kernel and in passes: 200
+// queries of each of 1000 tokens, 33 passes, 2228 and 1847, 130 passes 2224 and 3203; of 65 passes 500 of 1000
+// 5025 and 4287, 200 of 3000 5605 and 4975, but 200 of 200 1056 and 1379, 70 of 1000 958 and 1438.
 constexpr int64_t kMostPasses = 64;
+// Of a call that can be split there are more passes where the few-query kernel has so many segments for each:
+// most of them are empty, and still cost 2 ns, and it leaves segments whole (kMostParts).  A chunk beside single
+// queries of 2047 sequences, table of 131072 tokens, 40/8 heads of 128, us there and in passes, the others of
+// 1000 to 4000 tokens and of 100 to 200:
+//   64 queries, 2200 segments a pass    2694 and 2692, 634 and 1395
+//   128, 4200                           5078 and 3093, 1216 and 1820
+//   256, 8000                           5415 and 3266, 1550 and 1917
+//   512, 14400                          6076 and 3452, 2239 and 2076
+// of 255 sequences, 65 passes: 2048 queries, 10000 segments a pass, 1384 and 916.
+constexpr int64_t kPassSegments = 4000;
 // A prompt's workgroups a CU at most, slices counted: those that the lengths do not ask for end at once.
 constexpr int64_t kMostGroups = 8;
-// Bytes of parts for which the few-query kernel still cuts: a call of more has segments enough.
+// Bytes of parts for which the few-query kernel still cuts.  A call of more has 64 thousand segments (of 32 rows
+// of 128), which fill the CUs though some are empty; but a long one among them stays whole.
 constexpr int64_t kMostParts = (int64_t)1 << 30;
 
 // Workgroups of a launch, which has fewer than 2^32 threads.
@@ -194,10 +208,14 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
   const int64_t images = std::min<int64_t>(batch, total_q / (p.split + 1)) * cap;
   p.per_pass = (int)std::max<int64_t>(1, std::min(images, pass_bytes / image));
   const int64_t passes = (images + p.per_pass - 1) / p.per_pass;
-  p.prompt = rows >= kPromptRows && images > 0 && passes <= kMostPasses && images <= INT32_MAX - 4096 &&
-             (queries * g.nh * tokens >= kPromptWork ||
-              blocks(32) * g.nkv >= kPromptRounds * jacq::few_groups(g.hd, 2) * device_cus() ||
-              (p.split && (int64_t)batch * g.nkv * ((rows + 31) / 32) >= kSplitSegments));
+  const int64_t segments = (int64_t)batch * g.nkv * ((rows + 31) / 32);  // of the few-query kernel alone
+  const bool pays = rows >= kPromptRows &&
+                    (passes <= kMostPasses || (p.split && passes * kPassSegments <= segments)) &&
+                    (queries * g.nh * tokens >= kPromptWork ||
+                     blocks(32) * g.nkv >= kPromptRounds * jacq::few_groups(g.hd, 2) * device_cus() ||
+                     (p.split && segments >= kSplitSegments));
+  // Split, the few-query kernel has a segment a sequence and kv head: it may be the only way to launch it.
+  p.prompt = images > 0 && images <= INT32_MAX - 4096 && (pays || (p.split && segments >= kMostSegments));
   p.few = !p.prompt || p.split;
   if (p.prompt) {
     p.passes = (int)passes;

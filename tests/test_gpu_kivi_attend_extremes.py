@@ -4,6 +4,7 @@ values as large as fp16's."""
 from __future__ import annotations
 
 import ctypes
+import random
 
 import pytest
 
@@ -14,6 +15,7 @@ from tests.test_gpu_kivi_attend import check, ints, is_prompt, kivi, make, offse
 from tests.test_gpu_kivi_attend_edges import SIZES, call  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+POOL = ("k_code", "k_scale", "k_zero", "v_code", "v_scale", "v_zero")
 
 
 @pytest.fixture
@@ -152,3 +154,32 @@ def test_the_queries_of_one_head_may_lie_apart(kivi):  # noqa: F811
     got = cache.prefill(x, ints(*cu), most, seq, tables)
     assert torch.equal(got, cache.prefill(q, ints(*cu), most, seq, tables))
     check(cache, tables, [300, 77], q, cu, got)
+
+
+def test_a_chunk_beside_the_steps_of_many_sequences_under_a_wide_table(kivi, pass_bytes):  # noqa: F811
+    """max_q for every sequence would be more workgroups than a launch takes, the tiles of the table's width
+    more passes than pay for prompts alone."""
+    nh, nkv, hd, batch, chunk = 32, 2, 64, 2048, 8200
+    rng = random.Random(3)
+    lens = [rng.choice((0, 1, 20, 33, 64, 90)) for _ in range(batch)]
+    m = [rng.choice((0, 1, 1, 2, 3)) for _ in lens]
+    lens[700], m[700] = 400, chunk  # most of them before the first token
+    lens[1500], m[1500] = 700, 1
+    cache, tables, seq = make(kivi, nh, nkv, hd, 16, 32, lens, seed=1, width=2048)
+    cu = offsets(m)
+    pass_bytes(1 << 28)
+    assert is_prompt(kivi, cache, cu[-1], chunk)
+    gen = torch.Generator("cuda").manual_seed(1)
+    q = randn(gen, cu[-1], nh, hd)
+    some = [b for b in range(batch) if b % 29 == 0 or b in (699, 700, 701, 1500, batch - 1)]
+    for window, sinks in ((None, 0), (50, 3)):
+        lse = torch.full((cu[-1], nh), 7.0, device="cuda")
+        got = cache.prefill(q, ints(*cu), chunk, seq, tables, window=window, sinks=sinks, lse=lse)
+        assert not bool((lse == 7.0).all(-1).any())  # every row is written
+        for b in some:
+            rows = slice(cu[b], cu[b + 1])
+            part = kivi.PagedKiviCache.from_tensors(cache.geo, {
+                **dict(zip(POOL, cache.pool()[:6])), "k_scr": cache.k_scr[b:b + 1],
+                "v_scr": cache.v_scr[b:b + 1]})
+            check(part, tables[b:b + 1], lens[b:b + 1], q[rows], [0, m[b]], got[rows], lse[rows], window,
+                  sinks)

@@ -6,7 +6,8 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from jacq_amd import kivi  # noqa: E402
-from tests.test_kivi_attend import CU, EINVAL, LENS, TABLES, attend, cpu_cache, error, q  # noqa: E402
+from tests.test_kivi_attend import (CU, EINVAL, ENOMEM, GOOD, LENS, TABLES, attend,  # noqa: E402
+                                    cpu_cache, error, q)
 
 
 @pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
@@ -31,3 +32,18 @@ def test_the_queries_of_one_head_may_lie_apart(call):
         assert x.shape == (3, 1, 64) and not x.is_contiguous()
         with pytest.raises(kivi.KiviCheckError, match="GPU device"):  # and nothing else is wrong
             getattr(cache, call)(x, CU, 2, LENS, TABLES)
+
+
+@pytest.mark.parametrize("heads", [(40, 8, 128), (16, 16, 128), (64, 4, 64)])
+@pytest.mark.parametrize("batch,tokens,chunk", [
+    (2048, 32768, 8192), (1024, 131072, 16384), (2048, 131072, 32768), (65535, 8192, 2048),
+    (65535, 262000, 8192), (30000, 131072, 20000)])
+def test_a_chunk_beside_single_queries_is_taken_under_a_wide_table(heads, batch, tokens, chunk):
+    """Whatever the table's width and max_q x sequences; no workspace is given, so nothing is launched."""
+    geo = dict(num_heads=heads[0], num_kv_heads=heads[1], head_dim=heads[2], max_pages_per_seq=tokens // 16)
+    total = batch - 1 + chunk
+    size = kivi.lib().jacq_kivi_attend_workspace_size(kivi.KiviGeometry(**{**GOOD, **geo}).ref, batch, total,
+                                                      chunk)
+    assert 0 < size < 2 ** 33
+    rc = attend(geo=geo, batch=batch, total_q=total, max_q=chunk, q_stride=heads[0] * heads[2])
+    error(rc, ENOMEM, str(size))
