@@ -237,10 +237,11 @@ __device__ inline float over_sum(float l, bool sees) {
   return l != 0.0f ? 1.0f / l : sees ? __builtin_nanf("") : 0.0f;
 }
 
-// What a value of O is bounded by before it becomes fp16; a cache without a rule of its own has no bound.
-template <class G, class A>
-__device__ inline float bounded(const G&, const A&, float x) {
-  return x;
+// A weighted sum of values, bounded by the largest value times the sum l of the weights; of a cache without a
+// rule of its own there is no largest value.
+template <class G>
+__device__ inline float bounded(const G&, float sum, float /*l*/) {
+  return sum;
 }
 
 // Bits 0 to n - 1; n in any range.
@@ -274,10 +275,9 @@ __device__ inline void merge_slices(const G& g, const A& a) {
     mx = to;
   }
   const float inv = over_sum(l, sees_any(g, a, p.n, p.n - p.all, (int)(i / (HD / 4)) / g.nh));
-  acc *= inv;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) acc[c] = bounded(g, a, acc[c]);
-  store4(a, at * HD + ch, acc);
+  for (int c = 0; c < 4; ++c) acc[c] = bounded(g, acc[c], l);
+  store4(a, at * HD + ch, acc * inv);
   if (a.lse && ch == 0) a.lse[at] = l == 0.0f ? kNegInf : (mx + log2_(l)) / kLog2e;
 }
 
@@ -314,7 +314,7 @@ template <class G, class A>
 __device__ inline void finish_row(const G& g, const A& a, const Segment<G>& s, int row, int hd, int ch, float* x, int n, float l, float m) {
   const int r = s.rb * a.rows + row, tok = s.q0 + r / g.gqa, head = s.h * g.gqa + r % g.gqa;
   const float inv = over_sum(l, sees_any(g, a, s.span.n, s.span.first, r / g.gqa));
-  for (int i = 0; i < n; ++i) x[i] = bounded(g, a, x[i] * inv);
+  for (int i = 0; i < n; ++i) x[i] = bounded(g, x[i], l) * inv;
   store_row(a, ((int64_t)tok * g.nh + head) * hd + ch, x, n);
   if (ch == 0) {
     const float lse = l == 0.0f ? kNegInf : m + log2_(l);

@@ -143,10 +143,10 @@ __device__ inline bool sees_any(const KiviGeo&, const KiviAttendArgs& a, int n, 
 }
 
 // A mean of fp16 values is one, but the sum of the weights that they are multiplied by, each rounded to
-// fp16, may be a 2^-11th above the sum that divides it: beside 65504 that is beyond fp16.  NaN stays.
-__device__ inline float bounded(const KiviGeo&, const KiviAttendArgs& a, float x) {
-  if (a.o_type != kFp16) return x;
-  return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+// fp16, may be a 2^-11th above the sum l that divides it: beside 65504 that is beyond fp16.  An instruction a
+// value (a sum that is NaN comes with an l that is).
+__device__ inline float bounded(const KiviGeo&, float sum, float l) {
+  return __builtin_amdgcn_fmed3f(sum, -65504.0f * l, 65504.0f * l);
 }
 
 template <>

@@ -536,7 +536,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, prompt_groups(HD)) void kivi_pro
     for (int i = 0; i < 4; ++i) {
       f4 x;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[c] = bounded(g, a, acc[d][4 * i + c] * inv);
+      for (int c = 0; c < 4; ++c) x[c] = bounded(g, acc[d][4 * i + c], l) * inv;
       store4(a, at * HD + d * 32 + i * 8 + hh_ * 4, x);
     }
 }
