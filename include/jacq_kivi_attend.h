@@ -14,7 +14,11 @@
  *   old = max(0, n - R) / 32 * 32  (at most what the table addresses)
  * with K = code * scale + zero of its group and channel, V = code * scale +
  * zero of itself and its 32 channels; else it is row t - old of the scratch.
- * Values are rounded to fp16 once.  A token that a query does not see may hold
+ * The products take both rounded to fp16 once, queries in fp16 (bf16 ones times
+ * a power of two of the row) and softmax weights rounded to fp16; sums, maxima
+ * and LSE are fp32.  An output of fp16 or fp32 is off by about 6e-4 of its norm,
+ * mostly by K's rounding, where the codes hold K to a thirtieth of a group's
+ * range.  A token that a query does not see may hold
  * anything.  To a query that sees it, a V that is not finite (fp16 V; or zero
  * or zero + 15 scale of 32 of its channels beyond fp16) counts as a NaN key:
  * all of the query's output is NaN.  A table entry outside
@@ -92,7 +96,8 @@ int jacq_kivi_attend(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool,
 
 /* The values of tokens STARTS[b] to ENDS[b] of each sequence of ENDS[b] tokens,
  * one sequence after another: K, V [total, NKV, HD] of `dtype`, each rounded to
- * it once.  Tokens past `total` are dropped. */
+ * it once (bf16: from its fp32 value, which differs from the exact one only where
+ * scale and zero are 2^9 apart or more).  Tokens past `total` are dropped. */
 int jacq_kivi_read(const jacq_kivi_geometry* geo, const jacq_kivi_pool* pool, const int32_t* STARTS,
                    const int32_t* ENDS, const int32_t* BLOCK_TABLES, int32_t batch, int32_t total,
                    void* K, void* V, int32_t dtype, hipStream_t stream);

@@ -832,7 +832,11 @@ class PagedKiviCache:
         has, the rows after its first max_q are left as they are, and so are rows outside every
         sequence (undefined in a fresh output).  lse [tokens, NH] fp32 takes the log of the sum
         of exponentials.  A query that sees nothing gives 0 (lse -inf); one whose scores all are
-        -inf, as keys with infinities give them, NaN."""
+        -inf, as keys with infinities give them, NaN.  The output carries no autograd graph.
+
+        max_q None takes all of q for one sequence's: the call is planned, and its workspace sized, for
+        that and for sequences as long as the table is wide, so a step of many sequences under a wide
+        table should give its own."""
         return self._attend(q, cu_q, max_q, seq_lens, block_tables, window, sinks, 1, scale, out,
                             lse, workspace)
 

@@ -51,7 +51,10 @@ class Scaling:
     turns    by how often a pair turns over ``length`` tokens (what the model learned):
              frequencies of at most ``slow`` turns by the factor, of ``fast`` and more not at
              all, in between a mean of both that is linear in the turns; cosines and sines
-             times ``amplitude`` (by default 0.1 ln(factor) + 1)"""
+             times ``amplitude`` (by default 0.1 ln(factor) + 1)
+
+    A model whose mean of both is linear in the pair's index, or another one, gives its frequencies
+    to ``Rotary`` as ``speeds``."""
     kind: str
     factor: float
     length: int = 4096
@@ -171,7 +174,8 @@ class Rotary:
         same rotated: new tensors of their type (k of k_dtype: the int4 cache takes fp16), or
         q_out, k_out, of any type, which may be q and k themselves and must overlap neither
         otherwise.  k may be None.  inverse: by the negative angles; with an amplitude of 1 the
-        way back, with any the gradient of this rotation for the gradient of its outputs."""
+        way back, with any the gradient of this rotation for the gradient of its outputs, which
+        carry no autograd graph themselves."""
         shape, dtype, index = q.shape, q.dtype, q.get_device()
         tokens = shape[0] if len(shape) else 0
         q_stride, k_stride = self._quick(q, index), 0
