@@ -214,8 +214,8 @@ Plan plan_attend(const KiviGeo& g, int batch, int total_q, int max_q) {
                     (queries * g.nh * tokens >= kPromptWork ||
                      blocks(32) * g.nkv >= kPromptRounds * jacq::few_groups(g.hd, 2) * device_cus() ||
                      (p.split && segments >= kSplitSegments));
-  // Split, the few-query kernel has a segment a sequence and kv head: it may be the only way to launch it.
-  p.prompt = images > 0 && images <= INT32_MAX - 4096 && (pays || (p.split && segments >= kMostSegments));
+  // more segments than a launch takes: row tiles are of the call's queries alone, and four times as long
+  p.prompt = images > 0 && images <= INT32_MAX - 4096 && (pays || segments >= kMostSegments);
   p.few = !p.prompt || p.split;
   if (p.prompt) {
     p.passes = (int)passes;

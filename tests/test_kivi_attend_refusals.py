@@ -47,3 +47,12 @@ def test_a_chunk_beside_single_queries_is_taken_under_a_wide_table(heads, batch,
     assert 0 < size < 2 ** 33
     rc = attend(geo=geo, batch=batch, total_q=total, max_q=chunk, q_stride=heads[0] * heads[2])
     error(rc, ENOMEM, str(size))
+
+
+def test_many_long_chunks_are_taken_under_a_wide_table():
+    """More blocks of 32 rows than a launch has workgroups, but not more row tiles; nothing is launched."""
+    geo = dict(num_heads=16, num_kv_heads=1, head_dim=64, max_pages_per_seq=16384 // 16)
+    kw = dict(batch=65535, total_q=65535 * 520, max_q=520)
+    size = kivi.lib().jacq_kivi_attend_workspace_size(kivi.KiviGeometry(**{**GOOD, **geo}).ref, *kw.values())
+    assert 0 < size < 2 ** 33
+    error(attend(geo=geo, q_stride=16 * 64, **kw), ENOMEM, str(size))
